@@ -12,6 +12,7 @@ LIB_PATH = os.environ.get("GPT_LIB") or os.path.join(_HERE, "libgptools_hip.so")
 
 GPT_OK, GPT_ERR_NOT_PD, GPT_ERR_SHAPE, GPT_ERR_UNSUPPORTED, GPT_ERR_TIMEOUT = 0, 1, 2, 3, 4
 GPT_ROW_MAJOR, GPT_COL_MAJOR = 0, 1
+GPT_F64, GPT_F32, GPT_F16, GPT_BF16 = 0, 1, 2, 3
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
@@ -50,6 +51,14 @@ _SIGNATURES = {
     "gpt_gp_inv_rfft2_obs_lpdf_kernel_vjp": [c_int, c_int, c_dbl, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_dbl, c_ptr, c_i64,
                                              c_i64, c_i64, c_ptr, c_int, c_i64, c_i64, c_i64, c_int, c_ptr, c_ptr, c_ptr,
                                              c_ptr, c_ptr, c_ptr],
+    # read-out of several latent fields
+    "gpt_layer_norm": [c_int, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_dbl, c_ptr, c_ptr, c_ptr, c_ptr, ctypes.c_size_t],
+    "gpt_layer_norm_vjp": [c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr,
+                           ctypes.c_size_t],
+    "gpt_categorical_logit_glm_lpmf": [c_int, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr,
+                                       ctypes.c_size_t],
+    "gpt_categorical_logit_glm_lpmf_vjp": [c_int, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr,
+                                           c_ptr, c_ptr, c_ptr, c_ptr, ctypes.c_size_t],
     # host-pointer entry points
     "gpt_gp_rfft2_host": [c_int, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr],
     "gpt_gp_inv_rfft2_host": [c_int, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr],
@@ -93,6 +102,8 @@ _PLAIN = {
     "gpt_path_for_shape": ([c_i64, c_i64], c_int),
     "gpt_host_copy_slice": ([ctypes.c_size_t, c_int, c_int, ctypes.POINTER(ctypes.c_size_t),
                              ctypes.POINTER(ctypes.c_size_t)], None),
+    "gpt_layer_norm_workspace": ([c_int, c_i64, c_i64, c_int], ctypes.c_size_t),
+    "gpt_categorical_logit_glm_workspace": ([c_int, c_i64, c_i64, c_i64, c_int], ctypes.c_size_t),
     # cross-chain batching
     "gpt_batcher_create": ([c_int, c_int, c_int, c_i64, c_i64, c_int, ctypes.POINTER(c_ptr)], c_int),
     "gpt_batcher_destroy": ([c_ptr], c_int),

@@ -1,0 +1,498 @@
+// Layer norm and its reverse mode (gpt_layer_norm, gpt_layer_norm_vjp): rows of n values, standardised one by one.
+//
+//   mean = sum x / n, var = sum (x - mean)^2 / n, rstd = 1 / sqrt(var + eps), h = (x - mean) rstd, y = h w + b
+//   g = ybar w, xbar = rstd (g - <g> - h <g h>), wbar = sum_rows ybar h, bbar = sum_rows ybar
+//
+// Both are bound by HBM: forward reads x and writes y, reverse reads x and ybar and writes xbar. A row of up to ROW_BYTES
+// stays in the registers of the threads that read it (norm_row, norm_row_vjp): every value is read once, and the variance is
+// a sum of squares about the mean, not a difference of two sums. A longer row (a whole lattice) is cut into pieces that
+// many workgroups take (norm_long_*): statistics of the pieces, then a second sweep.
+#include "gpt_readout.h"
+#include "gpt_types.h"
+
+using namespace gptt;
+
+namespace {
+
+// ---- rows that fit the registers of one workgroup ---------------------------------------------------------------------
+// THREADS consecutive threads take a row, ITER 16-byte vectors each, THREADS apart.
+template <typename T, int THREADS, int ITER> struct RowRegs {
+    static constexpr int N = Vec16<T>::N;
+    acc_t<T> v[ITER * N];
+    __device__ __forceinline__ void load(const T* p, int64_t n, int t) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int64_t k = (int64_t)(i * THREADS + t) * N;
+            if (k + N <= n) {
+                const auto u = load16(p + k);
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i * N + e] = (acc_t<T>)u[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i * N + e] = k + e < n ? (acc_t<T>)p[k + e] : (acc_t<T>)0;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* p, int64_t n, int t) const {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int64_t k = (int64_t)(i * THREADS + t) * N;
+            if (k + N <= n) {
+                typename Vec16<T>::V u;
+#pragma unroll
+                for (int e = 0; e < N; ++e) u[e] = (T)v[i * N + e];
+                store16(p + k, u);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (k + e < n) p[k + e] = (T)v[i * N + e];
+            }
+        }
+    }
+    // in the first n values of the row? (index of register j)
+    static __device__ __forceinline__ bool inside(int j, int64_t n, int t) {
+        return (int64_t)((j / N) * THREADS + t) * N + j % N < n;
+    }
+};
+
+template <typename T, int THREADS, int ITER>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, K = ITER * Vec16<T>::N;
+    __shared__ A red[THREADS / 64];
+    const int t = threadIdx.x % THREADS;
+    const int64_t row = (int64_t)blockIdx.x * (BLOCK / THREADS) + threadIdx.x / THREADS;
+    if (row >= a.rows) return; // (whole waves; a workgroup with barriers has one row)
+    const int64_t n = a.width;
+    RowRegs<T, THREADS, ITER> x;
+    x.load((const T*)a.x + row * n, n, t);
+    A s[1] = {0};
+#pragma unroll
+    for (int j = 0; j < K; ++j) s[0] += x.v[j];
+    row_sum<THREADS>(s, red, false);
+    const A mean = s[0] / (A)n;
+    s[0] = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        x.v[j] -= mean;
+        if (RowRegs<T, THREADS, ITER>::inside(j, n, t)) s[0] += x.v[j] * x.v[j];
+    }
+    row_sum<THREADS>(s, red, true);
+    const A rstd = (A)1 / sqrt(s[0] / (A)n + (A)a.eps);
+    if (t == 0) {
+        ((A*)a.mean)[row] = mean;
+        ((A*)a.rstd)[row] = rstd;
+    }
+    RowRegs<T, THREADS, ITER> w;
+#pragma unroll
+    for (int j = 0; j < K; ++j) x.v[j] *= rstd;
+    if (a.weight) {
+        w.load((const T*)a.weight, n, t);
+#pragma unroll
+        for (int j = 0; j < K; ++j) x.v[j] *= w.v[j];
+    }
+    if (a.bias) {
+        w.load((const T*)a.bias, n, t);
+#pragma unroll
+        for (int j = 0; j < K; ++j) x.v[j] += w.v[j];
+    }
+    x.store((T*)a.y + row * n, n, t);
+}
+
+// A workgroup takes rows blockIdx.x, + gridDim.x, ...; its sums for the parameters' gradients stay in registers, and go to
+// partial[2][gridDim.x][n] at the end (norm_param_sum adds them up in a fixed order).
+template <typename T, int THREADS, int ITER, bool PARAMS>
+__global__ __launch_bounds__(THREADS) void norm_row_vjp(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int K = ITER * Vec16<T>::N;
+    __shared__ A red[THREADS / 64 * 2];
+    const int t = threadIdx.x;
+    const int64_t n = a.width;
+    A wbar[PARAMS ? K : 1], bbar[PARAMS ? K : 1];
+    if (PARAMS) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) wbar[j] = bbar[j] = 0;
+    }
+    RowRegs<T, THREADS, ITER> w;
+    if (a.weight) w.load((const T*)a.weight, n, t);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        RowRegs<T, THREADS, ITER> x, g;
+        x.load((const T*)a.x + row * n, n, t);
+        g.load((const T*)a.ybar + row * n, n, t);
+        const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+        A s[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            x.v[j] = (x.v[j] - mean) * rstd;
+            if (PARAMS) {
+                wbar[j] += g.v[j] * x.v[j];
+                bbar[j] += g.v[j];
+            }
+            if (a.weight) g.v[j] *= w.v[j];
+            s[0] += g.v[j]; // (zero behind the row's end: g is)
+            s[1] += g.v[j] * x.v[j];
+        }
+        row_sum<THREADS>(s, red, false);
+        const A c0 = s[0] / (A)n, c1 = s[1] / (A)n;
+#pragma unroll
+        for (int j = 0; j < K; ++j) x.v[j] = rstd * (g.v[j] - c0 - x.v[j] * c1);
+        x.store((T*)a.xbar + row * n, n, t);
+    }
+    if (PARAMS) {
+        A* p = (A*)a.partial + (int64_t)blockIdx.x * n;
+        const int64_t other = (int64_t)gridDim.x * n;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+            for (int e = 0; e < Vec16<T>::N; ++e) {
+                const int64_t k = (int64_t)(i * THREADS + t) * Vec16<T>::N + e;
+                if (k < n) {
+                    p[k] = wbar[i * Vec16<T>::N + e];
+                    p[k + other] = bbar[i * Vec16<T>::N + e];
+                }
+            }
+        }
+    }
+}
+
+// wbar, bbar <- the sums over the `parts` rows of partial[2][parts][n]: 64 columns a workgroup, 16 waves share the parts
+template <typename T> __global__ __launch_bounds__(1024) void norm_param_sum(const acc_t<T>* partial, int64_t parts, int64_t n,
+                                                                            T* wbar, T* bbar) {
+    typedef acc_t<T> A;
+    __shared__ A red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t k = (int64_t)blockIdx.x * 64 + lane;
+    const A* p = partial + (int64_t)blockIdx.y * parts * n;
+    A s = 0;
+    if (k < n)
+        for (int64_t i = w; i < parts; i += 16) s += p[i * n + k];
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && k < n) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += red[i][lane];
+        (blockIdx.y ? bbar : wbar)[k] = (T)s;
+    }
+}
+
+// ---- rows cut into pieces ---------------------------------------------------------------------------------------------
+constexpr int LONG_THREADS = 256;
+constexpr int LONG_ITER = 8; // a sweep of a workgroup: 256 threads x 8 vectors = 32 KB, in registers
+template <typename T> constexpr int64_t long_sweep() { return (int64_t)LONG_THREADS * LONG_ITER * Vec16<T>::N; }
+
+// Statistics of piece blockIdx.x of row blockIdx.y: partial[row][piece] = (c, sum (x - c), sum (x - c)^2) with c the mean of
+// the piece's first sweep, as rounded. Sums about a value near the piece's mean keep what a level far from zero would take
+// from them, and they join without the error of a rounded piece's mean: about any other m,
+// sum (x - m)^2 = sum (x - c)^2 + 2 (c - m) sum (x - c) + n (c - m)^2.
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_stats(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int K = LONG_ITER * Vec16<T>::N;
+    __shared__ A red[LONG_THREADS / 64 * 2];
+    const int t = threadIdx.x;
+    const T* x = (const T*)a.x + (int64_t)blockIdx.y * a.width;
+    const int64_t k0 = (int64_t)blockIdx.x * a.piece, k1 = k0 + a.piece < a.width ? k0 + a.piece : a.width;
+    A c = 0, s[2] = {0, 0};
+    for (int64_t k = k0; k < k1; k += long_sweep<T>()) {
+        const int64_t n = k1 - k < long_sweep<T>() ? k1 - k : long_sweep<T>();
+        RowRegs<T, LONG_THREADS, LONG_ITER> r;
+        r.load(x + k, n, t);
+        if (k == k0) {
+            A m[1] = {0};
+#pragma unroll
+            for (int j = 0; j < K; ++j) m[0] += r.v[j];
+            row_sum<LONG_THREADS>(m, red, false);
+            c = m[0] / (A)n;
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const A d = RowRegs<T, LONG_THREADS, LONG_ITER>::inside(j, n, t) ? r.v[j] - c : (A)0;
+            s[0] += d;
+            s[1] += d * d;
+        }
+    }
+    row_sum<LONG_THREADS>(s, red, true);
+    if (t == 0) {
+        A* p = (A*)a.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 3;
+        p[0] = c;
+        p[1] = s[0];
+        p[2] = s[1];
+    }
+}
+
+// The row's statistics from its pieces' (every workgroup for itself, in the same order), then the second sweep.
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int K = LONG_ITER * Vec16<T>::N;
+    __shared__ A red[LONG_THREADS / 64];
+    const int t = threadIdx.x;
+    const A* p = (const A*)a.partial + (int64_t)blockIdx.y * gridDim.x * 3;
+    A s[1] = {0};
+    const A whole = (A)a.piece, tail = (A)(a.width - (int64_t)(gridDim.x - 1) * a.piece); // values of a piece, of the last
+    for (int i = t; i < (int)gridDim.x; i += LONG_THREADS) s[0] += (i + 1 < (int)gridDim.x ? whole : tail) * p[3 * i] + p[3 * i + 1];
+    row_sum<LONG_THREADS>(s, red, false);
+    const A mean = s[0] / (A)a.width;
+    s[0] = 0;
+    for (int i = t; i < (int)gridDim.x; i += LONG_THREADS) {
+        const A d = p[3 * i] - mean;
+        s[0] += p[3 * i + 2] + d * ((A)2 * p[3 * i + 1] + (i + 1 < (int)gridDim.x ? whole : tail) * d);
+    }
+    row_sum<LONG_THREADS>(s, red, true);
+    const A rstd = (A)1 / sqrt(s[0] / (A)a.width + (A)a.eps);
+    if (t == 0 && blockIdx.x == 0) {
+        ((A*)a.mean)[blockIdx.y] = mean;
+        ((A*)a.rstd)[blockIdx.y] = rstd;
+    }
+    const T* x = (const T*)a.x + (int64_t)blockIdx.y * a.width;
+    T* y = (T*)a.y + (int64_t)blockIdx.y * a.width;
+    const int64_t k0 = (int64_t)blockIdx.x * a.piece, k1 = k0 + a.piece < a.width ? k0 + a.piece : a.width;
+    for (int64_t k = k0; k < k1; k += long_sweep<T>()) {
+        const int64_t n = k1 - k < long_sweep<T>() ? k1 - k : long_sweep<T>();
+        RowRegs<T, LONG_THREADS, LONG_ITER> r, w;
+        r.load(x + k, n, t);
+#pragma unroll
+        for (int j = 0; j < K; ++j) r.v[j] = (r.v[j] - mean) * rstd;
+        if (a.weight) {
+            w.load((const T*)a.weight + k, n, t);
+#pragma unroll
+            for (int j = 0; j < K; ++j) r.v[j] *= w.v[j];
+        }
+        if (a.bias) {
+            w.load((const T*)a.bias + k, n, t);
+#pragma unroll
+            for (int j = 0; j < K; ++j) r.v[j] += w.v[j];
+        }
+        r.store(y + k, n, t);
+    }
+}
+
+// Reverse mode, first sweep: columns [blockIdx.x * sweep, + sweep) of the rows of group blockIdx.y: the columns' gradient
+// sums over these rows (partial2[2][groups][n], or the outputs themselves where there is one group) and this piece's part of
+// the rows' two sums, partial[row][piece] = (sum g, sum g h).
+constexpr int LONGB_ITER = 4;
+template <typename T> constexpr int64_t longb_sweep() { return (int64_t)LONG_THREADS * LONGB_ITER * Vec16<T>::N; }
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_sums(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int K = LONGB_ITER * Vec16<T>::N;
+    __shared__ A red[LONG_THREADS / 64 * 2];
+    const int t = threadIdx.x;
+    const int64_t k0 = (int64_t)blockIdx.x * longb_sweep<T>();
+    const int64_t n = a.width - k0 < longb_sweep<T>() ? a.width - k0 : longb_sweep<T>();
+    RowRegs<T, LONG_THREADS, LONGB_ITER> w;
+    if (a.weight) w.load((const T*)a.weight + k0, n, t);
+    A wbar[K], bbar[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) wbar[j] = bbar[j] = 0;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        RowRegs<T, LONG_THREADS, LONGB_ITER> x, g;
+        x.load((const T*)a.x + row * a.width + k0, n, t);
+        g.load((const T*)a.ybar + row * a.width + k0, n, t);
+        const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+        A s[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const A h = (x.v[j] - mean) * rstd;
+            wbar[j] += g.v[j] * h;
+            bbar[j] += g.v[j];
+            const A gw = a.weight ? g.v[j] * w.v[j] : g.v[j];
+            s[0] += gw;
+            s[1] += gw * h;
+        }
+        row_sum<LONG_THREADS>(s, red, false);
+        if (t == 0) {
+            A* p = (A*)a.partial + (row * gridDim.x + blockIdx.x) * 2;
+            p[0] = s[0];
+            p[1] = s[1];
+        }
+    }
+    if (!a.wbar) return;
+    const bool direct = gridDim.y == 1;
+    A* q = (A*)a.partial2 + (int64_t)blockIdx.y * a.width + k0;
+    const int64_t other = (int64_t)gridDim.y * a.width;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const int64_t k = (int64_t)((j / Vec16<T>::N) * LONG_THREADS + t) * Vec16<T>::N + j % Vec16<T>::N;
+        if (k >= n) continue;
+        if (direct) {
+            ((T*)a.wbar)[k0 + k] = (T)wbar[j];
+            ((T*)a.bbar)[k0 + k] = (T)bbar[j];
+        } else {
+            q[k] = wbar[j];
+            q[k + other] = bbar[j];
+        }
+    }
+}
+
+// sums[row] = (<g>, <g h>): one workgroup a row
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_rows(NormArgs a, int64_t pieces) {
+    typedef acc_t<T> A;
+    __shared__ A red[LONG_THREADS / 64 * 2];
+    const A* p = (const A*)a.partial + (int64_t)blockIdx.x * pieces * 2;
+    A s[2] = {0, 0};
+    for (int64_t i = threadIdx.x; i < pieces; i += LONG_THREADS) {
+        s[0] += p[2 * i];
+        s[1] += p[2 * i + 1];
+    }
+    row_sum<LONG_THREADS>(s, red, true);
+    if (threadIdx.x == 0) {
+        ((A*)a.sums)[2 * (int64_t)blockIdx.x] = s[0] / (A)a.width;
+        ((A*)a.sums)[2 * (int64_t)blockIdx.x + 1] = s[1] / (A)a.width;
+    }
+}
+
+// second sweep: xbar
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_apply(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int K = LONGB_ITER * Vec16<T>::N;
+    const int t = threadIdx.x;
+    const int64_t row = blockIdx.y, k0 = (int64_t)blockIdx.x * longb_sweep<T>();
+    const int64_t n = a.width - k0 < longb_sweep<T>() ? a.width - k0 : longb_sweep<T>();
+    const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+    const A c0 = ((const A*)a.sums)[2 * row], c1 = ((const A*)a.sums)[2 * row + 1];
+    RowRegs<T, LONG_THREADS, LONGB_ITER> x, g, w;
+    x.load((const T*)a.x + row * a.width + k0, n, t);
+    g.load((const T*)a.ybar + row * a.width + k0, n, t);
+    if (a.weight) {
+        w.load((const T*)a.weight + k0, n, t);
+#pragma unroll
+        for (int j = 0; j < K; ++j) g.v[j] *= w.v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) x.v[j] = rstd * (g.v[j] - c0 - (x.v[j] - mean) * rstd * c1);
+    x.store((T*)a.xbar + row * a.width + k0, n, t);
+}
+
+// ---- plans ------------------------------------------------------------------------------------------------------------
+constexpr int64_t ROW_BYTES = 65536;   // longest row that one workgroup keeps in registers (1024 threads x 4 vectors)
+constexpr int64_t VJP_ROW_BYTES = 32768; // ... with its cotangent and its gradient sums (1024 threads x 2 vectors)
+constexpr int64_t MAX_GRID_Y = 65535;
+
+struct LongPlan {
+    int64_t piece, pieces;   // forward: elements of a piece (a multiple of the sweep), pieces of a row
+    int64_t vpieces, groups; // reverse: pieces of a row, row groups
+};
+template <typename T> LongPlan long_plan(int64_t rows, int64_t n) {
+    LongPlan p;
+    const int64_t sweeps = (n + long_sweep<T>() - 1) / long_sweep<T>();
+    // at most 1024 pieces a row (the second sweep's workgroups add them up, each for itself)
+    const int64_t per = (sweeps + 1023) / 1024;
+    p.piece = per * long_sweep<T>();
+    p.pieces = (n + p.piece - 1) / p.piece;
+    p.vpieces = (n + longb_sweep<T>() - 1) / longb_sweep<T>();
+    p.groups = 1;
+    while (p.groups < rows && p.groups < 256 && p.vpieces * p.groups < 1024) p.groups *= 2;
+    if (p.groups > rows) p.groups = rows;
+    return p;
+}
+int64_t row_blocks(int64_t rows) { return rows < 512 ? rows : 512; }
+
+template <typename T> size_t workspace(int64_t rows, int64_t n, bool vjp) {
+    const size_t A = sizeof(acc_t<T>);
+    if (n * (int64_t)sizeof(T) <= (vjp ? VJP_ROW_BYTES : ROW_BYTES)) return vjp ? A * 2 * (size_t)(row_blocks(rows) * n) : 0;
+    const LongPlan p = long_plan<T>(rows, n);
+    if (!vjp) return A * 3 * (size_t)(rows * p.pieces);
+    return A * (2 * (size_t)(rows * p.vpieces) + 2 * (size_t)rows + (p.groups > 1 ? 2 * (size_t)(p.groups * n) : 0));
+}
+
+template <typename T, int THREADS, int ITER> void launch_row(const NormArgs& a, hipStream_t st) {
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, RPB = BLOCK / THREADS;
+    norm_row<T, THREADS, ITER><<<dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, st>>>(a);
+}
+template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
+    const int64_t vecs = (a.width + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (a.width * (int64_t)sizeof(T) <= ROW_BYTES) {
+        // a wave a row where that is at most two vectors a lane; then 256 threads, then 1024
+        if (vecs <= 64) launch_row<T, 64, 1>(a, st);
+        else if (vecs <= 128) launch_row<T, 64, 2>(a, st);
+        else if (vecs <= 256) launch_row<T, 256, 1>(a, st);
+        else if (vecs <= 512) launch_row<T, 256, 2>(a, st);
+        else if (vecs <= 1024) launch_row<T, 256, 4>(a, st);
+        else if (vecs <= 2048) launch_row<T, 1024, 2>(a, st);
+        else launch_row<T, 1024, 4>(a, st);
+        return hipGetLastError();
+    }
+    const LongPlan p = long_plan<T>(a.rows, a.width);
+    const size_t es = sizeof(T), as = sizeof(acc_t<T>);
+    a.piece = p.piece;
+    for (int64_t r0 = 0; r0 < a.rows; r0 += MAX_GRID_Y) {
+        NormArgs s = a;
+        s.rows = a.rows - r0 < MAX_GRID_Y ? a.rows - r0 : MAX_GRID_Y;
+        s.x = (const char*)a.x + es * (size_t)(r0 * a.width);
+        s.y = (char*)a.y + es * (size_t)(r0 * a.width);
+        s.mean = (char*)a.mean + as * (size_t)r0;
+        s.rstd = (char*)a.rstd + as * (size_t)r0;
+        s.partial = (char*)a.partial + as * 3 * (size_t)(r0 * p.pieces);
+        const dim3 grid((unsigned)p.pieces, (unsigned)s.rows);
+        norm_long_stats<T><<<grid, dim3(LONG_THREADS), 0, st>>>(s);
+        norm_long_apply<T><<<grid, dim3(LONG_THREADS), 0, st>>>(s);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, int THREADS, int ITER> void launch_row_vjp(const NormArgs& a, unsigned blocks, hipStream_t st) {
+    if (a.wbar) norm_row_vjp<T, THREADS, ITER, true><<<dim3(blocks), dim3(THREADS), 0, st>>>(a);
+    else norm_row_vjp<T, THREADS, ITER, false><<<dim3(blocks), dim3(THREADS), 0, st>>>(a);
+}
+template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
+    typedef acc_t<T> A;
+    const int64_t n = a.width, vecs = (n + Vec16<T>::N - 1) / Vec16<T>::N;
+    int64_t parts = 0;
+    A* parted = (A*)a.partial;
+    if (n * (int64_t)sizeof(T) <= VJP_ROW_BYTES) {
+        parts = row_blocks(a.rows);
+        const unsigned b = (unsigned)parts;
+        if (vecs <= 64) launch_row_vjp<T, 64, 1>(a, b, st);
+        else if (vecs <= 256) launch_row_vjp<T, 256, 1>(a, b, st);
+        else if (vecs <= 512) launch_row_vjp<T, 256, 2>(a, b, st);
+        else if (vecs <= 1024) launch_row_vjp<T, 1024, 1>(a, b, st);
+        else launch_row_vjp<T, 1024, 2>(a, b, st);
+    } else {
+        const LongPlan p = long_plan<T>(a.rows, n);
+        a.sums = (A*)a.partial + 2 * a.rows * p.vpieces;
+        a.partial2 = (A*)a.sums + 2 * a.rows;
+        norm_long_vjp_sums<T><<<dim3((unsigned)p.vpieces, (unsigned)p.groups), dim3(LONG_THREADS), 0, st>>>(a);
+        norm_long_vjp_rows<T><<<dim3((unsigned)a.rows), dim3(LONG_THREADS), 0, st>>>(a, p.vpieces);
+        for (int64_t r0 = 0; r0 < a.rows; r0 += MAX_GRID_Y) {
+            NormArgs s = a;
+            s.rows = a.rows - r0 < MAX_GRID_Y ? a.rows - r0 : MAX_GRID_Y;
+            s.x = (const T*)a.x + r0 * n;
+            s.ybar = (const T*)a.ybar + r0 * n;
+            s.xbar = (T*)a.xbar + r0 * n;
+            s.mean = (A*)a.mean + r0;
+            s.rstd = (A*)a.rstd + r0;
+            s.sums = (A*)a.sums + 2 * r0;
+            norm_long_vjp_apply<T><<<dim3((unsigned)p.vpieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
+        }
+        parts = p.groups > 1 ? p.groups : 0;
+        parted = (A*)a.partial2;
+    }
+    if (a.wbar && parts > 0)
+        norm_param_sum<T><<<dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
+    return hipGetLastError();
+}
+
+} // namespace
+
+size_t gpt_norm_workspace(int dtype, int64_t rows, int64_t width, bool vjp) {
+    switch (dtype) {
+    case GPT_F64: return workspace<double>(rows, width, vjp);
+    case GPT_F32: return workspace<float>(rows, width, vjp);
+    case GPT_F16: return workspace<half_t>(rows, width, vjp);
+    default: return workspace<bf16_t>(rows, width, vjp);
+    }
+}
+hipError_t gpt_launch_norm(int dtype, const NormArgs& a, hipStream_t st) {
+    switch (dtype) {
+    case GPT_F64: return forward<double>(a, st);
+    case GPT_F32: return forward<float>(a, st);
+    case GPT_F16: return forward<half_t>(a, st);
+    default: return forward<bf16_t>(a, st);
+    }
+}
+hipError_t gpt_launch_norm_vjp(int dtype, const NormArgs& a, hipStream_t st) {
+    switch (dtype) {
+    case GPT_F64: return reverse<double>(a, st);
+    case GPT_F32: return reverse<float>(a, st);
+    case GPT_F16: return reverse<half_t>(a, st);
+    default: return reverse<bf16_t>(a, st);
+    }
+}

@@ -1,0 +1,66 @@
+// Element types of the read-out operators (gpt_norm.hip, gpt_class.hip): fp64, fp32, fp16, bf16. Sums, statistics and
+// accumulators are held in Acc (fp32, or fp64 for fp64 data); a value is rounded to the element type once, on its way out.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace gptt {
+
+typedef _Float16 half_t;
+typedef __bf16 bf16_t;
+
+template <typename T> struct Elem {
+    typedef float Acc;
+};
+template <> struct Elem<double> {
+    typedef double Acc;
+};
+template <typename T> using acc_t = typename Elem<T>::Acc;
+
+// 16 bytes of elements at an address that is aligned to the element only (gfx950 reads and writes such vectors in one
+// instruction): rows of odd length keep wide accesses
+template <typename T> struct Vec16 {
+    static constexpr int N = 16 / (int)sizeof(T);
+    typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+    typedef T U __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+template <typename T> __device__ __forceinline__ typename Vec16<T>::V load16(const T* p) {
+    return *reinterpret_cast<const typename Vec16<T>::U*>(p);
+}
+template <typename T> __device__ __forceinline__ void store16(T* p, typename Vec16<T>::V v) {
+    *reinterpret_cast<typename Vec16<T>::U*>(p) = v;
+}
+
+// sum over the 64 lanes of a wave, in every lane
+template <typename A> __device__ __forceinline__ A wave_sum(A v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+
+// K sums over the THREADS consecutive threads that share a row (THREADS is 64, or the whole workgroup), in every one of
+// them. red: THREADS / 64 * K values of LDS; two calls that use the same red need a barrier between them (`last` false
+// leaves one behind).
+template <int THREADS, int K, typename A> __device__ __forceinline__ void row_sum(A (&v)[K], A* red, bool last) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    if (THREADS > 64) {
+        constexpr int NW = THREADS / 64;
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[w * K + k] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            A s = red[k];
+#pragma unroll
+            for (int i = 1; i < NW; ++i) s += red[i * K + k];
+            v[k] = s;
+        }
+        if (!last) __syncthreads();
+    }
+}
+
+} // namespace gptt

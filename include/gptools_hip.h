@@ -54,6 +54,8 @@ enum {
     GPT_ERR_ALLOC = -2
 };
 enum { GPT_ROW_MAJOR = 0, GPT_COL_MAJOR = 1 };
+/* element types of the read-out entry points (everything else is fp64) */
+enum { GPT_F64 = 0, GPT_F32 = 1, GPT_F16 = 2, GPT_BF16 = 3 };
 
 /* ---- context ------------------------------------------------------------------------------------- */
 /* `stream` is a hipStream_t the caller owns (NULL: HIP's default stream). */
@@ -343,6 +345,42 @@ int gpt_gp_periodic_exp_quad_cov_rfft2_vjp_host(gpt_ctx*, int layout, int64_t he
 int gpt_gp_periodic_matern_cov_rfft2_vjp_host(gpt_ctx*, int layout, double nu, int64_t height, int64_t width,
                                               const double* params, const double* covbar, int dim1,
                                               double* params_bar);
+
+/* ---- read-out of several latent fields (no counterpart in the reference) -------------------------------------------
+ * A model with classes as data (species, land-cover types) reads them off several fields at each site: each field is
+ * standardised, and the classes' log odds are linear in the fields. Device pointers, asynchronous on the context's stream.
+ * `dtype` is the element type of the arrays marked T; Acc is float, or double where dtype is GPT_F64: sums and statistics are
+ * held in Acc, and a result is rounded to T once. Arrays need the alignment of their elements only. Nothing is allocated:
+ * `workspace` is the caller's, at least gpt_*_workspace() bytes for the same sizes, 256-byte aligned, not shared with a call
+ * that may run at the same time (a smaller one is GPT_ERR_SHAPE). rows == 0 is allowed (the sums over rows are then zero).
+ *
+ * Layer norm: each of `rows` rows of `width` values T (a site's features; a whole lattice, width = height * width) is
+ * standardised, mean = sum x / n, rstd = 1 / sqrt(sum (x - mean)^2 / n + eps), and y = (x - mean) rstd weight + bias. weight,
+ * bias: [width] T, NULL for 1 and 0. mean, rstd: [rows] Acc. A NaN or an infinity spoils its own row only. */
+size_t gpt_layer_norm_workspace(int dtype, int64_t rows, int64_t width, int vjp);
+int gpt_layer_norm(gpt_ctx*, int dtype, const void* x, const void* weight, const void* bias, int64_t rows, int64_t width,
+                   double eps, void* y, void* mean, void* rstd, void* workspace, size_t workspace_bytes);
+/* Its reverse mode from the forward call's mean and rstd: ybar -> xbar [rows][width] T and the sums over the rows, wbar and
+ * bbar [width] T (both NULL: not wanted). Sums are taken in a fixed order: the same call gives the same bits. */
+int gpt_layer_norm_vjp(gpt_ctx*, int dtype, const void* x, const void* weight, const void* mean, const void* rstd,
+                       const void* ybar, int64_t rows, int64_t width, void* xbar, void* wbar, void* bbar, void* workspace,
+                       size_t workspace_bytes);
+/* Log probability of observed classes, Stan's categorical_logit_glm_lpmf row by row: eta = alpha + beta x,
+ * lp[n] = eta[y[n]] - log sum_v exp eta[v] (Acc). x: `rows` rows of `features` T, ldx elements apart; beta: `classes` rows of
+ * `features` T, ldbeta apart (the memory of Stan's column-major features x classes matrix); alpha: [classes] T or NULL, -inf
+ * excludes a class (a row whose classes are all excluded has lp = -inf and no gradient). y: [rows] classes from 0;
+ * y < 0: not observed -- lp = 0, no gradient, and that row of x may hold anything; y >= classes: lp and the gradients of
+ * that row (so the sums over rows too) are NaN. The rows x classes logits are never stored. */
+size_t gpt_categorical_logit_glm_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, int vjp);
+int gpt_categorical_logit_glm_lpmf(gpt_ctx*, int dtype, const int64_t* y, const void* x, int64_t ldx, const void* alpha,
+                                   const void* beta, int64_t ldbeta, int64_t rows, int64_t features, int64_t classes, void* lp,
+                                   void* workspace, size_t workspace_bytes);
+/* ... and its reverse mode: lpbar [rows] Acc (NULL: ones) -> xbar [rows][features], alphabar [classes] (may be NULL) and
+ * betabar [classes][features], T, dense. Fixed order of sums. */
+int gpt_categorical_logit_glm_lpmf_vjp(gpt_ctx*, int dtype, const int64_t* y, const void* x, int64_t ldx, const void* alpha,
+                                       const void* beta, int64_t ldbeta, const void* lpbar, int64_t rows, int64_t features,
+                                       int64_t classes, void* lp, void* xbar, void* alphabar, void* betabar, void* workspace,
+                                       size_t workspace_bytes);
 
 #ifdef __cplusplus
 }
