@@ -9,10 +9,11 @@
 // contiguously for both operands: r is written in both orders, x and the piece of beta are transposed once.
 //
 // Sums, statistics and accumulators are Acc (fp32; fp64 for fp64 data). One intermediate is rounded to 16 bits where the data
-// have 16 bits: r, because the matrix instructions take both operands in one type. Its error (half a step, 2^-9 of each
-// entry in bf16) is independent from entry to entry, and no larger than that of rounding the result. fp16 has too few exponents
-// for the small probabilities of a large vocabulary: there r is stored times a power of two that brings max |lpbar| to 2^14
-// and taken back from the products' Acc results.
+// have 16 bits: r, because the matrix instructions take both operands in one type. Its error (half a step of each entry) is
+// independent from entry to entry, and no larger than that of rounding the result. The rows' cotangents stay out of that
+// rounding where they can: for xbar they multiply the product's Acc rows, for betabar (whose sum runs over the rows) r
+// holds them divided by the largest of them, so that cotangents that are all alike (a sum's, a mean's) leave [v = y] exact. fp16
+// has too few exponents for the small probabilities of a large vocabulary: there r is stored times 2^14.
 #include "gpt_readout.h"
 #include "gpt_tile.h"
 #include <type_traits>
@@ -22,17 +23,57 @@ using namespace gptt;
 namespace {
 
 template <typename A> __device__ __forceinline__ A neg_inf() { return -(A)__builtin_inf(); }
-__device__ __forceinline__ float exp_(float x) { return expf(x); }
-__device__ __forceinline__ double exp_(double x) { return exp(x); }
 __device__ __forceinline__ float log_(float x) { return logf(x); }
 __device__ __forceinline__ double log_(double x) { return log(x); }
 
-struct Scale { // of the stored r: host value, or (device) [scale, 1 / scale]
-    const float* dev;
-    float host, inverse;
-    __device__ __forceinline__ float times() const { return dev ? dev[0] : host; }
-    __device__ __forceinline__ float back() const { return dev ? dev[1] : inverse; }
+template <typename T> __host__ __device__ constexpr float stored_scale() { return std::is_same<T, half_t>::value ? 16384.f : 1.f; }
+
+constexpr int SCALE_PARTS = 64;
+// largest |lpbar| of the observed rows from class_scale's parts (null: no lpbar, 1), for a whole wave; 1 where it is no scale
+template <typename A> struct Largest {
+    const A* parts;
+    __device__ __forceinline__ A get() const {
+        if (!parts) return 1;
+        A m = parts[threadIdx.x & 63];
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
+        return m > 0 && m < (A)__builtin_inf() ? m : (A)1;
+    }
 };
+
+// sum over the 16 lanes of a row of lanes, in each of them
+__device__ __forceinline__ float sum16(float v) {
+#define GPT_ADD_DPP(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true))
+    GPT_ADD_DPP(0xb1);  // lane ^ 1
+    GPT_ADD_DPP(0x4e);  // lane ^ 2
+    GPT_ADD_DPP(0x141); // the other four of eight
+    GPT_ADD_DPP(0x140); // the other eight
+#undef GPT_ADD_DPP
+    return v;
+}
+__device__ __forceinline__ double sum16(double v) {
+#pragma unroll
+    for (int k = 8; k >= 1; k >>= 1) v += __shfl_xor(v, k, 64);
+    return v;
+}
+
+// The 4 x 4 transpose within every four neighbouring lanes: lane b gives value r in place r, and takes lane k's value b in
+// place k. 16-bit values, two a word.
+__device__ __forceinline__ void transpose4(uint32_t& lo, uint32_t& hi) {
+    const int b = threadIdx.x & 3;
+    const uint32_t give = b & 2 ? lo : hi;
+    const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)give, 0x4e, 0xf, 0xf, true); // lane ^ 2
+    const uint32_t p = b & 2 ? got : lo, q = b & 2 ? hi : got; // values 2 (b / 2), + 1 of lanes b & 1 and (b & 1) + 2
+    const uint32_t po = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p, 0xb1, 0xf, 0xf, true); // lane ^ 1
+    const uint32_t qo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)q, 0xb1, 0xf, 0xf, true);
+    const uint32_t sel = b & 1 ? 0x03020706u : 0x05040100u;
+    lo = __builtin_amdgcn_perm(po, p, sel);
+    hi = __builtin_amdgcn_perm(qo, q, sel);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T V2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, V2{(T)a, (T)b});
+}
 
 template <typename T> struct LogitArgs {
     Operand<T> beta, x; // beta: the classes from v0 on
@@ -42,42 +83,50 @@ template <typename T> struct LogitArgs {
     int64_t tiles_v, tiles_n;
     // statistics
     acc_t<T>*part_max, *part_sum, *eta_y; // [tiles_v][rows], [tiles_v][rows], [rows]
-    // r
+    // r, and r with the rows' cotangents in the other order: [rows][ldr] and [classes of the piece][ldrt], in whole tiles
     const acc_t<T>*lse, *lpbar;
-    T *r, *rt; // [rows][ldr] and [classes of the piece][ldrt], zero up to ldr and ldrt
+    T *r, *rt;
     int64_t ldr, ldrt;
     acc_t<T>* part_alpha; // [tiles_n][ldr] or null
-    Scale scale;
+    Largest<acc_t<T>> largest;
 };
 
-constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
+// In fp32 logits, maxima and lse are kept times log2(e): an exponential is one instruction then
+__device__ __forceinline__ float times_log2e(float v) { return v * 1.44269504088896340736f; }
+__device__ __forceinline__ float exp_log2e(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float from_log2e(float v) { return v * 0.69314718055994530942f; }
+__device__ __forceinline__ double times_log2e(double v) { return v; }
+__device__ __forceinline__ double from_log2e(double v) { return v; }
+__device__ __forceinline__ double exp_log2e(double v) { return exp(v); }
 
 // Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r.
-template <typename T, bool STATS> __global__ __launch_bounds__(64 * WM * WN) void class_logits(LogitArgs<T> a) {
+template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::THREADS) void class_logits(LogitArgs<T> a) {
     typedef acc_t<T> A;
-    typedef Tile<T, BM, BN, WM, WN> Tl;
     __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
-    __shared__ A red[2][WM > WN ? WM : WN][BM > BN ? BM : BN];
-    const int64_t m0 = (int64_t)(blockIdx.x / a.tiles_n) * BM, n0 = (int64_t)(blockIdx.x % a.tiles_n) * BN;
+    __shared__ A red[2][Tl::WM > Tl::WN ? Tl::WM : Tl::WN][Tl::BM > Tl::BN ? Tl::BM : Tl::BN];
+    int64_t tm, tn;
+    if (!tile_place(blockIdx.x, a.tiles_v, a.tiles_n, tm, tn)) return;
+    const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
     Tl tl;
     tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
-    const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / WN, wn = (threadIdx.x >> 6) % WN;
-    const int64_t nv = a.beta.rows; // classes of this launch
+    const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Tl::WN, wn = (threadIdx.x >> 6) % Tl::WN;
+    const int nv = (int)(a.beta.rows - m0 < Tl::BM ? a.beta.rows - m0 : Tl::BM); // classes of this tile
 #pragma unroll
     for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int64_t m = m0 + Tl::row(i, r);
-            const A al = m < nv ? (a.alpha ? (A)a.alpha[m] : (A)0) : neg_inf<A>();
+            const int m = Tl::row(i, r);
+            const A al = times_log2e(m < nv ? (a.alpha ? (A)a.alpha[m0 + m] : (A)0) : neg_inf<A>());
 #pragma unroll
-            for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] += al;
+            for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + al;
         }
     if (STATS) {
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j) {
             const int64_t n = n0 + Tl::col(j);
-            const int64_t y = n < a.x.rows ? a.y[n] : -1;
-            A mx = neg_inf<A>();
+            const int64_t y = n < a.x.rows ? a.y[n] - m0 : -1;
+            const int at = y >= 0 && y < Tl::BM ? (int)y : -1;
+            A mx = neg_inf<A>(), here = 0;
             bool nan = false;
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
@@ -85,20 +134,27 @@ template <typename T, bool STATS> __global__ __launch_bounds__(64 * WM * WN) voi
                 for (int r = 0; r < 4; ++r) {
                     mx = fmax(mx, tl.acc[i][j][r]);
                     nan |= tl.acc[i][j][r] != tl.acc[i][j][r];
-                    if (m0 + Tl::row(i, r) == y) a.eta_y[n] = tl.acc[i][j][r];
+                    here = Tl::row(i, r) == at ? tl.acc[i][j][r] : here;
                 }
+            // (one lane group of one wave holds the row's class)
+            bool mine = false;
+#pragma unroll
+            for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mine |= Tl::row(i, r) == at;
+            if (mine && at < nv) a.eta_y[n] = here;
             A s = 0;
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += mx == neg_inf<A>() ? (A)0 : exp_(tl.acc[i][j][r] - mx);
+                for (int r = 0; r < 4; ++r) s += mx == neg_inf<A>() ? (A)0 : exp_log2e(tl.acc[i][j][r] - mx);
             if (nan) s = mx = (A)__builtin_nan("");
             // the four lane groups hold other classes of the same rows
 #pragma unroll
             for (int k = 16; k <= 32; k <<= 1) {
                 const A mo = __shfl_xor(mx, k, 64), so = __shfl_xor(s, k, 64);
                 const A mm = (mx != mx || mo != mo) ? (A)__builtin_nan("") : fmax(mx, mo);
-                s = mm == neg_inf<A>() ? (A)0 : s * exp_(mx - mm) + so * exp_(mo - mm);
+                s = mm == neg_inf<A>() ? (A)0 : s * exp_log2e(mx - mm) + so * exp_log2e(mo - mm);
                 mx = mm;
             }
             if (lane < 16) {
@@ -107,66 +163,109 @@ template <typename T, bool STATS> __global__ __launch_bounds__(64 * WM * WN) voi
             }
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < BN; c += Tl::THREADS) {
+        for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
             A mx = red[0][0][c], s = red[1][0][c];
 #pragma unroll
-            for (int w = 1; w < WM; ++w) {
+            for (int w = 1; w < Tl::WM; ++w) {
                 const A mo = red[0][w][c], so = red[1][w][c];
                 const A mm = (mx != mx || mo != mo) ? (A)__builtin_nan("") : fmax(mx, mo);
-                s = mm == neg_inf<A>() ? (A)0 : s * exp_(mx - mm) + so * exp_(mo - mm);
+                s = mm == neg_inf<A>() ? (A)0 : s * exp_log2e(mx - mm) + so * exp_log2e(mo - mm);
                 mx = mm;
             }
             if (n0 + c < a.x.rows) {
-                a.part_max[(m0 / BM) * a.x.rows + n0 + c] = mx;
-                a.part_sum[(m0 / BM) * a.x.rows + n0 + c] = s;
+                a.part_max[tm * a.x.rows + n0 + c] = mx;
+                a.part_sum[tm * a.x.rows + n0 + c] = s;
             }
         }
         return;
     }
     A lse[Tl::TN], w[Tl::TN];
-    int64_t at[Tl::TN];
-    const A up = (A)a.scale.times();
+    bool none[Tl::TN];
+    int at[Tl::TN];
+    const A largest = a.largest.get();
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
         const int64_t n = n0 + Tl::col(j), y = n < a.x.rows ? a.y[n] : -1;
-        lse[j] = y >= 0 ? a.lse[n] : neg_inf<A>();
-        w[j] = y < 0 ? (A)0 : y >= a.classes ? (A)__builtin_nan("") : a.lpbar ? a.lpbar[n] * up : up;
-        at[j] = y - a.v0;
+        lse[j] = y < 0 ? (A)0 : y >= a.classes ? (A)__builtin_nan("") : a.lse[n];
+        none[j] = y < 0 || lse[j] == neg_inf<A>(); // no observation, or no possible class
+        w[j] = none[j] ? (A)0 : a.lpbar ? a.lpbar[n] / largest : (A)1;
+        const int64_t from = y - a.v0 - m0;
+        at[j] = y >= 0 && from >= 0 && from < Tl::BM ? (int)from : -1;
     }
+    constexpr A up = stored_scale<T>();
+    A total[Tl::TM][4];
 #pragma unroll
     for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int64_t m = m0 + Tl::row(i, r);
-            A total = 0;
+            total[i][r] = 0;
 #pragma unroll
             for (int j = 0; j < Tl::TN; ++j) {
-                const int64_t n = n0 + Tl::col(j);
-                // a row without an observation, a class behind the last, a row without any possible class: nothing
-                const bool none = (lse[j] == neg_inf<A>() && w[j] == w[j]) || m >= nv;
-                const A p = exp_(tl.acc[i][j][r] - lse[j]);
-                const A v = none ? (A)0 : w[j] * ((m == at[j] ? (A)1 : (A)0) - p);
-                total += v;
-                if (m < a.ldr && n < a.x.rows) a.r[n * a.ldr + m] = (T)v;
-                if (m < nv && n < a.ldrt) a.rt[m * a.ldrt + n] = (T)v;
-            }
-            if (a.part_alpha) {
-#pragma unroll
-                for (int k = 8; k >= 1; k >>= 1) total += __shfl_xor(total, k, 64);
-                if ((lane & 15) == 0) red[0][wn][Tl::row(i, r)] = total;
+                const A p = exp_log2e(tl.acc[i][j][r] - lse[j]);
+                const A v = none[j] ? (A)0 : (Tl::row(i, r) == at[j] ? up : (A)0) - up * p;
+                tl.acc[i][j][r] = v;
+                total[i][r] += v * w[j];
             }
         }
+    if constexpr (Tl::TM == 8 && sizeof(T) == 2) {
+        // r: 16 neighbouring classes of one row a lane; rt: after the transpose, 16 neighbouring rows of one class a lane
+        const int64_t mq = m0 + Tl::row(0, 0), nq = n0 + Tl::col(0);
+#pragma unroll
+        for (int j = 0; j < Tl::TN; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4* to = reinterpret_cast<uint4*>(a.r + (nq + Tl::fragment(j)) * a.ldr + mq + 64 * h);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const auto &c = tl.acc[4 * h + 2 * k][j], &d = tl.acc[4 * h + 2 * k + 1][j];
+                    to[k] = make_uint4(pack2<T>(c[0], c[1]), pack2<T>(c[2], c[3]), pack2<T>(d[0], d[1]), pack2<T>(d[2], d[3]));
+                }
+            }
+        const int64_t nb = nq - (lane & 3), mb = mq + (lane & 3);
+#pragma unroll
+        for (int i = 0; i < Tl::TM; ++i) {
+            uint32_t u[Tl::TN][2];
+#pragma unroll
+            for (int j = 0; j < Tl::TN; ++j) {
+                const auto& c = tl.acc[i][j];
+                u[j][0] = pack2<T>(c[0] * w[j], c[1] * w[j]);
+                u[j][1] = pack2<T>(c[2] * w[j], c[3] * w[j]);
+                transpose4(u[j][0], u[j][1]);
+            }
+            uint4* to = reinterpret_cast<uint4*>(a.rt + (mb + Tl::fragment(i)) * a.ldrt + nb);
+            to[0] = make_uint4(u[0][0], u[0][1], u[1][0], u[1][1]);
+            to[1] = make_uint4(u[2][0], u[2][1], u[3][0], u[3][1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < Tl::TN; ++j) {
+                    const int64_t m = m0 + Tl::row(i, r), n = n0 + Tl::col(j);
+                    a.r[n * a.ldr + m] = (T)tl.acc[i][j][r];
+                    a.rt[m * a.ldrt + n] = (T)(tl.acc[i][j][r] * w[j]);
+                }
+    }
     if (!a.part_alpha) return;
+#pragma unroll
+    for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const A s = sum16(total[i][r]);
+            if ((lane & 15) == 0) red[0][wn][Tl::row(i, r)] = s;
+        }
     __syncthreads();
-    for (int c = threadIdx.x; c < BM; c += Tl::THREADS) {
+    for (int c = threadIdx.x; c < nv; c += Tl::THREADS) {
         A s = red[0][0][c];
 #pragma unroll
-        for (int k = 1; k < WN; ++k) s += red[0][k][c];
-        if (m0 + c < nv) a.part_alpha[(n0 / BN) * a.ldr + m0 + c] = s * (A)a.scale.back();
+        for (int k = 1; k < Tl::WN; ++k) s += red[0][k][c];
+        a.part_alpha[tn * a.ldr + m0 + c] = s * (largest / up);
     }
 }
 
-// lse and lp of 16 rows from their tiles' statistics, 16 slices of the tiles in parallel
+// lse (times log2(e) in fp32) and lp of 16 rows from their tiles' statistics, 16 slices of the tiles in parallel
 template <typename T> __global__ __launch_bounds__(256) void class_join(const acc_t<T>* part_max, const acc_t<T>* part_sum,
                                                                        const acc_t<T>* eta_y, const int64_t* y, int64_t tiles,
                                                                        int64_t rows, int64_t classes, acc_t<T>* lse, acc_t<T>* lp) {
@@ -181,7 +280,7 @@ template <typename T> __global__ __launch_bounds__(256) void class_join(const ac
             const A mo = part_max[i * rows + n], so = part_sum[i * rows + n];
             nan |= mo != mo;
             const A mm = fmax(mx, mo);
-            if (mm != neg_inf<A>()) s = s * exp_(mx - mm) + so * exp_(mo - mm);
+            if (mm != neg_inf<A>()) s = s * exp_log2e(mx - mm) + so * exp_log2e(mo - mm);
             mx = mm;
         }
     red[0][k][c] = nan ? (A)__builtin_nan("") : mx;
@@ -195,11 +294,10 @@ template <typename T> __global__ __launch_bounds__(256) void class_join(const ac
     }
     A sum = 0;
     for (int i = 0; i < 16; ++i)
-        if (red[0][i][c] != neg_inf<A>()) sum += red[1][i][c] * exp_(red[0][i][c] - top);
-    const A l = nan ? (A)__builtin_nan("") : top == neg_inf<A>() ? top : top + log_(sum);
-    if (lse) lse[n] = l;
+        if (red[0][i][c] != neg_inf<A>()) sum += red[1][i][c] * exp_log2e(red[0][i][c] - top);
     const int64_t yn = y[n];
-    lp[n] = yn < 0 ? (A)0 : yn >= classes ? (A)__builtin_nan("") : l == neg_inf<A>() ? l : eta_y[n] - l;
+    lp[n] = yn < 0 ? (A)0 : yn >= classes || nan ? (A)__builtin_nan("") : top == neg_inf<A>() ? top : from_log2e(eta_y[n] - top) - log_(sum);
+    if (lse) lse[n] = nan ? (A)__builtin_nan("") : top == neg_inf<A>() ? top : top + times_log2e(log_(sum));
 }
 
 // out[c][r] = in[r][c], rows behind the last, and (y given) those without an observation, zero. 64 x 64 through LDS
@@ -219,45 +317,113 @@ template <typename T> __global__ __launch_bounds__(256) void class_transpose(con
     }
 }
 
+// out[r][0..ldo) = in[r][0..cols), zeros behind: rows that start on 16 bytes and end with a step of k
+template <typename T> __global__ __launch_bounds__(256) void class_align(const T* in, int64_t ld, int64_t rows, int64_t cols, T* out,
+                                                                        int64_t ldo) {
+    constexpr int N = Vec16<T>::N;
+    const int64_t per = ldo / N, count = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per, k = (i - r * per) * N;
+        *reinterpret_cast<typename Vec16<T>::V*>(out + r * ldo + k) = tile_chunk<T>({in, ld, rows}, r, k, cols);
+    }
+}
+
 // The products with r: out[n][m] = sum_k A[m][k] B[n][k] over this launch's share of k.
 template <typename T> struct ProductArgs {
     Operand<T> A, B;
     int64_t K, share; // k of one split (a multiple of the tile's step)
-    int64_t tiles_n;
+    int64_t tiles_m, tiles_n;
     acc_t<T>* acc; // [splits][B.rows][A.rows]: sums so far
     int64_t plane; // elements from one split's sums to the next
     T* out;        // the result, where this launch completes it; else null
     int64_t ldo;
-    bool add;        // acc holds earlier launches' sums
-    const int64_t* y; // of B's rows, where those without an observation give zero; or null
-    Scale scale;
+    bool add; // acc holds earlier launches' sums
+    // xbar: B's rows are the rows of x, each times its cotangent (zero without an observation). betabar: y null
+    const int64_t* y;
+    const acc_t<T>* lpbar;
+    Largest<acc_t<T>> largest;
 };
-template <typename T> __global__ __launch_bounds__(64 * WM * WN) void class_product(ProductArgs<T> a) {
+template <typename T, typename Tl> __global__ __launch_bounds__(Tl::THREADS) void class_product(ProductArgs<T> a) {
     typedef acc_t<T> A;
-    typedef Tile<T, BM, BN, WM, WN> Tl;
     __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
-    const int64_t m0 = (int64_t)(blockIdx.x / a.tiles_n) * BM, n0 = (int64_t)(blockIdx.x % a.tiles_n) * BN;
+    int64_t tm, tn;
+    if (!tile_place(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn)) return;
+    const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
     const int64_t k0 = (int64_t)blockIdx.y * a.share, k1 = k0 + a.share < a.K ? k0 + a.share : a.K;
     Tl tl;
     tl.run(a.A, m0, a.B, n0, k0, k1, lds);
-    const A back = (A)a.scale.back();
     A* acc = a.acc + (int64_t)blockIdx.y * a.plane;
+    const A largest = a.y ? (A)1 : a.largest.get();
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
         const int64_t n = n0 + Tl::col(j);
         if (n >= a.B.rows) continue;
-        const bool none = a.y && a.y[n] < 0;
+        A back = largest;
+        bool none = false;
+        if (a.y) {
+            none = a.y[n] < 0;
+            if (a.lpbar && !none) back = a.lpbar[n];
+        }
+        back /= (A)stored_scale<T>();
+        if constexpr (Tl::TM == 8) {
+            // 16 neighbouring values a lane: whole vectors where the rows of the result allow them
 #pragma unroll
-        for (int i = 0; i < Tl::TM; ++i)
+            for (int h = 0; h < 2; ++h) {
+                const int64_t m = m0 + Tl::row(4 * h, 0);
+                A v[16];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t m = m0 + Tl::row(i, r);
-                if (m >= a.A.rows) continue;
-                A v = none ? (A)0 : tl.acc[i][j][r] * back;
-                if (a.add) v += acc[n * a.A.rows + m];
-                if (a.out) a.out[n * a.ldo + m] = (T)v;
-                else acc[n * a.A.rows + m] = v;
+                for (int k = 0; k < 16; ++k) v[k] = none ? (A)0 : tl.acc[4 * h + k / 4][j][k % 4] * back;
+                A* s = acc + n * a.A.rows + m;
+                T* o = a.out + n * a.ldo + m;
+                if (m + 16 <= a.A.rows) {
+                    if (a.add) {
+#pragma unroll
+                        for (int k = 0; k < 16; k += Vec16<A>::N) {
+                            const auto u = load16(s + k);
+#pragma unroll
+                            for (int e = 0; e < Vec16<A>::N; ++e) v[k + e] += u[e];
+                        }
+                    }
+                    if (a.out) {
+#pragma unroll
+                        for (int k = 0; k < 16; k += Vec16<T>::N) {
+                            typename Vec16<T>::V u;
+#pragma unroll
+                            for (int e = 0; e < Vec16<T>::N; ++e) u[e] = (T)v[k + e];
+                            store16(o + k, u);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; k += Vec16<A>::N) {
+                            typename Vec16<A>::V u;
+#pragma unroll
+                            for (int e = 0; e < Vec16<A>::N; ++e) u[e] = v[k + e];
+                            store16(s + k, u);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        if (m + k >= a.A.rows) continue;
+                        if (a.add) v[k] += s[k];
+                        if (a.out) o[k] = (T)v[k];
+                        else s[k] = v[k];
+                    }
+                }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t m = m0 + Tl::row(i, r);
+                    if (m >= a.A.rows) continue;
+                    A v = none ? (A)0 : tl.acc[i][j][r] * back;
+                    if (a.add) v += acc[n * a.A.rows + m];
+                    if (a.out) a.out[n * a.ldo + m] = (T)v;
+                    else acc[n * a.A.rows + m] = v;
+                }
+        }
     }
 }
 // out[i] <- sum over the splits
@@ -287,32 +453,28 @@ template <typename T> __global__ __launch_bounds__(256) void class_alpha(const a
     if (out) out[v] = (T)s;
     else acc[v] = s;
 }
-// fp16: scale = the power of two that brings max |lpbar| to [2^13, 2^14], and its inverse
-__global__ __launch_bounds__(1024) void class_scale(const float* lpbar, const int64_t* y, int64_t rows, float* scale) {
-    __shared__ float red[16];
-    float m = 0.f;
-    for (int64_t i = threadIdx.x; i < rows; i += 1024)
-        if (y[i] >= 0) m = fmaxf(m, fabsf(lpbar[i]));
+// parts[b] = the largest |lpbar| of the observed rows that workgroup b of SCALE_PARTS takes
+template <typename A> __global__ __launch_bounds__(256) void class_scale(const A* lpbar, const int64_t* y, int64_t rows, A* parts) {
+    __shared__ A red[4];
+    A m = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += 256 * SCALE_PARTS)
+        if (y[i] >= 0) m = fmax(m, fabs(lpbar[i]));
 #pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+    for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
-    int e = 0;
-    if (m > 0.f && m < __builtin_inff()) (void)frexpf(m, &e); // m < 2^e
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
-    scale[0] = ldexpf(1.f, 14 - e);
-    scale[1] = ldexpf(1.f, e - 14);
+    if (threadIdx.x == 0) parts[blockIdx.x] = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
 }
 
 // ---- plan -------------------------------------------------------------------------------------------------------------
 int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
 
-constexpr int64_t ROW_BLOCK = 1 << 18;             // rows taken at a time
+constexpr int64_t ROW_BLOCK = 1 << 18;              // rows taken at a time
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20; // r in both orders, of a piece of the classes and a block of the rows
 constexpr int64_t FILL = 512;                       // workgroups that fill the card
+constexpr int64_t EDGE = 256;                       // the largest tile's edge
+constexpr int64_t WIDE_TILES = 96;                  // wide tiles from this many on
 
 // Splits of a product's k: enough workgroups to fill the card, at least 4 steps of k each
 int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
@@ -321,18 +483,22 @@ int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
     if (s > most) s = most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
 }
+// 256 x 256 tiles for a product of m x n results?
+template <typename T> bool wide(int64_t m, int64_t n) {
+    return sizeof(T) == 2 && tiles_of(m, WideTile<T>::BM) * tiles_of(n, WideTile<T>::BN) >= WIDE_TILES;
+}
 
 template <typename T> struct Plan {
-    int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt;
+    int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
     int64_t xsplits, bsplits;
     // offsets in bytes
-    size_t part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, bytes;
+    size_t part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
     Plan(int64_t rows, int64_t features, int64_t classes, bool vjp) {
         const size_t A = sizeof(acc_t<T>), E = sizeof(T);
         block = rows < ROW_BLOCK ? rows : ROW_BLOCK;
         blocks = tiles_of(rows, block);
-        tiles_v = tiles_of(classes, BM);
-        tiles_n = tiles_of(block, BN);
+        tiles_v = tiles_of(classes, SmallTile<T>::BM);
+        tiles_n = tiles_of(block, SmallTile<T>::BN);
         size_t at = 0;
         auto take = [&](size_t n) {
             const size_t p = at;
@@ -342,52 +508,85 @@ template <typename T> struct Plan {
         part_max = take(A * (size_t)(tiles_v * block));
         part_sum = take(A * (size_t)(tiles_v * block));
         eta_y = take(A * (size_t)block);
+        ldk = 0;
+        if (wide<T>(classes, block) && features * E % 16) { // copies whose rows start on 16 bytes
+            ldk = up_to(features, tile_k<T>());
+            xa = take(E * (size_t)(block * ldk));
+            ba = take(E * (size_t)(classes * ldk));
+        }
         if (vjp) {
-            piece = PIECE_BYTES / (int64_t)(2 * E) / up_to(block, BN) / BM * BM;
-            if (piece < BM) piece = BM;
-            if (piece > up_to(classes, BM)) piece = up_to(classes, BM);
+            piece = PIECE_BYTES / (int64_t)(2 * E) / up_to(block, EDGE) / EDGE * EDGE;
+            if (piece < EDGE) piece = EDGE;
+            if (piece > up_to(classes, EDGE)) piece = up_to(classes, EDGE);
             pieces = tiles_of(classes, piece);
-            piece = up_to(tiles_of(classes, pieces), BM); // of about the same size
+            piece = up_to(tiles_of(classes, pieces), EDGE); // of about the same size
             pieces = tiles_of(classes, piece);
             ldr = piece;
-            ldrt = up_to(block, BN);
+            ldrt = up_to(block, EDGE);
             lse = take(A * (size_t)block);
-            scale = take(8);
-            r = take(E * (size_t)(block * ldr));
-            rt = take(E * (size_t)(piece * ldrt));
+            scale = take(A * SCALE_PARTS);
+            r = take(E * (size_t)(ldrt * ldr));
+            rt = take(E * (size_t)(ldr * ldrt));
             xt = take(E * (size_t)(features * ldrt));
             bt = take(E * (size_t)(features * ldr));
             part_alpha = take(A * (size_t)(tiles_n * ldr));
             alpha_acc = blocks > 1 ? take(A * (size_t)classes) : 0;
-            xsplits = splits_of(tiles_of(features, BM) * tiles_n, piece, tile_k<T>());
-            bsplits = splits_of(tiles_of(features, BM) * tiles_of(piece, BN), block, tile_k<T>());
+            xsplits = product_splits(features, block, piece);
+            bsplits = product_splits(features, piece, block);
             xacc = xsplits > 1 || pieces > 1 ? take(A * (size_t)(xsplits * block * features)) : 0;
             bacc = blocks > 1 ? take(A * (size_t)(bsplits * classes * features))
                               : bsplits > 1 ? take(A * (size_t)(bsplits * piece * features)) : 0;
         }
         bytes = at;
     }
+    static int64_t product_splits(int64_t m, int64_t n, int64_t K) {
+        const int64_t edge = wide<T>(m, n) ? WideTile<T>::BM : SmallTile<T>::BM;
+        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * (wide<T>(m, n) ? 2 : 1), K, tile_k<T>());
+    }
 };
 
-template <typename T> hipError_t product(const Operand<T>& A, const Operand<T>& B, int64_t K, int64_t splits, acc_t<T>* acc,
-                                         int64_t plane, bool add, bool last, T* out, const int64_t* y, Scale scale, hipStream_t st) {
-    ProductArgs<T> p;
-    p.A = A;
-    p.B = B;
-    p.K = K;
-    p.share = up_to(tiles_of(K, splits), tile_k<T>());
-    p.tiles_n = tiles_of(B.rows, BN);
-    p.acc = acc;
-    p.plane = plane;
+template <typename T, typename Tl> void logits(LogitArgs<T> l, bool stats, hipStream_t st) {
+    l.tiles_v = tiles_of(l.beta.rows, Tl::BM);
+    l.tiles_n = tiles_of(l.x.rows, Tl::BN);
+    const dim3 grid(tile_grid(l.tiles_v, l.tiles_n));
+    if (stats) class_logits<T, Tl, true><<<grid, dim3(Tl::THREADS), 0, st>>>(l);
+    else class_logits<T, Tl, false><<<grid, dim3(Tl::THREADS), 0, st>>>(l);
+}
+// -> edge of the tiles taken
+template <typename T> int64_t logits_any(const LogitArgs<T>& l, bool use_wide, bool stats, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (use_wide) {
+            logits<T, WideTile<T>>(l, stats, st);
+            return WideTile<T>::BM;
+        }
+    }
+    logits<T, SmallTile<T>>(l, stats, st);
+    return SmallTile<T>::BM;
+}
+
+template <typename T> hipError_t product(ProductArgs<T> p, int64_t splits, bool last, T* out, hipStream_t st) {
+    p.share = up_to(tiles_of(p.K, splits), tile_k<T>());
     p.out = last && splits == 1 ? out : nullptr;
-    p.ldo = A.rows;
-    p.add = add;
-    p.y = y;
-    p.scale = scale;
-    class_product<T><<<dim3((unsigned)(tiles_of(A.rows, BM) * p.tiles_n), (unsigned)splits), dim3(64 * WM * WN), 0, st>>>(p);
+    p.ldo = p.A.rows;
+    bool done = false;
+    if constexpr (sizeof(T) == 2) {
+        typedef WideTile<T> Tl;
+        if (wide<T>(p.A.rows, p.B.rows)) {
+            p.tiles_m = tiles_of(p.A.rows, Tl::BM);
+            p.tiles_n = tiles_of(p.B.rows, Tl::BN);
+            class_product<T, Tl><<<dim3(tile_grid(p.tiles_m, p.tiles_n), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
+            done = true;
+        }
+    }
+    if (!done) {
+        typedef SmallTile<T> Tl;
+        p.tiles_m = tiles_of(p.A.rows, Tl::BM);
+        p.tiles_n = tiles_of(p.B.rows, Tl::BN);
+        class_product<T, Tl><<<dim3(tile_grid(p.tiles_m, p.tiles_n), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
+    }
     if (last && splits > 1) {
-        const int64_t count = A.rows * B.rows;
-        class_join_splits<T><<<dim3((unsigned)tiles_of(count, 256)), dim3(256), 0, st>>>(acc, (int)splits, plane, count, out);
+        const int64_t count = p.A.rows * p.B.rows;
+        class_join_splits<T><<<dim3((unsigned)tiles_of(count, 256)), dim3(256), 0, st>>>(p.acc, (int)splits, p.plane, count, out);
     }
     return hipGetLastError();
 }
@@ -398,43 +597,51 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     char* ws = (char*)c.ws;
     const int64_t D = c.features, V = c.classes;
     hipError_t e;
-    Scale scale = {nullptr, 1.f, 1.f};
-    if (vjp && std::is_same<T, half_t>::value) {
-        if (c.lpbar) {
-            scale.dev = (const float*)(ws + p.scale);
-            class_scale<<<1, 1024, 0, st>>>((const float*)c.lpbar, c.y, c.rows, (float*)(ws + p.scale));
-        } else {
-            scale.host = 16384.f;
-            scale.inverse = 1.f / 16384.f;
-        }
+    Operand<T> beta = {(const T*)c.beta, c.ldbeta, V};
+    int64_t K = D;
+    if (p.ldk) {
+        T* to = (T*)(ws + p.ba);
+        class_align<T><<<dim3(2048), dim3(256), 0, st>>>(beta.p, beta.ld, V, D, to, p.ldk);
+        beta = {to, p.ldk, V};
+        K = p.ldk;
+    }
+    Largest<A> largest = {nullptr};
+    if (vjp && c.lpbar) {
+        largest.parts = (A*)(ws + p.scale);
+        class_scale<A><<<dim3(SCALE_PARTS), dim3(256), 0, st>>>((const A*)c.lpbar, c.y, c.rows, (A*)(ws + p.scale));
     }
     for (int64_t n0 = 0; n0 < c.rows; n0 += p.block) {
         const int64_t N = c.rows - n0 < p.block ? c.rows - n0 : p.block;
         const bool first_block = n0 == 0, last_block = n0 + N == c.rows;
-        LogitArgs<T> l;
-        l.beta = {(const T*)c.beta, c.ldbeta, V};
-        l.x = {(const T*)c.x + n0 * c.ldx, c.ldx, N};
+        const T* x = (const T*)c.x + n0 * c.ldx;
+        LogitArgs<T> l = {};
+        l.beta = beta;
+        l.x = {x, c.ldx, N};
+        if (p.ldk) {
+            T* to = (T*)(ws + p.xa);
+            class_align<T><<<dim3(1024), dim3(256), 0, st>>>(x, c.ldx, N, D, to, p.ldk);
+            l.x = {to, p.ldk, N};
+        }
+        bool use_wide = false;
+        if constexpr (sizeof(T) == 2) use_wide = wide<T>(V, N) && WideTile<T>::fits(l.beta) && WideTile<T>::fits(l.x);
         l.alpha = (const T*)c.alpha;
-        l.features = D;
-        l.v0 = 0;
+        l.features = K;
         l.classes = V;
         l.y = c.y + n0;
-        l.tiles_v = p.tiles_v;
-        l.tiles_n = tiles_of(N, BN);
         l.part_max = (A*)(ws + p.part_max);
         l.part_sum = (A*)(ws + p.part_sum);
         l.eta_y = (A*)(ws + p.eta_y);
-        l.scale = scale;
-        class_logits<T, true><<<dim3((unsigned)(l.tiles_v * l.tiles_n)), dim3(64 * WM * WN), 0, st>>>(l);
+        l.largest = largest;
+        const int64_t edge = logits_any<T>(l, use_wide, true, st);
         A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
-        class_join<T><<<dim3((unsigned)tiles_of(N, 16)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, p.tiles_v, N, V,
-                                                                             lse, (A*)c.lp + n0);
+        class_join<T><<<dim3((unsigned)tiles_of(N, 16)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, tiles_of(V, edge), N,
+                                                                             V, lse, (A*)c.lp + n0);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if (!vjp) continue;
-        const int64_t ldrt = up_to(N, BN);
+        const int64_t ldrt = up_to(N, edge); // (r is written in whole tiles)
         T *r = (T*)(ws + p.r), *rt = (T*)(ws + p.rt), *xt = (T*)(ws + p.xt), *bt = (T*)(ws + p.bt);
-        class_transpose<T><<<dim3((unsigned)tiles_of(ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(
-            l.x.p, c.ldx, N, D, l.y, xt, ldrt);
+        class_transpose<T><<<dim3((unsigned)tiles_of(ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(x, c.ldx, N, D, l.y, xt,
+                                                                                                              ldrt);
         l.lse = lse;
         l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
         l.r = r;
@@ -444,26 +651,36 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
         for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
             const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
             const bool first = v0 == 0, last = v0 + nv == V;
-            l.beta = {(const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv};
+            l.beta = {beta.p + v0 * beta.ld, beta.ld, nv};
             l.alpha = c.alpha ? (const T*)c.alpha + v0 : nullptr;
             l.v0 = v0;
-            l.tiles_v = tiles_of(nv, BM);
-            l.ldr = up_to(nv, BM);
-            class_logits<T, false><<<dim3((unsigned)(l.tiles_v * l.tiles_n)), dim3(64 * WM * WN), 0, st>>>(l);
+            l.ldr = up_to(nv, edge);
+            logits_any<T>(l, use_wide, false, st);
             class_transpose<T><<<dim3((unsigned)tiles_of(l.ldr, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(
-                l.beta.p, c.ldbeta, nv, D, nullptr, bt, l.ldr);
+                (const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv, D, nullptr, bt, l.ldr);
             if (c.alphabar)
                 class_alpha<T><<<dim3((unsigned)tiles_of(nv, 64)), dim3(256), 0, st>>>(
-                    l.part_alpha, l.tiles_n, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
+                    l.part_alpha, tiles_of(N, edge), l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
                     last_block ? (T*)c.alphabar + v0 : nullptr);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-            if ((e = product<T>({bt, l.ldr, D}, {r, l.ldr, N}, l.ldr, p.xsplits, (A*)(ws + p.xacc), p.block * D, !first, last,
-                                (T*)c.xbar + n0 * D, l.y, scale, st)) != hipSuccess)
-                return e;
-            A* bacc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
-            if ((e = product<T>({xt, ldrt, D}, {rt, ldrt, nv}, ldrt, p.bsplits, bacc, (p.blocks > 1 ? V : p.piece) * D, !first_block,
-                                last_block, (T*)c.betabar + v0 * D, nullptr, scale, st)) != hipSuccess)
-                return e;
+            ProductArgs<T> x_ = {}, b_ = {};
+            x_.A = {bt, l.ldr, D};
+            x_.B = {r, l.ldr, N};
+            x_.K = l.ldr;
+            x_.acc = (A*)(ws + p.xacc);
+            x_.plane = p.block * D;
+            x_.add = !first;
+            x_.y = l.y;
+            x_.lpbar = l.lpbar;
+            if ((e = product<T>(x_, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
+            b_.A = {xt, ldrt, D};
+            b_.B = {rt, ldrt, nv};
+            b_.K = ldrt;
+            b_.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
+            b_.plane = (p.blocks > 1 ? V : p.piece) * D;
+            b_.add = !first_block;
+            b_.largest = largest;
+            if ((e = product<T>(b_, p.bsplits, last_block, (T*)c.betabar + v0 * D, st)) != hipSuccess) return e;
         }
     }
     return hipSuccess;

@@ -67,7 +67,8 @@ template <typename T> __device__ __forceinline__ typename Vec16<T>::V tile_chunk
     return v;
 }
 
-template <typename T, int BM, int BN, int WM, int WN> struct Tile {
+template <typename T> struct SmallTile {
+    static constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
     static constexpr int THREADS = 64 * WM * WN;
@@ -137,5 +138,171 @@ template <typename T, int BM, int BN, int WM, int WN> struct Tile {
         return ((int)(threadIdx.x >> 6) % WN) * (BN / WN) + 16 * j + (threadIdx.x & 15);
     }
 };
+
+// The same product for operands whose rows start on 16 bytes (in 16 bits and fp32): 256 x 256 of C for 8 waves, each step's 64 KB of rows taken
+// from memory straight into LDS, two steps deep. Registers hold the fragments of the half step that is being multiplied
+// and receive those of the next half from LDS meanwhile; one barrier a step. The stay of a step:
+//   loads are issued in the middle of step s for step s + 2 (its buffer is free then: every wave holds the second half of
+//   step s in registers), and must have landed in the middle of step s + 1.
+// A rest of k behind the last whole step goes through registers at the end.
+//
+// Which rows of the operands stand in a fragment is free, and chosen so that the results leave in whole lines: lane group q
+// holds rows 16 q .. 16 q + 15 of C in registers r of fragments 4 i' .. 4 i' + 3 (and four neighbouring lanes 16 columns), so
+// that 16 neighbouring values of a column are one lane's, and the four groups' fill 128 bytes in 16 bits. The chunks of a row
+// are swizzled by the row bits that differ within such a fragment.
+template <typename T> struct WideTile {
+    typedef typename Vec16<T>::V Vec;
+    typedef typename Mma<T>::C C;
+    static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
+    static constexpr int THREADS = 512, TM = 8, TN = 4;
+    static constexpr int STEP = (BM + BN) * TILE_CHUNKS; // chunks
+    static __device__ __forceinline__ int key(int row) { return (row & 3) | (row >> 2 & 4); }
+    static __device__ __forceinline__ int fragment(int i) { return 64 * (i >> 2) + 4 * (i & 3); } // first row of fragment i
+    static constexpr int LDS_BYTES = 2 * STEP * 16;
+    C acc[TM][TN];
+
+    static bool fits(const Operand<T>& o) {
+        return ((uintptr_t)o.p & 15) == 0 && (o.ld * (int64_t)sizeof(T)) % 16 == 0 && o.ld < ((int64_t)1 << 22);
+    }
+
+    // bytes of row's chunk from the tile's first row on (rows behind the last repeat it: their products are not used)
+    static __device__ __forceinline__ uint32_t source(const Operand<T>& o, int64_t r0, int row, int slot) {
+        const int64_t last = o.rows - 1 - r0;
+        const int64_t r = row < last ? row : last;
+        return (uint32_t)(r * o.ld * (int64_t)sizeof(T)) + (uint32_t)(slot ^ key(row)) * 16;
+    }
+    // 8 loads of 16 bytes a lane into LDS (a wave's 64 lanes side by side). The LDS address goes through m0; the waits that
+    // the hardware does not make by itself: a scalar register that a vector instruction wrote, m0 before its use
+    static __device__ __forceinline__ void take(const T* a, const T* b, const uint32_t (&from)[8], uint32_t to) {
+        asm volatile("s_nop 4\n\t"
+                     "s_mov_b32 m0, %10\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\t"
+                     "s_add_u32 m0, %10, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0\n\t"
+                     "s_add_u32 m0, %10, 0x4000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %0\n\t"
+                     "s_add_u32 m0, %10, 0x6000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %0\n\t"
+                     "s_add_u32 m0, %10, 0x8000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %1\n\t"
+                     "s_add_u32 m0, %10, 0xa000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %7, %1\n\t"
+                     "s_add_u32 m0, %10, 0xc000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %8, %1\n\t"
+                     "s_add_u32 m0, %10, 0xe000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %9, %1"
+                     :
+                     : "s"(a), "s"(b), "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "v"(from[4]), "v"(from[5]),
+                       "v"(from[6]), "v"(from[7]), "s"(to)
+                     : "memory", "scc"); // (m0 is the compiler's scratch: it sets it before each use of its own)
+    }
+    static __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+    __device__ __forceinline__ void run(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0, int64_t k1,
+                                        Vec* lds) {
+        const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4;
+        const int at16 = 16 * (lane >> 2 & 3) + (lane & 3); // this lane's row within a fragment
+        const int fm = (wave / WN) * (BM / WM) + at16, fn = BM + (wave % WN) * (BN / WN) + at16;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = C{0, 0, 0, 0};
+        const int64_t steps = (k1 - k0) / tile_k<T>();
+        // one half step: acc += a b, while a and bn take the fragments of half g of the step at `at`
+        Vec a[TM];
+        auto half = [&](const Vec(&b)[TN], Vec(&bn)[TN], const Vec* at, int g) {
+            const int cm = (4 * g + q) ^ key(fm), cn = (4 * g + q) ^ key(fn);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::mul(a[i], b[j], acc[i][j]);
+                a[i] = at[(fm + fragment(i)) * TILE_CHUNKS + cm];
+                if (i < TN) bn[i] = at[(fn + fragment(i)) * TILE_CHUNKS + cn];
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) { // matrix instructions, reads of LDS
+                __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);
+                if (i < TN) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        };
+        auto first = [&](Vec(&b)[TN], const Vec* at) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) b[j] = at[(fn + fragment(j)) * TILE_CHUNKS + (q ^ key(fn))];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[i] = at[(fm + fragment(i)) * TILE_CHUNKS + (q ^ key(fm))];
+        };
+        auto mul = [&](const Vec(&b)[TN]) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::mul(a[i], b[j], acc[i][j]);
+        };
+        auto second = [&](Vec(&b)[TN], const Vec* at) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) b[j] = at[(fn + fragment(j)) * TILE_CHUNKS + ((4 + q) ^ key(fn))];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[i] = at[(fm + fragment(i)) * TILE_CHUNKS + ((4 + q) ^ key(fm))];
+        };
+        Vec b0[TN], b1[TN];
+        if (steps > 0) {
+            uint32_t from[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int id = (i & 3) * THREADS + t;
+                from[i] = source(i < 4 ? A : B, i < 4 ? m0 : n0, id / TILE_CHUNKS, id % TILE_CHUNKS);
+            }
+            const T *pa = A.p + m0 * A.ld + k0, *pb = B.p + n0 * B.ld + k0;
+            const uint32_t to = __builtin_amdgcn_readfirstlane(
+                (uint32_t)(uintptr_t)(__attribute__((address_space(3))) Vec*)lds + (uint32_t)wave * 1024);
+            take(pa, pb, from, to);
+            pa += tile_k<T>(), pb += tile_k<T>();
+            arrive();
+            if (steps > 1) take(pa, pb, from, to + STEP * 16);
+            pa += tile_k<T>(), pb += tile_k<T>();
+            first(b0, lds);
+            int side = 0;
+            for (int64_t s = 0; s + 1 < steps; ++s) {
+                half(b0, b1, lds + side * STEP, 1);
+                arrive(); // step s + 1 is there, and step s is in registers to its end
+                if (s + 2 < steps) take(pa, pb, from, to + side * STEP * 16);
+                pa += tile_k<T>(), pb += tile_k<T>();
+                side ^= 1;
+                half(b1, b0, lds + side * STEP, 0);
+            }
+            half(b0, b1, lds + side * STEP, 1);
+            mul(b1);
+        }
+        const int64_t k = k0 + steps * tile_k<T>();
+        if (k < k1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int id = (i & 3) * THREADS + t, row = id / TILE_CHUNKS, c = id % TILE_CHUNKS;
+                lds[(i < 4 ? 0 : BM * TILE_CHUNKS) + row * TILE_CHUNKS + (c ^ key(row))] =
+                    tile_chunk(i < 4 ? A : B, (i < 4 ? m0 : n0) + row, k + c * Vec16<T>::N, k1);
+            }
+            __syncthreads();
+            first(b0, lds);
+            mul(b0);
+            second(b0, lds);
+            mul(b0);
+        }
+        __syncthreads();
+    }
+    static __device__ __forceinline__ int row(int i, int r) {
+        return ((int)(threadIdx.x >> 6) / WN) * (BM / WM) + fragment(i) + 16 * ((threadIdx.x & 63) >> 4) + r;
+    }
+    static __device__ __forceinline__ int col(int j) {
+        return ((int)(threadIdx.x >> 6) % WN) * (BN / WN) + fragment(j) + 16 * (threadIdx.x >> 2 & 3) + (threadIdx.x & 3);
+    }
+};
+
+// Which tile a workgroup takes: workgroups go round the 8 XCDs, each of which has an L2 of its own, so each XCD takes a
+// contiguous run of tiles, and a run goes through 8 columns of tiles row by row (32 tiles at work share 4 + 8 panels).
+// false: none (the grid is rounded up to the XCDs)
+__device__ __forceinline__ bool tile_place(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t& m, int64_t& n) {
+    const int64_t total = tiles_m * tiles_n, run = (total + 7) / 8;
+    const int64_t at = (id & 7) * run + (id >> 3);
+    if (id >> 3 >= run || at >= total) return false;
+    const int64_t band = at / (8 * tiles_m), in = at - band * 8 * tiles_m;
+    const int64_t wide = tiles_n - 8 * band < 8 ? tiles_n - 8 * band : 8;
+    m = in / wide;
+    n = 8 * band + in % wide;
+    return true;
+}
+inline unsigned tile_grid(int64_t tiles_m, int64_t tiles_n) { return (unsigned)((tiles_m * tiles_n + 7) / 8 * 8); }
 
 } // namespace gptt

@@ -201,6 +201,10 @@ def _check_class(glm, name, y, x, alpha, beta, lpbar=None):
     _within("lp of the reverse mode", lp2, lp, dlp)
     # r: the probability's relative error, and its rounding to the element type
     dr = scale.abs().unsqueeze(1) * p * (de + dlp.unsqueeze(1) + 4 * ea) + 4 * ea * r.abs()
+    if dtype != torch.float64:
+        # fp32's exponential gives 0 for results below its smallest normal number 2^-126 (a logit 87.3 below the sum's
+        # logarithm): the probability is then off by itself, less than 2^-126, and each entry of r by that times its cotangent
+        dr = dr + 2.0**-126 * scale.abs().unsqueeze(1)
     if et > ea:
         dr = dr + et / 2 * r.abs() * (1 + et)
         if name == "f16":  # r is stored times 2^13 / max |lpbar| at least
