@@ -1,0 +1,57 @@
+// What the kernels of the categorical log density share (gpt_class.hip, gpt_class_narrow.hip).
+#pragma once
+#include "gpt_types.h"
+
+namespace gptt {
+
+template <typename A> __device__ __forceinline__ A neg_inf() { return -(A)__builtin_inf(); }
+
+// In fp32 logits, maxima and lse are kept times log2(e): an exponential is one instruction then
+__device__ __forceinline__ float times_log2e(float v) { return v * 1.44269504088896340736f; }
+__device__ __forceinline__ float from_log2e(float v) { return v * 0.69314718055994530942f; }
+__device__ __forceinline__ float exp_log2e(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ double times_log2e(double v) { return v; }
+__device__ __forceinline__ double from_log2e(double v) { return v; }
+__device__ __forceinline__ double exp_log2e(double v) { return exp(v); }
+__device__ __forceinline__ float log_(float x) { return logf(x); }
+__device__ __forceinline__ double log_(double x) { return log(x); }
+// alpha: a finite one stays finite (the type's lowest value is no exclusion)
+__device__ __forceinline__ float level_log2e(float v) {
+    return v == neg_inf<float>() ? v : fmaxf(times_log2e(v), -3.40282346638528859812e38f);
+}
+__device__ __forceinline__ double level_log2e(double v) { return v; }
+
+// the value that exponentials are taken about: the maximum, or zero where no class is possible (their sum is then zero)
+template <typename A> __device__ __forceinline__ A about(A mx) { return mx == neg_inf<A>() ? (A)0 : mx; }
+// (mx, s) <- maximum and sum of exponentials about it of two sets of classes. A NaN among the logits is a NaN in s
+template <typename A> __device__ __forceinline__ void join(A& mx, A& s, A mo, A so) {
+    const A mm = fmax(mx, mo), ref = about(mm);
+    s = s * exp_log2e(mx - ref) + so * exp_log2e(mo - ref);
+    mx = mm;
+}
+// a row's log probability from all classes' maximum and sum, and its lse (times log2(e) in fp32)
+template <typename A> __device__ __forceinline__ A row_lp(int64_t y, int64_t classes, A mx, A s, A eta_y, A& lse) {
+    const bool empty = mx == neg_inf<A>() && s == 0;
+    const A ls = log_(s);
+    lse = empty ? neg_inf<A>() : about(mx) + times_log2e(ls);
+    return y < 0 ? (A)0 : y >= classes ? (A)__builtin_nan("") : empty ? neg_inf<A>() : from_log2e(eta_y - about(mx)) - ls;
+}
+
+// sum over the 16 lanes of a row of lanes, in each of them
+__device__ __forceinline__ float sum16(float v) {
+#define GPT_ADD_DPP(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true))
+    GPT_ADD_DPP(0xb1);  // lane ^ 1
+    GPT_ADD_DPP(0x4e);  // lane ^ 2
+    GPT_ADD_DPP(0x141); // the other four of eight
+    GPT_ADD_DPP(0x140); // the other eight
+#undef GPT_ADD_DPP
+    return v;
+}
+__device__ __forceinline__ double sum16(double v) {
+#pragma unroll
+    for (int k = 8; k >= 1; k >>= 1) v += __shfl_xor(v, k, 64);
+    return v;
+}
+
+
+} // namespace gptt

@@ -14,6 +14,7 @@
 // rounding where they can: for xbar they multiply the product's Acc rows, for betabar (whose sum runs over the rows) r
 // holds them divided by the largest of them, so that cotangents that are all alike (a sum's, a mean's) leave [v = y] exact. fp16
 // has too few exponents for the small probabilities of a large vocabulary: there r is stored times 2^14.
+#include "gpt_class.h"
 #include "gpt_readout.h"
 #include "gpt_tile.h"
 #include <type_traits>
@@ -21,10 +22,6 @@
 using namespace gptt;
 
 namespace {
-
-template <typename A> __device__ __forceinline__ A neg_inf() { return -(A)__builtin_inf(); }
-__device__ __forceinline__ float log_(float x) { return logf(x); }
-__device__ __forceinline__ double log_(double x) { return log(x); }
 
 template <typename T> __host__ __device__ constexpr float stored_scale() { return std::is_same<T, half_t>::value ? 16384.f : 1.f; }
 
@@ -40,22 +37,6 @@ template <typename A> struct Largest {
         return m > 0 && m < (A)__builtin_inf() ? m : (A)1;
     }
 };
-
-// sum over the 16 lanes of a row of lanes, in each of them
-__device__ __forceinline__ float sum16(float v) {
-#define GPT_ADD_DPP(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true))
-    GPT_ADD_DPP(0xb1);  // lane ^ 1
-    GPT_ADD_DPP(0x4e);  // lane ^ 2
-    GPT_ADD_DPP(0x141); // the other four of eight
-    GPT_ADD_DPP(0x140); // the other eight
-#undef GPT_ADD_DPP
-    return v;
-}
-__device__ __forceinline__ double sum16(double v) {
-#pragma unroll
-    for (int k = 8; k >= 1; k >>= 1) v += __shfl_xor(v, k, 64);
-    return v;
-}
 
 // The 4 x 4 transpose within every four neighbouring lanes: lane b gives value r in place r, and takes lane k's value b in
 // place k. 16-bit values, two a word.
@@ -91,14 +72,6 @@ template <typename T> struct LogitArgs {
     Largest<acc_t<T>> largest;
 };
 
-// In fp32 logits, maxima and lse are kept times log2(e): an exponential is one instruction then
-__device__ __forceinline__ float times_log2e(float v) { return v * 1.44269504088896340736f; }
-__device__ __forceinline__ float exp_log2e(float v) { return __builtin_amdgcn_exp2f(v); }
-__device__ __forceinline__ float from_log2e(float v) { return v * 0.69314718055994530942f; }
-__device__ __forceinline__ double times_log2e(double v) { return v; }
-__device__ __forceinline__ double from_log2e(double v) { return v; }
-__device__ __forceinline__ double exp_log2e(double v) { return exp(v); }
-
 // Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r.
 template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::THREADS) void class_logits(LogitArgs<T> a) {
     typedef acc_t<T> A;
@@ -116,7 +89,7 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int m = Tl::row(i, r);
-            const A al = times_log2e(m < nv ? (a.alpha ? (A)a.alpha[m0 + m] : (A)0) : neg_inf<A>());
+            const A al = m < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + m]) : (A)0) : neg_inf<A>();
 #pragma unroll
             for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + al;
         }
@@ -127,36 +100,26 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
             const int64_t y = n < a.x.rows ? a.y[n] - m0 : -1;
             const int at = y >= 0 && y < Tl::BM ? (int)y : -1;
             A mx = neg_inf<A>(), here = 0;
-            bool nan = false;
+            bool mine = false; // (one lane group of one wave holds the row's class)
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     mx = fmax(mx, tl.acc[i][j][r]);
-                    nan |= tl.acc[i][j][r] != tl.acc[i][j][r];
-                    here = Tl::row(i, r) == at ? tl.acc[i][j][r] : here;
+                    const bool is = Tl::row(i, r) == at;
+                    mine |= is;
+                    here = is ? tl.acc[i][j][r] : here;
                 }
-            // (one lane group of one wave holds the row's class)
-            bool mine = false;
-#pragma unroll
-            for (int i = 0; i < Tl::TM; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mine |= Tl::row(i, r) == at;
             if (mine && at < nv) a.eta_y[n] = here;
             A s = 0;
+            const A ref = about(mx);
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += mx == neg_inf<A>() ? (A)0 : exp_log2e(tl.acc[i][j][r] - mx);
-            if (nan) s = mx = (A)__builtin_nan("");
+                for (int r = 0; r < 4; ++r) s += exp_log2e(tl.acc[i][j][r] - ref);
             // the four lane groups hold other classes of the same rows
 #pragma unroll
-            for (int k = 16; k <= 32; k <<= 1) {
-                const A mo = __shfl_xor(mx, k, 64), so = __shfl_xor(s, k, 64);
-                const A mm = (mx != mx || mo != mo) ? (A)__builtin_nan("") : fmax(mx, mo);
-                s = mm == neg_inf<A>() ? (A)0 : s * exp_log2e(mx - mm) + so * exp_log2e(mo - mm);
-                mx = mm;
-            }
+            for (int k = 16; k <= 32; k <<= 1) join(mx, s, __shfl_xor(mx, k, 64), __shfl_xor(s, k, 64));
             if (lane < 16) {
                 red[0][wm][Tl::col(j)] = mx;
                 red[1][wm][Tl::col(j)] = s;
@@ -166,12 +129,7 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
         for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
             A mx = red[0][0][c], s = red[1][0][c];
 #pragma unroll
-            for (int w = 1; w < Tl::WM; ++w) {
-                const A mo = red[0][w][c], so = red[1][w][c];
-                const A mm = (mx != mx || mo != mo) ? (A)__builtin_nan("") : fmax(mx, mo);
-                s = mm == neg_inf<A>() ? (A)0 : s * exp_log2e(mx - mm) + so * exp_log2e(mo - mm);
-                mx = mm;
-            }
+            for (int w = 1; w < Tl::WM; ++w) join(mx, s, red[0][w][c], red[1][w][c]);
             if (n0 + c < a.x.rows) {
                 a.part_max[tm * a.x.rows + n0 + c] = mx;
                 a.part_sum[tm * a.x.rows + n0 + c] = s;
@@ -274,30 +232,17 @@ template <typename T> __global__ __launch_bounds__(256) void class_join(const ac
     const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
     const int64_t n = (int64_t)blockIdx.x * 16 + c;
     A mx = neg_inf<A>(), s = 0;
-    bool nan = false;
     if (n < rows)
-        for (int64_t i = k; i < tiles; i += 16) {
-            const A mo = part_max[i * rows + n], so = part_sum[i * rows + n];
-            nan |= mo != mo;
-            const A mm = fmax(mx, mo);
-            if (mm != neg_inf<A>()) s = s * exp_log2e(mx - mm) + so * exp_log2e(mo - mm);
-            mx = mm;
-        }
-    red[0][k][c] = nan ? (A)__builtin_nan("") : mx;
+        for (int64_t i = k; i < tiles; i += 16) join(mx, s, part_max[i * rows + n], part_sum[i * rows + n]);
+    red[0][k][c] = mx;
     red[1][k][c] = s;
     __syncthreads();
     if (k || n >= rows) return;
-    A top = neg_inf<A>();
-    for (int i = 0; i < 16; ++i) {
-        nan |= red[0][i][c] != red[0][i][c];
-        top = fmax(top, red[0][i][c]);
-    }
-    A sum = 0;
-    for (int i = 0; i < 16; ++i)
-        if (red[0][i][c] != neg_inf<A>()) sum += red[1][i][c] * exp_log2e(red[0][i][c] - top);
+    for (int i = 1; i < 16; ++i) join(mx, s, red[0][i][c], red[1][i][c]);
     const int64_t yn = y[n];
-    lp[n] = yn < 0 ? (A)0 : yn >= classes || nan ? (A)__builtin_nan("") : top == neg_inf<A>() ? top : from_log2e(eta_y[n] - top) - log_(sum);
-    if (lse) lse[n] = nan ? (A)__builtin_nan("") : top == neg_inf<A>() ? top : top + times_log2e(log_(sum));
+    A l;
+    lp[n] = row_lp(yn, classes, mx, s, yn >= 0 && yn < classes ? eta_y[n] : (A)0, l);
+    if (lse) lse[n] = l;
 }
 
 // out[c][r] = in[r][c], rows behind the last, and (y given) those without an observation, zero. 64 x 64 through LDS
@@ -689,6 +634,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
 } // namespace
 
 size_t gpt_class_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, bool vjp) {
+    if (gpt_class_narrow(dtype, rows, features, classes)) return gpt_class_narrow_workspace(dtype, rows, features, classes, vjp);
     switch (dtype) {
     case GPT_F64: return Plan<double>(rows, features, classes, vjp).bytes;
     case GPT_F32: return Plan<float>(rows, features, classes, vjp).bytes;
@@ -697,6 +643,7 @@ size_t gpt_class_workspace(int dtype, int64_t rows, int64_t features, int64_t cl
     }
 }
 hipError_t gpt_launch_class(int dtype, const ClassArgs& a, bool vjp, hipStream_t st) {
+    if (gpt_class_narrow(dtype, a.rows, a.features, a.classes)) return gpt_launch_class_narrow(dtype, a, vjp, st);
     switch (dtype) {
     case GPT_F64: return launch<double>(a, vjp, st);
     case GPT_F32: return launch<float>(a, vjp, st);

@@ -9,7 +9,8 @@
 
 namespace gptt {
 
-template <typename T> struct Mma; // C fragment, product of two 16-byte chunks, row of C that register r of lane group q holds
+template <typename T> struct Mma; // C fragment, product of two 16-byte chunks, row of C that register r of lane group q holds;
+                                 // mul1: of one value a lane, that of lane group q standing for k = q
 template <> struct Mma<bf16_t> {
     typedef float C __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ C mul(Vec16<bf16_t>::V a, Vec16<bf16_t>::V b, C c) {
@@ -28,18 +29,20 @@ template <> struct Mma<float> {
     typedef float C __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ C mul(Vec16<float>::V a, Vec16<float>::V b, C c) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+        for (int j = 0; j < 4; ++j) c = mul1(a[j], b[j], c);
         return c;
     }
+    static __device__ __forceinline__ C mul1(float a, float b, C c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ int row(int q, int r) { return 4 * q + r; }
 };
 template <> struct Mma<double> {
     typedef double C __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ C mul(Vec16<double>::V a, Vec16<double>::V b, C c) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[j], b[j], c, 0, 0, 0);
+        for (int j = 0; j < 2; ++j) c = mul1(a[j], b[j], c);
         return c;
     }
+    static __device__ __forceinline__ C mul1(double a, double b, C c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ int row(int q, int r) { return q + 4 * r; }
 };
 
