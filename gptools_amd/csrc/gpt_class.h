@@ -1,6 +1,7 @@
 // What the kernels of the categorical log density share (gpt_class.hip, gpt_class_narrow.hip).
 #pragma once
 #include "gpt_types.h"
+#include <type_traits>
 
 namespace gptt {
 
@@ -53,5 +54,20 @@ __device__ __forceinline__ double sum16(double v) {
     return v;
 }
 
+
+template <typename T> __host__ __device__ constexpr float stored_scale() { return std::is_same<T, half_t>::value ? 16384.f : 1.f; }
+
+constexpr int SCALE_PARTS = 64;
+// largest |lpbar| of the observed rows from class_scale's parts (null: no lpbar, 1), for a whole wave; 1 where it is no scale
+template <typename A> struct Largest {
+    const A* parts;
+    __device__ __forceinline__ A get() const {
+        if (!parts) return 1;
+        A m = parts[threadIdx.x & 63];
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
+        return m > 0 && m < (A)__builtin_inf() ? m : (A)1;
+    }
+};
 
 } // namespace gptt

@@ -14,7 +14,7 @@
 // rounding where they can: for xbar they multiply the product's Acc rows, for betabar (whose sum runs over the rows) r
 // holds them divided by the largest of them, so that cotangents that are all alike (a sum's, a mean's) leave [v = y] exact. fp16
 // has too few exponents for the small probabilities of a large vocabulary: there r is stored times 2^14.
-#include "gpt_class.h"
+#include "gpt_class_few.h"
 #include "gpt_readout.h"
 #include "gpt_tile.h"
 #include <type_traits>
@@ -22,21 +22,6 @@
 using namespace gptt;
 
 namespace {
-
-template <typename T> __host__ __device__ constexpr float stored_scale() { return std::is_same<T, half_t>::value ? 16384.f : 1.f; }
-
-constexpr int SCALE_PARTS = 64;
-// largest |lpbar| of the observed rows from class_scale's parts (null: no lpbar, 1), for a whole wave; 1 where it is no scale
-template <typename A> struct Largest {
-    const A* parts;
-    __device__ __forceinline__ A get() const {
-        if (!parts) return 1;
-        A m = parts[threadIdx.x & 63];
-#pragma unroll
-        for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
-        return m > 0 && m < (A)__builtin_inf() ? m : (A)1;
-    }
-};
 
 // The 4 x 4 transpose within every four neighbouring lanes: lane b gives value r in place r, and takes lane k's value b in
 // place k. 16-bit values, two a word.
@@ -536,8 +521,103 @@ template <typename T> hipError_t product(ProductArgs<T> p, int64_t splits, bool 
     return hipGetLastError();
 }
 
+// ---- few rows
+template <typename T> struct FewPlan {
+    // class tiles of a workgroup where the classes are enough to fill the card that way (fp64 has not the LDS for more)
+    static constexpr int CT = sizeof(T) == 8 ? 2 : 4;
+    bool large;
+    int64_t tiles, ldv, ldrt, share, splits;
+    size_t part_max, part_sum, eta, lse, largest, r, rt, xt, xpart, bytes;
+    FewPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
+        const size_t A = sizeof(acc_t<T>), E = sizeof(T);
+        size_t at = 0;
+        auto take = [&](size_t n) {
+            const size_t p = at;
+            at += (n + 255) / 256 * 256;
+            return p;
+        };
+        large = V >= 16 * CT * FILL / 2;
+        tiles = tiles_of(V, large ? 16 * CT : 16);
+        part_max = take(A * (size_t)(rows * tiles));
+        part_sum = take(A * (size_t)(rows * tiles));
+        if (vjp) {
+            ldv = up_to(V, 64);
+            ldrt = rows <= 32 ? 32 : 64;
+            const int64_t slabs = tiles_of(D, 16 * Vec16<T>::N);
+            splits = tiles_of(2 * FILL, slabs);
+            if (splits > tiles_of(V, 128)) splits = tiles_of(V, 128);
+            share = up_to(tiles_of(V, splits), 128);
+            splits = tiles_of(V, share);
+            eta = take(A * (size_t)(rows * ldv));
+            lse = take(A * (size_t)rows);
+            largest = take(A * FEW);
+            r = take(E * (size_t)(rows * ldv));
+            rt = take(E * (size_t)(V * ldrt));
+            xt = take(E * (size_t)(D * ldrt));
+            xpart = take(A * (size_t)(splits * rows * D));
+        }
+        bytes = at;
+    }
+};
+template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStream_t st) {
+    typedef acc_t<T> A;
+    const int64_t D = c.features, V = c.classes;
+    const FewPlan<T> p(c.rows, D, V, vjp);
+    char* ws = (char*)c.ws;
+    FewArgs<T> a = {};
+    a.x = {(const T*)c.x, c.ldx, c.rows};
+    a.beta = {(const T*)c.beta, c.ldbeta, V};
+    a.alpha = (const T*)c.alpha;
+    a.y = c.y;
+    a.lpbar = (const A*)c.lpbar;
+    a.features = D;
+    a.part_max = (A*)(ws + p.part_max);
+    a.part_sum = (A*)(ws + p.part_sum);
+    a.tiles = p.tiles;
+    a.lp = (A*)c.lp;
+    if (vjp) {
+        a.eta = (A*)(ws + p.eta);
+        a.ldv = p.ldv;
+        a.lse = (A*)(ws + p.lse);
+        a.largest = (A*)(ws + p.largest);
+        a.r = (T*)(ws + p.r);
+        a.rt = (T*)(ws + p.rt);
+        a.ldrt = p.ldrt;
+        a.alphabar = (T*)c.alphabar;
+        a.xpart = (A*)(ws + p.xpart);
+        a.share = p.share;
+    }
+    const dim3 grid((unsigned)p.tiles);
+    if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4><<<grid, dim3(256), 0, st>>>(a);
+    else class_few_logits<T, NT, 1, 8><<<grid, dim3(512), 0, st>>>(a);
+    class_few_join<T><<<dim3((unsigned)c.rows), dim3(256), 0, st>>>(a);
+    if (!vjp) return hipGetLastError();
+    const Largest<A> largest = {c.lpbar ? a.largest : nullptr};
+    class_few_r<T><<<dim3((unsigned)(p.ldv / 64)), dim3(256), 0, st>>>(a, largest);
+    class_few_xbar<T, NT><<<dim3((unsigned)tiles_of(D, 16 * Vec16<T>::N), (unsigned)p.splits), dim3(256), 0, st>>>(a);
+    class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits, (T*)c.xbar);
+    T* xt = (T*)(ws + p.xt);
+    class_transpose<T><<<dim3((unsigned)tiles_of(p.ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(a.x.p, c.ldx, c.rows, D,
+                                                                                                            c.y, xt, p.ldrt);
+    constexpr int NG = (NT <= 2 ? 32 : 64) / (4 * Vec16<T>::N);
+    const int64_t slabs = tiles_of(D, Slab<T>::WIDTH);
+    int64_t shares = tiles_of(4 * FILL, slabs);
+    if (shares > tiles_of(V, 128)) shares = tiles_of(V, 128);
+    class_few_beta<T, NG><<<dim3((unsigned)slabs, (unsigned)shares), dim3(256), 0, st>>>(a, xt, (T*)c.betabar, largest);
+    return hipGetLastError();
+}
+template <typename T> size_t space(int64_t rows, int64_t features, int64_t classes, bool vjp) {
+    return rows <= FEW ? FewPlan<T>(rows, features, classes, vjp).bytes : Plan<T>(rows, features, classes, vjp).bytes;
+}
+template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStream_t st) {
+    if (c.rows <= 16) return launch_few<T, 1>(c, vjp, st);
+    if (c.rows <= 32) return launch_few<T, 2>(c, vjp, st);
+    return launch_few<T, 4>(c, vjp, st);
+}
+
 template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_t st) {
     typedef acc_t<T> A;
+    if (c.rows <= FEW) return launch_few<T>(c, vjp, st);
     const Plan<T> p(c.rows, c.features, c.classes, vjp);
     char* ws = (char*)c.ws;
     const int64_t D = c.features, V = c.classes;
@@ -636,10 +716,10 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
 size_t gpt_class_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, bool vjp) {
     if (gpt_class_narrow(dtype, rows, features, classes)) return gpt_class_narrow_workspace(dtype, rows, features, classes, vjp);
     switch (dtype) {
-    case GPT_F64: return Plan<double>(rows, features, classes, vjp).bytes;
-    case GPT_F32: return Plan<float>(rows, features, classes, vjp).bytes;
-    case GPT_F16: return Plan<half_t>(rows, features, classes, vjp).bytes;
-    default: return Plan<bf16_t>(rows, features, classes, vjp).bytes;
+    case GPT_F64: return space<double>(rows, features, classes, vjp);
+    case GPT_F32: return space<float>(rows, features, classes, vjp);
+    case GPT_F16: return space<half_t>(rows, features, classes, vjp);
+    default: return space<bf16_t>(rows, features, classes, vjp);
     }
 }
 hipError_t gpt_launch_class(int dtype, const ClassArgs& a, bool vjp, hipStream_t st) {

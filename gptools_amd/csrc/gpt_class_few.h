@@ -1,0 +1,385 @@
+// The categorical log density for few rows (up to 64; gpt_class.hip includes this): a token or a batch of tokens of a generating
+// model. Bound by reading beta (and writing betabar): the products have few columns, so beta's rows go from memory straight
+// into the registers that the matrix instruction reads, no LDS between.
+//
+//   class_few_logits  16 classes a workgroup or 64 (32 in fp64), whose waves share the features; their logits' maximum and sum for every row,
+//                     and for the reverse mode the logits themselves (64 rows of logits are a piece as r is one)
+//   class_few_r       r in both orders, alphabar
+//   class_few_xbar    xbar = r beta. beta's rows lie along the features, the sum runs over the classes: a lane reads 16 bytes of
+//                     eight classes and turns the block over in its registers (in 16 bits one byte permutation for two values)
+//   class_few_beta    betabar = r^T x, bound by writing it
+#pragma once
+#include "gpt_class.h"
+#include "gpt_tile.h"
+
+namespace gptt {
+
+constexpr int FEW = 64; // rows
+
+template <typename T> struct FewArgs {
+    Operand<T> x, beta;
+    const T* alpha;
+    const int64_t* y;
+    const acc_t<T>* lpbar;
+    int64_t features;
+    acc_t<T>*part_max, *part_sum; // [rows][tiles]
+    int64_t tiles;
+    acc_t<T>* eta; // [rows][ldv], times log2(e) in fp32
+    int64_t ldv;
+    acc_t<T>*lse, *lp, *largest; // largest: |lpbar| of each observed row, zero to FEW
+    T *r, *rt;                   // [rows][ldv], [classes][ldrt]
+    int64_t ldrt;
+    T* alphabar;
+    acc_t<T>* xpart; // [splits][rows][features]
+    int64_t share;   // classes of a split
+};
+
+// NT tiles of 16 rows, CT of 16 classes, WK waves that share the features
+template <typename T, int NT, int CT, int WK> __global__ __launch_bounds__(64 * WK) void class_few_logits(FewArgs<T> a) {
+    typedef acc_t<T> A;
+    typedef typename Vec16<T>::V Vec;
+    typedef typename Mma<T>::C C;
+    constexpr int N = Vec16<T>::N, STEP = 4 * N; // a wave's step: 64 bytes of a row
+    __shared__ A sum[WK][CT * 16][NT * 16 + 1];
+    const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
+    const int64_t v0 = (int64_t)blockIdx.x * CT * 16, V = a.beta.rows, D = a.features;
+    C c[CT][NT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) c[i][t] = C{0, 0, 0, 0};
+    const T *pb[CT], *px[NT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) { // (rows behind the last repeat it: their results are not used)
+        const int64_t v = v0 + 16 * i + (lane & 15);
+        pb[i] = a.beta.p + (v < V ? v : V - 1) * a.beta.ld + q * N;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int64_t n = 16 * t + (lane & 15);
+        px[t] = a.x.p + (n < a.x.rows ? n : a.x.rows - 1) * a.x.ld + q * N;
+    }
+    const int64_t whole = D / STEP;
+    // Runs of AHEAD steps a wave. Few steps on their way, and many waves, read beta faster than the other way round; and four
+    // class tiles share each read of x, which comes from the caches at the same rate: bf16, 64 rows x 128000 classes x 4096
+    // features 262 us with CT = 4, AHEAD = 2 (284 with 4; CT = 2 421, 8 370); 16 x 69974 x 3584 106 us (CT = 1 142); one row x
+    // 32000 x 4096 39 us (45)
+    constexpr int AHEAD = CT >= 4 ? 2 : 4;
+    const int64_t runs = whole / AHEAD;
+    for (int64_t g = wave; g < runs; g += WK) {
+        Vec b[AHEAD][CT], x[AHEAD][NT];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i) b[u][i] = load16(pb[i] + (g * AHEAD + u) * STEP);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) x[u][t] = load16(px[t] + (g * AHEAD + u) * STEP);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) c[i][t] = Mma<T>::mul(b[u][i], x[u][t], c[i][t]);
+    }
+    for (int64_t s = runs * AHEAD + wave; s < whole; s += WK) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const Vec b = load16(pb[i] + s * STEP);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) c[i][t] = Mma<T>::mul(b, load16(px[t] + s * STEP), c[i][t]);
+        }
+    }
+    if (whole * STEP < D && wave == (int)(whole % WK)) {
+        const int64_t k = whole * STEP + q * N;
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const int64_t v = v0 + 16 * i + (lane & 15);
+            const Vec b = tile_chunk(a.beta, v, k, D);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) c[i][t] = Mma<T>::mul(b, tile_chunk(a.x, (int64_t)16 * t + (lane & 15), k, D), c[i][t]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[wave][16 * i + Mma<T>::row(q, r)][16 * t + (lane & 15)] = c[i][t][r];
+    __syncthreads();
+    // 16 threads a row (NT * 16 rows; the workgroup may take them in several goes), CT classes each
+    const int k = threadIdx.x & 15;
+    for (int n = threadIdx.x >> 4; n < NT * 16; n += 4 * WK) {
+        A e[CT], mx = neg_inf<A>(), s = 0;
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const int64_t v = v0 + 16 * i + k;
+            A u = 0;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) u += sum[w][16 * i + k][n];
+            e[i] = times_log2e(u) + (v < V ? (a.alpha ? level_log2e((A)a.alpha[v]) : (A)0) : neg_inf<A>());
+            mx = fmax(mx, e[i]);
+            if (a.eta && n < a.x.rows && v < a.ldv) a.eta[n * a.ldv + v] = e[i];
+        }
+#pragma unroll
+        for (int m = 8; m >= 1; m >>= 1) mx = fmax(mx, __shfl_xor(mx, m, 64));
+#pragma unroll
+        for (int i = 0; i < CT; ++i) s += exp_log2e(e[i] - about(mx));
+        s = sum16(s);
+        if (k == 0 && n < a.x.rows) {
+            a.part_max[n * a.tiles + blockIdx.x] = mx;
+            a.part_sum[n * a.tiles + blockIdx.x] = s;
+        }
+    }
+}
+
+// one workgroup a row: lse and lp. The row's logit of its class comes from x and beta again (one dot product)
+template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewArgs<T> a) {
+    typedef acc_t<T> A;
+    __shared__ A red[3][4];
+    const int64_t n = blockIdx.x, y = a.y[n], V = a.beta.rows;
+    const bool known = y >= 0 && y < V;
+    A mx = neg_inf<A>(), s = 0, eta = 0;
+    for (int64_t i = threadIdx.x; i < a.tiles; i += 256) join(mx, s, a.part_max[n * a.tiles + i], a.part_sum[n * a.tiles + i]);
+    if (known)
+#pragma unroll 4
+        for (int k = threadIdx.x; k < (int)a.features; k += 256) eta += (A)a.x.p[n * a.x.ld + k] * (A)a.beta.p[y * a.beta.ld + k];
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        join(mx, s, __shfl_xor(mx, m, 64), __shfl_xor(s, m, 64));
+        eta += __shfl_xor(eta, m, 64);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        red[0][threadIdx.x >> 6] = mx;
+        red[1][threadIdx.x >> 6] = s;
+        red[2][threadIdx.x >> 6] = eta;
+    }
+    __syncthreads();
+    if (a.largest && n == 0) // (rows behind the last)
+        for (int64_t i = gridDim.x + threadIdx.x; i < FEW; i += 256) a.largest[i] = 0;
+    if (threadIdx.x) return;
+    for (int w = 1; w < 4; ++w) {
+        join(mx, s, red[0][w], red[1][w]);
+        eta += red[2][w];
+    }
+    eta = times_log2e(eta);
+    if (known && a.alpha) eta += level_log2e((A)a.alpha[y]);
+    A lse;
+    a.lp[n] = row_lp(y, V, mx, s, eta, lse);
+    if (a.lse) a.lse[n] = lse;
+    if (a.largest) a.largest[n] = y < 0 || !a.lpbar ? (A)0 : fabs(a.lpbar[n]);
+}
+
+// r of 64 classes: a wave takes a quarter of the rows, a lane a class -- rt's entries side by side, r's column, alphabar
+template <typename T> __global__ __launch_bounds__(256) void class_few_r(FewArgs<T> a, Largest<acc_t<T>> largest_of) {
+    typedef acc_t<T> A;
+    constexpr int N = Vec16<T>::N;
+    __shared__ A lse[FEW], w[FEW], sum[4][64];
+    __shared__ int64_t y[FEW];
+    const A largest = largest_of.get();
+    const int64_t V = a.beta.rows;
+    const int rows = (int)a.x.rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x < FEW) {
+        const int n = threadIdx.x;
+        const int64_t yn = n < rows ? a.y[n] : -1;
+        const A l = yn >= 0 ? a.lse[n] : neg_inf<A>();
+        const bool none = l == neg_inf<A>();
+        y[n] = none ? -1 : yn;
+        lse[n] = yn >= V ? (A)__builtin_nan("") : l;
+        w[n] = none ? (A)0 : a.lpbar ? a.lpbar[n] / largest : (A)1;
+    }
+    __syncthreads();
+    const int64_t v = (int64_t)blockIdx.x * 64 + lane; // (below ldv, a multiple of 64)
+    constexpr A up = stored_scale<T>();
+    A total = 0;
+    const int share = (int)a.ldrt / 4;
+    for (int n0 = wave * share; n0 < (wave + 1) * share; n0 += N) {
+        typename Vec16<T>::V u;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int n = n0 + e;
+            A g = 0;
+            if (n < rows) {
+                g = y[n] < 0 || v >= V ? (A)0 : (y[n] == v ? up : (A)0) - up * exp_log2e(a.eta[n * a.ldv + v] - lse[n]);
+                a.r[n * a.ldv + v] = (T)g;
+                g *= w[n];
+            }
+            total += g;
+            u[e] = (T)g;
+        }
+        if (v < V) *reinterpret_cast<typename Vec16<T>::V*>(a.rt + v * a.ldrt + n0) = u;
+    }
+    if (!a.alphabar) return;
+    sum[wave][lane] = total;
+    __syncthreads();
+    if (wave == 0 && v < V) a.alphabar[v] = (T)(((sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane])) * (largest / up));
+}
+
+// Fragment j (feature 16-byte chunk's element j) of eight classes' chunks
+template <typename T> struct Turn;
+template <> struct Turn<float> {
+    static __device__ __forceinline__ void mul(const Vec16<float>::V (&b)[8], int j, const float (&r)[8], Mma<float>::C& c) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c = Mma<float>::mul1(b[u][j], r[u], c);
+    }
+};
+template <> struct Turn<double> {
+    static __device__ __forceinline__ void mul(const Vec16<double>::V (&b)[8], int j, const double (&r)[8], Mma<double>::C& c) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c = Mma<double>::mul1(b[u][j], r[u], c);
+    }
+};
+template <typename T> struct Turn { // 16 bits
+    static __device__ __forceinline__ void mul(const typename Vec16<T>::V (&b)[8], int j, const T (&r)[8], typename Mma<T>::C& c) {
+        typename Vec16<T>::V f, g;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            f[u] = b[u][j];
+            g[u] = r[u];
+        }
+        c = Mma<T>::mul(f, g, c);
+    }
+};
+
+// xbar's sums over a share of the classes for 16 chunks of features: four waves with a quarter of the share each
+template <typename T, int NT> __global__ __launch_bounds__(256) void class_few_xbar(FewArgs<T> a) {
+    typedef acc_t<T> A;
+    typedef typename Vec16<T>::V Vec;
+    typedef typename Mma<T>::C C;
+    constexpr int N = Vec16<T>::N;
+    __shared__ A sum[4][16][16 * N + 1];
+    const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
+    const int64_t d0 = (int64_t)blockIdx.x * 16 * N, d = d0 + (lane & 15) * N, D = a.features, V = a.beta.rows;
+    const int64_t s0 = (int64_t)blockIdx.y * a.share, s1 = s0 + a.share < V ? s0 + a.share : V;
+    C c[NT][N];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < N; ++j) c[t][j] = C{0, 0, 0, 0};
+    const bool full = d0 + 16 * N <= D;
+    // lane group q: classes v + 8 q .. + 7 (r is zero behind the last class, up to ldv, a multiple of 32)
+    for (int64_t v = s0 + 32 * wave; v < s1; v += 128) {
+        Vec b[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int64_t at = v + 8 * q + u, row = at < V ? at : V - 1;
+            b[u] = full ? load16(a.beta.p + row * a.beta.ld + d) : tile_chunk(a.beta, row, d, D);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int64_t n = 16 * t + (lane & 15);
+            T r[8];
+#pragma unroll
+            for (int k = 0; k < 8; k += N) {
+                const Vec u = *reinterpret_cast<const Vec*>(a.r + (n < a.x.rows ? n : a.x.rows - 1) * a.ldv + v + 8 * q + k);
+#pragma unroll
+                for (int e = 0; e < N && k + e < 8; ++e) r[k + e] = u[e];
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) Turn<T>::mul(b, j, r, c[t][j]);
+        }
+    }
+    // c[t][j] register r: row of x 16 t + (lane & 15), feature (row(q, r)) N + j
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[wave][lane & 15][Mma<T>::row(q, r) * N + j] = c[t][j][r];
+        __syncthreads();
+        for (int id = threadIdx.x; id < 16 * 16 * N; id += 256) {
+            const int n = id / (16 * N), k = id % (16 * N);
+            if (16 * t + n < a.x.rows && d0 + k < D)
+                a.xpart[((int64_t)blockIdx.y * a.x.rows + 16 * t + n) * D + d0 + k] =
+                    (sum[0][n][k] + sum[1][n][k]) + (sum[2][n][k] + sum[3][n][k]);
+        }
+        __syncthreads();
+    }
+}
+// xbar <- the splits' sums times the rows' cotangents
+template <typename T> __global__ __launch_bounds__(256) void class_few_xbar_join(FewArgs<T> a, int splits, T* xbar) {
+    typedef acc_t<T> A;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, count = a.x.rows * a.features;
+    if (i >= count) return;
+    const int64_t n = i / a.features, y = a.y[n];
+    A s = 0;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += a.xpart[k * count + i];
+    xbar[i] = (T)(y < 0 ? (A)0 : s * ((a.lpbar ? a.lpbar[n] : (A)1) / (A)stored_scale<T>()));
+}
+
+// betabar[v][d] = sum_n rt[v][n] x[n][d] for a slab of features and a share of the classes: the slab's x stays in registers (xt, its
+// transpose: [features][ldrt]), 16 classes at a time pass by. NG: steps of k, ldrt = NG * 4 chunks. As in WideTile the features of a
+// fragment's rows are chosen so that a lane's results lie side by side (16 bytes of them, four lanes 64).
+template <typename T> struct Slab {
+    static constexpr int FRAGS = 64 / (4 * (int)sizeof(T)) < 2 ? 2 : 64 / (4 * (int)sizeof(T)), WIDTH = 16 * FRAGS;
+    static constexpr int RUN = sizeof(T) == 2 ? 8 : 4; // results side by side
+    static __device__ __forceinline__ int feature(int j, int row) {
+        if (sizeof(T) == 2) return 32 * (j >> 1) + 8 * (row >> 2) + 4 * (j & 1) + (row & 3);
+        if (sizeof(T) == 4) return 16 * j + row;
+        return 16 * j + 4 * (row & 3) + (row >> 2);
+    }
+};
+template <typename T, int NG> __global__ __launch_bounds__(256) void class_few_beta(FewArgs<T> a, const T* xt, T* betabar,
+                                                                                   Largest<acc_t<T>> largest) {
+    typedef acc_t<T> A;
+    typedef typename Vec16<T>::V Vec;
+    typedef typename Mma<T>::C C;
+    typedef Slab<T> S;
+    constexpr int N = Vec16<T>::N, AHEAD = NG <= 2 ? 4 : 2;
+    const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
+    const int64_t d0 = (int64_t)blockIdx.x * S::WIDTH, D = a.features, V = a.beta.rows, ldrt = a.ldrt;
+    const A back = largest.get() / (A)stored_scale<T>();
+    Vec x[S::FRAGS][NG];
+#pragma unroll
+    for (int j = 0; j < S::FRAGS; ++j) {
+        const int64_t d = d0 + S::feature(j, lane & 15);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) x[j][g] = d < D ? *reinterpret_cast<const Vec*>(xt + d * ldrt + (4 * g + q) * N) : Vec{};
+    }
+    const bool full = d0 + S::WIDTH <= D;
+    const int64_t step = (int64_t)gridDim.y * 4 * 16 * AHEAD;
+    for (int64_t v0 = ((int64_t)blockIdx.y * 4 + wave) * 16 * AHEAD; v0 < V; v0 += step) {
+        Vec b[AHEAD][NG];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int64_t v = v0 + 16 * u + (lane & 15), at = v < V ? v : V - 1;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) b[u][g] = *reinterpret_cast<const Vec*>(a.rt + at * ldrt + (4 * g + q) * N);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int64_t v = v0 + 16 * u + (lane & 15);
+            A out[S::FRAGS * 4];
+#pragma unroll
+            for (int j = 0; j < S::FRAGS; ++j) {
+                C c = {0, 0, 0, 0};
+#pragma unroll
+                for (int g = 0; g < NG; ++g) c = Mma<T>::mul(x[j][g], b[u][g], c);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out[4 * j + r] = c[r] * back;
+            }
+            if (v >= V) continue;
+#pragma unroll
+            for (int i = 0; i < S::FRAGS * 4 / S::RUN; ++i) {
+                const int64_t d = d0 + i * 4 * S::RUN + q * S::RUN;
+                T* to = betabar + v * D + d;
+#pragma unroll
+                for (int k = 0; k < S::RUN; k += N) {
+                    if (full) {
+                        Vec w;
+#pragma unroll
+                        for (int e = 0; e < N; ++e) w[e] = (T)out[i * S::RUN + k + e];
+                        store16(to + k, w);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < N; ++e)
+                            if (d + k + e < D) to[k + e] = (T)out[i * S::RUN + k + e];
+                    }
+                }
+            }
+        }
+    }
+}
+
+} // namespace gptt
