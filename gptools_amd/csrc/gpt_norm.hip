@@ -99,80 +99,157 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row(NormAr
     x.store((T*)a.y + row * n, n, t);
 }
 
-// A workgroup takes rows blockIdx.x, + gridDim.x, ...; its sums for the parameters' gradients stay in registers, and go to
-// partial[2][gridDim.x][n] at the end (norm_param_sum adds them up in a fixed order).
+// A row's vectors as they lie in memory
+template <typename T, int THREADS, int ITER> struct RowRaw {
+    static constexpr int N = Vec16<T>::N;
+    typename Vec16<T>::V v[ITER];
+    __device__ __forceinline__ void load(const T* p, int64_t n, int t) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int64_t k = (int64_t)(i * THREADS + t) * N;
+            if (k + N <= n) v[i] = load16(p + k);
+            else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i][e] = k + e < n ? p[k + e] : (T)0;
+            }
+        }
+    }
+    __device__ __forceinline__ acc_t<T> at(int j) const { return (acc_t<T>)v[j / N][j % N]; }
+};
+
+// Rows go round the workgroups' groups of THREADS threads; the next row's vectors are on their way while this one is
+// reduced. The sums for the parameters' gradients stay in registers, and go to partial[2][gridDim.x][n] at the end
+// (norm_param_sum adds them up in a fixed order).
 template <typename T, int THREADS, int ITER, bool PARAMS>
-__global__ __launch_bounds__(THREADS) void norm_row_vjp(NormArgs a) {
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row_vjp(NormArgs a) {
     typedef acc_t<T> A;
-    constexpr int K = ITER * Vec16<T>::N;
-    __shared__ A red[THREADS / 64 * 2];
-    const int t = threadIdx.x;
-    const int64_t n = a.width;
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, GROUPS = BLOCK / THREADS, N = Vec16<T>::N, K = ITER * N;
+    __shared__ A red[2][THREADS / 64 * 2];
+    __shared__ A joined[PARAMS && GROUPS > 1 ? GROUPS - 1 : 1][PARAMS && GROUPS > 1 ? 2 * K * THREADS : 1];
+    const int t = threadIdx.x % THREADS, group = threadIdx.x / THREADS;
+    const int64_t n = a.width, step = (int64_t)gridDim.x * GROUPS;
     A wbar[PARAMS ? K : 1], bbar[PARAMS ? K : 1];
     if (PARAMS) {
 #pragma unroll
         for (int j = 0; j < K; ++j) wbar[j] = bbar[j] = 0;
     }
-    RowRegs<T, THREADS, ITER> w;
+    RowRaw<T, THREADS, ITER> w, xn, gn;
     if (a.weight) w.load((const T*)a.weight, n, t);
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+    A mean = 0, rstd = 0;
+    if (row < a.rows) {
+        xn.load((const T*)a.x + row * n, n, t);
+        gn.load((const T*)a.ybar + row * n, n, t);
+        mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+    }
+    int side = 0;
+    for (; row < a.rows; row += step) { // (a group of several waves is the whole workgroup: its barriers are met by all)
         RowRegs<T, THREADS, ITER> x, g;
-        x.load((const T*)a.x + row * n, n, t);
-        g.load((const T*)a.ybar + row * n, n, t);
-        const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+        const A mu = mean, rs = rstd;
         A s[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            x.v[j] = (x.v[j] - mean) * rstd;
+            x.v[j] = (xn.at(j) - mu) * rs;
+            g.v[j] = gn.at(j);
+        }
+        if (row + step < a.rows) {
+            xn.load((const T*)a.x + (row + step) * n, n, t);
+            gn.load((const T*)a.ybar + (row + step) * n, n, t);
+            mean = ((const A*)a.mean)[row + step], rstd = ((const A*)a.rstd)[row + step];
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
             if (PARAMS) {
                 wbar[j] += g.v[j] * x.v[j];
                 bbar[j] += g.v[j];
             }
-            if (a.weight) g.v[j] *= w.v[j];
+            if (a.weight) g.v[j] *= w.at(j);
             s[0] += g.v[j]; // (zero behind the row's end: g is)
             s[1] += g.v[j] * x.v[j];
         }
-        row_sum<THREADS>(s, red, false);
+        row_sum<THREADS>(s, red[side], true); // (the other half is next: one barrier a row)
+        side ^= 1;
         const A c0 = s[0] / (A)n, c1 = s[1] / (A)n;
 #pragma unroll
-        for (int j = 0; j < K; ++j) x.v[j] = rstd * (g.v[j] - c0 - x.v[j] * c1);
+        for (int j = 0; j < K; ++j) x.v[j] = rs * (g.v[j] - c0 - x.v[j] * c1);
         x.store((T*)a.xbar + row * n, n, t);
     }
     if (PARAMS) {
+        if (GROUPS > 1) {
+            if (group) {
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    joined[group - 1][j * THREADS + t] = wbar[j];
+                    joined[group - 1][(K + j) * THREADS + t] = bbar[j];
+                }
+            }
+            __syncthreads();
+            if (group) return;
+#pragma unroll
+            for (int k = 0; k < GROUPS - 1; ++k)
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    wbar[j] += joined[k][j * THREADS + t];
+                    bbar[j] += joined[k][(K + j) * THREADS + t];
+                }
+        }
         A* p = (A*)a.partial + (int64_t)blockIdx.x * n;
         const int64_t other = (int64_t)gridDim.x * n;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
+            const int64_t k = (int64_t)(i * THREADS + t) * N;
+            if (k + N <= n) {
 #pragma unroll
-            for (int e = 0; e < Vec16<T>::N; ++e) {
-                const int64_t k = (int64_t)(i * THREADS + t) * Vec16<T>::N + e;
-                if (k < n) {
-                    p[k] = wbar[i * Vec16<T>::N + e];
-                    p[k + other] = bbar[i * Vec16<T>::N + e];
+                for (int e = 0; e < N; e += Vec16<A>::N) {
+                    typename Vec16<A>::V u, v;
+#pragma unroll
+                    for (int f = 0; f < Vec16<A>::N; ++f) {
+                        u[f] = wbar[i * N + e + f];
+                        v[f] = bbar[i * N + e + f];
+                    }
+                    store16(p + k + e, u);
+                    store16(p + other + k + e, v);
                 }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (k + e < n) {
+                        p[k + e] = wbar[i * N + e];
+                        p[other + k + e] = bbar[i * N + e];
+                    }
             }
         }
     }
 }
 
-// wbar, bbar <- the sums over the `parts` rows of partial[2][parts][n]: 64 columns a workgroup, 16 waves share the parts
-template <typename T> __global__ __launch_bounds__(1024) void norm_param_sum(const acc_t<T>* partial, int64_t parts, int64_t n,
-                                                                            T* wbar, T* bbar) {
+// wbar, bbar <- the sums over the `parts` rows of partial[2][parts][n]: COLS columns a workgroup, whose threads share the parts
+template <typename T, int COLS> __global__ __launch_bounds__(1024) void norm_param_sum(const acc_t<T>* partial, int64_t parts, int64_t n,
+                                                                                      T* wbar, T* bbar) {
     typedef acc_t<T> A;
-    __shared__ A red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t k = (int64_t)blockIdx.x * 64 + lane;
-    const A* p = partial + (int64_t)blockIdx.y * parts * n;
-    A s = 0;
-    if (k < n)
-        for (int64_t i = w; i < parts; i += 16) s += p[i * n + k];
-    red[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && k < n) {
+    constexpr int SLICES = 1024 / COLS;
+    __shared__ A red[SLICES][COLS];
+    const int c = threadIdx.x % COLS, w = threadIdx.x / COLS;
+    const int64_t k = (int64_t)blockIdx.x * COLS + c;
+    const A* p = partial + (int64_t)blockIdx.y * parts * n + k;
+    A s[4] = {0, 0, 0, 0};
+    if (k < n) {
+        int64_t i = w;
+        for (; i + 7 * SLICES < parts; i += 8 * SLICES) {
+            A v[8];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][lane];
-        (blockIdx.y ? bbar : wbar)[k] = (T)s;
+            for (int u = 0; u < 8; ++u) v[u] = p[(i + u * SLICES) * n];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[u & 3] += v[u];
+        }
+        for (; i < parts; i += SLICES) s[0] += p[i * n];
     }
+    red[w][c] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (w || k >= n) return;
+    A t = red[0][c];
+#pragma unroll
+    for (int i = 1; i < SLICES; ++i) t += red[i][c];
+    (blockIdx.y ? bbar : wbar)[k] = (T)t;
 }
 
 // ---- rows cut into pieces ---------------------------------------------------------------------------------------------
@@ -181,28 +258,28 @@ constexpr int LONG_ITER = 8; // a sweep of a workgroup: 256 threads x 8 vectors 
 template <typename T> constexpr int64_t long_sweep() { return (int64_t)LONG_THREADS * LONG_ITER * Vec16<T>::N; }
 
 // Statistics of piece blockIdx.x of row blockIdx.y: partial[row][piece] = (c, sum (x - c), sum (x - c)^2) with c the mean of
-// the piece's first sweep, as rounded. Sums about a value near the piece's mean keep what a level far from zero would take
+// the piece's first values, as rounded. Sums about a value near the piece's mean keep what a level far from zero would take
 // from them, and they join without the error of a rounded piece's mean: about any other m,
 // sum (x - m)^2 = sum (x - c)^2 + 2 (c - m) sum (x - c) + n (c - m)^2.
 template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_stats(NormArgs a) {
     typedef acc_t<T> A;
-    constexpr int K = LONG_ITER * Vec16<T>::N;
+    constexpr int N = Vec16<T>::N, K = LONG_ITER * N;
     __shared__ A red[LONG_THREADS / 64 * 2];
     const int t = threadIdx.x;
     const T* x = (const T*)a.x + (int64_t)blockIdx.y * a.width;
     const int64_t k0 = (int64_t)blockIdx.x * a.piece, k1 = k0 + a.piece < a.width ? k0 + a.piece : a.width;
+    // each wave sums the first 64 vectors (or what there is of them) for itself
+    const int64_t lead = k1 - k0 < 64 * N ? k1 - k0 : 64 * N;
+    RowRegs<T, 64, 1> r0;
+    r0.load(x + k0, lead, t & 63);
     A c = 0, s[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < N; ++j) c += r0.v[j];
+    c = wave_sum(c) / (A)lead;
     for (int64_t k = k0; k < k1; k += long_sweep<T>()) {
         const int64_t n = k1 - k < long_sweep<T>() ? k1 - k : long_sweep<T>();
         RowRegs<T, LONG_THREADS, LONG_ITER> r;
         r.load(x + k, n, t);
-        if (k == k0) {
-            A m[1] = {0};
-#pragma unroll
-            for (int j = 0; j < K; ++j) m[0] += r.v[j];
-            row_sum<LONG_THREADS>(m, red, false);
-            c = m[0] / (A)n;
-        }
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const A d = RowRegs<T, LONG_THREADS, LONG_ITER>::inside(j, n, t) ? r.v[j] - c : (A)0;
@@ -219,50 +296,53 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
     }
 }
 
-// The row's statistics from its pieces' (every workgroup for itself, in the same order), then the second sweep.
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a) {
+// mean and rstd of a row from its pieces', one workgroup a row
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_join(NormArgs a, int pieces) {
     typedef acc_t<T> A;
-    constexpr int K = LONG_ITER * Vec16<T>::N;
     __shared__ A red[LONG_THREADS / 64];
     const int t = threadIdx.x;
-    const A* p = (const A*)a.partial + (int64_t)blockIdx.y * gridDim.x * 3;
+    const A* p = (const A*)a.partial + (int64_t)blockIdx.x * pieces * 3;
+    const A whole = (A)a.piece, tail = (A)(a.width - (int64_t)(pieces - 1) * a.piece); // values of a piece, of the last
     A s[1] = {0};
-    const A whole = (A)a.piece, tail = (A)(a.width - (int64_t)(gridDim.x - 1) * a.piece); // values of a piece, of the last
-    for (int i = t; i < (int)gridDim.x; i += LONG_THREADS) s[0] += (i + 1 < (int)gridDim.x ? whole : tail) * p[3 * i] + p[3 * i + 1];
+    for (int i = t; i < pieces; i += LONG_THREADS) s[0] += (i + 1 < pieces ? whole : tail) * p[3 * i] + p[3 * i + 1];
     row_sum<LONG_THREADS>(s, red, false);
     const A mean = s[0] / (A)a.width;
     s[0] = 0;
-    for (int i = t; i < (int)gridDim.x; i += LONG_THREADS) {
+    for (int i = t; i < pieces; i += LONG_THREADS) {
         const A d = p[3 * i] - mean;
-        s[0] += p[3 * i + 2] + d * ((A)2 * p[3 * i + 1] + (i + 1 < (int)gridDim.x ? whole : tail) * d);
+        s[0] += p[3 * i + 2] + d * ((A)2 * p[3 * i + 1] + (i + 1 < pieces ? whole : tail) * d);
     }
     row_sum<LONG_THREADS>(s, red, true);
-    const A rstd = (A)1 / sqrt(s[0] / (A)a.width + (A)a.eps);
-    if (t == 0 && blockIdx.x == 0) {
-        ((A*)a.mean)[blockIdx.y] = mean;
-        ((A*)a.rstd)[blockIdx.y] = rstd;
+    if (t == 0) {
+        ((A*)a.mean)[blockIdx.x] = mean;
+        ((A*)a.rstd)[blockIdx.x] = (A)1 / sqrt(s[0] / (A)a.width + (A)a.eps);
     }
-    const T* x = (const T*)a.x + (int64_t)blockIdx.y * a.width;
-    T* y = (T*)a.y + (int64_t)blockIdx.y * a.width;
-    const int64_t k0 = (int64_t)blockIdx.x * a.piece, k1 = k0 + a.piece < a.width ? k0 + a.piece : a.width;
-    for (int64_t k = k0; k < k1; k += long_sweep<T>()) {
-        const int64_t n = k1 - k < long_sweep<T>() ? k1 - k : long_sweep<T>();
-        RowRegs<T, LONG_THREADS, LONG_ITER> r, w;
-        r.load(x + k, n, t);
+}
+
+// The second sweep, 32 KB a workgroup. (Taking the rows one lattice at a time, so that it finds them in the last-level cache,
+// costs more in short launches than it saves: 16 lattices of 4096 x 4096 in fp64 1350 us against 1170.)
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a) {
+    typedef acc_t<T> A;
+    constexpr int K = LONG_ITER * Vec16<T>::N;
+    const int t = threadIdx.x;
+    const int64_t row = blockIdx.y, k = (int64_t)blockIdx.x * long_sweep<T>();
+    const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+    const int64_t n = a.width - k < long_sweep<T>() ? a.width - k : long_sweep<T>();
+    RowRegs<T, LONG_THREADS, LONG_ITER> r, w;
+    r.load((const T*)a.x + row * a.width + k, n, t);
 #pragma unroll
-        for (int j = 0; j < K; ++j) r.v[j] = (r.v[j] - mean) * rstd;
-        if (a.weight) {
-            w.load((const T*)a.weight + k, n, t);
+    for (int j = 0; j < K; ++j) r.v[j] = (r.v[j] - mean) * rstd;
+    if (a.weight) {
+        w.load((const T*)a.weight + k, n, t);
 #pragma unroll
-            for (int j = 0; j < K; ++j) r.v[j] *= w.v[j];
-        }
-        if (a.bias) {
-            w.load((const T*)a.bias + k, n, t);
-#pragma unroll
-            for (int j = 0; j < K; ++j) r.v[j] += w.v[j];
-        }
-        r.store(y + k, n, t);
+        for (int j = 0; j < K; ++j) r.v[j] *= w.v[j];
     }
+    if (a.bias) {
+        w.load((const T*)a.bias + k, n, t);
+#pragma unroll
+        for (int j = 0; j < K; ++j) r.v[j] += w.v[j];
+    }
+    r.store((T*)a.y + row * a.width + k, n, t);
 }
 
 // Reverse mode, first sweep: columns [blockIdx.x * sweep, + sweep) of the rows of group blockIdx.y: the columns' gradient
@@ -373,21 +453,27 @@ struct LongPlan {
 template <typename T> LongPlan long_plan(int64_t rows, int64_t n) {
     LongPlan p;
     const int64_t sweeps = (n + long_sweep<T>() - 1) / long_sweep<T>();
-    // at most 1024 pieces a row (the second sweep's workgroups add them up, each for itself)
-    const int64_t per = (sweeps + 1023) / 1024;
+    // at most 2048 pieces a row: one row alone fills the card, and its join stays short
+    const int64_t per = (sweeps + 2047) / 2048;
     p.piece = per * long_sweep<T>();
     p.pieces = (n + p.piece - 1) / p.piece;
     p.vpieces = (n + longb_sweep<T>() - 1) / longb_sweep<T>();
     p.groups = 1;
-    while (p.groups < rows && p.groups < 256 && p.vpieces * p.groups < 1024) p.groups *= 2;
+    while (p.groups < rows && p.groups < 256 && p.vpieces * p.groups < 512) p.groups *= 2;
     if (p.groups > rows) p.groups = rows;
     return p;
 }
-int64_t row_blocks(int64_t rows) { return rows < 512 ? rows : 512; }
+// Workgroups of the reverse mode on whole rows: enough to fill the card, and at least 8 rows each where there are as many (each
+// leaves 2 n partial sums). small: four rows at a time
+int64_t row_blocks(int64_t rows, bool small) {
+    const int64_t groups = small ? (rows + 3) / 4 : rows;
+    return groups < 256 ? groups : groups < 8192 ? (groups / 8 > 256 ? groups / 8 : 256) : 1024;
+}
+template <typename T> bool small_row(int64_t n) { return n <= 128 * Vec16<T>::N; }
 
 template <typename T> size_t workspace(int64_t rows, int64_t n, bool vjp) {
     const size_t A = sizeof(acc_t<T>);
-    if (n * (int64_t)sizeof(T) <= (vjp ? VJP_ROW_BYTES : ROW_BYTES)) return vjp ? A * 2 * (size_t)(row_blocks(rows) * n) : 0;
+    if (n * (int64_t)sizeof(T) <= (vjp ? VJP_ROW_BYTES : ROW_BYTES)) return vjp ? A * 2 * (size_t)(row_blocks(rows, small_row<T>(n)) * n) : 0;
     const LongPlan p = long_plan<T>(rows, n);
     if (!vjp) return A * 3 * (size_t)(rows * p.pieces);
     return A * (2 * (size_t)(rows * p.vpieces) + 2 * (size_t)rows + (p.groups > 1 ? 2 * (size_t)(p.groups * n) : 0));
@@ -421,16 +507,17 @@ template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
         s.mean = (char*)a.mean + as * (size_t)r0;
         s.rstd = (char*)a.rstd + as * (size_t)r0;
         s.partial = (char*)a.partial + as * 3 * (size_t)(r0 * p.pieces);
-        const dim3 grid((unsigned)p.pieces, (unsigned)s.rows);
-        norm_long_stats<T><<<grid, dim3(LONG_THREADS), 0, st>>>(s);
-        norm_long_apply<T><<<grid, dim3(LONG_THREADS), 0, st>>>(s);
+        norm_long_stats<T><<<dim3((unsigned)p.pieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
+        norm_long_join<T><<<dim3((unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s, (int)p.pieces);
+        norm_long_apply<T><<<dim3((unsigned)((a.width + long_sweep<T>() - 1) / long_sweep<T>()), (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
     }
     return hipGetLastError();
 }
 
 template <typename T, int THREADS, int ITER> void launch_row_vjp(const NormArgs& a, unsigned blocks, hipStream_t st) {
-    if (a.wbar) norm_row_vjp<T, THREADS, ITER, true><<<dim3(blocks), dim3(THREADS), 0, st>>>(a);
-    else norm_row_vjp<T, THREADS, ITER, false><<<dim3(blocks), dim3(THREADS), 0, st>>>(a);
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS;
+    if (a.wbar) norm_row_vjp<T, THREADS, ITER, true><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
+    else norm_row_vjp<T, THREADS, ITER, false><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
 }
 template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
     typedef acc_t<T> A;
@@ -438,9 +525,10 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
     int64_t parts = 0;
     A* parted = (A*)a.partial;
     if (n * (int64_t)sizeof(T) <= VJP_ROW_BYTES) {
-        parts = row_blocks(a.rows);
+        parts = row_blocks(a.rows, small_row<T>(n));
         const unsigned b = (unsigned)parts;
         if (vecs <= 64) launch_row_vjp<T, 64, 1>(a, b, st);
+        else if (vecs <= 128) launch_row_vjp<T, 64, 2>(a, b, st);
         else if (vecs <= 256) launch_row_vjp<T, 256, 1>(a, b, st);
         else if (vecs <= 512) launch_row_vjp<T, 256, 2>(a, b, st);
         else if (vecs <= 1024) launch_row_vjp<T, 1024, 1>(a, b, st);
@@ -465,8 +553,10 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
         parts = p.groups > 1 ? p.groups : 0;
         parted = (A*)a.partial2;
     }
-    if (a.wbar && parts > 0)
-        norm_param_sum<T><<<dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
+    if (a.wbar && parts > 16)
+        norm_param_sum<T, 64><<<dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
+    else if (a.wbar && parts > 0)
+        norm_param_sum<T, 512><<<dim3((unsigned)((n + 511) / 512), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
     return hipGetLastError();
 }
 

@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .fft import _p, get_context
+from .fft import get_context
 
 _TYPES = {torch.float64: _lib.GPT_F64, torch.float32: _lib.GPT_F32, torch.float16: _lib.GPT_F16,
           torch.bfloat16: _lib.GPT_BF16}
@@ -41,13 +41,17 @@ def _given(x, like=None):
 
 
 def _alike(what, t, shape, dtype, device):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}; expected {tuple(shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what} has type {t.dtype}; expected {dtype}")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}; expected {device}")
     return t.contiguous()
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _wide(dtype):
@@ -67,11 +71,12 @@ def _workspace(device, name, *sizes):
 def _core(x, core_ndim):
     if core_ndim < 1 or x.ndim < core_ndim:
         raise ValueError(f"core_ndim must lie between 1 and the number of dimensions of x ({x.ndim})")
-    core = x.shape[x.ndim - core_ndim:]
+    shape = tuple(x.shape)
+    core = shape[x.ndim - core_ndim:]
     width = math.prod(core)
     if width < 1:
         raise ValueError("layer norm needs at least one value in a row")
-    return tuple(x.shape[: x.ndim - core_ndim]), tuple(core), width
+    return shape[: x.ndim - core_ndim], core, width
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, core_ndim=1):
@@ -90,8 +95,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, core_ndim=1):
     mean, rstd = torch.empty((2, *bshape), dtype=_wide(x.dtype), device=x.device).unbind(0)
     kind = _TYPES[x.dtype]
     ws, n = _workspace(x.device, "gpt_layer_norm_workspace", kind, rows, width, 0)
-    get_context(x.device).call("gpt_layer_norm", kind, _p(x), _p(weight), _p(bias), rows, width, float(eps), _p(y), _p(mean),
-                               _p(rstd), _p(ws), n)
+    get_context(x.device).call("gpt_layer_norm", kind, x.data_ptr(), _at(weight), _at(bias), rows, width, eps, y.data_ptr(),
+                               mean.data_ptr(), rstd.data_ptr(), _at(ws), n)
     return y, mean, rstd
 
 
@@ -110,11 +115,11 @@ def layer_norm_vjp(x, weight, mean, rstd, ybar, core_ndim=1, need_param_grad=Tru
     xbar = torch.empty_like(x)
     wbar = bbar = None
     if need_param_grad:
-        wbar, bbar = (torch.empty(core, dtype=x.dtype, device=x.device) for _ in range(2))
+        wbar, bbar = torch.empty((2, *core), dtype=x.dtype, device=x.device).unbind(0)
     kind = _TYPES[x.dtype]
     ws, n = _workspace(x.device, "gpt_layer_norm_workspace", kind, rows, width, 1)
-    get_context(x.device).call("gpt_layer_norm_vjp", kind, _p(x), _p(weight), _p(mean), _p(rstd), _p(ybar), rows, width,
-                               _p(xbar), _p(wbar), _p(bbar), _p(ws), n)
+    get_context(x.device).call("gpt_layer_norm_vjp", kind, x.data_ptr(), _at(weight), mean.data_ptr(), rstd.data_ptr(),
+                               ybar.data_ptr(), rows, width, xbar.data_ptr(), _at(wbar), _at(bbar), _at(ws), n)
     return xbar, wbar, bbar
 
 
@@ -122,34 +127,37 @@ def _matrix(t):
     """Two-dimensional with the last dimension contiguous, and the distance of its rows (a slice of wider rows is taken as it is)."""
     if t.ndim != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] <= 1 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-        return t, t.shape[1]
-    return t, t.stride(0)
+    rows, cols = t.shape
+    ld, one = t.stride()
+    if rows > 1 and one == 1 and ld >= cols:
+        return t, ld
+    return t.contiguous(), cols
 
 
 def _glm(y, x, alpha, beta, check):
     x = _given(x)
     beta = _given(beta, x)
-    if x.ndim < 1 or beta.ndim != 2 or beta.shape[1] != x.shape[-1] or beta.numel() == 0:
+    shape = tuple(x.shape)
+    if not shape or beta.ndim != 2 or beta.shape[1] != shape[-1] or beta.numel() == 0:
         raise ValueError(f"x has shape {tuple(x.shape)} and beta {tuple(beta.shape)}; expected (..., features) and (classes, features)")
-    if beta.dtype != x.dtype or beta.device != x.device:
+    if beta.dtype is not x.dtype or beta.device != x.device:
         raise ValueError(f"beta is {beta.dtype} on {beta.device}; expected {x.dtype} on {x.device}")
-    bshape = tuple(x.shape[:-1])
+    bshape = shape[:-1]
     if alpha is not None:
         alpha = _alike("alpha", _given(alpha, x), (beta.shape[0],), x.dtype, x.device)
     if not isinstance(y, torch.Tensor):
         y = torch.as_tensor(np.asarray(y))
-    if y.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8):
+    if y.dtype is not torch.int64 and y.dtype not in (torch.int32, torch.int16, torch.int8):
         raise ValueError(f"y has type {y.dtype}; expected integers")
-    if tuple(y.shape) != bshape:
+    if y.shape != bshape:
         raise ValueError(f"y has shape {tuple(y.shape)}; expected {bshape}")
     if y.is_cuda and y.device != x.device:
         raise ValueError(f"y is on {y.device}; expected {x.device}")
-    y = y.to(x.device, torch.int64).contiguous()
-    classes = beta.shape[0]
-    if check and y.numel() and int(y.max()) >= classes:
-        raise ValueError(f"y holds class {int(y.max())}; there are {classes}, counted from 0")
+    y = (y if y.is_cuda and y.dtype is torch.int64 else y.to(x.device, torch.int64)).contiguous()
+    if check and y.numel():
+        most = int(y.max())
+        if most >= beta.shape[0]:
+            raise ValueError(f"y holds class {most}; there are {beta.shape[0]}, counted from 0")
     return y, x, alpha, beta, bshape
 
 
@@ -166,8 +174,8 @@ def categorical_logit_glm_lpmf(y, x, alpha, beta, check=True):
     lp = torch.empty(bshape, dtype=_wide(x.dtype), device=x.device)
     kind = _TYPES[x.dtype]
     ws, n = _workspace(x.device, "gpt_categorical_logit_glm_workspace", kind, rows, features, classes, 0)
-    get_context(x.device).call("gpt_categorical_logit_glm_lpmf", kind, _p(y), _p(xm), ldx, _p(alpha), _p(bm), ldb, rows, features,
-                               classes, _p(lp), _p(ws), n)
+    get_context(x.device).call("gpt_categorical_logit_glm_lpmf", kind, y.data_ptr(), xm.data_ptr(), ldx, _at(alpha),
+                               bm.data_ptr(), ldb, rows, features, classes, lp.data_ptr(), ws.data_ptr() if n else None, n)
     return lp
 
 
@@ -188,6 +196,7 @@ def categorical_logit_glm_lpmf_vjp(y, x, alpha, beta, lpbar=None, check=True):
     betabar = torch.empty((classes, features), dtype=x.dtype, device=x.device)
     kind = _TYPES[x.dtype]
     ws, n = _workspace(x.device, "gpt_categorical_logit_glm_workspace", kind, rows, features, classes, 1)
-    get_context(x.device).call("gpt_categorical_logit_glm_lpmf_vjp", kind, _p(y), _p(xm), ldx, _p(alpha), _p(bm), ldb, _p(lpbar),
-                               rows, features, classes, _p(lp), _p(xbar), _p(alphabar), _p(betabar), _p(ws), n)
+    get_context(x.device).call("gpt_categorical_logit_glm_lpmf_vjp", kind, y.data_ptr(), xm.data_ptr(), ldx, _at(alpha),
+                               bm.data_ptr(), ldb, _at(lpbar), rows, features, classes, lp.data_ptr(), xbar.data_ptr(),
+                               _at(alphabar), betabar.data_ptr(), ws.data_ptr() if n else None, n)
     return lp, xbar, alphabar, betabar
