@@ -13,7 +13,12 @@
 // independent from entry to entry, and no larger than that of rounding the result. The rows' cotangents stay out of that
 // rounding where they can: for xbar they multiply the product's Acc rows, for betabar (whose sum runs over the rows) r
 // holds them divided by the largest of them, so that cotangents that are all alike (a sum's, a mean's) leave [v = y] exact. fp16
-// has too few exponents for the small probabilities of a large vocabulary: there r is stored times 2^14.
+// has too few exponents for the small probabilities of a large vocabulary: there r is stored times 2^14. Large products of fp32 data
+// run on the bf16 matrix cores, each value split in three (gpt_tile.h): six bf16 products, which take a little over half the time
+// of the fp32 instructions' one, at fp32's precision.
+//
+// Rows without an observation cost nothing: the others are numbered first (class_index), and their x copied side by side; all
+// that follows counts in those numbers, up to a count that only the device knows.
 #include "gpt_class_few.h"
 #include "gpt_readout.h"
 #include "gpt_tile.h"
@@ -42,29 +47,60 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
 }
 
 template <typename T> struct LogitArgs {
-    Operand<T> beta, x; // beta: the classes from v0 on
-    const T* alpha;     // from v0 on, or null
-    int64_t features, v0, classes; // classes: all of them
-    const int64_t* y;
-    int64_t tiles_v, tiles_n;
+    typedef typename T::Element E;
+    typedef typename T::Acc A;
+    Operand<E> beta, x; // beta: the classes from v0 on; x: the observed rows (x.rows: the most there can be)
+    const int* count;   // observed rows
+    const typename T::Data* alpha; // from v0 on, or null
+    int64_t features, v0, classes; // features: k of the operands; classes: all of them
+    const int* y;                  // class of an observed row; `classes` or more: none such
+    const int* row;                // its row
+    int64_t tiles_v;
     // statistics
-    acc_t<T>*part_max, *part_sum, *eta_y; // [tiles_v][rows], [tiles_v][rows], [rows]
+    A *part_max, *part_sum, *eta_y; // [tiles_v][rows], [tiles_v][rows], [rows]
     // r, and r with the rows' cotangents in the other order: [rows][ldr] and [classes of the piece][ldrt], in whole tiles
-    const acc_t<T>*lse, *lpbar;
-    T *r, *rt;
-    int64_t ldr, ldrt;
-    acc_t<T>* part_alpha; // [tiles_n][ldr] or null
-    Largest<acc_t<T>> largest;
+    const A *lse, *lpbar; // lpbar: of all rows
+    E *r, *rt;
+    int64_t ldr, ldrt, r_plane, rt_plane;
+    A* part_alpha; // [tiles_n][ldr] or null
+    Largest<A> largest;
 };
 
+// One way to run the products: data type, tile, type and number of planes of its operands
+template <typename T, typename Tl_, int PLANES_> struct Way {
+    typedef T Data;
+    typedef acc_t<T> Acc;
+    typedef Tl_ Tl;
+    typedef typename Tl::Element Element;
+    static constexpr int PLANES = PLANES_;
+    static constexpr bool WIDE = Tl::BM == 256;
+};
+
+// Two values in one word (plane p of them)
+template <typename W> __device__ __forceinline__ void words(float a, float b, uint32_t (&u)[W::PLANES]) {
+    if constexpr (W::PLANES == 3) {
+        bf16_t x[3], y[3];
+        split3(a, x[0], x[1], x[2]);
+        split3(b, y[0], y[1], y[2]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            typedef bf16_t V2 __attribute__((ext_vector_type(2)));
+            u[p] = __builtin_bit_cast(uint32_t, V2{x[p], y[p]});
+        }
+    } else u[0] = pack2<typename W::Element>(a, b);
+}
+
 // Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r.
-template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::THREADS) void class_logits(LogitArgs<T> a) {
-    typedef acc_t<T> A;
+template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) void class_logits(LogitArgs<W> a) {
+    typedef typename W::Acc A;
+    typedef typename W::Tl Tl;
     __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
     __shared__ A red[2][Tl::WM > Tl::WN ? Tl::WM : Tl::WN][Tl::BM > Tl::BN ? Tl::BM : Tl::BN];
+    const int64_t rows = *a.count, ld = a.x.rows;
     int64_t tm, tn;
-    if (!tile_place(blockIdx.x, a.tiles_v, a.tiles_n, tm, tn)) return;
+    if (!tile_place(blockIdx.x, a.tiles_v, (rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
     const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
+    a.x.rows = rows;
     Tl tl;
     tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
     const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Tl::WN, wn = (threadIdx.x >> 6) % Tl::WN;
@@ -82,7 +118,7 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j) {
             const int64_t n = n0 + Tl::col(j);
-            const int64_t y = n < a.x.rows ? a.y[n] - m0 : -1;
+            const int64_t y = n < rows ? a.y[n] - m0 : -1;
             const int at = y >= 0 && y < Tl::BM ? (int)y : -1;
             A mx = neg_inf<A>(), here = 0;
             bool mine = false; // (one lane group of one wave holds the row's class)
@@ -115,9 +151,9 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
             A mx = red[0][0][c], s = red[1][0][c];
 #pragma unroll
             for (int w = 1; w < Tl::WM; ++w) join(mx, s, red[0][w][c], red[1][w][c]);
-            if (n0 + c < a.x.rows) {
-                a.part_max[tm * a.x.rows + n0 + c] = mx;
-                a.part_sum[tm * a.x.rows + n0 + c] = s;
+            if (n0 + c < rows) {
+                a.part_max[tm * ld + n0 + c] = mx;
+                a.part_sum[tm * ld + n0 + c] = s;
             }
         }
         return;
@@ -128,14 +164,14 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
     const A largest = a.largest.get();
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
-        const int64_t n = n0 + Tl::col(j), y = n < a.x.rows ? a.y[n] : -1;
+        const int64_t n = n0 + Tl::col(j), y = n < rows ? a.y[n] : -1;
         lse[j] = y < 0 ? (A)0 : y >= a.classes ? (A)__builtin_nan("") : a.lse[n];
-        none[j] = y < 0 || lse[j] == neg_inf<A>(); // no observation, or no possible class
-        w[j] = none[j] ? (A)0 : a.lpbar ? a.lpbar[n] / largest : (A)1;
+        none[j] = y < 0 || lse[j] == neg_inf<A>(); // behind the last row, or no possible class
+        w[j] = none[j] ? (A)0 : a.lpbar ? a.lpbar[a.row[n]] / largest : (A)1;
         const int64_t from = y - a.v0 - m0;
         at[j] = y >= 0 && from >= 0 && from < Tl::BM ? (int)from : -1;
     }
-    constexpr A up = stored_scale<T>();
+    constexpr A up = stored_scale<typename W::Data>();
     A total[Tl::TM][4];
 #pragma unroll
     for (int i = 0; i < Tl::TM; ++i)
@@ -150,35 +186,47 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
                 total[i][r] += v * w[j];
             }
         }
-    if constexpr (Tl::TM == 8 && sizeof(T) == 2) {
+    if constexpr (W::WIDE) {
         // r: 16 neighbouring classes of one row a lane; rt: after the transpose, 16 neighbouring rows of one class a lane
         const int64_t mq = m0 + Tl::row(0, 0), nq = n0 + Tl::col(0);
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint4* to = reinterpret_cast<uint4*>(a.r + (nq + Tl::fragment(j)) * a.ldr + mq + 64 * h);
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const auto &c = tl.acc[4 * h + 2 * k][j], &d = tl.acc[4 * h + 2 * k + 1][j];
-                    to[k] = make_uint4(pack2<T>(c[0], c[1]), pack2<T>(c[2], c[3]), pack2<T>(d[0], d[1]), pack2<T>(d[2], d[3]));
+                    uint32_t u[4][W::PLANES];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const auto& c = tl.acc[4 * h + 2 * k + e / 2][j];
+                        words<W>(c[2 * (e & 1)], c[2 * (e & 1) + 1], u[e]);
+                    }
+#pragma unroll
+                    for (int p = 0; p < W::PLANES; ++p)
+                        *reinterpret_cast<uint4*>(a.r + p * a.r_plane + (nq + Tl::fragment(j)) * a.ldr + mq + 64 * h + 8 * k) =
+                            make_uint4(u[0][p], u[1][p], u[2][p], u[3][p]);
                 }
-            }
         const int64_t nb = nq - (lane & 3), mb = mq + (lane & 3);
 #pragma unroll
-        for (int i = 0; i < Tl::TM; ++i) {
-            uint32_t u[Tl::TN][2];
+        for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
-            for (int j = 0; j < Tl::TN; ++j) {
-                const auto& c = tl.acc[i][j];
-                u[j][0] = pack2<T>(c[0] * w[j], c[1] * w[j]);
-                u[j][1] = pack2<T>(c[2] * w[j], c[3] * w[j]);
-                transpose4(u[j][0], u[j][1]);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t lo[2][W::PLANES], hi[2][W::PLANES];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int j = 2 * h + e;
+                    const auto& c = tl.acc[i][j];
+                    words<W>(c[0] * w[j], c[1] * w[j], lo[e]);
+                    words<W>(c[2] * w[j], c[3] * w[j], hi[e]);
+                }
+#pragma unroll
+                for (int p = 0; p < W::PLANES; ++p) {
+                    transpose4(lo[0][p], hi[0][p]);
+                    transpose4(lo[1][p], hi[1][p]);
+                    *reinterpret_cast<uint4*>(a.rt + p * a.rt_plane + (mb + Tl::fragment(i)) * a.ldrt + nb + 8 * h) =
+                        make_uint4(lo[0][p], hi[0][p], lo[1][p], hi[1][p]);
+                }
             }
-            uint4* to = reinterpret_cast<uint4*>(a.rt + (mb + Tl::fragment(i)) * a.ldrt + nb);
-            to[0] = make_uint4(u[0][0], u[0][1], u[1][0], u[1][1]);
-            to[1] = make_uint4(u[2][0], u[2][1], u[3][0], u[3][1]);
-        }
     } else {
 #pragma unroll
         for (int i = 0; i < Tl::TM; ++i)
@@ -187,8 +235,8 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
 #pragma unroll
                 for (int j = 0; j < Tl::TN; ++j) {
                     const int64_t m = m0 + Tl::row(i, r), n = n0 + Tl::col(j);
-                    a.r[n * a.ldr + m] = (T)tl.acc[i][j][r];
-                    a.rt[m * a.ldrt + n] = (T)(tl.acc[i][j][r] * w[j]);
+                    a.r[n * a.ldr + m] = (typename W::Element)tl.acc[i][j][r];
+                    a.rt[m * a.ldrt + n] = (typename W::Element)(tl.acc[i][j][r] * w[j]);
                 }
     }
     if (!a.part_alpha) return;
@@ -208,17 +256,114 @@ template <typename T, typename Tl, bool STATS> __global__ __launch_bounds__(Tl::
     }
 }
 
-// lse (times log2(e) in fp32) and lp of 16 rows from their tiles' statistics, 16 slices of the tiles in parallel
-template <typename T> __global__ __launch_bounds__(256) void class_join(const acc_t<T>* part_max, const acc_t<T>* part_sum,
-                                                                       const acc_t<T>* eta_y, const int64_t* y, int64_t tiles,
-                                                                       int64_t rows, int64_t classes, acc_t<T>* lse, acc_t<T>* lp) {
-    typedef acc_t<T> A;
+// Numbers the observed rows: place[row] (-1: none), row[number], y[number] (any y that is no class as `classes`), their count; lp = 0 for
+// the others. A workgroup takes INDEX_ROWS rows and counts those before them for itself.
+constexpr int INDEX_ROWS = 4096;
+template <typename A> __global__ __launch_bounds__(1024) void class_index(const int64_t* y, int64_t rows, int64_t classes, int* place, int* row,
+                                                                         int* y_of, int* count, A* lp) {
+    __shared__ int red[2][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * INDEX_ROWS, mine = first + 4 * threadIdx.x;
+    int before = 0, n = 0;
+    for (int64_t i = threadIdx.x; i < first; i += 1024) before += y[i] >= 0;
+    int64_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[k] = mine + k < rows ? y[mine + k] : -1;
+        n += v[k] >= 0;
+    }
+    int upto = n; // of this wave's lanes up to this one
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const int o = __shfl_up(upto, k, 64);
+        if (lane >= k) upto += o;
+    }
+    before = wave_sum(before);
+    if (lane == 63) {
+        red[0][wave] = before;
+        red[1][wave] = upto;
+    }
+    __syncthreads();
+    int at = upto - n, all = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        at += red[0][k] + (k < wave ? red[1][k] : 0);
+        all += red[0][k] + red[1][k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (mine + k >= rows) continue;
+        const bool seen = v[k] >= 0;
+        place[mine + k] = seen ? at : -1;
+        if (seen) {
+            row[at] = (int)(mine + k);
+            y_of[at] = (int)(v[k] < classes ? v[k] : classes);
+            ++at;
+        } else lp[mine + k] = 0;
+    }
+    if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *count = all;
+}
+
+// The observed rows of x side by side, as operands (zeros behind their features); zeros into xbar's other rows
+template <typename W> __global__ __launch_bounds__(256) void class_gather(const typename W::Data* x, int64_t ld, int64_t rows, int64_t cols,
+                                                                         const int* place, typename W::Element* out, int64_t ldo,
+                                                                         int64_t plane, typename W::Data* xbar) {
+    typedef typename W::Data T;
+    constexpr int N = 8;
+    const int64_t per = ldo / N, total = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per, k = (i - r * per) * N;
+        const int at = place ? place[r] : (int)r;
+        if (at < 0) {
+            if (xbar)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (k + e < cols) xbar[r * cols + k + e] = (T)0;
+            continue;
+        }
+        T v[N];
+#pragma unroll
+        for (int h = 0; h < N; h += Vec16<T>::N) {
+            const auto u = tile_chunk<T>({x, ld, rows}, r, k + h, cols);
+#pragma unroll
+            for (int e = 0; e < Vec16<T>::N; ++e) v[h + e] = u[e];
+        }
+        typename W::Element* to = out + at * ldo + k;
+        if constexpr (W::PLANES == 3) {
+            typename Vec16<bf16_t>::V u[3];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                bf16_t a, b, c;
+                split3(v[e], a, b, c);
+                u[0][e] = a;
+                u[1][e] = b;
+                u[2][e] = c;
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<typename Vec16<bf16_t>::V*>(to + p * plane) = u[p];
+        } else {
+#pragma unroll
+            for (int h = 0; h < N; h += Vec16<T>::N) {
+                typename Vec16<T>::V u;
+#pragma unroll
+                for (int e = 0; e < Vec16<T>::N; ++e) u[e] = v[h + e];
+                *reinterpret_cast<typename Vec16<T>::V*>(to + h) = u;
+            }
+        }
+    }
+}
+
+// lse (times log2(e) in fp32) and lp of 16 observed rows from their tiles' statistics, 16 slices of the tiles in parallel
+template <typename A> __global__ __launch_bounds__(256) void class_join(const A* part_max, const A* part_sum, const A* eta_y, const int* y,
+                                                                       const int* row, const int* count, int64_t tiles, int64_t ld,
+                                                                       int64_t classes, A* lse, A* lp) {
     __shared__ A red[2][16][17];
     const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-    const int64_t n = (int64_t)blockIdx.x * 16 + c;
+    const int64_t n = (int64_t)blockIdx.x * 16 + c, rows = *count;
+    if ((int64_t)blockIdx.x * 16 >= rows) return;
     A mx = neg_inf<A>(), s = 0;
     if (n < rows)
-        for (int64_t i = k; i < tiles; i += 16) join(mx, s, part_max[i * rows + n], part_sum[i * rows + n]);
+        for (int64_t i = k; i < tiles; i += 16) join(mx, s, part_max[i * ld + n], part_sum[i * ld + n]);
     red[0][k][c] = mx;
     red[1][k][c] = s;
     __syncthreads();
@@ -226,85 +371,112 @@ template <typename T> __global__ __launch_bounds__(256) void class_join(const ac
     for (int i = 1; i < 16; ++i) join(mx, s, red[0][i][c], red[1][i][c]);
     const int64_t yn = y[n];
     A l;
-    lp[n] = row_lp(yn, classes, mx, s, yn >= 0 && yn < classes ? eta_y[n] : (A)0, l);
+    lp[row[n]] = row_lp(yn, classes, mx, s, yn < classes ? eta_y[n] : (A)0, l);
     if (lse) lse[n] = l;
 }
 
-// out[c][r] = in[r][c], rows behind the last, and (y given) those without an observation, zero. 64 x 64 through LDS
-template <typename T> __global__ __launch_bounds__(256) void class_transpose(const T* in, int64_t ld, int64_t rows, int64_t cols,
-                                                                            const int64_t* y, T* out, int64_t ldo) {
-    __shared__ T tile[64][65];
+// out[c][r] = in[row[r]][c] as operands (row null: r itself), zeros behind the last row up to ldo. 64 x 64 through LDS; each side in
+// vectors of eight
+template <typename W> __global__ __launch_bounds__(256) void class_transpose(const typename W::Data* in, int64_t ld, int64_t rows,
+                                                                            const int* count, int64_t cols, const int* row,
+                                                                            typename W::Element* out, int64_t ldo, int64_t plane) {
+    typedef typename W::Data T;
+    __shared__ T tile[64][66];
     const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int i = w; i < 64; i += 4) {
-        const int64_t r = r0 + i, c = c0 + lane;
-        tile[i][lane] = r < rows && c < cols && !(y && y[r] < 0) ? in[r * ld + c] : (T)0;
+    if (count) rows = *count;
+    const int a = threadIdx.x >> 3, b = 8 * (threadIdx.x & 7);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t r = r0 + a + 32 * h;
+        const T* from = r < rows ? in + (row ? row[r] : r) * ld : nullptr;
+#pragma unroll
+        for (int k = 0; k < 8; k += Vec16<T>::N) {
+            typename Vec16<T>::V v = {};
+            if (from) v = tile_chunk<T>({from, ld, 1}, 0, c0 + b + k, cols);
+#pragma unroll
+            for (int e = 0; e < Vec16<T>::N; ++e) tile[a + 32 * h][b + k + e] = v[e];
+        }
     }
     __syncthreads();
-    for (int i = w; i < 64; i += 4) {
-        const int64_t c = c0 + i, r = r0 + lane;
-        if (c < cols && r < ldo) out[c * ldo + r] = tile[lane][i];
-    }
-}
-
-// out[r][0..ldo) = in[r][0..cols), zeros behind: rows that start on 16 bytes and end with a step of k
-template <typename T> __global__ __launch_bounds__(256) void class_align(const T* in, int64_t ld, int64_t rows, int64_t cols, T* out,
-                                                                        int64_t ldo) {
-    constexpr int N = Vec16<T>::N;
-    const int64_t per = ldo / N, count = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per, k = (i - r * per) * N;
-        *reinterpret_cast<typename Vec16<T>::V*>(out + r * ldo + k) = tile_chunk<T>({in, ld, rows}, r, k, cols);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t c = c0 + a + 32 * h, r = r0 + b;
+        if (c >= cols || r >= ldo) continue;
+        typename W::Element* to = out + c * ldo + r;
+        if constexpr (W::PLANES == 3) {
+            typename Vec16<bf16_t>::V u[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bf16_t x, y, z;
+                split3(tile[b + e][a + 32 * h], x, y, z);
+                u[0][e] = x;
+                u[1][e] = y;
+                u[2][e] = z;
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<typename Vec16<bf16_t>::V*>(to + p * plane) = u[p];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k += Vec16<T>::N) {
+                typename Vec16<T>::V u;
+#pragma unroll
+                for (int e = 0; e < Vec16<T>::N; ++e) u[e] = tile[b + k + e][a + 32 * h];
+                *reinterpret_cast<typename Vec16<T>::V*>(to + k) = u;
+            }
+        }
     }
 }
 
 // The products with r: out[n][m] = sum_k A[m][k] B[n][k] over this launch's share of k.
-template <typename T> struct ProductArgs {
-    Operand<T> A, B;
-    int64_t K, share; // k of one split (a multiple of the tile's step)
-    int64_t tiles_m, tiles_n;
-    acc_t<T>* acc; // [splits][B.rows][A.rows]: sums so far
+template <typename T, typename E> struct ProductArgs {
+    typedef acc_t<T> Acc;
+    Operand<E> A, B;
+    int64_t K;        // (betabar: the observed rows', rounded up to k_edge)
+    int64_t k_edge;
+    const int* count; // observed rows: B's rows (xbar), or k (betabar)
+    int64_t tiles_m;
+    Acc* acc;      // [splits][B.rows][A.rows]: sums so far
     int64_t plane; // elements from one split's sums to the next
     T* out;        // the result, where this launch completes it; else null
     int64_t ldo;
     bool add; // acc holds earlier launches' sums
-    // xbar: B's rows are the rows of x, each times its cotangent (zero without an observation). betabar: y null
-    const int64_t* y;
-    const acc_t<T>* lpbar;
-    Largest<acc_t<T>> largest;
+    // xbar: B's rows are the observed rows, each times its cotangent, and go where row says. betabar: row null
+    const int* row;
+    const Acc* lpbar;
+    Largest<Acc> largest;
 };
-template <typename T, typename Tl> __global__ __launch_bounds__(Tl::THREADS) void class_product(ProductArgs<T> a) {
-    typedef acc_t<T> A;
+template <typename W> __global__ __launch_bounds__(W::Tl::THREADS) void class_product(ProductArgs<typename W::Data, typename W::Element> a) {
+    typedef typename W::Acc A;
+    typedef typename W::Data T;
+    typedef typename W::Tl Tl;
     __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
+    if (a.row) a.B.rows = *a.count;
+    else a.K = (*a.count + a.k_edge - 1) / a.k_edge * a.k_edge;
     int64_t tm, tn;
-    if (!tile_place(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn)) return;
-    const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
-    const int64_t k0 = (int64_t)blockIdx.y * a.share, k1 = k0 + a.share < a.K ? k0 + a.share : a.K;
+    if (!tile_place(blockIdx.x, a.tiles_m, (a.B.rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
+    const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN, step = tile_k<typename W::Element>();
+    const int64_t share = ((a.K + gridDim.y - 1) / gridDim.y + step - 1) / step * step;
+    const int64_t k0 = (int64_t)blockIdx.y * share, k1 = k0 + share < a.K ? k0 + share : a.K;
     Tl tl;
     tl.run(a.A, m0, a.B, n0, k0, k1, lds);
     A* acc = a.acc + (int64_t)blockIdx.y * a.plane;
-    const A largest = a.y ? (A)1 : a.largest.get();
+    const A largest = a.row ? (A)1 : a.largest.get();
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
         const int64_t n = n0 + Tl::col(j);
         if (n >= a.B.rows) continue;
-        A back = largest;
-        bool none = false;
-        if (a.y) {
-            none = a.y[n] < 0;
-            if (a.lpbar && !none) back = a.lpbar[n];
-        }
-        back /= (A)stored_scale<T>();
-        if constexpr (Tl::TM == 8) {
+        const int64_t to = a.row ? a.row[n] : n;
+        const A back = (a.row && a.lpbar ? a.lpbar[to] : largest) / (A)stored_scale<T>();
+        if constexpr (W::WIDE) {
             // 16 neighbouring values a lane: whole vectors where the rows of the result allow them
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int64_t m = m0 + Tl::row(4 * h, 0);
                 A v[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = none ? (A)0 : tl.acc[4 * h + k / 4][j][k % 4] * back;
+                for (int k = 0; k < 16; ++k) v[k] = tl.acc[4 * h + k / 4][j][k % 4] * back;
                 A* s = acc + n * a.A.rows + m;
-                T* o = a.out + n * a.ldo + m;
+                T* o = a.out + to * a.ldo + m;
                 if (m + 16 <= a.A.rows) {
                     if (a.add) {
 #pragma unroll
@@ -348,30 +520,32 @@ template <typename T, typename Tl> __global__ __launch_bounds__(Tl::THREADS) voi
                 for (int r = 0; r < 4; ++r) {
                     const int64_t m = m0 + Tl::row(i, r);
                     if (m >= a.A.rows) continue;
-                    A v = none ? (A)0 : tl.acc[i][j][r] * back;
+                    A v = tl.acc[i][j][r] * back;
                     if (a.add) v += acc[n * a.A.rows + m];
-                    if (a.out) a.out[n * a.ldo + m] = (T)v;
+                    if (a.out) a.out[to * a.ldo + m] = (T)v;
                     else acc[n * a.A.rows + m] = v;
                 }
         }
     }
 }
-// out[i] <- sum over the splits
-template <typename T> __global__ __launch_bounds__(256) void class_join_splits(const acc_t<T>* acc, int splits, int64_t plane,
-                                                                              int64_t count, T* out) {
+// out[row[n]][0..cols) <- sum over the splits (row null: all `rows` rows, else the observed ones)
+template <typename T> __global__ __launch_bounds__(256) void class_join_splits(const acc_t<T>* acc, int splits, int64_t plane, int64_t rows,
+                                                                              int64_t cols, const int* count, const int* row, T* out) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= count) return;
-    acc_t<T> s = acc[i];
-    for (int k = 1; k < splits; ++k) s += acc[k * plane + i];
-    out[i] = (T)s;
+    if (i >= (row ? *count : rows) * cols) return;
+    acc_t<T> s = 0;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += acc[k * plane + i];
+    const int64_t n = i / cols;
+    out[row ? row[n] * cols + (i - n * cols) : i] = (T)s;
 }
 // alphabar of a piece from the tiles' sums: 64 classes a workgroup, 4 waves share the tiles. acc: sums over row blocks
-template <typename T> __global__ __launch_bounds__(256) void class_alpha(const acc_t<T>* part, int64_t tiles, int64_t ld, int64_t nv,
-                                                                        acc_t<T>* acc, bool add, T* out) {
+template <typename T> __global__ __launch_bounds__(256) void class_alpha(const acc_t<T>* part, const int* count, int64_t edge, int64_t ld,
+                                                                        int64_t nv, acc_t<T>* acc, bool add, T* out) {
     typedef acc_t<T> A;
     __shared__ A red[4][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t v = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t v = (int64_t)blockIdx.x * 64 + lane, tiles = (*count + edge - 1) / edge;
     A s = 0;
     if (v < nv)
         for (int64_t i = w; i < tiles; i += 4) s += part[i * ld + v];
@@ -403,7 +577,6 @@ int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
 constexpr int64_t ROW_BLOCK = 1 << 18;              // rows taken at a time
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20; // r in both orders, of a piece of the classes and a block of the rows
 constexpr int64_t FILL = 512;                       // workgroups that fill the card
-constexpr int64_t EDGE = 256;                       // the largest tile's edge
 constexpr int64_t WIDE_TILES = 96;                  // wide tiles from this many on
 
 // Splits of a product's k: enough workgroups to fill the card, at least 4 steps of k each
@@ -413,39 +586,46 @@ int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
     if (s > most) s = most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
 }
-// 256 x 256 tiles for a product of m x n results?
-template <typename T> bool wide(int64_t m, int64_t n) {
-    return sizeof(T) == 2 && tiles_of(m, WideTile<T>::BM) * tiles_of(n, WideTile<T>::BN) >= WIDE_TILES;
-}
+// 256 x 256 tiles for a product of m x n results? (fp64 has no registers for them)
+template <typename T> bool wide(int64_t m, int64_t n) { return sizeof(T) < 8 && tiles_of(m, 256) * tiles_of(n, 256) >= WIDE_TILES; }
 
-template <typename T> struct Plan {
+// W: the way of the logits. The products with r take wide tiles where the logits do and there are enough of them (always with
+// planes)
+template <typename W> struct Plan {
+    typedef typename W::Data T;
+    typedef typename W::Element E;
+    static constexpr int64_t EDGE = W::Tl::BM;
     int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
     int64_t xsplits, bsplits;
+    bool copy; // beta as operands of its own
     // offsets in bytes
-    size_t part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
+    size_t place, row, y, count, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
+    static bool product_wide(int64_t m, int64_t n) { return W::WIDE && (W::PLANES == 3 || wide<T>(m, n)); }
     Plan(int64_t rows, int64_t features, int64_t classes, bool vjp) {
-        const size_t A = sizeof(acc_t<T>), E = sizeof(T);
+        const size_t A = sizeof(acc_t<T>), S = sizeof(E) * W::PLANES;
         block = rows < ROW_BLOCK ? rows : ROW_BLOCK;
         blocks = tiles_of(rows, block);
-        tiles_v = tiles_of(classes, SmallTile<T>::BM);
-        tiles_n = tiles_of(block, SmallTile<T>::BN);
+        tiles_v = tiles_of(classes, EDGE);
+        tiles_n = tiles_of(block, EDGE);
         size_t at = 0;
         auto take = [&](size_t n) {
             const size_t p = at;
             at += (n + 255) / 256 * 256;
             return p;
         };
+        place = take(4 * (size_t)block);
+        row = take(4 * (size_t)block);
+        y = take(4 * (size_t)block);
+        count = take(4);
         part_max = take(A * (size_t)(tiles_v * block));
         part_sum = take(A * (size_t)(tiles_v * block));
         eta_y = take(A * (size_t)block);
-        ldk = 0;
-        if (wide<T>(classes, block) && features * E % 16) { // copies whose rows start on 16 bytes
-            ldk = up_to(features, tile_k<T>());
-            xa = take(E * (size_t)(block * ldk));
-            ba = take(E * (size_t)(classes * ldk));
-        }
+        ldk = up_to(features, tile_k<E>());
+        xa = take(S * (size_t)(block * ldk));
+        copy = W::PLANES == 3 || (W::WIDE && features * sizeof(T) % 16);
+        if (copy) ba = take(S * (size_t)(classes * ldk));
         if (vjp) {
-            piece = PIECE_BYTES / (int64_t)(2 * E) / up_to(block, EDGE) / EDGE * EDGE;
+            piece = PIECE_BYTES / (int64_t)(2 * S) / up_to(block, EDGE) / EDGE * EDGE;
             if (piece < EDGE) piece = EDGE;
             if (piece > up_to(classes, EDGE)) piece = up_to(classes, EDGE);
             pieces = tiles_of(classes, piece);
@@ -455,10 +635,10 @@ template <typename T> struct Plan {
             ldrt = up_to(block, EDGE);
             lse = take(A * (size_t)block);
             scale = take(A * SCALE_PARTS);
-            r = take(E * (size_t)(ldrt * ldr));
-            rt = take(E * (size_t)(ldr * ldrt));
-            xt = take(E * (size_t)(features * ldrt));
-            bt = take(E * (size_t)(features * ldr));
+            r = take(S * (size_t)(ldrt * ldr));
+            rt = take(S * (size_t)(ldr * ldrt));
+            xt = take(S * (size_t)(features * ldrt));
+            bt = take(S * (size_t)(features * ldr));
             part_alpha = take(A * (size_t)(tiles_n * ldr));
             alpha_acc = blocks > 1 ? take(A * (size_t)classes) : 0;
             xsplits = product_splits(features, block, piece);
@@ -470,55 +650,141 @@ template <typename T> struct Plan {
         bytes = at;
     }
     static int64_t product_splits(int64_t m, int64_t n, int64_t K) {
-        const int64_t edge = wide<T>(m, n) ? WideTile<T>::BM : SmallTile<T>::BM;
-        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * (wide<T>(m, n) ? 2 : 1), K, tile_k<T>());
+        const bool large = product_wide(m, n);
+        const int64_t edge = large ? 256 : 128;
+        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * (large ? 2 : 1), K, tile_k<E>());
     }
 };
 
-template <typename T, typename Tl> void logits(LogitArgs<T> l, bool stats, hipStream_t st) {
+template <typename W, bool STATS> void logits(LogitArgs<W> l, hipStream_t st) {
+    typedef typename W::Tl Tl;
     l.tiles_v = tiles_of(l.beta.rows, Tl::BM);
-    l.tiles_n = tiles_of(l.x.rows, Tl::BN);
-    const dim3 grid(tile_grid(l.tiles_v, l.tiles_n));
-    if (stats) class_logits<T, Tl, true><<<grid, dim3(Tl::THREADS), 0, st>>>(l);
-    else class_logits<T, Tl, false><<<grid, dim3(Tl::THREADS), 0, st>>>(l);
-}
-// -> edge of the tiles taken
-template <typename T> int64_t logits_any(const LogitArgs<T>& l, bool use_wide, bool stats, hipStream_t st) {
-    if constexpr (sizeof(T) == 2) {
-        if (use_wide) {
-            logits<T, WideTile<T>>(l, stats, st);
-            return WideTile<T>::BM;
-        }
-    }
-    logits<T, SmallTile<T>>(l, stats, st);
-    return SmallTile<T>::BM;
+    class_logits<W, STATS><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
-template <typename T> hipError_t product(ProductArgs<T> p, int64_t splits, bool last, T* out, hipStream_t st) {
-    p.share = up_to(tiles_of(p.K, splits), tile_k<T>());
+template <typename W> hipError_t product(ProductArgs<typename W::Data, typename W::Element> p, int64_t splits, bool last,
+                                         typename W::Data* out, hipStream_t st) {
+    typedef typename W::Data T;
     p.out = last && splits == 1 ? out : nullptr;
     p.ldo = p.A.rows;
-    bool done = false;
-    if constexpr (sizeof(T) == 2) {
-        typedef WideTile<T> Tl;
-        if (wide<T>(p.A.rows, p.B.rows)) {
-            p.tiles_m = tiles_of(p.A.rows, Tl::BM);
-            p.tiles_n = tiles_of(p.B.rows, Tl::BN);
-            class_product<T, Tl><<<dim3(tile_grid(p.tiles_m, p.tiles_n), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
-            done = true;
+    auto run = [&](auto way) {
+        typedef decltype(way) U;
+        typedef typename U::Tl Tl;
+        p.tiles_m = tiles_of(p.A.rows, Tl::BM);
+        class_product<U><<<dim3(tile_grid(p.tiles_m, tiles_of(p.B.rows, Tl::BN)), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
+    };
+    if constexpr (W::PLANES == 3) run(W());
+    else if constexpr (W::WIDE) {
+        if (Plan<W>::product_wide(p.A.rows, p.B.rows)) run(W());
+        else run(Way<T, SmallTile<T>, 1>());
+    } else run(W());
+    if (last && splits > 1)
+        class_join_splits<T><<<dim3((unsigned)tiles_of(p.A.rows * p.B.rows, 256)), dim3(256), 0, st>>>(p.acc, (int)splits, p.plane, p.B.rows,
+                                                                                                      p.A.rows, p.count, p.row, out);
+    return hipGetLastError();
+}
+
+template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipStream_t st) {
+    typedef typename W::Data T;
+    typedef typename W::Element E;
+    typedef acc_t<T> A;
+    constexpr int64_t EDGE = W::Tl::BM;
+    const Plan<W> p(c.rows, c.features, c.classes, vjp);
+    char* ws = (char*)c.ws;
+    const int64_t D = c.features, V = c.classes;
+    hipError_t e;
+    int *place = (int*)(ws + p.place), *row = (int*)(ws + p.row), *count = (int*)(ws + p.count);
+    Operand<E> beta;
+    int64_t K = D;
+    if (p.copy) {
+        E* to = (E*)(ws + p.ba);
+        class_gather<W><<<dim3(2048), dim3(256), 0, st>>>((const T*)c.beta, c.ldbeta, V, D, nullptr, to, p.ldk, V * p.ldk, nullptr);
+        beta = {to, p.ldk, V, V * p.ldk};
+        K = p.ldk;
+    } else beta = {(const E*)c.beta, c.ldbeta, V, 0};
+    Largest<A> largest = {nullptr};
+    if (vjp && c.lpbar) {
+        largest.parts = (A*)(ws + p.scale);
+        class_scale<A><<<dim3(SCALE_PARTS), dim3(256), 0, st>>>((const A*)c.lpbar, c.y, c.rows, (A*)(ws + p.scale));
+    }
+    for (int64_t n0 = 0; n0 < c.rows; n0 += p.block) {
+        const int64_t N = c.rows - n0 < p.block ? c.rows - n0 : p.block;
+        const bool first_block = n0 == 0, last_block = n0 + N == c.rows;
+        const T* x = (const T*)c.x + n0 * c.ldx;
+        LogitArgs<W> l = {};
+        class_index<A><<<dim3((unsigned)tiles_of(N, INDEX_ROWS)), dim3(1024), 0, st>>>(c.y + n0, N, V, place, row, (int*)(ws + p.y), count,
+                                                                                      (A*)c.lp + n0);
+        E* xa = (E*)(ws + p.xa);
+        class_gather<W><<<dim3(1024), dim3(256), 0, st>>>(x, c.ldx, N, D, place, xa, p.ldk, p.block * p.ldk,
+                                                          vjp ? (T*)c.xbar + n0 * D : nullptr);
+        l.beta = beta;
+        l.x = {xa, p.ldk, N, p.block * p.ldk};
+        l.count = count;
+        l.alpha = (const T*)c.alpha;
+        l.features = K;
+        l.classes = V;
+        l.y = (const int*)(ws + p.y);
+        l.row = row;
+        l.part_max = (A*)(ws + p.part_max);
+        l.part_sum = (A*)(ws + p.part_sum);
+        l.eta_y = (A*)(ws + p.eta_y);
+        l.largest = largest;
+        logits<W, true>(l, st);
+        A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
+        class_join<A><<<dim3((unsigned)tiles_of(N, 16)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
+                                                                             tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        if (!vjp) continue;
+        const int64_t ldrt = up_to(N, EDGE); // (r is written in whole tiles)
+        E *r = (E*)(ws + p.r), *rt = (E*)(ws + p.rt), *xt = (E*)(ws + p.xt), *bt = (E*)(ws + p.bt);
+        class_transpose<W><<<dim3((unsigned)tiles_of(ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(x, c.ldx, N, count, D, row, xt,
+                                                                                                              ldrt, D * ldrt);
+        l.lse = lse;
+        l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
+        l.r = r;
+        l.rt = rt;
+        l.ldrt = ldrt;
+        l.part_alpha = c.alphabar ? (A*)(ws + p.part_alpha) : nullptr;
+        for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+            const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
+            const bool first = v0 == 0, last = v0 + nv == V;
+            l.beta = {beta.p + v0 * beta.ld, beta.ld, nv, beta.plane};
+            l.alpha = c.alpha ? (const T*)c.alpha + v0 : nullptr;
+            l.v0 = v0;
+            l.ldr = up_to(nv, EDGE);
+            l.r_plane = ldrt * l.ldr;
+            l.rt_plane = l.ldr * ldrt;
+            logits<W, false>(l, st);
+            class_transpose<W><<<dim3((unsigned)tiles_of(l.ldr, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(
+                (const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv, nullptr, D, nullptr, bt, l.ldr, D * l.ldr);
+            if (c.alphabar)
+                class_alpha<T><<<dim3((unsigned)tiles_of(nv, 64)), dim3(256), 0, st>>>(
+                    l.part_alpha, count, EDGE, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
+                    last_block ? (T*)c.alphabar + v0 : nullptr);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+            ProductArgs<T, E> x_ = {}, b_ = {};
+            x_.A = {bt, l.ldr, D, D * l.ldr};
+            x_.B = {r, l.ldr, N, l.r_plane};
+            x_.K = l.ldr;
+            x_.count = count;
+            x_.acc = (A*)(ws + p.xacc);
+            x_.plane = p.block * D;
+            x_.add = !first;
+            x_.row = row;
+            x_.lpbar = l.lpbar;
+            if ((e = product<W>(x_, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
+            b_.A = {xt, ldrt, D, D * ldrt};
+            b_.B = {rt, ldrt, nv, l.rt_plane};
+            b_.k_edge = EDGE;
+            b_.count = count;
+            b_.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
+            b_.plane = (p.blocks > 1 ? V : p.piece) * D;
+            b_.add = !first_block;
+            b_.largest = largest;
+            if ((e = product<W>(b_, p.bsplits, last_block, (T*)c.betabar + v0 * D, st)) != hipSuccess) return e;
         }
     }
-    if (!done) {
-        typedef SmallTile<T> Tl;
-        p.tiles_m = tiles_of(p.A.rows, Tl::BM);
-        p.tiles_n = tiles_of(p.B.rows, Tl::BN);
-        class_product<T, Tl><<<dim3(tile_grid(p.tiles_m, p.tiles_n), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
-    }
-    if (last && splits > 1) {
-        const int64_t count = p.A.rows * p.B.rows;
-        class_join_splits<T><<<dim3((unsigned)tiles_of(count, 256)), dim3(256), 0, st>>>(p.acc, (int)splits, p.plane, count, out);
-    }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 // ---- few rows
@@ -597,8 +863,7 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
     class_few_xbar<T, NT><<<dim3((unsigned)tiles_of(D, 16 * Vec16<T>::N), (unsigned)p.splits), dim3(256), 0, st>>>(a);
     class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits, (T*)c.xbar);
     T* xt = (T*)(ws + p.xt);
-    class_transpose<T><<<dim3((unsigned)tiles_of(p.ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(a.x.p, c.ldx, c.rows, D,
-                                                                                                            c.y, xt, p.ldrt);
+    class_few_turn<T><<<dim3((unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(a, xt);
     constexpr int NG = (NT <= 2 ? 32 : 64) / (4 * Vec16<T>::N);
     const int64_t slabs = tiles_of(D, Slab<T>::WIDTH);
     int64_t shares = tiles_of(4 * FILL, slabs);
@@ -606,109 +871,36 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
     class_few_beta<T, NG><<<dim3((unsigned)slabs, (unsigned)shares), dim3(256), 0, st>>>(a, xt, (T*)c.betabar, largest);
     return hipGetLastError();
 }
-template <typename T> size_t space(int64_t rows, int64_t features, int64_t classes, bool vjp) {
-    return rows <= FEW ? FewPlan<T>(rows, features, classes, vjp).bytes : Plan<T>(rows, features, classes, vjp).bytes;
-}
 template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStream_t st) {
     if (c.rows <= 16) return launch_few<T, 1>(c, vjp, st);
     if (c.rows <= 32) return launch_few<T, 2>(c, vjp, st);
     return launch_few<T, 4>(c, vjp, st);
 }
 
+template <typename T> struct WideWay {
+    typedef Way<T, WideTile<T>, 1> type;
+};
+template <> struct WideWay<float> {
+    typedef Way<float, WideTile<bf16_t, 3>, 3> type;
+};
+template <> struct WideWay<double> { // (never taken)
+    typedef Way<double, SmallTile<double>, 1> type;
+};
+template <typename T> size_t space(int64_t rows, int64_t features, int64_t classes, bool vjp) {
+    if (rows <= FEW) return FewPlan<T>(rows, features, classes, vjp).bytes;
+    // (an operand that does not start on 16 bytes goes the small way: its workspace is enough for both)
+    const size_t small = Plan<Way<T, SmallTile<T>, 1>>(rows, features, classes, vjp).bytes;
+    if (!wide<T>(classes, rows < ROW_BLOCK ? rows : ROW_BLOCK)) return small;
+    const size_t large = Plan<typename WideWay<T>::type>(rows, features, classes, vjp).bytes;
+    return small > large ? small : large;
+}
 template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_t st) {
-    typedef acc_t<T> A;
     if (c.rows <= FEW) return launch_few<T>(c, vjp, st);
-    const Plan<T> p(c.rows, c.features, c.classes, vjp);
-    char* ws = (char*)c.ws;
-    const int64_t D = c.features, V = c.classes;
-    hipError_t e;
-    Operand<T> beta = {(const T*)c.beta, c.ldbeta, V};
-    int64_t K = D;
-    if (p.ldk) {
-        T* to = (T*)(ws + p.ba);
-        class_align<T><<<dim3(2048), dim3(256), 0, st>>>(beta.p, beta.ld, V, D, to, p.ldk);
-        beta = {to, p.ldk, V};
-        K = p.ldk;
-    }
-    Largest<A> largest = {nullptr};
-    if (vjp && c.lpbar) {
-        largest.parts = (A*)(ws + p.scale);
-        class_scale<A><<<dim3(SCALE_PARTS), dim3(256), 0, st>>>((const A*)c.lpbar, c.y, c.rows, (A*)(ws + p.scale));
-    }
-    for (int64_t n0 = 0; n0 < c.rows; n0 += p.block) {
-        const int64_t N = c.rows - n0 < p.block ? c.rows - n0 : p.block;
-        const bool first_block = n0 == 0, last_block = n0 + N == c.rows;
-        const T* x = (const T*)c.x + n0 * c.ldx;
-        LogitArgs<T> l = {};
-        l.beta = beta;
-        l.x = {x, c.ldx, N};
-        if (p.ldk) {
-            T* to = (T*)(ws + p.xa);
-            class_align<T><<<dim3(1024), dim3(256), 0, st>>>(x, c.ldx, N, D, to, p.ldk);
-            l.x = {to, p.ldk, N};
-        }
-        bool use_wide = false;
-        if constexpr (sizeof(T) == 2) use_wide = wide<T>(V, N) && WideTile<T>::fits(l.beta) && WideTile<T>::fits(l.x);
-        l.alpha = (const T*)c.alpha;
-        l.features = K;
-        l.classes = V;
-        l.y = c.y + n0;
-        l.part_max = (A*)(ws + p.part_max);
-        l.part_sum = (A*)(ws + p.part_sum);
-        l.eta_y = (A*)(ws + p.eta_y);
-        l.largest = largest;
-        const int64_t edge = logits_any<T>(l, use_wide, true, st);
-        A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
-        class_join<T><<<dim3((unsigned)tiles_of(N, 16)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, tiles_of(V, edge), N,
-                                                                             V, lse, (A*)c.lp + n0);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-        if (!vjp) continue;
-        const int64_t ldrt = up_to(N, edge); // (r is written in whole tiles)
-        T *r = (T*)(ws + p.r), *rt = (T*)(ws + p.rt), *xt = (T*)(ws + p.xt), *bt = (T*)(ws + p.bt);
-        class_transpose<T><<<dim3((unsigned)tiles_of(ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(x, c.ldx, N, D, l.y, xt,
-                                                                                                              ldrt);
-        l.lse = lse;
-        l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
-        l.r = r;
-        l.rt = rt;
-        l.ldrt = ldrt;
-        l.part_alpha = c.alphabar ? (A*)(ws + p.part_alpha) : nullptr;
-        for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
-            const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
-            const bool first = v0 == 0, last = v0 + nv == V;
-            l.beta = {beta.p + v0 * beta.ld, beta.ld, nv};
-            l.alpha = c.alpha ? (const T*)c.alpha + v0 : nullptr;
-            l.v0 = v0;
-            l.ldr = up_to(nv, edge);
-            logits_any<T>(l, use_wide, false, st);
-            class_transpose<T><<<dim3((unsigned)tiles_of(l.ldr, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(
-                (const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv, D, nullptr, bt, l.ldr);
-            if (c.alphabar)
-                class_alpha<T><<<dim3((unsigned)tiles_of(nv, 64)), dim3(256), 0, st>>>(
-                    l.part_alpha, tiles_of(N, edge), l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
-                    last_block ? (T*)c.alphabar + v0 : nullptr);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-            ProductArgs<T> x_ = {}, b_ = {};
-            x_.A = {bt, l.ldr, D};
-            x_.B = {r, l.ldr, N};
-            x_.K = l.ldr;
-            x_.acc = (A*)(ws + p.xacc);
-            x_.plane = p.block * D;
-            x_.add = !first;
-            x_.y = l.y;
-            x_.lpbar = l.lpbar;
-            if ((e = product<T>(x_, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
-            b_.A = {xt, ldrt, D};
-            b_.B = {rt, ldrt, nv};
-            b_.K = ldrt;
-            b_.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
-            b_.plane = (p.blocks > 1 ? V : p.piece) * D;
-            b_.add = !first_block;
-            b_.largest = largest;
-            if ((e = product<T>(b_, p.bsplits, last_block, (T*)c.betabar + v0 * D, st)) != hipSuccess) return e;
-        }
-    }
-    return hipSuccess;
+    typedef typename WideWay<T>::type W;
+    typedef typename W::Element E;
+    const bool fits = W::PLANES == 3 || c.features * sizeof(T) % 16 || tile_fits(Operand<E>{(const E*)c.beta, c.ldbeta, c.classes, 0});
+    if (wide<T>(c.classes, c.rows < ROW_BLOCK ? c.rows : ROW_BLOCK) && fits) return launch_rows<W>(c, vjp, st);
+    return launch_rows<Way<T, SmallTile<T>, 1>>(c, vjp, st);
 }
 
 } // namespace

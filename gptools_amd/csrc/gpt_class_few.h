@@ -308,6 +308,18 @@ template <typename T> __global__ __launch_bounds__(256) void class_few_xbar_join
     xbar[i] = (T)(y < 0 ? (A)0 : s * ((a.lpbar ? a.lpbar[n] : (A)1) / (A)stored_scale<T>()));
 }
 
+// xt[d][n] = x[n][d] (zero without an observation, and behind the last row): 64 features a workgroup
+template <typename T> __global__ __launch_bounds__(256) void class_few_turn(FewArgs<T> a, T* xt) {
+    __shared__ T tile[FEW][66];
+    const int64_t d0 = (int64_t)blockIdx.x * 64;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int n = w; n < (int)a.ldrt; n += 4)
+        tile[n][lane] = n < a.x.rows && d0 + lane < a.features && a.y[n] >= 0 ? a.x.p[n * a.x.ld + d0 + lane] : (T)0;
+    __syncthreads();
+    for (int k = w; k < 64; k += 4)
+        if (lane < a.ldrt && d0 + k < a.features) xt[(d0 + k) * a.ldrt + lane] = tile[lane][k];
+}
+
 // betabar[v][d] = sum_n rt[v][n] x[n][d] for a slab of features and a share of the classes: the slab's x stays in registers (xt, its
 // transpose: [features][ldrt]), 16 classes at a time pass by. NG: steps of k, ldrt = NG * 4 chunks. As in WideTile the features of a
 // fragment's rows are chosen so that a lane's results lie side by side (16 bytes of them, four lanes 64).

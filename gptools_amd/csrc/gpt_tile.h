@@ -50,9 +50,21 @@ constexpr int TILE_CHUNKS = 8; // 16-byte chunks of a row in one k step
 template <typename T> constexpr int tile_k() { return TILE_CHUNKS * Vec16<T>::N; }
 
 template <typename T> struct Operand {
-    const T* p; // [rows][ld]
+    const T* p; // [rows][ld], or several planes of that
     int64_t ld, rows;
+    int64_t plane; // elements from one plane to the next
 };
+
+// fp32 as a sum of three bf16 values, each half a step (2^-8) or less of the one before (an infinity or a NaN stands in the
+// first alone). Six of the nine products of two such sums are taken, those down to 2^-16 of the whole; each one left out, and the
+// rest of the sum, is at most 2^-24, fp32's own rounding.
+__device__ __forceinline__ void split3(float v, bf16_t& a, bf16_t& b, bf16_t& c) {
+    a = (bf16_t)v;
+    const float r = v - (float)a;
+    const bool fine = r == r; // (inf - inf is not)
+    b = fine ? (bf16_t)r : (bf16_t)0.f;
+    c = fine ? (bf16_t)(r - (float)b) : (bf16_t)0.f;
+}
 
 // One 16-byte chunk, zeros where it lies outside rows x [0, k1)
 template <typename T> __device__ __forceinline__ typename Vec16<T>::V tile_chunk(const Operand<T>& o, int64_t row, int64_t k, int64_t k1) {
@@ -71,6 +83,7 @@ template <typename T> __device__ __forceinline__ typename Vec16<T>::V tile_chunk
 }
 
 template <typename T> struct SmallTile {
+    typedef T Element;
     static constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
@@ -142,7 +155,12 @@ template <typename T> struct SmallTile {
     }
 };
 
-// The same product for operands whose rows start on 16 bytes (in 16 bits and fp32): 256 x 256 of C for 8 waves, each step's 64 KB of rows taken
+// May WideTile read it? (its rows start on 16 bytes, a tile of them spans less than 4 GB)
+template <typename T> bool tile_fits(const Operand<T>& o) {
+    return ((uintptr_t)o.p & 15) == 0 && (o.ld * (int64_t)sizeof(T)) % 16 == 0 && o.ld < ((int64_t)1 << 22);
+}
+
+// The same product for operands whose rows start on 16 bytes (in 16 bits): 256 x 256 of C for 8 waves, each step's 64 KB of rows taken
 // from memory straight into LDS, two steps deep. Registers hold the fragments of the half step that is being multiplied
 // and receive those of the next half from LDS meanwhile; one barrier a step. The stay of a step:
 //   loads are issued in the middle of step s for step s + 2 (its buffer is free then: every wave holds the second half of
@@ -153,7 +171,10 @@ template <typename T> struct SmallTile {
 // holds rows 16 q .. 16 q + 15 of C in registers r of fragments 4 i' .. 4 i' + 3 (and four neighbouring lanes 16 columns), so
 // that 16 neighbouring values of a column are one lane's, and the four groups' fill 128 bytes in 16 bits. The chunks of a row
 // are swizzled by the row bits that differ within such a fragment.
-template <typename T> struct WideTile {
+//
+// PLANES == 3: the operands are fp32 values split in three (split3), and k runs through six pairs of planes.
+template <typename T, int PLANES = 1> struct WideTile {
+    typedef T Element;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
     static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
@@ -163,10 +184,6 @@ template <typename T> struct WideTile {
     static __device__ __forceinline__ int fragment(int i) { return 64 * (i >> 2) + 4 * (i & 3); } // first row of fragment i
     static constexpr int LDS_BYTES = 2 * STEP * 16;
     C acc[TM][TN];
-
-    static bool fits(const Operand<T>& o) {
-        return ((uintptr_t)o.p & 15) == 0 && (o.ld * (int64_t)sizeof(T)) % 16 == 0 && o.ld < ((int64_t)1 << 22);
-    }
 
     // bytes of row's chunk from the tile's first row on (rows behind the last repeat it: their products are not used)
     static __device__ __forceinline__ uint32_t source(const Operand<T>& o, int64_t r0, int row, int slot) {
@@ -202,7 +219,8 @@ template <typename T> struct WideTile {
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = C{0, 0, 0, 0};
-        const int64_t steps = (k1 - k0) / tile_k<T>();
+        constexpr int PAIRS = PLANES == 3 ? 6 : 1;
+        const int64_t each = (k1 - k0) / tile_k<T>(), steps = PAIRS * each; // (with planes k1 - k0 is a whole number of steps)
         // one half step: acc += a b, while a and bn take the fragments of half g of the step at `at`
         Vec a[TM];
         auto half = [&](const Vec(&b)[TN], Vec(&bn)[TN], const Vec* at, int g) {
@@ -247,29 +265,40 @@ template <typename T> struct WideTile {
                 const int id = (i & 3) * THREADS + t;
                 from[i] = source(i < 4 ? A : B, i < 4 ? m0 : n0, id / TILE_CHUNKS, id % TILE_CHUNKS);
             }
-            const T *pa = A.p + m0 * A.ld + k0, *pb = B.p + n0 * B.ld + k0;
+            const T *const a0 = A.p + m0 * A.ld + k0, *const b0_ = B.p + n0 * B.ld + k0, *pa = a0, *pb = b0_;
+            int64_t left = each;
+            int pair = 0;
+            auto onward = [&]() {
+                pa += tile_k<T>(), pb += tile_k<T>();
+                if (PLANES == 3 && --left == 0) { // pairs of planes (0,0) (0,1) (1,0) (1,1) (0,2) (2,0)
+                    left = each;
+                    ++pair;
+                    pa = a0 + (0x001102 >> 4 * (pair > 5 ? 0 : 5 - pair) & 15) * A.plane;
+                    pb = b0_ + (0x010120 >> 4 * (pair > 5 ? 0 : 5 - pair) & 15) * B.plane;
+                }
+            };
             const uint32_t to = __builtin_amdgcn_readfirstlane(
                 (uint32_t)(uintptr_t)(__attribute__((address_space(3))) Vec*)lds + (uint32_t)wave * 1024);
             take(pa, pb, from, to);
-            pa += tile_k<T>(), pb += tile_k<T>();
+            onward();
             arrive();
             if (steps > 1) take(pa, pb, from, to + STEP * 16);
-            pa += tile_k<T>(), pb += tile_k<T>();
+            onward();
             first(b0, lds);
             int side = 0;
             for (int64_t s = 0; s + 1 < steps; ++s) {
                 half(b0, b1, lds + side * STEP, 1);
                 arrive(); // step s + 1 is there, and step s is in registers to its end
                 if (s + 2 < steps) take(pa, pb, from, to + side * STEP * 16);
-                pa += tile_k<T>(), pb += tile_k<T>();
+                onward();
                 side ^= 1;
                 half(b1, b0, lds + side * STEP, 0);
             }
             half(b0, b1, lds + side * STEP, 1);
             mul(b1);
         }
-        const int64_t k = k0 + steps * tile_k<T>();
-        if (k < k1) {
+        const int64_t k = k0 + each * tile_k<T>();
+        if (PLANES == 1 && k < k1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

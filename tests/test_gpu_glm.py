@@ -246,7 +246,15 @@ def test_class_sizes(glm, name, n, d, v):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
-@pytest.mark.parametrize("n,d,v", [(40, 16, 20), (333, 100, 1000), (16, 256, 4000)])
+@pytest.mark.parametrize("n,d,v", [(700, 128, 8192), (520, 200, 8300), (1030, 65, 5003), (300, 1000, 13001), (9000, 130, 700),
+                                   (5000, 100, 1300)])
+def test_class_large_sizes(glm, name, n, d, v):
+    """Products of enough tiles for the large ones; aligned and not."""
+    _check_class(glm, name, *_class_data(name, n, d, v, seed=n + d + v, masked=0.1))
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n,d,v", [(40, 16, 20), (333, 100, 1000), (16, 256, 4000), (1500, 96, 6000)])
 @pytest.mark.parametrize("masked", [0.3, 1.0])
 def test_class_masked_rows(glm, name, n, d, v, masked):
     y, x, alpha, beta = _class_data(name, n, d, v, 7, masked)
@@ -267,7 +275,7 @@ def test_class_cotangents(glm, name, size):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
-@pytest.mark.parametrize("n,d,v", [(50, 20, 30), (70, 200, 700)])
+@pytest.mark.parametrize("n,d,v", [(50, 20, 30), (70, 200, 700), (800, 80, 7000)])
 def test_class_excluded_classes(glm, name, n, d, v):
     y, x, alpha, beta = _class_data(name, n, d, v, 13)
     alpha[1::2] = -float("inf")
@@ -296,7 +304,7 @@ def test_class_large_logits(glm, name):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
-@pytest.mark.parametrize("n,d,v", [(30, 7, 50), (65, 160, 300)])
+@pytest.mark.parametrize("n,d,v", [(30, 7, 50), (65, 160, 300), (800, 80, 7000)])
 def test_class_spoilt_rows(glm, name, n, d, v):
     y, x, alpha, beta = _class_data(name, n, d, v, 19)
     y[4] = v  # no class: refused, or NaN where the check is left out
@@ -315,11 +323,11 @@ def test_class_spoilt_rows(glm, name, n, d, v):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n,v", [(30, 210), (90, 210), (900, 6300)])
 @pytest.mark.parametrize("d", [8, 64, 100, 131])
-def test_class_strides_and_shapes(glm, name, d):
+def test_class_strides_and_shapes(glm, name, d, n, v):
     dtype = DTYPES[name]
     g = _rng(23)
-    n, v = 90, 210
     wide_x, wide_b = _normal(g, (n, d + 9), dtype), _normal(g, (v, d + 5), dtype, 1 / d**0.5)
     y = torch.randint(0, v, (n,), generator=g, device="cuda")
     x, beta = wide_x[:, 3:3 + d], wide_b[:, 1:1 + d]  # rows apart, not aligned to 16 bytes
@@ -327,9 +335,11 @@ def test_class_strides_and_shapes(glm, name, d):
     base = glm.categorical_logit_glm_lpmf_vjp(y, x.contiguous(), None, beta.contiguous())
     for got in (glm.categorical_logit_glm_lpmf_vjp(y, x, None, beta),
                 glm.categorical_logit_glm_lpmf_vjp(y.int(), x.T.contiguous().T, None, beta.T.contiguous().T),
-                glm.categorical_logit_glm_lpmf_vjp(y.view(2, 3, 15), x.reshape(2, 3, 15, d), None, beta)):
+                glm.categorical_logit_glm_lpmf_vjp(y.view(2, 3, -1), x.reshape(2, 3, -1, d), None, beta)):
         for a, b in zip(got, base):
-            assert (a is None and b is None) or torch.equal(a.reshape(b.shape), b)
+            # (rows that do not start on 16 bytes may be added up in another order: the bound above holds for both)
+            assert (a is None and b is None) or torch.allclose(a.reshape(b.shape).double(), b.double(), rtol=4 * _eps(b.dtype),
+                                                               atol=64 * _eps(b.dtype) * float(b.double().abs().max()))
 
 
 @pytest.mark.parametrize("name,n,d,v", [("f64", 262144 + 300, 3, 300), ("f64", 262144 + 1, 90, 129), ("bf16", 262144 + 129, 130, 1100)])
@@ -429,7 +439,7 @@ def _training_calls(glm, name, x, weight, bias, alpha, beta, y):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
-@pytest.mark.parametrize("n,d,v", [(60, 16, 50), (150, 192, 1000)])
+@pytest.mark.parametrize("n,d,v", [(60, 16, 50), (150, 192, 1000), (1000, 128, 6500)])
 def test_captured_and_replayed(glm, name, n, d, v):
     """A training step's calls in a graph, replayed on new data, with eager calls of other sizes in between; two graphs alive."""
     dtype = DTYPES[name]
