@@ -70,4 +70,84 @@ template <typename A> struct Largest {
     }
 };
 
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T V2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, V2{(T)a, (T)b});
+}
+
+namespace { // (a kernel of its own in each of the two)
+
+// Numbers the observed rows: row[number], y[number] (any y that is no class as `classes`), their count; behind them row lists the
+// others, whose lp is 0. place (or null): the rows' numbers, -1 where there is no observation. A workgroup takes INDEX_ROWS rows and
+// counts those before them for itself.
+constexpr int INDEX_ROWS = 4096;
+template <typename A> __global__ __launch_bounds__(1024) void class_index(const int64_t* y, int64_t rows, int64_t classes, int* place, int* row,
+                                                                         int* y_of, int* count, A* lp) {
+    __shared__ int red[2][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * INDEX_ROWS, mine = first + 4 * threadIdx.x;
+    int before = 0, n = 0;
+    for (int64_t i = threadIdx.x; i < first; i += 4096) { // (whole runs of 4096)
+        int64_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = y[i + 1024 * k];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) before += u[k] >= 0;
+    }
+    int64_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[k] = mine + k < rows ? y[mine + k] : -1;
+        n += v[k] >= 0;
+    }
+    int upto = n; // of this wave's lanes up to this one
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const int o = __shfl_up(upto, k, 64);
+        if (lane >= k) upto += o;
+    }
+    before = wave_sum(before);
+    if (lane == 63) {
+        red[0][wave] = before;
+        red[1][wave] = upto;
+    }
+    __syncthreads();
+    int at = upto - n, all = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        at += red[0][k] + (k < wave ? red[1][k] : 0);
+        all += red[0][k] + red[1][k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t i = mine + k;
+        if (i >= rows) continue;
+        const bool seen = v[k] >= 0;
+        if (place) place[i] = seen ? at : -1;
+        if (seen) {
+            row[at] = (int)i;
+            y_of[at] = (int)(v[k] < classes ? v[k] : classes);
+            ++at;
+        } else {
+            row[rows - 1 - (i - at)] = (int)i; // (i - at rows before this one have no observation)
+            lp[i] = 0;
+        }
+    }
+    if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *count = all;
+}
+
+// parts[b] = the largest |lpbar| of the observed rows that workgroup b of SCALE_PARTS takes
+template <typename A> __global__ __launch_bounds__(256) void class_scale(const A* lpbar, const int64_t* y, int64_t rows, A* parts) {
+    __shared__ A red[4];
+    A m = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += 256 * SCALE_PARTS)
+        if (y[i] >= 0) m = fmax(m, fabs(lpbar[i]));
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[blockIdx.x] = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
+}
+
+} // namespace
 } // namespace gptt

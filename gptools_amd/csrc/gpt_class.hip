@@ -41,11 +41,6 @@ __device__ __forceinline__ void transpose4(uint32_t& lo, uint32_t& hi) {
     lo = __builtin_amdgcn_perm(po, p, sel);
     hi = __builtin_amdgcn_perm(qo, q, sel);
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    typedef T V2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, V2{(T)a, (T)b});
-}
-
 template <typename T> struct LogitArgs {
     typedef typename T::Element E;
     typedef typename T::Acc A;
@@ -100,38 +95,54 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
     int64_t tm, tn;
     if (!tile_place(blockIdx.x, a.tiles_v, (rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
     const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
+    const int nv = (int)(a.beta.rows - m0 < Tl::BM ? a.beta.rows - m0 : Tl::BM); // classes of this tile
+    // what the tile's classes and rows need besides, on its way into LDS while the product runs (which ends with a barrier)
+    __shared__ A al[Tl::BM], lse_of[STATS ? 1 : Tl::BN], w_of[STATS ? 1 : Tl::BN];
+    __shared__ int at_of[Tl::BN];
+    A largest = 1;
+    if (!STATS) largest = a.largest.get();
+    for (int c = threadIdx.x; c < Tl::BM; c += Tl::THREADS)
+        al[c] = c < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + c]) : (A)0) : neg_inf<A>();
+    for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
+        const int64_t n = n0 + c, y = n < rows ? a.y[n] : -1, from = y - (a.v0 + m0);
+        at_of[c] = y >= 0 && from >= 0 && from < nv ? (int)from : -1; // the row's class within the tile
+        if (!STATS) {
+            // lse: NaN where the row's class is none, infinite (no probability) behind the last row and without a possible class
+            const A l = y < 0 ? neg_inf<A>() : y >= a.classes ? (A)__builtin_nan("") : a.lse[n];
+            const bool none = l == neg_inf<A>();
+            lse_of[c] = none ? -neg_inf<A>() : l;
+            w_of[c] = none ? (A)0 : a.lpbar ? a.lpbar[a.row[n]] / largest : (A)1;
+        }
+    }
     a.x.rows = rows;
     Tl tl;
     tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
     const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Tl::WN, wn = (threadIdx.x >> 6) % Tl::WN;
-    const int nv = (int)(a.beta.rows - m0 < Tl::BM ? a.beta.rows - m0 : Tl::BM); // classes of this tile
 #pragma unroll
     for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int m = Tl::row(i, r);
-            const A al = m < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + m]) : (A)0) : neg_inf<A>();
+            const A v = al[Tl::row(i, r)];
 #pragma unroll
-            for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + al;
+            for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + v;
         }
     if (STATS) {
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j) {
-            const int64_t n = n0 + Tl::col(j);
-            const int64_t y = n < rows ? a.y[n] - m0 : -1;
-            const int at = y >= 0 && y < Tl::BM ? (int)y : -1;
-            A mx = neg_inf<A>(), here = 0;
-            bool mine = false; // (one lane group of one wave holds the row's class)
+            const int at = at_of[Tl::col(j)];
+            A mx = neg_inf<A>();
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    mx = fmax(mx, tl.acc[i][j][r]);
-                    const bool is = Tl::row(i, r) == at;
-                    mine |= is;
-                    here = is ? tl.acc[i][j][r] : here;
-                }
-            if (mine && at < nv) a.eta_y[n] = here;
+                for (int r = 0; r < 4; ++r) mx = fmax(mx, tl.acc[i][j][r]);
+            if (at >= 0 && Tl::holds(at)) { // (few tiles hold a row's class)
+                A here = 0;
+#pragma unroll
+                for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) here = Tl::row(i, r) == at ? tl.acc[i][j][r] : here;
+                a.eta_y[n0 + Tl::col(j)] = here;
+            }
             A s = 0;
             const A ref = about(mx);
 #pragma unroll
@@ -159,17 +170,12 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
         return;
     }
     A lse[Tl::TN], w[Tl::TN];
-    bool none[Tl::TN];
     int at[Tl::TN];
-    const A largest = a.largest.get();
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
-        const int64_t n = n0 + Tl::col(j), y = n < rows ? a.y[n] : -1;
-        lse[j] = y < 0 ? (A)0 : y >= a.classes ? (A)__builtin_nan("") : a.lse[n];
-        none[j] = y < 0 || lse[j] == neg_inf<A>(); // behind the last row, or no possible class
-        w[j] = none[j] ? (A)0 : a.lpbar ? a.lpbar[a.row[n]] / largest : (A)1;
-        const int64_t from = y - a.v0 - m0;
-        at[j] = y >= 0 && from >= 0 && from < Tl::BM ? (int)from : -1;
+        lse[j] = lse_of[Tl::col(j)];
+        w[j] = w_of[Tl::col(j)];
+        at[j] = lse[j] == -neg_inf<A>() ? -1 : at_of[Tl::col(j)];
     }
     constexpr A up = stored_scale<typename W::Data>();
     A total[Tl::TM][4];
@@ -181,7 +187,7 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
 #pragma unroll
             for (int j = 0; j < Tl::TN; ++j) {
                 const A p = exp_log2e(tl.acc[i][j][r] - lse[j]);
-                const A v = none[j] ? (A)0 : (Tl::row(i, r) == at[j] ? up : (A)0) - up * p;
+                const A v = (Tl::row(i, r) == at[j] ? up : (A)0) - up * p;
                 tl.acc[i][j][r] = v;
                 total[i][r] += v * w[j];
             }
@@ -256,54 +262,6 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
     }
 }
 
-// Numbers the observed rows: place[row] (-1: none), row[number], y[number] (any y that is no class as `classes`), their count; lp = 0 for
-// the others. A workgroup takes INDEX_ROWS rows and counts those before them for itself.
-constexpr int INDEX_ROWS = 4096;
-template <typename A> __global__ __launch_bounds__(1024) void class_index(const int64_t* y, int64_t rows, int64_t classes, int* place, int* row,
-                                                                         int* y_of, int* count, A* lp) {
-    __shared__ int red[2][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t first = (int64_t)blockIdx.x * INDEX_ROWS, mine = first + 4 * threadIdx.x;
-    int before = 0, n = 0;
-    for (int64_t i = threadIdx.x; i < first; i += 1024) before += y[i] >= 0;
-    int64_t v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        v[k] = mine + k < rows ? y[mine + k] : -1;
-        n += v[k] >= 0;
-    }
-    int upto = n; // of this wave's lanes up to this one
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const int o = __shfl_up(upto, k, 64);
-        if (lane >= k) upto += o;
-    }
-    before = wave_sum(before);
-    if (lane == 63) {
-        red[0][wave] = before;
-        red[1][wave] = upto;
-    }
-    __syncthreads();
-    int at = upto - n, all = 0;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        at += red[0][k] + (k < wave ? red[1][k] : 0);
-        all += red[0][k] + red[1][k];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (mine + k >= rows) continue;
-        const bool seen = v[k] >= 0;
-        place[mine + k] = seen ? at : -1;
-        if (seen) {
-            row[at] = (int)(mine + k);
-            y_of[at] = (int)(v[k] < classes ? v[k] : classes);
-            ++at;
-        } else lp[mine + k] = 0;
-    }
-    if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *count = all;
-}
-
 // The observed rows of x side by side, as operands (zeros behind their features); zeros into xbar's other rows
 template <typename W> __global__ __launch_bounds__(256) void class_gather(const typename W::Data* x, int64_t ld, int64_t rows, int64_t cols,
                                                                          const int* place, typename W::Element* out, int64_t ldo,
@@ -353,22 +311,34 @@ template <typename W> __global__ __launch_bounds__(256) void class_gather(const 
     }
 }
 
-// lse (times log2(e) in fp32) and lp of 16 observed rows from their tiles' statistics, 16 slices of the tiles in parallel
+// lse (times log2(e) in fp32) and lp of 8 observed rows from their tiles' statistics, 32 slices of the tiles in parallel
 template <typename A> __global__ __launch_bounds__(256) void class_join(const A* part_max, const A* part_sum, const A* eta_y, const int* y,
                                                                        const int* row, const int* count, int64_t tiles, int64_t ld,
                                                                        int64_t classes, A* lse, A* lp) {
-    __shared__ A red[2][16][17];
-    const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-    const int64_t n = (int64_t)blockIdx.x * 16 + c, rows = *count;
-    if ((int64_t)blockIdx.x * 16 >= rows) return;
+    __shared__ A red[2][32][9];
+    const int c = threadIdx.x & 7, k = threadIdx.x >> 3;
+    const int64_t n = (int64_t)blockIdx.x * 8 + c, rows = *count;
+    if ((int64_t)blockIdx.x * 8 >= rows) return;
     A mx = neg_inf<A>(), s = 0;
-    if (n < rows)
-        for (int64_t i = k; i < tiles; i += 16) join(mx, s, part_max[i * ld + n], part_sum[i * ld + n]);
+    if (n < rows) {
+        int64_t i = k;
+        for (; i + 96 < tiles; i += 128) {
+            A m[4], t[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                m[u] = part_max[(i + 32 * u) * ld + n];
+                t[u] = part_sum[(i + 32 * u) * ld + n];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) join(mx, s, m[u], t[u]);
+        }
+        for (; i < tiles; i += 32) join(mx, s, part_max[i * ld + n], part_sum[i * ld + n]);
+    }
     red[0][k][c] = mx;
     red[1][k][c] = s;
     __syncthreads();
     if (k || n >= rows) return;
-    for (int i = 1; i < 16; ++i) join(mx, s, red[0][i][c], red[1][i][c]);
+    for (int i = 1; i < 32; ++i) join(mx, s, red[0][i][c], red[1][i][c]);
     const int64_t yn = y[n];
     A l;
     lp[row[n]] = row_lp(yn, classes, mx, s, yn < classes ? eta_y[n] : (A)0, l);
@@ -557,19 +527,6 @@ template <typename T> __global__ __launch_bounds__(256) void class_alpha(const a
     if (out) out[v] = (T)s;
     else acc[v] = s;
 }
-// parts[b] = the largest |lpbar| of the observed rows that workgroup b of SCALE_PARTS takes
-template <typename A> __global__ __launch_bounds__(256) void class_scale(const A* lpbar, const int64_t* y, int64_t rows, A* parts) {
-    __shared__ A red[4];
-    A m = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += 256 * SCALE_PARTS)
-        if (y[i] >= 0) m = fmax(m, fabs(lpbar[i]));
-#pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) parts[blockIdx.x] = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
-}
-
 // ---- plan -------------------------------------------------------------------------------------------------------------
 int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
@@ -597,10 +554,16 @@ template <typename W> struct Plan {
     static constexpr int64_t EDGE = W::Tl::BM;
     int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
     int64_t xsplits, bsplits;
-    bool copy; // beta as operands of its own
+    bool xwide, bwide; // wide tiles for xbar, betabar
+    bool copy;         // beta as operands of its own
     // offsets in bytes
     size_t place, row, y, count, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
-    static bool product_wide(int64_t m, int64_t n) { return W::WIDE && (W::PLANES == 3 || wide<T>(m, n)); }
+    // a product's splits of k count too: 16 rows of wide tiles with a sixteenth of a long k each fill the card as well
+    static bool product_wide(int64_t m, int64_t n, int64_t K) {
+        if (!W::WIDE || W::PLANES == 3) return W::WIDE;
+        const int64_t tiles = tiles_of(m, 256) * tiles_of(n, 256);
+        return tiles * splits_of(2 * tiles, K, 2 * tile_k<E>()) >= WIDE_TILES;
+    }
     Plan(int64_t rows, int64_t features, int64_t classes, bool vjp) {
         const size_t A = sizeof(acc_t<T>), S = sizeof(E) * W::PLANES;
         block = rows < ROW_BLOCK ? rows : ROW_BLOCK;
@@ -641,6 +604,8 @@ template <typename W> struct Plan {
             bt = take(S * (size_t)(features * ldr));
             part_alpha = take(A * (size_t)(tiles_n * ldr));
             alpha_acc = blocks > 1 ? take(A * (size_t)classes) : 0;
+            xwide = product_wide(features, block, piece);
+            bwide = product_wide(features, piece, block);
             xsplits = product_splits(features, block, piece);
             bsplits = product_splits(features, piece, block);
             xacc = xsplits > 1 || pieces > 1 ? take(A * (size_t)(xsplits * block * features)) : 0;
@@ -650,9 +615,8 @@ template <typename W> struct Plan {
         bytes = at;
     }
     static int64_t product_splits(int64_t m, int64_t n, int64_t K) {
-        const bool large = product_wide(m, n);
-        const int64_t edge = large ? 256 : 128;
-        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * (large ? 2 : 1), K, tile_k<E>());
+        const int64_t large = product_wide(m, n, K) ? 2 : 1, edge = 128 * large;
+        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * large, K, large * tile_k<E>());
     }
 };
 
@@ -662,7 +626,8 @@ template <typename W, bool STATS> void logits(LogitArgs<W> l, hipStream_t st) {
     class_logits<W, STATS><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
-template <typename W> hipError_t product(ProductArgs<typename W::Data, typename W::Element> p, int64_t splits, bool last,
+// large: wide tiles, where the logits have them
+template <typename W> hipError_t product(ProductArgs<typename W::Data, typename W::Element> p, bool large, int64_t splits, bool last,
                                          typename W::Data* out, hipStream_t st) {
     typedef typename W::Data T;
     p.out = last && splits == 1 ? out : nullptr;
@@ -675,7 +640,7 @@ template <typename W> hipError_t product(ProductArgs<typename W::Data, typename 
     };
     if constexpr (W::PLANES == 3) run(W());
     else if constexpr (W::WIDE) {
-        if (Plan<W>::product_wide(p.A.rows, p.B.rows)) run(W());
+        if (large) run(W());
         else run(Way<T, SmallTile<T>, 1>());
     } else run(W());
     if (last && splits > 1)
@@ -731,7 +696,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         l.largest = largest;
         logits<W, true>(l, st);
         A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
-        class_join<A><<<dim3((unsigned)tiles_of(N, 16)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
+        class_join<A><<<dim3((unsigned)tiles_of(N, 8)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
                                                                              tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if (!vjp) continue;
@@ -772,7 +737,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
             x_.add = !first;
             x_.row = row;
             x_.lpbar = l.lpbar;
-            if ((e = product<W>(x_, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
+            if ((e = product<W>(x_, p.xwide, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
             b_.A = {xt, ldrt, D, D * ldrt};
             b_.B = {rt, ldrt, nv, l.rt_plane};
             b_.k_edge = EDGE;
@@ -781,7 +746,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
             b_.plane = (p.blocks > 1 ? V : p.piece) * D;
             b_.add = !first_block;
             b_.largest = largest;
-            if ((e = product<W>(b_, p.bsplits, last_block, (T*)c.betabar + v0 * D, st)) != hipSuccess) return e;
+            if ((e = product<W>(b_, p.bwide, p.bsplits, last_block, (T*)c.betabar + v0 * D, st)) != hipSuccess) return e;
         }
     }
     return hipSuccess;
@@ -906,7 +871,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
 } // namespace
 
 size_t gpt_class_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, bool vjp) {
-    if (gpt_class_narrow(dtype, rows, features, classes)) return gpt_class_narrow_workspace(dtype, rows, features, classes, vjp);
+    if (gpt_class_narrow(dtype, rows, features, classes, vjp)) return gpt_class_narrow_workspace(dtype, rows, features, classes, vjp);
     switch (dtype) {
     case GPT_F64: return space<double>(rows, features, classes, vjp);
     case GPT_F32: return space<float>(rows, features, classes, vjp);
@@ -915,7 +880,7 @@ size_t gpt_class_workspace(int dtype, int64_t rows, int64_t features, int64_t cl
     }
 }
 hipError_t gpt_launch_class(int dtype, const ClassArgs& a, bool vjp, hipStream_t st) {
-    if (gpt_class_narrow(dtype, a.rows, a.features, a.classes)) return gpt_launch_class_narrow(dtype, a, vjp, st);
+    if (gpt_class_narrow(dtype, a.rows, a.features, a.classes, vjp)) return gpt_launch_class_narrow(dtype, a, vjp, st);
     switch (dtype) {
     case GPT_F64: return launch<double>(a, vjp, st);
     case GPT_F32: return launch<float>(a, vjp, st);

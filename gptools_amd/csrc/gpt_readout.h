@@ -28,6 +28,6 @@ struct ClassArgs {
 size_t gpt_class_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, bool vjp);
 hipError_t gpt_launch_class(int dtype, const ClassArgs& a, bool vjp, hipStream_t st);
 // Few features (gpt_class_narrow.hip): what the two above turn to where it applies
-bool gpt_class_narrow(int dtype, int64_t rows, int64_t features, int64_t classes);
+bool gpt_class_narrow(int dtype, int64_t rows, int64_t features, int64_t classes, bool vjp);
 size_t gpt_class_narrow_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, bool vjp);
 hipError_t gpt_launch_class_narrow(int dtype, const ClassArgs& a, bool vjp, hipStream_t st);

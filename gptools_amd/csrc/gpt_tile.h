@@ -10,12 +10,14 @@
 namespace gptt {
 
 template <typename T> struct Mma; // C fragment, product of two 16-byte chunks, row of C that register r of lane group q holds;
-                                 // mul1: of one value a lane, that of lane group q standing for k = q
+                                 // mul1: of one value a lane, that of lane group q standing for k = q; mul4: of four, k = 4 q + r
 template <> struct Mma<bf16_t> {
     typedef float C __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ C mul(Vec16<bf16_t>::V a, Vec16<bf16_t>::V b, C c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    typedef short V4 __attribute__((ext_vector_type(4))); // bf16 bits
+    static __device__ __forceinline__ C mul4(V4 a, V4 b, C c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ int row(int q, int r) { return 4 * q + r; }
 };
 template <> struct Mma<half_t> {
@@ -23,6 +25,8 @@ template <> struct Mma<half_t> {
     static __device__ __forceinline__ C mul(Vec16<half_t>::V a, Vec16<half_t>::V b, C c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
+    typedef half_t V4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ C mul4(V4 a, V4 b, C c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ int row(int q, int r) { return 4 * q + r; }
 };
 template <> struct Mma<float> {
@@ -145,6 +149,11 @@ template <typename T> struct SmallTile {
             }
             __syncthreads();
         }
+    }
+    // does this lane hold row m of C (within the tile)?
+    static __device__ __forceinline__ bool holds(int m) {
+        const int q = (threadIdx.x & 63) >> 4;
+        return m / (BM / WM) == (int)(threadIdx.x >> 6) / WN && (Mma<T>::row(1, 0) == 1 ? (m & 3) : (m >> 2 & 3)) == q;
     }
     // row of C (within the tile) of register r of fragment i; column of fragment j
     static __device__ __forceinline__ int row(int i, int r) {
@@ -313,6 +322,9 @@ template <typename T, int PLANES = 1> struct WideTile {
             mul(b0);
         }
         __syncthreads();
+    }
+    static __device__ __forceinline__ bool holds(int m) {
+        return m / (BM / WM) == (int)(threadIdx.x >> 6) / WN && (m >> 4 & 3) == (int)(threadIdx.x & 63) >> 4;
     }
     static __device__ __forceinline__ int row(int i, int r) {
         return ((int)(threadIdx.x >> 6) / WN) * (BM / WM) + fragment(i) + 16 * ((threadIdx.x & 63) >> 4) + r;
