@@ -68,7 +68,7 @@ template <typename T, typename Tl_, int PLANES_> struct Way {
     typedef Tl_ Tl;
     typedef typename Tl::Element Element;
     static constexpr int PLANES = PLANES_;
-    static constexpr bool WIDE = Tl::BM == 256;
+    static constexpr bool LINES = Tl::TN == 4 && !std::is_same<Tl, SmallTile<T>>::value; // a LineTile
 };
 
 // Two values in one word (plane p of them)
@@ -192,13 +192,13 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
                 total[i][r] += v * w[j];
             }
         }
-    if constexpr (W::WIDE) {
+    if constexpr (W::LINES) {
         // r: 16 neighbouring classes of one row a lane; rt: after the transpose, 16 neighbouring rows of one class a lane
         const int64_t mq = m0 + Tl::row(0, 0), nq = n0 + Tl::col(0);
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < Tl::TM / 4; ++h)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     uint32_t u[4][W::PLANES];
@@ -437,10 +437,10 @@ template <typename W> __global__ __launch_bounds__(W::Tl::THREADS) void class_pr
         if (n >= a.B.rows) continue;
         const int64_t to = a.row ? a.row[n] : n;
         const A back = (a.row && a.lpbar ? a.lpbar[to] : largest) / (A)stored_scale<T>();
-        if constexpr (W::WIDE) {
+        if constexpr (W::LINES) {
             // 16 neighbouring values a lane: whole vectors where the rows of the result allow them
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < Tl::TM / 4; ++h) {
                 const int64_t m = m0 + Tl::row(4 * h, 0);
                 A v[16];
 #pragma unroll
@@ -534,7 +534,7 @@ int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
 constexpr int64_t ROW_BLOCK = 1 << 18;              // rows taken at a time
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20; // r in both orders, of a piece of the classes and a block of the rows
 constexpr int64_t FILL = 512;                       // workgroups that fill the card
-constexpr int64_t WIDE_TILES = 96;                  // wide tiles from this many on
+constexpr int64_t WIDE_TILES = 192;                 // 256 x 256 tiles from this many on
 
 // Splits of a product's k: enough workgroups to fill the card, at least 4 steps of k each
 int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
@@ -543,11 +543,10 @@ int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
     if (s > most) s = most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
 }
-// 256 x 256 tiles for a product of m x n results? (fp64 has no registers for them)
-template <typename T> bool wide(int64_t m, int64_t n) { return sizeof(T) < 8 && tiles_of(m, 256) * tiles_of(n, 256) >= WIDE_TILES; }
+// 256 x 256 tiles for a product of m x n results?
+bool wide(int64_t m, int64_t n) { return tiles_of(m, 256) * tiles_of(n, 256) >= WIDE_TILES; }
 
-// W: the way of the logits. The products with r take wide tiles where the logits do and there are enough of them (always with
-// planes)
+// W: the way of the logits. The products with r take the larger tile or the smaller by themselves
 template <typename W> struct Plan {
     typedef typename W::Data T;
     typedef typename W::Element E;
@@ -558,11 +557,10 @@ template <typename W> struct Plan {
     bool copy;         // beta as operands of its own
     // offsets in bytes
     size_t place, row, y, count, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
-    // a product's splits of k count too: 16 rows of wide tiles with a sixteenth of a long k each fill the card as well
+    // (a product's splits of k count too: 16 rows of large tiles with a sixteenth of a long k each fill the card as well)
     static bool product_wide(int64_t m, int64_t n, int64_t K) {
-        if (!W::WIDE || W::PLANES == 3) return W::WIDE;
         const int64_t tiles = tiles_of(m, 256) * tiles_of(n, 256);
-        return tiles * splits_of(2 * tiles, K, 2 * tile_k<E>()) >= WIDE_TILES;
+        return W::LINES && tiles * splits_of(2 * tiles, K, 4 * tile_k<E>()) >= WIDE_TILES;
     }
     Plan(int64_t rows, int64_t features, int64_t classes, bool vjp) {
         const size_t A = sizeof(acc_t<T>), S = sizeof(E) * W::PLANES;
@@ -585,7 +583,7 @@ template <typename W> struct Plan {
         eta_y = take(A * (size_t)block);
         ldk = up_to(features, tile_k<E>());
         xa = take(S * (size_t)(block * ldk));
-        copy = W::PLANES == 3 || (W::WIDE && features * sizeof(T) % 16);
+        copy = W::PLANES == 3 || (W::LINES && features * sizeof(T) % 16);
         if (copy) ba = take(S * (size_t)(classes * ldk));
         if (vjp) {
             piece = PIECE_BYTES / (int64_t)(2 * S) / up_to(block, EDGE) / EDGE * EDGE;
@@ -616,7 +614,7 @@ template <typename W> struct Plan {
     }
     static int64_t product_splits(int64_t m, int64_t n, int64_t K) {
         const int64_t large = product_wide(m, n, K) ? 2 : 1, edge = 128 * large;
-        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * large, K, large * tile_k<E>());
+        return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * large, K, 2 * large * tile_k<E>());
     }
 };
 
@@ -626,7 +624,7 @@ template <typename W, bool STATS> void logits(LogitArgs<W> l, hipStream_t st) {
     class_logits<W, STATS><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
-// large: wide tiles, where the logits have them
+// large: 256 x 256 tiles
 template <typename W> hipError_t product(ProductArgs<typename W::Data, typename W::Element> p, bool large, int64_t splits, bool last,
                                          typename W::Data* out, hipStream_t st) {
     typedef typename W::Data T;
@@ -638,10 +636,10 @@ template <typename W> hipError_t product(ProductArgs<typename W::Data, typename 
         p.tiles_m = tiles_of(p.A.rows, Tl::BM);
         class_product<U><<<dim3(tile_grid(p.tiles_m, tiles_of(p.B.rows, Tl::BN)), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
     };
-    if constexpr (W::PLANES == 3) run(W());
-    else if constexpr (W::WIDE) {
-        if (large) run(W());
-        else run(Way<T, SmallTile<T>, 1>());
+    typedef typename W::Element E;
+    if constexpr (W::LINES) {
+        if (large) run(Way<T, WideTile<E, W::PLANES>, W::PLANES>());
+        else run(Way<T, MidTile<E, W::PLANES>, W::PLANES>());
     } else run(W());
     if (last && splits > 1)
         class_join_splits<T><<<dim3((unsigned)tiles_of(p.A.rows * p.B.rows, 256)), dim3(256), 0, st>>>(p.acc, (int)splits, p.plane, p.B.rows,
@@ -842,30 +840,46 @@ template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStr
     return launch_few<T, 4>(c, vjp, st);
 }
 
-template <typename T> struct WideWay {
-    typedef Way<T, WideTile<T>, 1> type;
+// fp32 runs in three planes of bf16; fp64 has neither the instructions nor the registers for line tiles
+template <typename T> struct Ways {
+    typedef Way<T, WideTile<T>, 1> Wide;
+    typedef Way<T, MidTile<T>, 1> Mid;
+    typedef Way<T, SmallTile<T>, 1> Other; // operands that do not start on 16 bytes
 };
-template <> struct WideWay<float> {
-    typedef Way<float, WideTile<bf16_t, 3>, 3> type;
+template <> struct Ways<float> {
+    typedef Way<float, WideTile<bf16_t, 3>, 3> Wide;
+    typedef Way<float, MidTile<bf16_t, 3>, 3> Mid;
 };
-template <> struct WideWay<double> { // (never taken)
-    typedef Way<double, SmallTile<double>, 1> type;
+template <> struct Ways<double> {
+    typedef Way<double, SmallTile<double>, 1> Other;
 };
 template <typename T> size_t space(int64_t rows, int64_t features, int64_t classes, bool vjp) {
     if (rows <= FEW) return FewPlan<T>(rows, features, classes, vjp).bytes;
-    // (an operand that does not start on 16 bytes goes the small way: its workspace is enough for both)
-    const size_t small = Plan<Way<T, SmallTile<T>, 1>>(rows, features, classes, vjp).bytes;
-    if (!wide<T>(classes, rows < ROW_BLOCK ? rows : ROW_BLOCK)) return small;
-    const size_t large = Plan<typename WideWay<T>::type>(rows, features, classes, vjp).bytes;
-    return small > large ? small : large;
+    typedef Ways<T> Y;
+    if constexpr (sizeof(T) == 8) return Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
+    else {
+        const bool large = wide(classes, rows < ROW_BLOCK ? rows : ROW_BLOCK);
+        const size_t n = large ? Plan<typename Y::Wide>(rows, features, classes, vjp).bytes : Plan<typename Y::Mid>(rows, features, classes, vjp).bytes;
+        if constexpr (sizeof(T) == 2) { // (whether beta starts on 16 bytes shows only in the call)
+            const size_t other = Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
+            return n > other ? n : other;
+        }
+        return n;
+    }
 }
 template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_t st) {
     if (c.rows <= FEW) return launch_few<T>(c, vjp, st);
-    typedef typename WideWay<T>::type W;
-    typedef typename W::Element E;
-    const bool fits = W::PLANES == 3 || c.features * sizeof(T) % 16 || tile_fits(Operand<E>{(const E*)c.beta, c.ldbeta, c.classes, 0});
-    if (wide<T>(c.classes, c.rows < ROW_BLOCK ? c.rows : ROW_BLOCK) && fits) return launch_rows<W>(c, vjp, st);
-    return launch_rows<Way<T, SmallTile<T>, 1>>(c, vjp, st);
+    typedef Ways<T> Y;
+    if constexpr (sizeof(T) == 8) return launch_rows<typename Y::Other>(c, vjp, st);
+    else {
+        if constexpr (sizeof(T) == 2) {
+            // (rows of an odd length are copied, whole ones need to start on 16 bytes where they are)
+            if (c.features * sizeof(T) % 16 == 0 && !tile_fits(Operand<T>{(const T*)c.beta, c.ldbeta, c.classes, 0}))
+                return launch_rows<typename Y::Other>(c, vjp, st);
+        }
+        return wide(c.classes, c.rows < ROW_BLOCK ? c.rows : ROW_BLOCK) ? launch_rows<typename Y::Wide>(c, vjp, st)
+                                                                         : launch_rows<typename Y::Mid>(c, vjp, st);
+    }
 }
 
 } // namespace

@@ -164,13 +164,13 @@ template <typename T> struct SmallTile {
     }
 };
 
-// May WideTile read it? (its rows start on 16 bytes, a tile of them spans less than 4 GB)
+// May a LineTile read it? (its rows start on 16 bytes, a tile of them spans less than 4 GB)
 template <typename T> bool tile_fits(const Operand<T>& o) {
     return ((uintptr_t)o.p & 15) == 0 && (o.ld * (int64_t)sizeof(T)) % 16 == 0 && o.ld < ((int64_t)1 << 22);
 }
 
-// The same product for operands whose rows start on 16 bytes (in 16 bits): 256 x 256 of C for 8 waves, each step's 64 KB of rows taken
-// from memory straight into LDS, two steps deep. Registers hold the fragments of the half step that is being multiplied
+// The same product for operands whose rows start on 16 bytes (in 16 bits): 256 x 256 of C for 8 waves or 128 x 128 for 4
+// (WideTile, MidTile), each step's rows (64 KB, 32) taken from memory straight into LDS, two steps deep. Registers hold the fragments of the half step that is being multiplied
 // and receive those of the next half from LDS meanwhile; one barrier a step. The stay of a step:
 //   loads are issued in the middle of step s for step s + 2 (its buffer is free then: every wave holds the second half of
 //   step s in registers), and must have landed in the middle of step s + 1.
@@ -182,12 +182,13 @@ template <typename T> bool tile_fits(const Operand<T>& o) {
 // are swizzled by the row bits that differ within such a fragment.
 //
 // PLANES == 3: the operands are fp32 values split in three (split3), and k runs through six pairs of planes.
-template <typename T, int PLANES = 1> struct WideTile {
+template <typename T, int PLANES, int EDGE> struct LineTile {
     typedef T Element;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
-    static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
-    static constexpr int THREADS = 512, TM = 8, TN = 4;
+    static constexpr int BM = EDGE, BN = EDGE, WM = 2, WN = EDGE / 64;
+    static constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = 4;
+    static_assert((BM + BN) * TILE_CHUNKS == 8 * THREADS, "eight loads a step, four of each operand");
     static constexpr int STEP = (BM + BN) * TILE_CHUNKS; // chunks
     static __device__ __forceinline__ int key(int row) { return (row & 3) | (row >> 2 & 4); }
     static __device__ __forceinline__ int fragment(int i) { return 64 * (i >> 2) + 4 * (i & 3); } // first row of fragment i
@@ -205,16 +206,17 @@ template <typename T, int PLANES = 1> struct WideTile {
     static __device__ __forceinline__ void take(const T* a, const T* b, const uint32_t (&from)[8], uint32_t to) {
         asm volatile("s_nop 4\n\t"
                      "s_mov_b32 m0, %10\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\t"
-                     "s_add_u32 m0, %10, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0\n\t"
-                     "s_add_u32 m0, %10, 0x4000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %0\n\t"
-                     "s_add_u32 m0, %10, 0x6000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %0\n\t"
-                     "s_add_u32 m0, %10, 0x8000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %1\n\t"
-                     "s_add_u32 m0, %10, 0xa000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %7, %1\n\t"
-                     "s_add_u32 m0, %10, 0xc000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %8, %1\n\t"
-                     "s_add_u32 m0, %10, 0xe000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %9, %1"
+                     "s_add_u32 m0, %10, %11\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0\n\t"
+                     "s_add_u32 m0, %10, %12\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %0\n\t"
+                     "s_add_u32 m0, %10, %13\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %0\n\t"
+                     "s_add_u32 m0, %10, %14\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %1\n\t"
+                     "s_add_u32 m0, %10, %15\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %7, %1\n\t"
+                     "s_add_u32 m0, %10, %16\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %8, %1\n\t"
+                     "s_add_u32 m0, %10, %17\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %9, %1"
                      :
                      : "s"(a), "s"(b), "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "v"(from[4]), "v"(from[5]),
-                       "v"(from[6]), "v"(from[7]), "s"(to)
+                       "v"(from[6]), "v"(from[7]), "s"(to), "i"(16 * THREADS), "i"(32 * THREADS), "i"(48 * THREADS),
+                       "i"(64 * THREADS), "i"(80 * THREADS), "i"(96 * THREADS), "i"(112 * THREADS)
                      : "memory", "scc"); // (m0 is the compiler's scratch: it sets it before each use of its own)
     }
     static __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -333,6 +335,9 @@ template <typename T, int PLANES = 1> struct WideTile {
         return ((int)(threadIdx.x >> 6) % WN) * (BN / WN) + fragment(j) + 16 * (threadIdx.x >> 2 & 3) + (threadIdx.x & 3);
     }
 };
+
+template <typename T, int PLANES = 1> using WideTile = LineTile<T, PLANES, 256>;
+template <typename T, int PLANES = 1> using MidTile = LineTile<T, PLANES, 128>;
 
 // Which tile a workgroup takes: workgroups go round the 8 XCDs, each of which has an L2 of its own, so each XCD takes a
 // contiguous run of tiles, and a run goes through 8 columns of tiles row by row (32 tiles at work share 4 + 8 panels).
