@@ -87,13 +87,16 @@ template <typename A> __global__ __launch_bounds__(1024) void class_index(const 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * INDEX_ROWS, mine = first + 4 * threadIdx.x;
     int before = 0, n = 0;
-    for (int64_t i = threadIdx.x; i < first; i += 4096) { // (whole runs of 4096)
-        int64_t u[4];
+    auto some = [&](int64_t i, auto runs) { // (whole runs of 4096)
+        int64_t u[4 * decltype(runs)::value];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = y[i + 1024 * k];
+        for (int k = 0; k < 4 * runs; ++k) u[k] = y[i + threadIdx.x + 1024 * k];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) before += u[k] >= 0;
-    }
+        for (int k = 0; k < 4 * runs; ++k) before += u[k] >= 0;
+    };
+    int64_t done = 0;
+    for (; done + 4 * INDEX_ROWS <= first; done += 4 * INDEX_ROWS) some(done, std::integral_constant<int, 4>());
+    for (; done < first; done += INDEX_ROWS) some(done, std::integral_constant<int, 1>());
     int64_t v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {

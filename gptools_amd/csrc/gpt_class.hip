@@ -738,7 +738,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
             if ((e = product<W>(x_, p.xwide, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
             b_.A = {xt, ldrt, D, D * ldrt};
             b_.B = {rt, ldrt, nv, l.rt_plane};
-            b_.k_edge = EDGE;
+            b_.k_edge = tile_k<E>(); // (rt and xt are zero from the last row to ldrt)
             b_.count = count;
             b_.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
             b_.plane = (p.blocks > 1 ? V : p.piece) * D;

@@ -40,9 +40,9 @@ template <typename T> struct NarrowArgs {
     int64_t share; // rows of one share
 };
 
-// Tiles of 16 that a wave takes at a time of what it walks along. (fp64 with many features, and its prefetch spread over four
-// waves' shares, has not the registers for two)
-template <typename T, int DT, int SHARES> constexpr int VT_ = sizeof(T) == 8 && DT == 4 && SHARES == 4 ? 1 : 2;
+// Tiles of 16 that a wave takes at a time of what it walks along. (fp64 and fp32 with many features, and the prefetch spread over four
+// waves' shares, have not the registers and the LDS for two)
+template <typename T, int DT, int SHARES> constexpr int VT_ = sizeof(T) >= 4 && DT == 4 && SHARES == 4 ? 1 : 2;
 
 template <typename T, int DT> struct Narrow {
     typedef acc_t<T> A;
@@ -52,8 +52,73 @@ template <typename T, int DT> struct Narrow {
     static constexpr int G = DP / (4 * N);              // 16-byte chunks of a row that a lane holds
     static constexpr int LD = DP + N;                   // a row in LDS
     static constexpr bool TURN = sizeof(T) == 2;        // a transposed copy stands in LDS too
-    // rows of a step in LDS, and what they take: the rows, and their transpose [DP][STEP + 4]
-    template <int STEP> static constexpr int stage() { return STEP * LD + (TURN ? DP * (STEP + 4) : 0); }
+    // fp32: logits on the bf16 matrix cores, each value split in three (six products of 32 features take 96 cycles, the fp32
+    // instructions of their one 256); three planes of the rows stand in LDS
+    static constexpr bool SPLIT = std::is_same<T, float>::value && DT >= 2;
+    static constexpr int SLD = DP + 8, SG = DP / 32;
+    typedef Vec16<bf16_t>::V SVec;
+    // rows of a step in LDS, and what they take: the rows, their transpose [DP][STEP + 4] or planes [3][STEP][SLD]
+    template <int STEP> static constexpr int stage() { return STEP * LD + (TURN ? DP * (STEP + 4) : SPLIT ? 3 * STEP * SLD / 2 : 0); }
+    // a lane's part of one row (its column of the logits): chunks 4 g + q
+    struct Part {
+        Vec v[SPLIT ? 1 : G];
+        SVec s[SPLIT ? 3 : 1][SPLIT ? SG : 1];
+        __device__ __forceinline__ void load(const Operand<T>& o, int64_t row, int64_t D) {
+            const int q = (threadIdx.x & 63) >> 4;
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int g = 0; g < SG; ++g)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const Vec u = tile_chunk(o, row, (int64_t)((4 * g + q) * 8 + 4 * h), D);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            bf16_t a, b, c;
+                            split3(u[e], a, b, c);
+                            s[0][g][4 * h + e] = a;
+                            s[1][g][4 * h + e] = b;
+                            s[2][g][4 * h + e] = c;
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; ++g) v[g] = tile_chunk(o, row, (int64_t)(4 * g + q) * N, D);
+            }
+        }
+        __device__ __forceinline__ void clear() {
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int g = 0; g < SG; ++g) s[0][g] = s[1][g] = s[2][g] = SVec{};
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; ++g) v[g] = Vec{};
+            }
+        }
+        // this lane's share of the dot product with another row
+        __device__ __forceinline__ A dot(const Operand<T>& o, int64_t row, int64_t D) const {
+            const int q = (threadIdx.x & 63) >> 4;
+            A t = 0;
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int g = 0; g < SG; ++g)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const Vec u = tile_chunk(o, row, (int64_t)((4 * g + q) * 8 + 4 * h), D);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            t += ((float)s[0][g][4 * h + e] + ((float)s[1][g][4 * h + e] + (float)s[2][g][4 * h + e])) * u[e];
+                    }
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const Vec u = tile_chunk(o, row, (int64_t)(4 * g + q) * N, D);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) t += (A)v[g][e] * (A)u[e];
+                }
+            }
+            return t;
+        }
+    };
     template <int STEP> static constexpr int loads() { return STEP * (DP / N) / 256 > 0 ? STEP * (DP / N) / 256 : 1; }
 
     // Rows r0.. of an operand (order given: order[r0..], rows of which y says that they are observed) into registers, and from
@@ -75,20 +140,51 @@ template <typename T, int DT> struct Narrow {
             const int id = i * 256 + threadIdx.x, r = id / (DP / N), c = id % (DP / N);
             if (r >= STEP) continue;
             *reinterpret_cast<Vec*>(lds + r * LD + c * N) = v[i];
-            if (TURN) {
+            if constexpr (TURN) {
                 T* t = lds + STEP * LD + c * N * (STEP + 4) + r;
 #pragma unroll
                 for (int e = 0; e < N; ++e) t[e * (STEP + 4)] = v[i][e];
             }
+            if constexpr (SPLIT) {
+                bf16_t* t = reinterpret_cast<bf16_t*>(lds + STEP * LD) + r * SLD + c * N;
+                typedef bf16_t V4 __attribute__((ext_vector_type(4)));
+                V4 u[3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bf16_t x, y, z;
+                    split3(v[i][e], x, y, z);
+                    u[0][e] = x;
+                    u[1][e] = y;
+                    u[2][e] = z;
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<V4*>(t + p * STEP * SLD) = u[p];
+            }
         }
     }
     // C[row base + .. of lds][column held in f] and its use as an operand
-    static __device__ __forceinline__ C logits(const T* lds, int base, const Vec (&f)[G]) {
+    template <int STEP> static __device__ __forceinline__ C logits(const T* lds, int base, const Part& f) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
         C c = {0, 0, 0, 0};
+        if constexpr (SPLIT) {
+            const bf16_t* t = reinterpret_cast<const bf16_t*>(lds + STEP * LD) + (base + (lane & 15)) * SLD;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-            c = Mma<T>::mul(*reinterpret_cast<const Vec*>(lds + (base + (lane & 15)) * LD + (4 * g + q) * N), f[g], c);
+            for (int g = 0; g < SG; ++g) {
+                SVec a[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) a[p] = *reinterpret_cast<const SVec*>(t + p * STEP * SLD + (4 * g + q) * 8);
+                c = Mma<bf16_t>::mul(a[2], f.s[0][g], c); // (the smallest first)
+                c = Mma<bf16_t>::mul(a[0], f.s[2][g], c);
+                c = Mma<bf16_t>::mul(a[1], f.s[1][g], c);
+                c = Mma<bf16_t>::mul(a[1], f.s[0][g], c);
+                c = Mma<bf16_t>::mul(a[0], f.s[1][g], c);
+                c = Mma<bf16_t>::mul(a[0], f.s[0][g], c);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                c = Mma<T>::mul(*reinterpret_cast<const Vec*>(lds + (base + (lane & 15)) * LD + (4 * g + q) * N), f.v[g], c);
+        }
         return c;
     }
     template <int STEP> static __device__ __forceinline__ void gather(const T* lds, int base, const C& p, C (&o)[DT]) {
@@ -128,7 +224,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
     typedef typename W::A A;
     typedef typename W::C C;
     typedef typename W::Vec Vec;
-    constexpr int VT = VT_<T, DT, WV>, STEP = 16 * VT * WV, ROWS = 16 * NT * WR, N = W::N;
+    constexpr int VT = VT_<T, DT, WV>, STEP = 16 * VT * WV, ROWS = 16 * NT * WR;
     constexpr int STAGE = W::template stage<STEP>() * (int)sizeof(T), SPILL = VJP ? WV * ROWS * W::OLD * (int)sizeof(A) : 0;
     __shared__ uint4 room[(larger(STAGE, SPILL) + 15) / 16];
     __shared__ __attribute__((aligned(16))) A al[STEP];
@@ -144,7 +240,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
             }
         return;
     }
-    Vec x[NT][W::G];
+    typename W::Part x[NT];
     int64_t y[NT], row[NT];
     A ref[NT], sum[NT];
     C o[NT][DT];
@@ -153,8 +249,8 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         const int64_t n = n0 + (wr * NT + t) * 16 + (lane & 15);
         row[t] = n < a.x.rows ? (a.order ? a.order[n] : n) : -1;
         y[t] = row[t] >= 0 ? a.y[row[t]] : -1;
-#pragma unroll
-        for (int g = 0; g < W::G; ++g) x[t][g] = y[t] >= 0 ? tile_chunk(a.x, row[t], (int64_t)(4 * g + q) * N, D) : Vec{};
+        if (y[t] >= 0) x[t].load(a.x, row[t], D);
+        else x[t].clear();
         ref[t] = neg_inf<A>();
         sum[t] = 0;
 #pragma unroll
@@ -185,7 +281,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 #pragma unroll
             for (int v = 0; v < VT; ++v) {
                 const int base = (wv * VT + v) * 16;
-                p[t][v] = W::logits(lds, base, x[t]);
+                p[t][v] = W::template logits<STEP>(lds, base, x[t]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     p[t][v][r] = times_log2e(p[t][v][r]) + al[base + Mma<T>::row(q, r)];
@@ -248,14 +344,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         for (int k = 0; k < WV; ++k) join(mx, s, red[0][k][at], red[1][k][at]);
         const bool known = y[t] >= 0 && y[t] < V;
         A eta = 0; // of the row's class, as the matrix cores have it up to rounding
-        if (wv == 0 && known) {
-#pragma unroll
-            for (int g = 0; g < W::G; ++g) {
-                const Vec b = tile_chunk(a.beta, y[t], (int64_t)(4 * g + q) * N, D);
-#pragma unroll
-                for (int e = 0; e < N; ++e) eta += (A)x[t][g][e] * (A)b[e];
-            }
-        }
+        if (wv == 0 && known) eta = x[t].dot(a.beta, y[t], D);
         eta += __shfl_xor(eta, 16, 64);
         eta += __shfl_xor(eta, 32, 64);
         eta = times_log2e(eta);
@@ -305,7 +394,7 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     typedef typename W::A A;
     typedef typename W::C C;
     typedef typename W::Vec Vec;
-    constexpr int VT = VT_<T, DT, WR>, STEP = 16 * VT * WR, CLASSES = 16 * NT * WV, N = W::N;
+    constexpr int VT = VT_<T, DT, WR>, STEP = 16 * VT * WR, CLASSES = 16 * NT * WV;
     constexpr int STAGE = W::template stage<STEP>() * (int)sizeof(T), SPILL = WR * CLASSES * W::OLD * (int)sizeof(A);
     __shared__ uint4 room[(larger(STAGE, SPILL) + 15) / 16];
     __shared__ __attribute__((aligned(16))) A lse[STEP], wt[STEP];
@@ -314,7 +403,7 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6, wv = wave / WR, wr = wave % WR;
     const int64_t v0 = (int64_t)blockIdx.x * CLASSES, V = a.beta.rows, D = a.features;
     constexpr A up = stored_scale<T>();
-    Vec b[NT][W::G];
+    typename W::Part b[NT];
     A al[NT], abar[NT];
     C o[NT][DT];
     int me[NT];
@@ -322,8 +411,7 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     for (int t = 0; t < NT; ++t) {
         const int64_t v = v0 + (wv * NT + t) * 16 + (lane & 15);
         me[t] = (int)v;
-#pragma unroll
-        for (int g = 0; g < W::G; ++g) b[t][g] = tile_chunk(a.beta, v, (int64_t)(4 * g + q) * N, D);
+        b[t].load(a.beta, v, D);
         al[t] = v < V ? (a.alpha ? level_log2e((A)a.alpha[v]) : (A)0) : neg_inf<A>();
         abar[t] = 0;
 #pragma unroll
@@ -364,7 +452,7 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
             const int base = (wr * VT + u) * 16;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                C p = W::logits(lds, base, b[t]);
+                C p = W::template logits<STEP>(lds, base, b[t]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int n = base + Mma<T>::row(q, r);
@@ -407,6 +495,13 @@ template <typename T> __global__ __launch_bounds__(256) void class_narrow_join(c
     if (i >= count) return;
     A s[4] = {0, 0, 0, 0};
     int k = 0;
+    for (; k + 16 <= shares; k += 16) {
+        A u[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) u[e] = part[(k + e) * count + i];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e & 3] += u[e];
+    }
     for (; k + 4 <= shares; k += 4)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[e] += part[(k + e) * count + i];
@@ -434,7 +529,7 @@ template <typename T> struct NarrowPlan {
         const int64_t groups = tiles_of(V, 64 * NT);
         many_classes = groups * tiles_of(rows, 32 * 8) >= 512;
         const int64_t blocks = many_classes ? groups : tiles_of(V, 16 * NT), step = many_classes ? 32 : 128;
-        int64_t s = tiles_of(768, blocks);
+        int64_t s = tiles_of(1024, blocks);
         const int64_t most = tiles_of(rows, step);
         if (s > most) s = most;
         if (s > 1024) s = 1024;
@@ -467,7 +562,7 @@ template <typename T> struct NarrowPlan {
 template <typename T, int DT, bool VJP> void rows_kernel(const NarrowArgs<T>& a, const NarrowPlan<T>& p, hipStream_t st) {
     constexpr int NT = NarrowPlan<T>::NT;
     if (p.many_rows)
-        class_narrow_rows<T, DT, 4, 1, NT, VJP><<<dim3((unsigned)tiles_of(a.x.rows, 64 * NT)), dim3(256), 0, st>>>(a);
+        class_narrow_rows<T, DT, 2, 2, NT, VJP><<<dim3((unsigned)tiles_of(a.x.rows, 32 * NT)), dim3(256), 0, st>>>(a);
     else class_narrow_rows<T, DT, 1, 4, 1, VJP><<<dim3((unsigned)tiles_of(a.x.rows, 16)), dim3(256), 0, st>>>(a);
 }
 template <typename T, int DT> void run(const NarrowArgs<T>& a, const NarrowPlan<T>& p, bool vjp, hipStream_t st) {
