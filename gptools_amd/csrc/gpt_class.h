@@ -78,12 +78,13 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
 namespace { // (a kernel of its own in each of the two)
 
 // Numbers the observed rows: row[number], y[number] (any y that is no class as `classes`), their count; behind them row lists the
-// others, whose lp is 0. place (or null): the rows' numbers, -1 where there is no observation. A workgroup takes INDEX_ROWS rows and
-// counts those before them for itself.
+// others, whose lp is 0. place (or null): the rows' numbers, -1 where there is no observation. parts (or null): the largest |lpbar| of
+// the observed rows of a workgroup, as class_scale leaves it. A workgroup takes INDEX_ROWS rows and counts those before them for itself.
 constexpr int INDEX_ROWS = 4096;
 template <typename A> __global__ __launch_bounds__(1024) void class_index(const int64_t* y, int64_t rows, int64_t classes, int* place, int* row,
-                                                                         int* y_of, int* count, A* lp) {
+                                                                         int* y_of, int* count, A* lp, const A* lpbar, A* parts) {
     __shared__ int red[2][16];
+    __shared__ A most[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * INDEX_ROWS, mine = first + 4 * threadIdx.x;
     int before = 0, n = 0;
@@ -102,6 +103,15 @@ template <typename A> __global__ __launch_bounds__(1024) void class_index(const 
     for (int k = 0; k < 4; ++k) {
         v[k] = mine + k < rows ? y[mine + k] : -1;
         n += v[k] >= 0;
+    }
+    if (parts) {
+        A m = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (v[k] >= 0) m = fmax(m, fabs(lpbar[mine + k]));
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k, 64));
+        if (lane == 0) most[wave] = m;
     }
     int upto = n; // of this wave's lanes up to this one
 #pragma unroll
@@ -137,6 +147,14 @@ template <typename A> __global__ __launch_bounds__(1024) void class_index(const 
         }
     }
     if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *count = all;
+    if (parts && threadIdx.x == 0) {
+        A m = most[0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) m = fmax(m, most[k]);
+        parts[blockIdx.x] = m;
+        if (blockIdx.x == 0)
+            for (int k = gridDim.x; k < SCALE_PARTS; ++k) parts[k] = 0;
+    }
 }
 
 // parts[b] = the largest |lpbar| of the observed rows that workgroup b of SCALE_PARTS takes

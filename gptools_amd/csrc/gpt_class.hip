@@ -263,13 +263,22 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
 }
 
 // The observed rows of x side by side, as operands (zeros behind their features); zeros into xbar's other rows
-template <typename W> __global__ __launch_bounds__(256) void class_gather(const typename W::Data* x, int64_t ld, int64_t rows, int64_t cols,
-                                                                         const int* place, typename W::Element* out, int64_t ldo,
-                                                                         int64_t plane, typename W::Data* xbar) {
+template <typename W> struct GatherArgs {
+    const typename W::Data* x;
+    int64_t ld, rows, cols;
+    const int* place; // null: all rows
+    typename W::Element* out;
+    int64_t ldo, plane;
+    typename W::Data* xbar;
+};
+template <typename W> __device__ __forceinline__ void gather(const GatherArgs<W>& a, int64_t block, int64_t blocks) {
     typedef typename W::Data T;
     constexpr int N = 8;
-    const int64_t per = ldo / N, total = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const T* x = a.x;
+    const int64_t ld = a.ld, rows = a.rows, cols = a.cols, ldo = a.ldo, plane = a.plane, per = ldo / N, total = rows * per;
+    const int* place = a.place;
+    T* xbar = a.xbar;
+    for (int64_t i = block * 256 + threadIdx.x; i < total; i += blocks * 256) {
         const int64_t r = i / per, k = (i - r * per) * N;
         const int at = place ? place[r] : (int)r;
         if (at < 0) {
@@ -286,7 +295,7 @@ template <typename W> __global__ __launch_bounds__(256) void class_gather(const 
 #pragma unroll
             for (int e = 0; e < Vec16<T>::N; ++e) v[h + e] = u[e];
         }
-        typename W::Element* to = out + at * ldo + k;
+        typename W::Element* to = a.out + at * ldo + k;
         if constexpr (W::PLANES == 3) {
             typename Vec16<bf16_t>::V u[3];
 #pragma unroll
@@ -347,13 +356,23 @@ template <typename A> __global__ __launch_bounds__(256) void class_join(const A*
 
 // out[c][r] = in[row[r]][c] as operands (row null: r itself), zeros behind the last row up to ldo. 64 x 64 through LDS; each side in
 // vectors of eight
-template <typename W> __global__ __launch_bounds__(256) void class_transpose(const typename W::Data* in, int64_t ld, int64_t rows,
-                                                                            const int* count, int64_t cols, const int* row,
-                                                                            typename W::Element* out, int64_t ldo, int64_t plane) {
+template <typename W> struct TransposeArgs {
+    const typename W::Data* in;
+    int64_t ld, rows;
+    const int* count; // null: rows
+    int64_t cols;
+    const int* row; // null: as they come
+    typename W::Element* out;
+    int64_t ldo, plane;
+};
+template <typename W> __device__ __forceinline__ void transpose(const TransposeArgs<W>& t, int64_t block) {
     typedef typename W::Data T;
     __shared__ T tile[64][66];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    if (count) rows = *count;
+    const int64_t across = (t.ldo + 63) / 64, r0 = block % across * 64, c0 = block / across * 64;
+    const T* in = t.in;
+    const int64_t ld = t.ld, rows = t.count ? *t.count : t.rows, cols = t.cols, ldo = t.ldo, plane = t.plane;
+    const int* row = t.row;
+    typename W::Element* out = t.out;
     const int a = threadIdx.x >> 3, b = 8 * (threadIdx.x & 7);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -397,6 +416,21 @@ template <typename W> __global__ __launch_bounds__(256) void class_transpose(con
     }
 }
 
+// All that is copied before the logits, in one launch: the workgroups up to end[k] do part k. end[0], end[1]: x side by side, and beta
+// with rows that start on 16 bytes (gather); end[2], end[3]: the transposes of x and of beta's first piece
+template <typename W> struct PrepareArgs {
+    GatherArgs<W> g[2];
+    TransposeArgs<W> t[2];
+    int end[4];
+};
+template <typename W> __global__ __launch_bounds__(256) void class_prepare(PrepareArgs<W> a) {
+    const int id = blockIdx.x;
+    if (id < a.end[0]) gather<W>(a.g[0], id, a.end[0]);
+    else if (id < a.end[1]) gather<W>(a.g[1], id - a.end[0], a.end[1] - a.end[0]);
+    else if (id < a.end[2]) transpose<W>(a.t[0], id - a.end[1]);
+    else transpose<W>(a.t[1], id - a.end[2]);
+}
+
 // The products with r: out[n][m] = sum_k A[m][k] B[n][k] over this launch's share of k.
 template <typename T, typename E> struct ProductArgs {
     typedef acc_t<T> Acc;
@@ -404,7 +438,7 @@ template <typename T, typename E> struct ProductArgs {
     int64_t K;        // (betabar: the observed rows', rounded up to k_edge)
     int64_t k_edge;
     const int* count; // observed rows: B's rows (xbar), or k (betabar)
-    int64_t tiles_m;
+    int64_t tiles_m, splits, grid; // grid: workgroups of one split
     Acc* acc;      // [splits][B.rows][A.rows]: sums so far
     int64_t plane; // elements from one split's sums to the next
     T* out;        // the result, where this launch completes it; else null
@@ -415,21 +449,22 @@ template <typename T, typename E> struct ProductArgs {
     const Acc* lpbar;
     Largest<Acc> largest;
 };
-template <typename W> __global__ __launch_bounds__(W::Tl::THREADS) void class_product(ProductArgs<typename W::Data, typename W::Element> a) {
+template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<typename W::Data, typename W::Element> a, int64_t id,
+                                                                   typename W::Tl::Vec* lds) {
     typedef typename W::Acc A;
     typedef typename W::Data T;
     typedef typename W::Tl Tl;
-    __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
+    const int64_t split = id / a.grid;
     if (a.row) a.B.rows = *a.count;
     else a.K = (*a.count + a.k_edge - 1) / a.k_edge * a.k_edge;
     int64_t tm, tn;
-    if (!tile_place(blockIdx.x, a.tiles_m, (a.B.rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
+    if (!tile_place(id - split * a.grid, a.tiles_m, (a.B.rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
     const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN, step = tile_k<typename W::Element>();
-    const int64_t share = ((a.K + gridDim.y - 1) / gridDim.y + step - 1) / step * step;
-    const int64_t k0 = (int64_t)blockIdx.y * share, k1 = k0 + share < a.K ? k0 + share : a.K;
+    const int64_t share = ((a.K + a.splits - 1) / a.splits + step - 1) / step * step;
+    const int64_t k0 = split * share, k1 = k0 + share < a.K ? k0 + share : a.K;
     Tl tl;
     tl.run(a.A, m0, a.B, n0, k0, k1, lds);
-    A* acc = a.acc + (int64_t)blockIdx.y * a.plane;
+    A* acc = a.acc + split * a.plane;
     const A largest = a.row ? (A)1 : a.largest.get();
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
@@ -498,35 +533,70 @@ template <typename W> __global__ __launch_bounds__(W::Tl::THREADS) void class_pr
         }
     }
 }
+// alphabar of a piece from the tiles' sums: 64 classes a workgroup, its waves share the tiles. acc: sums over row blocks
+template <typename T> struct AlphaArgs {
+    const acc_t<T>* part;
+    const int* count;
+    int64_t edge, ld, nv;
+    acc_t<T>* acc;
+    bool add;
+    T* out;
+};
+template <typename T, int WAVES> __device__ __forceinline__ void alpha_sums(const AlphaArgs<T>& a, int64_t block, acc_t<T>* red) {
+    typedef acc_t<T> A;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t v = block * 64 + lane, tiles = (*a.count + a.edge - 1) / a.edge;
+    A s = 0;
+    if (v < a.nv)
+        for (int64_t i = w; i < tiles; i += WAVES) s += a.part[i * a.ld + v];
+    red[w * 64 + lane] = s;
+    __syncthreads();
+    if (w || v >= a.nv) return;
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) s += red[k * 64 + lane];
+    if (a.add) s += a.acc[v];
+    if (a.out) a.out[v] = (T)s;
+    else a.acc[v] = s;
+}
+// Both products with r, and alphabar, in one launch where they run the same way: the workgroups up to end[0] take xbar, those up to
+// end[1] betabar, the others alphabar
+template <typename W> struct ProductsArgs {
+    ProductArgs<typename W::Data, typename W::Element> x, b;
+    AlphaArgs<typename W::Data> alpha;
+    int end[2];
+};
+template <typename W> __global__ __launch_bounds__(W::Tl::THREADS) void class_products(ProductsArgs<W> a) {
+    typedef typename W::Tl Tl;
+    __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
+    const int id = blockIdx.x;
+    if (id < a.end[1]) { // (one call: the tile's code stands once)
+        const bool x = id < a.end[0];
+        product_tile<W>(x ? a.x : a.b, x ? id : id - a.end[0], lds);
+    } else alpha_sums<typename W::Data, Tl::THREADS / 64>(a.alpha, id - a.end[1], reinterpret_cast<typename W::Acc*>(lds));
+}
+
 // out[row[n]][0..cols) <- sum over the splits (row null: all `rows` rows, else the observed ones)
-template <typename T> __global__ __launch_bounds__(256) void class_join_splits(const acc_t<T>* acc, int splits, int64_t plane, int64_t rows,
-                                                                              int64_t cols, const int* count, const int* row, T* out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (row ? *count : rows) * cols) return;
+template <typename T> struct SplitsArgs {
+    const acc_t<T>* acc;
+    int splits;
+    int64_t plane, rows, cols;
+    const int *count, *row;
+    T* out;
+};
+template <typename T> __device__ __forceinline__ void join_splits(const SplitsArgs<T>& a, int64_t block) {
+    const int64_t i = block * 256 + threadIdx.x;
+    if (i >= (a.row ? *a.count : a.rows) * a.cols) return;
     acc_t<T> s = 0;
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) s += acc[k * plane + i];
-    const int64_t n = i / cols;
-    out[row ? row[n] * cols + (i - n * cols) : i] = (T)s;
+    for (int k = 0; k < a.splits; ++k) s += a.acc[k * a.plane + i];
+    const int64_t n = i / a.cols;
+    a.out[a.row ? a.row[n] * a.cols + (i - n * a.cols) : i] = (T)s;
 }
-// alphabar of a piece from the tiles' sums: 64 classes a workgroup, 4 waves share the tiles. acc: sums over row blocks
-template <typename T> __global__ __launch_bounds__(256) void class_alpha(const acc_t<T>* part, const int* count, int64_t edge, int64_t ld,
-                                                                        int64_t nv, acc_t<T>* acc, bool add, T* out) {
-    typedef acc_t<T> A;
-    __shared__ A red[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t v = (int64_t)blockIdx.x * 64 + lane, tiles = (*count + edge - 1) / edge;
-    A s = 0;
-    if (v < nv)
-        for (int64_t i = w; i < tiles; i += 4) s += part[i * ld + v];
-    red[w][lane] = s;
-    __syncthreads();
-    if (w || v >= nv) return;
-    s = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
-    if (add) s += acc[v];
-    if (out) out[v] = (T)s;
-    else acc[v] = s;
+template <typename T> __global__ __launch_bounds__(256) void class_join_splits(SplitsArgs<T> x, SplitsArgs<T> b, int64_t end) {
+    if (blockIdx.x < end) join_splits<T>(x, blockIdx.x);
+    else join_splits<T>(b, blockIdx.x - end);
 }
+
 // ---- plan -------------------------------------------------------------------------------------------------------------
 int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
@@ -624,26 +694,52 @@ template <typename W, bool STATS> void logits(LogitArgs<W> l, hipStream_t st) {
     class_logits<W, STATS><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
-// large: 256 x 256 tiles
-template <typename W> hipError_t product(ProductArgs<typename W::Data, typename W::Element> p, bool large, int64_t splits, bool last,
-                                         typename W::Data* out, hipStream_t st) {
+// xbar and betabar of a piece (each complete if its `last`), alphabar (blocks: its workgroups, or none)
+template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan, bool xlast, typename W::Data* xbar, bool blast,
+                                          typename W::Data* betabar, int64_t alpha_blocks, hipStream_t st) {
     typedef typename W::Data T;
-    p.out = last && splits == 1 ? out : nullptr;
-    p.ldo = p.A.rows;
-    auto run = [&](auto way) {
+    typedef typename W::Element E;
+    auto ready = [](auto& q, int64_t splits, bool last, T* out) {
+        q.splits = splits;
+        q.out = last && splits == 1 ? out : nullptr;
+        q.ldo = q.A.rows;
+    };
+    ready(p.x, plan.xsplits, xlast, xbar);
+    ready(p.b, plan.bsplits, blast, betabar);
+    auto run = [&](auto way, bool x, bool b) {
         typedef decltype(way) U;
         typedef typename U::Tl Tl;
-        p.tiles_m = tiles_of(p.A.rows, Tl::BM);
-        class_product<U><<<dim3(tile_grid(p.tiles_m, tiles_of(p.B.rows, Tl::BN)), (unsigned)splits), dim3(Tl::THREADS), 0, st>>>(p);
+        ProductsArgs<U> u = {p.x, p.b, p.alpha, {0, 0}};
+        auto size = [](auto& q) {
+            q.tiles_m = tiles_of(q.A.rows, Tl::BM);
+            q.grid = tile_grid(q.tiles_m, tiles_of(q.B.rows, Tl::BN));
+            return (int)(q.grid * q.splits);
+        };
+        u.end[0] = x ? size(u.x) : 0;
+        u.end[1] = u.end[0] + (b ? size(u.b) : 0);
+        class_products<U><<<dim3((unsigned)(u.end[1] + (b ? alpha_blocks : 0))), dim3(Tl::THREADS), 0, st>>>(u);
     };
-    typedef typename W::Element E;
     if constexpr (W::LINES) {
-        if (large) run(Way<T, WideTile<E, W::PLANES>, W::PLANES>());
-        else run(Way<T, MidTile<E, W::PLANES>, W::PLANES>());
-    } else run(W());
-    if (last && splits > 1)
-        class_join_splits<T><<<dim3((unsigned)tiles_of(p.A.rows * p.B.rows, 256)), dim3(256), 0, st>>>(p.acc, (int)splits, p.plane, p.B.rows,
-                                                                                                      p.A.rows, p.count, p.row, out);
+        typedef Way<T, WideTile<E, W::PLANES>, W::PLANES> Wide;
+        typedef Way<T, MidTile<E, W::PLANES>, W::PLANES> Mid;
+        if (plan.xwide == plan.bwide) {
+            if (plan.xwide) run(Wide(), true, true);
+            else run(Mid(), true, true);
+        } else {
+            if (plan.xwide) run(Wide(), true, false);
+            else run(Mid(), true, false);
+            if (plan.bwide) run(Wide(), false, true);
+            else run(Mid(), false, true);
+        }
+    } else run(W(), true, true);
+    const bool xjoin = xlast && plan.xsplits > 1, bjoin = blast && plan.bsplits > 1;
+    if (xjoin || bjoin) {
+        auto args = [](const auto& q, T* out) {
+            return SplitsArgs<T>{q.acc, (int)q.splits, q.plane, q.B.rows, q.A.rows, q.count, q.row, out};
+        };
+        const int64_t nx = xjoin ? tiles_of(p.x.A.rows * p.x.B.rows, 256) : 0, nb = bjoin ? tiles_of(p.b.A.rows * p.b.B.rows, 256) : 0;
+        class_join_splits<T><<<dim3((unsigned)(nx + nb)), dim3(256), 0, st>>>(args(p.x, xbar), args(p.b, betabar), nx);
+    }
     return hipGetLastError();
 }
 
@@ -657,34 +753,50 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
     const int64_t D = c.features, V = c.classes;
     hipError_t e;
     int *place = (int*)(ws + p.place), *row = (int*)(ws + p.row), *count = (int*)(ws + p.count);
-    Operand<E> beta;
-    int64_t K = D;
-    if (p.copy) {
-        E* to = (E*)(ws + p.ba);
-        class_gather<W><<<dim3(2048), dim3(256), 0, st>>>((const T*)c.beta, c.ldbeta, V, D, nullptr, to, p.ldk, V * p.ldk, nullptr);
-        beta = {to, p.ldk, V, V * p.ldk};
-        K = p.ldk;
-    } else beta = {(const E*)c.beta, c.ldbeta, V, 0};
+    E *xa = (E*)(ws + p.xa), *ba = (E*)(ws + p.ba);
+    E *r = (E*)(ws + p.r), *rt = (E*)(ws + p.rt), *xt = (E*)(ws + p.xt), *bt = (E*)(ws + p.bt);
+    const Operand<E> beta = p.copy ? Operand<E>{ba, p.ldk, V, V * p.ldk} : Operand<E>{(const E*)c.beta, c.ldbeta, V, 0};
     Largest<A> largest = {nullptr};
     if (vjp && c.lpbar) {
         largest.parts = (A*)(ws + p.scale);
-        class_scale<A><<<dim3(SCALE_PARTS), dim3(256), 0, st>>>((const A*)c.lpbar, c.y, c.rows, (A*)(ws + p.scale));
+        if (p.blocks > 1)
+            class_scale<A><<<dim3(SCALE_PARTS), dim3(256), 0, st>>>((const A*)c.lpbar, c.y, c.rows, (A*)(ws + p.scale));
     }
+    auto turn = [&](int64_t v0) { // a piece of beta
+        const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece, ldr = up_to(nv, EDGE);
+        return TransposeArgs<W>{(const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv, nullptr, D, nullptr, bt, ldr, D * ldr};
+    };
+    auto blocks_of = [&](const TransposeArgs<W>& t) { return tiles_of(t.ldo, 64) * tiles_of(t.cols, 64); };
     for (int64_t n0 = 0; n0 < c.rows; n0 += p.block) {
         const int64_t N = c.rows - n0 < p.block ? c.rows - n0 : p.block;
         const bool first_block = n0 == 0, last_block = n0 + N == c.rows;
         const T* x = (const T*)c.x + n0 * c.ldx;
+        const int64_t ldrt = up_to(N, EDGE); // (r is written in whole tiles)
+        const bool scale_here = largest.parts && p.blocks == 1;
+        class_index<A><<<dim3((unsigned)tiles_of(N, INDEX_ROWS)), dim3(1024), 0, st>>>(
+            c.y + n0, N, V, place, row, (int*)(ws + p.y), count, (A*)c.lp + n0, (const A*)c.lpbar, scale_here ? (A*)(ws + p.scale) : nullptr);
+        PrepareArgs<W> q = {};
+        q.g[0] = {x, c.ldx, N, D, place, xa, p.ldk, p.block * p.ldk, vjp ? (T*)c.xbar + n0 * D : nullptr};
+        q.end[0] = (int)(tiles_of(N * (p.ldk / 8), 256) < 1024 ? tiles_of(N * (p.ldk / 8), 256) : 1024);
+        q.end[1] = q.end[0];
+        if (p.copy && first_block) {
+            q.g[1] = {(const T*)c.beta, c.ldbeta, V, D, nullptr, ba, p.ldk, V * p.ldk, nullptr};
+            q.end[1] += (int)(tiles_of(V * (p.ldk / 8), 256) < 2048 ? tiles_of(V * (p.ldk / 8), 256) : 2048);
+        }
+        q.end[2] = q.end[3] = q.end[1];
+        if (vjp) {
+            q.t[0] = {x, c.ldx, N, count, D, row, xt, ldrt, D * ldrt};
+            q.t[1] = turn(0);
+            q.end[2] += (int)blocks_of(q.t[0]);
+            q.end[3] = q.end[2] + (first_block || p.pieces > 1 ? (int)blocks_of(q.t[1]) : 0);
+        }
+        class_prepare<W><<<dim3((unsigned)q.end[3]), dim3(256), 0, st>>>(q);
         LogitArgs<W> l = {};
-        class_index<A><<<dim3((unsigned)tiles_of(N, INDEX_ROWS)), dim3(1024), 0, st>>>(c.y + n0, N, V, place, row, (int*)(ws + p.y), count,
-                                                                                      (A*)c.lp + n0);
-        E* xa = (E*)(ws + p.xa);
-        class_gather<W><<<dim3(1024), dim3(256), 0, st>>>(x, c.ldx, N, D, place, xa, p.ldk, p.block * p.ldk,
-                                                          vjp ? (T*)c.xbar + n0 * D : nullptr);
         l.beta = beta;
         l.x = {xa, p.ldk, N, p.block * p.ldk};
         l.count = count;
         l.alpha = (const T*)c.alpha;
-        l.features = K;
+        l.features = p.copy ? p.ldk : D;
         l.classes = V;
         l.y = (const int*)(ws + p.y);
         l.row = row;
@@ -695,13 +807,9 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         logits<W, true>(l, st);
         A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
         class_join<A><<<dim3((unsigned)tiles_of(N, 8)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
-                                                                             tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
+                                                                            tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if (!vjp) continue;
-        const int64_t ldrt = up_to(N, EDGE); // (r is written in whole tiles)
-        E *r = (E*)(ws + p.r), *rt = (E*)(ws + p.rt), *xt = (E*)(ws + p.xt), *bt = (E*)(ws + p.bt);
-        class_transpose<W><<<dim3((unsigned)tiles_of(ldrt, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(x, c.ldx, N, count, D, row, xt,
-                                                                                                              ldrt, D * ldrt);
         l.lse = lse;
         l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
         l.r = r;
@@ -711,6 +819,11 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
             const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
             const bool first = v0 == 0, last = v0 + nv == V;
+            if (!first) {
+                PrepareArgs<W> t = {};
+                t.t[1] = turn(v0);
+                class_prepare<W><<<dim3((unsigned)blocks_of(t.t[1])), dim3(256), 0, st>>>(t);
+            }
             l.beta = {beta.p + v0 * beta.ld, beta.ld, nv, beta.plane};
             l.alpha = c.alpha ? (const T*)c.alpha + v0 : nullptr;
             l.v0 = v0;
@@ -718,33 +831,29 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
             l.r_plane = ldrt * l.ldr;
             l.rt_plane = l.ldr * ldrt;
             logits<W, false>(l, st);
-            class_transpose<W><<<dim3((unsigned)tiles_of(l.ldr, 64), (unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(
-                (const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv, nullptr, D, nullptr, bt, l.ldr, D * l.ldr);
+            ProductsArgs<W> m = {};
+            m.x.A = {bt, l.ldr, D, D * l.ldr};
+            m.x.B = {r, l.ldr, N, l.r_plane};
+            m.x.K = l.ldr;
+            m.x.count = count;
+            m.x.acc = (A*)(ws + p.xacc);
+            m.x.plane = p.block * D;
+            m.x.add = !first;
+            m.x.row = row;
+            m.x.lpbar = l.lpbar;
+            m.b.A = {xt, ldrt, D, D * ldrt};
+            m.b.B = {rt, ldrt, nv, l.rt_plane};
+            m.b.k_edge = tile_k<E>(); // (rt and xt are zero from the last row to ldrt)
+            m.b.count = count;
+            m.b.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
+            m.b.plane = (p.blocks > 1 ? V : p.piece) * D;
+            m.b.add = !first_block;
+            m.b.largest = largest;
             if (c.alphabar)
-                class_alpha<T><<<dim3((unsigned)tiles_of(nv, 64)), dim3(256), 0, st>>>(
-                    l.part_alpha, count, EDGE, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
-                    last_block ? (T*)c.alphabar + v0 : nullptr);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-            ProductArgs<T, E> x_ = {}, b_ = {};
-            x_.A = {bt, l.ldr, D, D * l.ldr};
-            x_.B = {r, l.ldr, N, l.r_plane};
-            x_.K = l.ldr;
-            x_.count = count;
-            x_.acc = (A*)(ws + p.xacc);
-            x_.plane = p.block * D;
-            x_.add = !first;
-            x_.row = row;
-            x_.lpbar = l.lpbar;
-            if ((e = product<W>(x_, p.xwide, p.xsplits, last, (T*)c.xbar + n0 * D, st)) != hipSuccess) return e;
-            b_.A = {xt, ldrt, D, D * ldrt};
-            b_.B = {rt, ldrt, nv, l.rt_plane};
-            b_.k_edge = tile_k<E>(); // (rt and xt are zero from the last row to ldrt)
-            b_.count = count;
-            b_.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
-            b_.plane = (p.blocks > 1 ? V : p.piece) * D;
-            b_.add = !first_block;
-            b_.largest = largest;
-            if ((e = product<W>(b_, p.bwide, p.bsplits, last_block, (T*)c.betabar + v0 * D, st)) != hipSuccess) return e;
+                m.alpha = {l.part_alpha, count, EDGE, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
+                           last_block ? (T*)c.alphabar + v0 : nullptr};
+            e = products<W>(m, p, last, (T*)c.xbar + n0 * D, last_block, (T*)c.betabar + v0 * D, c.alphabar ? tiles_of(nv, 64) : 0, st);
+            if (e != hipSuccess) return e;
         }
     }
     return hipSuccess;
@@ -775,6 +884,7 @@ template <typename T> struct FewPlan {
             const int64_t slabs = tiles_of(D, 16 * Vec16<T>::N);
             splits = tiles_of(2 * FILL, slabs);
             if (splits > tiles_of(V, 128)) splits = tiles_of(V, 128);
+            if (V <= 1024) splits = 1; // (eight rounds of one workgroup are shorter than another launch)
             share = up_to(tiles_of(V, splits), 128);
             splits = tiles_of(V, share);
             eta = take(A * (size_t)(rows * ldv));
@@ -783,7 +893,7 @@ template <typename T> struct FewPlan {
             r = take(E * (size_t)(rows * ldv));
             rt = take(E * (size_t)(V * ldrt));
             xt = take(E * (size_t)(D * ldrt));
-            xpart = take(A * (size_t)(splits * rows * D));
+            xpart = splits > 1 ? take(A * (size_t)(splits * rows * D)) : 0;
         }
         bytes = at;
     }
@@ -813,25 +923,25 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
         a.rt = (T*)(ws + p.rt);
         a.ldrt = p.ldrt;
         a.alphabar = (T*)c.alphabar;
-        a.xpart = (A*)(ws + p.xpart);
+        a.xpart = p.splits > 1 ? (A*)(ws + p.xpart) : nullptr;
+        a.xbar = (T*)c.xbar;
         a.share = p.share;
     }
     const dim3 grid((unsigned)p.tiles);
     if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4><<<grid, dim3(256), 0, st>>>(a);
     else class_few_logits<T, NT, 1, 8><<<grid, dim3(512), 0, st>>>(a);
-    class_few_join<T><<<dim3((unsigned)c.rows), dim3(256), 0, st>>>(a);
+    T* xt = vjp ? (T*)(ws + p.xt) : nullptr;
+    class_few_join<T><<<dim3((unsigned)(c.rows + (vjp ? tiles_of(D, 64) : 0))), dim3(256), 0, st>>>(a, xt);
     if (!vjp) return hipGetLastError();
     const Largest<A> largest = {c.lpbar ? a.largest : nullptr};
     class_few_r<T><<<dim3((unsigned)(p.ldv / 64)), dim3(256), 0, st>>>(a, largest);
-    class_few_xbar<T, NT><<<dim3((unsigned)tiles_of(D, 16 * Vec16<T>::N), (unsigned)p.splits), dim3(256), 0, st>>>(a);
-    class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits, (T*)c.xbar);
-    T* xt = (T*)(ws + p.xt);
-    class_few_turn<T><<<dim3((unsigned)tiles_of(D, 64)), dim3(256), 0, st>>>(a, xt);
     constexpr int NG = (NT <= 2 ? 32 : 64) / (4 * Vec16<T>::N);
-    const int64_t slabs = tiles_of(D, Slab<T>::WIDTH);
-    int64_t shares = tiles_of(4 * FILL, slabs);
+    const int64_t xslabs = tiles_of(D, 16 * Vec16<T>::N), bslabs = tiles_of(D, Slab<T>::WIDTH);
+    int64_t shares = tiles_of(4 * FILL, bslabs);
     if (shares > tiles_of(V, 128)) shares = tiles_of(V, 128);
-    class_few_beta<T, NG><<<dim3((unsigned)slabs, (unsigned)shares), dim3(256), 0, st>>>(a, xt, (T*)c.betabar, largest);
+    class_few_back<T, NT, NG><<<dim3((unsigned)(xslabs * p.splits + bslabs * shares)), dim3(256), 0, st>>>(
+        a, xt, (T*)c.betabar, largest, (int)xslabs, (int)p.splits, (int)bslabs, (int)shares);
+    if (p.splits > 1) class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits);
     return hipGetLastError();
 }
 template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStream_t st) {

@@ -5,9 +5,9 @@
 //   class_few_logits  16 classes a workgroup or 64 (32 in fp64), whose waves share the features; their logits' maximum and sum for every row,
 //                     and for the reverse mode the logits themselves (64 rows of logits are a piece as r is one)
 //   class_few_r       r in both orders, alphabar
-//   class_few_xbar    xbar = r beta. beta's rows lie along the features, the sum runs over the classes: a lane reads 16 bytes of
-//                     eight classes and turns the block over in its registers (in 16 bits one byte permutation for two values)
-//   class_few_beta    betabar = r^T x, bound by writing it
+//   class_few_back    xbar = r beta, and betabar = r^T x, which is bound by writing it. For xbar beta's rows lie along the
+//                     features, the sum runs over the classes: a lane reads 16 bytes of eight classes and turns the block over in
+//                     its registers (in 16 bits one byte permutation for two values)
 #pragma once
 #include "gpt_class.h"
 #include "gpt_tile.h"
@@ -30,7 +30,8 @@ template <typename T> struct FewArgs {
     T *r, *rt;                   // [rows][ldv], [classes][ldrt]
     int64_t ldrt;
     T* alphabar;
-    acc_t<T>* xpart; // [splits][rows][features]
+    acc_t<T>* xpart; // [splits][rows][features]; null: one split, the result itself
+    T* xbar;
     int64_t share;   // classes of a split
 };
 
@@ -133,10 +134,25 @@ template <typename T, int NT, int CT, int WK> __global__ __launch_bounds__(64 * 
     }
 }
 
-// one workgroup a row: lse and lp. The row's logit of its class comes from x and beta again (one dot product)
-template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewArgs<T> a) {
+// xt[d][n] = x[n][d] (zero without an observation, and behind the last row): 64 features
+template <typename T> __device__ __forceinline__ void few_turn(const FewArgs<T>& a, int64_t d0, T* xt) {
+    __shared__ T tile[FEW][66];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int n = w; n < (int)a.ldrt; n += 4)
+        tile[n][lane] = n < a.x.rows && d0 + lane < a.features && a.y[n] >= 0 ? a.x.p[n * a.x.ld + d0 + lane] : (T)0;
+    __syncthreads();
+    for (int k = w; k < 64; k += 4)
+        if (lane < a.ldrt && d0 + k < a.features) xt[(d0 + k) * a.ldrt + lane] = tile[lane][k];
+}
+// One workgroup a row: lse and lp. The row's logit of its class comes from x and beta again (one dot product). The workgroups behind
+// the last row turn x over
+template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewArgs<T> a, T* xt) {
     typedef acc_t<T> A;
     __shared__ A red[3][4];
+    if (blockIdx.x >= a.x.rows) {
+        few_turn(a, (blockIdx.x - a.x.rows) * 64, xt);
+        return;
+    }
     const int64_t n = blockIdx.x, y = a.y[n], V = a.beta.rows;
     const bool known = y >= 0 && y < V;
     A mx = neg_inf<A>(), s = 0, eta = 0;
@@ -156,7 +172,7 @@ template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewA
     }
     __syncthreads();
     if (a.largest && n == 0) // (rows behind the last)
-        for (int64_t i = gridDim.x + threadIdx.x; i < FEW; i += 256) a.largest[i] = 0;
+        for (int64_t i = a.x.rows + threadIdx.x; i < FEW; i += 256) a.largest[i] = 0;
     if (threadIdx.x) return;
     for (int w = 1; w < 4; ++w) {
         join(mx, s, red[0][w], red[1][w]);
@@ -241,16 +257,21 @@ template <typename T> struct Turn { // 16 bits
     }
 };
 
+// an entry of xbar from its sum: times the row's cotangent
+template <typename T> __device__ __forceinline__ T few_cotangent(const FewArgs<T>& a, int64_t n, acc_t<T> s) {
+    return (T)(a.y[n] < 0 ? (acc_t<T>)0 : s * ((a.lpbar ? a.lpbar[n] : (acc_t<T>)1) / (acc_t<T>)stored_scale<T>()));
+}
+
 // xbar's sums over a share of the classes for 16 chunks of features: four waves with a quarter of the share each
-template <typename T, int NT> __global__ __launch_bounds__(256) void class_few_xbar(FewArgs<T> a) {
+template <typename T, int NT> __device__ __forceinline__ void few_xbar(const FewArgs<T>& a, int64_t slab, int64_t split) {
     typedef acc_t<T> A;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
     constexpr int N = Vec16<T>::N;
     __shared__ A sum[4][16][16 * N + 1];
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
-    const int64_t d0 = (int64_t)blockIdx.x * 16 * N, d = d0 + (lane & 15) * N, D = a.features, V = a.beta.rows;
-    const int64_t s0 = (int64_t)blockIdx.y * a.share, s1 = s0 + a.share < V ? s0 + a.share : V;
+    const int64_t d0 = slab * 16 * N, d = d0 + (lane & 15) * N, D = a.features, V = a.beta.rows;
+    const int64_t s0 = split * a.share, s1 = s0 + a.share < V ? s0 + a.share : V;
     C c[NT][N];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -289,35 +310,22 @@ template <typename T, int NT> __global__ __launch_bounds__(256) void class_few_x
         __syncthreads();
         for (int id = threadIdx.x; id < 16 * 16 * N; id += 256) {
             const int n = id / (16 * N), k = id % (16 * N);
-            if (16 * t + n < a.x.rows && d0 + k < D)
-                a.xpart[((int64_t)blockIdx.y * a.x.rows + 16 * t + n) * D + d0 + k] =
-                    (sum[0][n][k] + sum[1][n][k]) + (sum[2][n][k] + sum[3][n][k]);
+            if (16 * t + n >= a.x.rows || d0 + k >= D) continue;
+            const A s = (sum[0][n][k] + sum[1][n][k]) + (sum[2][n][k] + sum[3][n][k]);
+            if (a.xpart) a.xpart[(split * a.x.rows + 16 * t + n) * D + d0 + k] = s;
+            else a.xbar[(16 * t + n) * D + d0 + k] = few_cotangent(a, 16 * t + n, s);
         }
         __syncthreads();
     }
 }
 // xbar <- the splits' sums times the rows' cotangents
-template <typename T> __global__ __launch_bounds__(256) void class_few_xbar_join(FewArgs<T> a, int splits, T* xbar) {
-    typedef acc_t<T> A;
+template <typename T> __global__ __launch_bounds__(256) void class_few_xbar_join(FewArgs<T> a, int splits) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, count = a.x.rows * a.features;
     if (i >= count) return;
-    const int64_t n = i / a.features, y = a.y[n];
-    A s = 0;
+    acc_t<T> s = 0;
 #pragma unroll 4
     for (int k = 0; k < splits; ++k) s += a.xpart[k * count + i];
-    xbar[i] = (T)(y < 0 ? (A)0 : s * ((a.lpbar ? a.lpbar[n] : (A)1) / (A)stored_scale<T>()));
-}
-
-// xt[d][n] = x[n][d] (zero without an observation, and behind the last row): 64 features a workgroup
-template <typename T> __global__ __launch_bounds__(256) void class_few_turn(FewArgs<T> a, T* xt) {
-    __shared__ T tile[FEW][66];
-    const int64_t d0 = (int64_t)blockIdx.x * 64;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int n = w; n < (int)a.ldrt; n += 4)
-        tile[n][lane] = n < a.x.rows && d0 + lane < a.features && a.y[n] >= 0 ? a.x.p[n * a.x.ld + d0 + lane] : (T)0;
-    __syncthreads();
-    for (int k = w; k < 64; k += 4)
-        if (lane < a.ldrt && d0 + k < a.features) xt[(d0 + k) * a.ldrt + lane] = tile[lane][k];
+    a.xbar[i] = few_cotangent(a, i / a.features, s);
 }
 
 // betabar[v][d] = sum_n rt[v][n] x[n][d] for a slab of features and a share of the classes: the slab's x stays in registers (xt, its
@@ -332,15 +340,15 @@ template <typename T> struct Slab {
         return 16 * j + 4 * (row & 3) + (row >> 2);
     }
 };
-template <typename T, int NG> __global__ __launch_bounds__(256) void class_few_beta(FewArgs<T> a, const T* xt, T* betabar,
-                                                                                   Largest<acc_t<T>> largest) {
+template <typename T, int NG> __device__ __forceinline__ void few_beta(const FewArgs<T>& a, const T* xt, T* betabar, Largest<acc_t<T>> largest,
+                                                                     int64_t slab, int64_t share, int64_t shares) {
     typedef acc_t<T> A;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
     typedef Slab<T> S;
     constexpr int N = Vec16<T>::N, AHEAD = NG <= 2 ? 4 : 2;
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
-    const int64_t d0 = (int64_t)blockIdx.x * S::WIDTH, D = a.features, V = a.beta.rows, ldrt = a.ldrt;
+    const int64_t d0 = slab * S::WIDTH, D = a.features, V = a.beta.rows, ldrt = a.ldrt;
     const A back = largest.get() / (A)stored_scale<T>();
     Vec x[S::FRAGS][NG];
 #pragma unroll
@@ -350,8 +358,8 @@ template <typename T, int NG> __global__ __launch_bounds__(256) void class_few_b
         for (int g = 0; g < NG; ++g) x[j][g] = d < D ? *reinterpret_cast<const Vec*>(xt + d * ldrt + (4 * g + q) * N) : Vec{};
     }
     const bool full = d0 + S::WIDTH <= D;
-    const int64_t step = (int64_t)gridDim.y * 4 * 16 * AHEAD;
-    for (int64_t v0 = ((int64_t)blockIdx.y * 4 + wave) * 16 * AHEAD; v0 < V; v0 += step) {
+    const int64_t step = shares * 4 * 16 * AHEAD;
+    for (int64_t v0 = (share * 4 + wave) * 16 * AHEAD; v0 < V; v0 += step) {
         Vec b[AHEAD][NG];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -392,6 +400,15 @@ template <typename T, int NG> __global__ __launch_bounds__(256) void class_few_b
             }
         }
     }
+}
+
+// xbar's sums by the first xslabs x splits workgroups, betabar by the others
+template <typename T, int NT, int NG> __global__ __launch_bounds__(256) void class_few_back(FewArgs<T> a, const T* xt, T* betabar,
+                                                                                           Largest<acc_t<T>> largest, int xslabs, int splits,
+                                                                                           int bslabs, int shares) {
+    const int id = blockIdx.x;
+    if (id < xslabs * splits) few_xbar<T, NT>(a, id % xslabs, id / xslabs);
+    else few_beta<T, NG>(a, xt, betabar, largest, (id - xslabs * splits) % bslabs, (id - xslabs * splits) / bslabs, shares);
 }
 
 } // namespace gptt

@@ -36,7 +36,8 @@ template <typename T> struct NarrowArgs {
     int* at;         // ... and the row's class
     Largest<A> largest;
     T* xbar;       // [rows][features]
-    A* part;       // [shares][classes][features + 1]: betabar, alphabar
+    A* part;       // [shares][classes][features + 1]: betabar, alphabar; null: one share, the results themselves
+    T *betabar, *alphabar;
     int64_t share; // rows of one share
 };
 
@@ -476,13 +477,16 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     }
     __syncthreads();
     A* part = a.part + (int64_t)blockIdx.y * V * (D + 1);
+    const A back = a.largest.get() / up;
     for (int id = threadIdx.x; id < CLASSES * W::OLD; id += 256) {
         const int c = id / W::OLD, d = id % W::OLD;
         if (v0 + c >= V || (d >= D && d != W::DP)) continue;
         A s = 0;
 #pragma unroll
         for (int k = 0; k < WR; ++k) s += spilt[(k * CLASSES + c) * W::OLD + d];
-        part[(v0 + c) * (D + 1) + (d == W::DP ? D : d)] = s;
+        if (a.part) part[(v0 + c) * (D + 1) + (d == W::DP ? D : d)] = s;
+        else if (d < D) a.betabar[(v0 + c) * D + d] = (T)(s * back);
+        else if (a.alphabar) a.alphabar[v0 + c] = (T)(s * back);
     }
 }
 
@@ -533,6 +537,7 @@ template <typename T> struct NarrowPlan {
         const int64_t most = tiles_of(rows, step);
         if (s > most) s = most;
         if (s > 1024) s = 1024;
+        if (rows <= 256) s = 1; // (two steps of one workgroup are shorter than another launch)
         share = tiles_of(tiles_of(rows, s), step) * step;
         shares = tiles_of(rows, share);
         indexed = rows >= INDEXED;
@@ -553,7 +558,7 @@ template <typename T> struct NarrowPlan {
             w = take(A * (size_t)rows);
             at = take(4 * (size_t)rows);
             scale = take(A * SCALE_PARTS);
-            part = take(A * (size_t)(shares * V * (D + 1)));
+            part = shares > 1 ? take(A * (size_t)(shares * V * (D + 1))) : 0;
         }
         bytes = to;
     }
@@ -591,7 +596,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     a.lp = (A*)c.lp;
     if (p.indexed) {
         class_index<A><<<dim3((unsigned)tiles_of(c.rows, INDEX_ROWS)), dim3(1024), 0, st>>>(
-            c.y, c.rows, c.classes, nullptr, (int*)(ws + p.order), (int*)(ws + p.y_of), (int*)(ws + p.count), a.lp);
+            c.y, c.rows, c.classes, nullptr, (int*)(ws + p.order), (int*)(ws + p.y_of), (int*)(ws + p.count), a.lp, nullptr, nullptr);
         a.order = (const int*)(ws + p.order);
         a.count = (const int*)(ws + p.count);
     }
@@ -600,7 +605,9 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
         a.w = (A*)(ws + p.w);
         a.at = (int*)(ws + p.at);
         a.xbar = (T*)c.xbar;
-        a.part = (A*)(ws + p.part);
+        a.part = p.shares > 1 ? (A*)(ws + p.part) : nullptr;
+        a.betabar = (T*)c.betabar;
+        a.alphabar = (T*)c.alphabar;
         a.share = p.share;
         if (sizeof(T) == 2 && c.lpbar) { // (r is not rounded otherwise)
             a.largest.parts = (const A*)(ws + p.scale);
@@ -616,7 +623,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
         else run<T, 4>(a, p, vjp, st);
     }
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !vjp) return e;
+    if (e != hipSuccess || !vjp || p.shares == 1) return e;
     class_narrow_join<T><<<dim3((unsigned)tiles_of(c.classes * (c.features + 1), 256)), dim3(256), 0, st>>>(
         a.part, (int)p.shares, c.classes, c.features, a.largest, (T*)c.betabar, (T*)c.alphabar);
     return hipGetLastError();

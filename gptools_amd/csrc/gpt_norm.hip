@@ -120,10 +120,11 @@ template <typename T, int THREADS, int ITER> struct RowRaw {
 // Rows go round the workgroups' groups of THREADS threads; the next row's vectors are on their way while this one is
 // reduced. The sums for the parameters' gradients stay in registers, and go to partial[2][gridDim.x][n] at the end
 // (norm_param_sum adds them up in a fixed order).
-template <typename T, int THREADS, int ITER, bool PARAMS>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row_vjp(NormArgs a) {
+// A workgroup alone (few rows) writes the results themselves.
+template <typename T, int THREADS, int ITER, bool PARAMS, int GROUPS>
+__global__ __launch_bounds__(THREADS * GROUPS) void norm_row_vjp(NormArgs a) {
     typedef acc_t<T> A;
-    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, GROUPS = BLOCK / THREADS, N = Vec16<T>::N, K = ITER * N;
+    constexpr int N = Vec16<T>::N, K = ITER * N;
     __shared__ A red[2][THREADS / 64 * 2];
     __shared__ A joined[PARAMS && GROUPS > 1 ? GROUPS - 1 : 1][PARAMS && GROUPS > 1 ? 2 * K * THREADS : 1];
     const int t = threadIdx.x % THREADS, group = threadIdx.x / THREADS;
@@ -192,6 +193,16 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row_vjp(No
                     wbar[j] += joined[k][j * THREADS + t];
                     bbar[j] += joined[k][(K + j) * THREADS + t];
                 }
+        }
+        if (gridDim.x == 1) {
+            RowRegs<T, THREADS, ITER> u;
+#pragma unroll
+            for (int j = 0; j < K; ++j) u.v[j] = wbar[j];
+            u.store((T*)a.wbar, n, t);
+#pragma unroll
+            for (int j = 0; j < K; ++j) u.v[j] = bbar[j];
+            u.store((T*)a.bbar, n, t);
+            return;
         }
         A* p = (A*)a.partial + (int64_t)blockIdx.x * n;
         const int64_t other = (int64_t)gridDim.x * n;
@@ -463,9 +474,11 @@ template <typename T> LongPlan long_plan(int64_t rows, int64_t n) {
     if (p.groups > rows) p.groups = rows;
     return p;
 }
-// Workgroups of the reverse mode on whole rows: enough to fill the card, and at least 8 rows each where there are as many (each
-// leaves 2 n partial sums). small: four rows at a time
+// Workgroups of the reverse mode on whole rows: one where the rows are few (its rounds are shorter than another launch), else
+// enough to fill the card, and at least 8 rows each where there are as many (each leaves 2 n partial sums). small: a wave takes a
+// row, a workgroup 4 at a time, or 16 if it is alone
 int64_t row_blocks(int64_t rows, bool small) {
+    if (rows <= (small ? 32 : 2)) return 1;
     const int64_t groups = small ? (rows + 3) / 4 : rows;
     return groups < 256 ? groups : groups < 8192 ? (groups / 8 > 256 ? groups / 8 : 256) : 1024;
 }
@@ -514,10 +527,14 @@ template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <typename T, int THREADS, int ITER, int GROUPS> void launch_groups(const NormArgs& a, unsigned blocks, hipStream_t st) {
+    if (a.wbar) norm_row_vjp<T, THREADS, ITER, true, GROUPS><<<dim3(blocks), dim3(THREADS * GROUPS), 0, st>>>(a);
+    else norm_row_vjp<T, THREADS, ITER, false, GROUPS><<<dim3(blocks), dim3(THREADS * GROUPS), 0, st>>>(a);
+}
 template <typename T, int THREADS, int ITER> void launch_row_vjp(const NormArgs& a, unsigned blocks, hipStream_t st) {
-    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS;
-    if (a.wbar) norm_row_vjp<T, THREADS, ITER, true><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
-    else norm_row_vjp<T, THREADS, ITER, false><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
+    if constexpr (THREADS > 64) launch_groups<T, THREADS, ITER, 1>(a, blocks, st);
+    else if (blocks == 1) launch_groups<T, THREADS, ITER, 16>(a, blocks, st);
+    else launch_groups<T, THREADS, ITER, 4>(a, blocks, st);
 }
 template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
     typedef acc_t<T> A;
@@ -527,6 +544,7 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
     if (n * (int64_t)sizeof(T) <= VJP_ROW_BYTES) {
         parts = row_blocks(a.rows, small_row<T>(n));
         const unsigned b = (unsigned)parts;
+        if (parts == 1) parts = 0; // (nothing left to add up)
         if (vecs <= 64) launch_row_vjp<T, 64, 1>(a, b, st);
         else if (vecs <= 128) launch_row_vjp<T, 64, 2>(a, b, st);
         else if (vecs <= 256) launch_row_vjp<T, 256, 1>(a, b, st);
