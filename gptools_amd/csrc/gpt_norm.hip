@@ -307,40 +307,53 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
     }
 }
 
-// mean and rstd of a row from its pieces', one workgroup a row
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_join(NormArgs a, int pieces) {
+// mean and rstd of a row from its pieces', for a whole workgroup
+template <typename T> __device__ __forceinline__ void long_moments(const NormArgs& a, int64_t row, int pieces, acc_t<T>& mean, acc_t<T>& rstd) {
     typedef acc_t<T> A;
     __shared__ A red[LONG_THREADS / 64];
     const int t = threadIdx.x;
-    const A* p = (const A*)a.partial + (int64_t)blockIdx.x * pieces * 3;
+    const A* p = (const A*)a.partial + row * pieces * 3;
     const A whole = (A)a.piece, tail = (A)(a.width - (int64_t)(pieces - 1) * a.piece); // values of a piece, of the last
     A s[1] = {0};
     for (int i = t; i < pieces; i += LONG_THREADS) s[0] += (i + 1 < pieces ? whole : tail) * p[3 * i] + p[3 * i + 1];
     row_sum<LONG_THREADS>(s, red, false);
-    const A mean = s[0] / (A)a.width;
+    mean = s[0] / (A)a.width;
     s[0] = 0;
     for (int i = t; i < pieces; i += LONG_THREADS) {
         const A d = p[3 * i] - mean;
         s[0] += p[3 * i + 2] + d * ((A)2 * p[3 * i + 1] + (i + 1 < pieces ? whole : tail) * d);
     }
     row_sum<LONG_THREADS>(s, red, true);
-    if (t == 0) {
-        ((A*)a.mean)[blockIdx.x] = mean;
-        ((A*)a.rstd)[blockIdx.x] = (A)1 / sqrt(s[0] / (A)a.width + (A)a.eps);
+    rstd = (A)1 / sqrt(s[0] / (A)a.width + (A)a.eps);
+}
+// ... one workgroup a row
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_join(NormArgs a, int pieces) {
+    acc_t<T> mean, rstd;
+    long_moments<T>(a, blockIdx.x, pieces, mean, rstd);
+    if (threadIdx.x == 0) {
+        ((acc_t<T>*)a.mean)[blockIdx.x] = mean;
+        ((acc_t<T>*)a.rstd)[blockIdx.x] = rstd;
     }
 }
 
-// The second sweep, 32 KB a workgroup. (Taking the rows one lattice at a time, so that it finds them in the last-level cache,
+// The second sweep, 32 KB a workgroup. join > 0: the row's moments from that many pieces, by each workgroup for itself. (Taking the rows one lattice at a time, so that it finds them in the last-level cache,
 // costs more in short launches than it saves: 16 lattices of 4096 x 4096 in fp64 1350 us against 1170.)
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a) {
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a, int join) {
     typedef acc_t<T> A;
     constexpr int K = LONG_ITER * Vec16<T>::N;
     const int t = threadIdx.x;
     const int64_t row = blockIdx.y, k = (int64_t)blockIdx.x * long_sweep<T>();
-    const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
     const int64_t n = a.width - k < long_sweep<T>() ? a.width - k : long_sweep<T>();
     RowRegs<T, LONG_THREADS, LONG_ITER> r, w;
     r.load((const T*)a.x + row * a.width + k, n, t);
+    A mean, rstd;
+    if (join) {
+        long_moments<T>(a, row, join, mean, rstd);
+        if (t == 0 && blockIdx.x == 0) {
+            ((A*)a.mean)[row] = mean;
+            ((A*)a.rstd)[row] = rstd;
+        }
+    } else mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
 #pragma unroll
     for (int j = 0; j < K; ++j) r.v[j] = (r.v[j] - mean) * rstd;
     if (a.weight) {
@@ -413,42 +426,51 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
     }
 }
 
-// sums[row] = (<g>, <g h>): one workgroup a row
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_rows(NormArgs a, int64_t pieces) {
+// (<g>, <g h>) of a row from its pieces', for a whole workgroup
+template <typename T> __device__ __forceinline__ void long_means(const NormArgs& a, int64_t row, int64_t pieces, acc_t<T> (&s)[2]) {
     typedef acc_t<T> A;
     __shared__ A red[LONG_THREADS / 64 * 2];
-    const A* p = (const A*)a.partial + (int64_t)blockIdx.x * pieces * 2;
-    A s[2] = {0, 0};
+    const A* p = (const A*)a.partial + row * pieces * 2;
+    s[0] = s[1] = 0;
     for (int64_t i = threadIdx.x; i < pieces; i += LONG_THREADS) {
         s[0] += p[2 * i];
         s[1] += p[2 * i + 1];
     }
     row_sum<LONG_THREADS>(s, red, true);
+    s[0] /= (A)a.width;
+    s[1] /= (A)a.width;
+}
+// ... one workgroup a row, into sums
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_rows(NormArgs a, int64_t pieces) {
+    acc_t<T> s[2];
+    long_means<T>(a, blockIdx.x, pieces, s);
     if (threadIdx.x == 0) {
-        ((A*)a.sums)[2 * (int64_t)blockIdx.x] = s[0] / (A)a.width;
-        ((A*)a.sums)[2 * (int64_t)blockIdx.x + 1] = s[1] / (A)a.width;
+        ((acc_t<T>*)a.sums)[2 * (int64_t)blockIdx.x] = s[0];
+        ((acc_t<T>*)a.sums)[2 * (int64_t)blockIdx.x + 1] = s[1];
     }
 }
 
-// second sweep: xbar
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_apply(NormArgs a) {
+// second sweep: xbar. join > 0: the row's means from that many pieces, by each workgroup for itself
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_apply(NormArgs a, int64_t join) {
     typedef acc_t<T> A;
     constexpr int K = LONGB_ITER * Vec16<T>::N;
     const int t = threadIdx.x;
     const int64_t row = blockIdx.y, k0 = (int64_t)blockIdx.x * longb_sweep<T>();
     const int64_t n = a.width - k0 < longb_sweep<T>() ? a.width - k0 : longb_sweep<T>();
     const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
-    const A c0 = ((const A*)a.sums)[2 * row], c1 = ((const A*)a.sums)[2 * row + 1];
     RowRegs<T, LONG_THREADS, LONGB_ITER> x, g, w;
     x.load((const T*)a.x + row * a.width + k0, n, t);
     g.load((const T*)a.ybar + row * a.width + k0, n, t);
+    A c[2];
+    if (join) long_means<T>(a, row, join, c);
+    else c[0] = ((const A*)a.sums)[2 * row], c[1] = ((const A*)a.sums)[2 * row + 1];
     if (a.weight) {
         w.load((const T*)a.weight + k0, n, t);
 #pragma unroll
         for (int j = 0; j < K; ++j) g.v[j] *= w.v[j];
     }
 #pragma unroll
-    for (int j = 0; j < K; ++j) x.v[j] = rstd * (g.v[j] - c0 - (x.v[j] - mean) * rstd * c1);
+    for (int j = 0; j < K; ++j) x.v[j] = rstd * (g.v[j] - c[0] - (x.v[j] - mean) * rstd * c[1]);
     x.store((T*)a.xbar + row * a.width + k0, n, t);
 }
 
@@ -456,6 +478,7 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
 constexpr int64_t ROW_BYTES = 65536;   // longest row that one workgroup keeps in registers (1024 threads x 4 vectors)
 constexpr int64_t VJP_ROW_BYTES = 32768; // ... with its cotangent and its gradient sums (1024 threads x 2 vectors)
 constexpr int64_t MAX_GRID_Y = 65535;
+constexpr int64_t FEW_PIECES = 256; // of a row that the second sweep's workgroups add up for themselves rather than in a launch before
 
 struct LongPlan {
     int64_t piece, pieces;   // forward: elements of a piece (a multiple of the sweep), pieces of a row
@@ -486,7 +509,10 @@ template <typename T> bool small_row(int64_t n) { return n <= 128 * Vec16<T>::N;
 
 template <typename T> size_t workspace(int64_t rows, int64_t n, bool vjp) {
     const size_t A = sizeof(acc_t<T>);
-    if (n * (int64_t)sizeof(T) <= (vjp ? VJP_ROW_BYTES : ROW_BYTES)) return vjp ? A * 2 * (size_t)(row_blocks(rows, small_row<T>(n)) * n) : 0;
+    if (n * (int64_t)sizeof(T) <= (vjp ? VJP_ROW_BYTES : ROW_BYTES)) {
+        const int64_t blocks = vjp ? row_blocks(rows, small_row<T>(n)) : 1;
+        return blocks > 1 ? A * 2 * (size_t)(blocks * n) : 0;
+    }
     const LongPlan p = long_plan<T>(rows, n);
     if (!vjp) return A * 3 * (size_t)(rows * p.pieces);
     return A * (2 * (size_t)(rows * p.vpieces) + 2 * (size_t)rows + (p.groups > 1 ? 2 * (size_t)(p.groups * n) : 0));
@@ -521,8 +547,10 @@ template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
         s.rstd = (char*)a.rstd + as * (size_t)r0;
         s.partial = (char*)a.partial + as * 3 * (size_t)(r0 * p.pieces);
         norm_long_stats<T><<<dim3((unsigned)p.pieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
-        norm_long_join<T><<<dim3((unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s, (int)p.pieces);
-        norm_long_apply<T><<<dim3((unsigned)((a.width + long_sweep<T>() - 1) / long_sweep<T>()), (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
+        const bool small = p.pieces <= FEW_PIECES;
+        if (!small) norm_long_join<T><<<dim3((unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s, (int)p.pieces);
+        norm_long_apply<T><<<dim3((unsigned)((a.width + long_sweep<T>() - 1) / long_sweep<T>()), (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(
+            s, small ? (int)p.pieces : 0);
     }
     return hipGetLastError();
 }
@@ -556,7 +584,8 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
         a.sums = (A*)a.partial + 2 * a.rows * p.vpieces;
         a.partial2 = (A*)a.sums + 2 * a.rows;
         norm_long_vjp_sums<T><<<dim3((unsigned)p.vpieces, (unsigned)p.groups), dim3(LONG_THREADS), 0, st>>>(a);
-        norm_long_vjp_rows<T><<<dim3((unsigned)a.rows), dim3(LONG_THREADS), 0, st>>>(a, p.vpieces);
+        const bool small = p.vpieces <= FEW_PIECES;
+        if (!small) norm_long_vjp_rows<T><<<dim3((unsigned)a.rows), dim3(LONG_THREADS), 0, st>>>(a, p.vpieces);
         for (int64_t r0 = 0; r0 < a.rows; r0 += MAX_GRID_Y) {
             NormArgs s = a;
             s.rows = a.rows - r0 < MAX_GRID_Y ? a.rows - r0 : MAX_GRID_Y;
@@ -566,7 +595,8 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
             s.mean = (A*)a.mean + r0;
             s.rstd = (A*)a.rstd + r0;
             s.sums = (A*)a.sums + 2 * r0;
-            norm_long_vjp_apply<T><<<dim3((unsigned)p.vpieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
+            s.partial = (A*)a.partial + 2 * r0 * p.vpieces;
+            norm_long_vjp_apply<T><<<dim3((unsigned)p.vpieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s, small ? p.vpieces : 0);
         }
         parts = p.groups > 1 ? p.groups : 0;
         parted = (A*)a.partial2;
