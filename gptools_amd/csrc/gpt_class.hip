@@ -74,14 +74,7 @@ template <typename T, typename Tl_, int PLANES_> struct Way {
 // Two values in one word (plane p of them)
 template <typename W> __device__ __forceinline__ void words(float a, float b, uint32_t (&u)[W::PLANES]) {
     if constexpr (W::PLANES == 3) {
-        bf16_t x[3], y[3];
-        split3(a, x[0], x[1], x[2]);
-        split3(b, y[0], y[1], y[2]);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            typedef bf16_t V2 __attribute__((ext_vector_type(2)));
-            u[p] = __builtin_bit_cast(uint32_t, V2{x[p], y[p]});
-        }
+        split3(a, b, u);
     } else u[0] = pack2<typename W::Element>(a, b);
 }
 
@@ -297,17 +290,11 @@ template <typename W> __device__ __forceinline__ void gather(const GatherArgs<W>
         }
         typename W::Element* to = a.out + at * ldo + k;
         if constexpr (W::PLANES == 3) {
-            typename Vec16<bf16_t>::V u[3];
+            uint32_t u[N / 2][3];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                bf16_t a, b, c;
-                split3(v[e], a, b, c);
-                u[0][e] = a;
-                u[1][e] = b;
-                u[2][e] = c;
-            }
+            for (int e = 0; e < N / 2; ++e) split3(v[2 * e], v[2 * e + 1], u[e]);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<typename Vec16<bf16_t>::V*>(to + p * plane) = u[p];
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(to + p * plane) = make_uint4(u[0][p], u[1][p], u[2][p], u[3][p]);
         } else {
 #pragma unroll
             for (int h = 0; h < N; h += Vec16<T>::N) {
@@ -393,17 +380,11 @@ template <typename W> __device__ __forceinline__ void transpose(const TransposeA
         if (c >= cols || r >= ldo) continue;
         typename W::Element* to = out + c * ldo + r;
         if constexpr (W::PLANES == 3) {
-            typename Vec16<bf16_t>::V u[3];
+            uint32_t u[4][3];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                bf16_t x, y, z;
-                split3(tile[b + e][a + 32 * h], x, y, z);
-                u[0][e] = x;
-                u[1][e] = y;
-                u[2][e] = z;
-            }
+            for (int e = 0; e < 4; ++e) split3(tile[b + 2 * e][a + 32 * h], tile[b + 2 * e + 1][a + 32 * h], u[e]);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<typename Vec16<bf16_t>::V*>(to + p * plane) = u[p];
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(to + p * plane) = make_uint4(u[0][p], u[1][p], u[2][p], u[3][p]);
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k += Vec16<T>::N) {

@@ -72,13 +72,15 @@ template <typename T, int DT> struct Narrow {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const Vec u = tile_chunk(o, row, (int64_t)((4 * g + q) * 8 + 4 * h), D);
+                        uint32_t w[2][3];
+                        split3(u[0], u[1], w[0]);
+                        split3(u[2], u[3], w[1]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            bf16_t a, b, c;
-                            split3(u[e], a, b, c);
-                            s[0][g][4 * h + e] = a;
-                            s[1][g][4 * h + e] = b;
-                            s[2][g][4 * h + e] = c;
+                        for (int p = 0; p < 3; ++p) {
+                            uint4 k = __builtin_bit_cast(uint4, s[p][g]);
+                            if (h) k.z = w[0][p], k.w = w[1][p];
+                            else k.x = w[0][p], k.y = w[1][p];
+                            s[p][g] = __builtin_bit_cast(SVec, k);
                         }
                     }
             } else {
@@ -126,13 +128,26 @@ template <typename T, int DT> struct Narrow {
     // there into LDS
     template <int STEP> static __device__ __forceinline__ void fetch(Vec (&v)[loads<STEP>()], const Operand<T>& o, int64_t r0, int64_t D,
                                                                      const int* order, const int64_t* y) {
+        const int left = (int)(o.rows - r0 < STEP ? o.rows - r0 : STEP);
+        const T* first = o.p + r0 * o.ld;
+        const int d = (int)D;
 #pragma unroll
         for (int i = 0; i < loads<STEP>(); ++i) {
-            const int id = i * 256 + threadIdx.x, r = id / (DP / N), c = id % (DP / N);
+            const int id = i * 256 + threadIdx.x, r = id / (DP / N), k = id % (DP / N) * N;
             v[i] = Vec{};
-            if (r >= STEP || r0 + r >= o.rows) continue;
-            const int64_t row = order ? order[r0 + r] : r0 + r;
-            if (!y || y[row] >= 0) v[i] = tile_chunk<T>({o.p, o.ld, row + 1, 0}, row, (int64_t)c * N, D);
+            if (r >= left || k >= d) continue;
+            const T* from = first + ((int64_t)r * o.ld + k);
+            if (order || y) {
+                const int64_t row = order ? order[r0 + r] : r0 + r;
+                if (y && y[row] < 0) continue;
+                from = o.p + row * o.ld + k;
+            }
+            if (k + N <= d) v[i] = load16(from);
+            else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (k + e < d) v[i][e] = from[e];
+            }
         }
     }
     template <int STEP> static __device__ __forceinline__ void put(const Vec (&v)[loads<STEP>()], T* lds) {
@@ -148,18 +163,11 @@ template <typename T, int DT> struct Narrow {
             }
             if constexpr (SPLIT) {
                 bf16_t* t = reinterpret_cast<bf16_t*>(lds + STEP * LD) + r * SLD + c * N;
-                typedef bf16_t V4 __attribute__((ext_vector_type(4)));
-                V4 u[3];
+                uint32_t u[2][3];
+                split3(v[i][0], v[i][1], u[0]);
+                split3(v[i][2], v[i][3], u[1]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    bf16_t x, y, z;
-                    split3(v[i][e], x, y, z);
-                    u[0][e] = x;
-                    u[1][e] = y;
-                    u[2][e] = z;
-                }
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<V4*>(t + p * STEP * SLD) = u[p];
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(t + p * STEP * SLD) = make_uint2(u[0][p], u[1][p]);
             }
         }
     }

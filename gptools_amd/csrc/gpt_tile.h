@@ -59,15 +59,23 @@ template <typename T> struct Operand {
     int64_t plane; // elements from one plane to the next
 };
 
-// fp32 as a sum of three bf16 values, each half a step (2^-8) or less of the one before (an infinity or a NaN stands in the
-// first alone). Six of the nine products of two such sums are taken, those down to 2^-16 of the whole; each one left out, and the
-// rest of the sum, is at most 2^-24, fp32's own rounding.
-__device__ __forceinline__ void split3(float v, bf16_t& a, bf16_t& b, bf16_t& c) {
-    a = (bf16_t)v;
-    const float r = v - (float)a;
-    const bool fine = r == r; // (inf - inf is not)
-    b = fine ? (bf16_t)r : (bf16_t)0.f;
-    c = fine ? (bf16_t)(r - (float)b) : (bf16_t)0.f;
+// fp32 as a sum of three bf16 values, by cutting off bits: each holds the eight leading bits of what is left (an infinity or a NaN
+// stands in the first). Six of the nine products of two such sums are taken; those left out are at most 2^-22 of the whole (the
+// second value is below 2^-7 of the first, the third below 2^-15), and 2^-26 on average. Here as fp32 values whose low halves are zero.
+__device__ __forceinline__ void split3(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
+    a = __builtin_bit_cast(uint32_t, v) & 0xffff0000u;
+    const float fa = __builtin_bit_cast(float, a);
+    const float r = v == fa ? 0.f : v - fa; // (inf - inf is not 0)
+    b = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
+    c = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, b));
+}
+// ... of two values, two bf16 in a word each
+__device__ __forceinline__ void split3(float v, float w, uint32_t (&u)[3]) {
+    uint32_t x[3], y[3];
+    split3(v, x[0], x[1], x[2]);
+    split3(w, y[0], y[1], y[2]);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) u[p] = __builtin_amdgcn_perm(y[p], x[p], 0x07060302u);
 }
 
 // One 16-byte chunk, zeros where it lies outside rows x [0, k1)

@@ -19,8 +19,8 @@ def test_workspace_sizes(lib, dtype):
         assert glm(dtype, *bad, 1) == 0
     assert norm(dtype, 1, 64, 0) == 0 and norm(dtype, 1, 64, 1) == 0 and norm(dtype, 100, 64, 1) > 0
     assert glm(dtype, 1, 1, 1, 1) > glm(dtype, 1, 1, 1, 0) >= 0 and glm(dtype, 100, 100, 100, 1) > glm(dtype, 100, 100, 100, 0) > 0
-    # the logits are not in it: 4096 rows of 128000 classes would take 2 GiB in fp32 alone
-    assert glm(dtype, 4096, 512, 128000, 0) < 128 << 20
+    # the logits are not in it: 4096 rows of 128000 classes would take 2 GiB in fp32 (a copy of beta may be, 6 bytes a value in fp32)
+    assert glm(dtype, 4096, 512, 128000, 0) < 512 << 20
     # r, for a piece of the classes and a block of the rows, is bounded; the rest grows with the rows or with the classes
     for rows in (1, 100, 4096, 100000, 1 << 20, 1 << 24):
         assert glm(dtype, rows, 64, 1000, 1) < (4 << 30)

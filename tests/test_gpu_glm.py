@@ -534,8 +534,10 @@ def test_refusals(glm):
         args[at] = value
         with pytest.raises(error):
             ctx.call(*args)
-    norm = ("gpt_layer_norm_vjp", 1, p[1], None, out.data_ptr(), out.data_ptr(), p[1], 4, 6, out.data_ptr(), out.data_ptr(),
-            out.data_ptr(), ws.data_ptr(), ws.numel())
+    many, sums = torch.zeros(100, 6, device="cuda"), torch.zeros(1000, device="cuda")
+    norm = ("gpt_layer_norm_vjp", 1, many.data_ptr(), None, sums.data_ptr(), sums.data_ptr(), many.data_ptr(), 100, 6, sums.data_ptr(),
+            sums.data_ptr(), sums.data_ptr(), ws.data_ptr(), glm._space("gpt_layer_norm_workspace", 1, 100, 6, 1))
+    assert 0 < norm[-1] <= ws.numel()
     for at, value, error in [(1, 9, NotImplementedError), (2, None, ValueError), (4, None, ValueError), (6, None, ValueError),
                              (7, -1, ValueError), (8, 0, ValueError), (9, None, ValueError), (10, None, ValueError),
                              (11, None, ValueError), (12, None, ValueError), (13, 0, ValueError)]:
@@ -544,4 +546,4 @@ def test_refusals(glm):
         with pytest.raises(error):
             ctx.call(*args)
     torch.cuda.synchronize()
-    assert not bool(out.any())
+    assert not bool(out.any()) and not bool(sums.any())
