@@ -33,7 +33,8 @@ int zero(gpt_ctx* c, void* p, size_t bytes) {
 
 bool known_type(int dtype) { return dtype == GPT_F64 || dtype == GPT_F32 || dtype == GPT_F16 || dtype == GPT_BF16; }
 size_t size_of(int dtype) { return dtype == GPT_F64 ? 8 : dtype == GPT_F32 ? 4 : 2; }
-constexpr int64_t MOST = 2147483647LL; // rows, features, classes (grids count them in 32 bits)
+constexpr int64_t MOST = 2147483647LL;                                       // rows
+constexpr int64_t MOST_FEATURES = (int64_t)1 << 21, MOST_CLASSES = (int64_t)1 << 26; // (grids count their tiles in 32 bits)
 constexpr int64_t MOST_WIDTH = (int64_t)1 << 40;
 
 int check_norm(gpt_ctx* c, int dtype, int64_t rows, int64_t width) {
@@ -46,7 +47,7 @@ int check_class(gpt_ctx* c, int dtype, int64_t ldx, int64_t ldbeta, int64_t rows
     if (!known_type(dtype)) return fail(c, GPT_ERR_UNSUPPORTED, "unknown element type");
     if (rows < 0 || features < 1 || classes < 1)
         return fail(c, GPT_ERR_SHAPE, "categorical_logit_glm needs rows >= 0, features >= 1 and classes >= 1");
-    if (rows > MOST || features > (1 << 21) || classes > MOST - 255)
+    if (rows > MOST || features > MOST_FEATURES || classes > MOST_CLASSES)
         return fail(c, GPT_ERR_SHAPE, "categorical_logit_glm: too many rows, features or classes");
     if (ldx < features || ldbeta < features) return fail(c, GPT_ERR_SHAPE, "rows of x and beta must not overlap (ldx, ldbeta >= features)");
     return GPT_OK;
@@ -140,7 +141,7 @@ int gpt_layer_norm_vjp(gpt_ctx* c, int dtype, const void* x, const void* weight,
 }
 
 size_t gpt_categorical_logit_glm_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, int vjp) {
-    return known_type(dtype) && rows > 0 && features > 0 && classes > 0 && rows <= MOST && features <= (1 << 21) && classes <= MOST - 255
+    return known_type(dtype) && rows > 0 && features > 0 && classes > 0 && rows <= MOST && features <= MOST_FEATURES && classes <= MOST_CLASSES
                ? gpt_class_workspace(dtype, rows, features, classes, vjp != 0)
                : 0;
 }

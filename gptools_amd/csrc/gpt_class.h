@@ -79,25 +79,43 @@ namespace { // (a kernel of its own in each of the two)
 
 // Numbers the observed rows: row[number], y[number] (any y that is no class as `classes`), their count; behind them row lists the
 // others, whose lp is 0. place (or null): the rows' numbers, -1 where there is no observation. parts (or null): the largest |lpbar| of
-// the observed rows of a workgroup, as class_scale leaves it. A workgroup takes INDEX_ROWS rows and counts those before them for itself.
+// the observed rows of a workgroup, as class_scale leaves it. A workgroup takes INDEX_ROWS rows; runs: the observed ones of every
+// INDEX_ROWS (class_count), or null, and it counts those before its own for itself.
 constexpr int INDEX_ROWS = 4096;
+constexpr int64_t INDEX_ALONE = 4 * INDEX_ROWS; // rows up to which counting the ones before is shorter than another launch
+__global__ __launch_bounds__(1024) void class_count(const int64_t* y, int64_t rows, int* runs) {
+    __shared__ int red[16];
+    const int64_t mine = (int64_t)blockIdx.x * INDEX_ROWS + 4 * threadIdx.x;
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n += mine + k < rows && y[mine + k] >= 0;
+    n = wave_sum(n);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) n += red[k];
+    runs[blockIdx.x] = n;
+}
 template <typename A> __global__ __launch_bounds__(1024) void class_index(const int64_t* y, int64_t rows, int64_t classes, int* place, int* row,
-                                                                         int* y_of, int* count, A* lp, const A* lpbar, A* parts) {
+                                                                         int* y_of, int* count, A* lp, const A* lpbar, A* parts,
+                                                                         const int* runs) {
     __shared__ int red[2][16];
     __shared__ A most[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * INDEX_ROWS, mine = first + 4 * threadIdx.x;
     int before = 0, n = 0;
-    auto some = [&](int64_t i, auto runs) { // (whole runs of 4096)
-        int64_t u[4 * decltype(runs)::value];
+    if (runs) {
+        for (int i = threadIdx.x; i < (int)blockIdx.x; i += 1024) before += runs[i];
+    } else {
+        for (int64_t i = threadIdx.x; i < first; i += INDEX_ROWS) { // (whole runs)
+            int64_t u[4];
 #pragma unroll
-        for (int k = 0; k < 4 * runs; ++k) u[k] = y[i + threadIdx.x + 1024 * k];
+            for (int k = 0; k < 4; ++k) u[k] = y[i + 1024 * k];
 #pragma unroll
-        for (int k = 0; k < 4 * runs; ++k) before += u[k] >= 0;
-    };
-    int64_t done = 0;
-    for (; done + 4 * INDEX_ROWS <= first; done += 4 * INDEX_ROWS) some(done, std::integral_constant<int, 4>());
-    for (; done < first; done += INDEX_ROWS) some(done, std::integral_constant<int, 1>());
+            for (int k = 0; k < 4; ++k) before += u[k] >= 0;
+        }
+    }
     int64_t v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -168,6 +186,15 @@ template <typename A> __global__ __launch_bounds__(256) void class_scale(const A
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0) parts[blockIdx.x] = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
+}
+
+// runs: room for a count of every INDEX_ROWS rows
+template <typename A> void number_rows(const int64_t* y, int64_t rows, int64_t classes, int* place, int* row, int* y_of, int* count, A* lp,
+                                       const A* lpbar, A* parts, int* runs, hipStream_t st) {
+    const dim3 grid((unsigned)((rows + INDEX_ROWS - 1) / INDEX_ROWS));
+    const bool alone = rows <= INDEX_ALONE;
+    if (!alone) class_count<<<grid, dim3(1024), 0, st>>>(y, rows, runs);
+    class_index<A><<<grid, dim3(1024), 0, st>>>(y, rows, classes, place, row, y_of, count, lp, lpbar, parts, alone ? nullptr : runs);
 }
 
 } // namespace

@@ -607,7 +607,7 @@ template <typename W> struct Plan {
     bool xwide, bwide; // wide tiles for xbar, betabar
     bool copy;         // beta as operands of its own
     // offsets in bytes
-    size_t place, row, y, count, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
+    size_t place, row, y, count, runs, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
     // (a product's splits of k count too: 16 rows of large tiles with a sixteenth of a long k each fill the card as well)
     static bool product_wide(int64_t m, int64_t n, int64_t K) {
         const int64_t tiles = tiles_of(m, 256) * tiles_of(n, 256);
@@ -629,6 +629,7 @@ template <typename W> struct Plan {
         row = take(4 * (size_t)block);
         y = take(4 * (size_t)block);
         count = take(4);
+        runs = take(4 * (size_t)tiles_of(block, INDEX_ROWS));
         part_max = take(A * (size_t)(tiles_v * block));
         part_sum = take(A * (size_t)(tiles_v * block));
         eta_y = take(A * (size_t)block);
@@ -754,8 +755,8 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         const T* x = (const T*)c.x + n0 * c.ldx;
         const int64_t ldrt = up_to(N, EDGE); // (r is written in whole tiles)
         const bool scale_here = largest.parts && p.blocks == 1;
-        class_index<A><<<dim3((unsigned)tiles_of(N, INDEX_ROWS)), dim3(1024), 0, st>>>(
-            c.y + n0, N, V, place, row, (int*)(ws + p.y), count, (A*)c.lp + n0, (const A*)c.lpbar, scale_here ? (A*)(ws + p.scale) : nullptr);
+        number_rows<A>(c.y + n0, N, V, place, row, (int*)(ws + p.y), count, (A*)c.lp + n0, (const A*)c.lpbar,
+                       scale_here ? (A*)(ws + p.scale) : nullptr, (int*)(ws + p.runs), st);
         PrepareArgs<W> q = {};
         q.g[0] = {x, c.ldx, N, D, place, xa, p.ldk, p.block * p.ldk, vjp ? (T*)c.xbar + n0 * D : nullptr};
         q.end[0] = (int)(tiles_of(N * (p.ldk / 8), 256) < 1024 ? tiles_of(N * (p.ldk / 8), 256) : 1024);

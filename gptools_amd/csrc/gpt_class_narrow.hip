@@ -45,6 +45,9 @@ template <typename T> struct NarrowArgs {
 // waves' shares, have not the registers and the LDS for two)
 template <typename T, int DT, int SHARES> constexpr int VT_ = sizeof(T) >= 4 && DT == 4 && SHARES == 4 ? 1 : 2;
 
+// waves of a SIMD that the registers have to leave room for
+template <typename T, int DT> constexpr int WAVES_ = sizeof(T) == 8 || (sizeof(T) == 4 && DT == 4) ? 2 : 4;
+
 template <typename T, int DT> struct Narrow {
     typedef acc_t<T> A;
     typedef typename Vec16<T>::V Vec;
@@ -228,7 +231,7 @@ template <typename T, int DT> struct Narrow {
 constexpr int larger(int a, int b) { return a > b ? a : b; }
 
 // WR groups of 16 NT rows x WV shares of the classes a workgroup
-template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __launch_bounds__(256, 2) void class_narrow_rows(NarrowArgs<T> a) {
+template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __launch_bounds__(256, (WAVES_<T, DT>)) void class_narrow_rows(NarrowArgs<T> a) {
     typedef Narrow<T, DT> W;
     typedef typename W::A A;
     typedef typename W::C C;
@@ -250,14 +253,15 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         return;
     }
     typename W::Part x[NT];
-    int64_t y[NT], row[NT];
+    int y[NT], row[NT]; // y: -1 without an observation, V where it is no class
     A ref[NT], sum[NT];
     C o[NT][DT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int64_t n = n0 + (wr * NT + t) * 16 + (lane & 15);
-        row[t] = n < a.x.rows ? (a.order ? a.order[n] : n) : -1;
-        y[t] = row[t] >= 0 ? a.y[row[t]] : -1;
+        row[t] = n < a.x.rows ? (a.order ? a.order[n] : (int)n) : -1;
+        const int64_t yn = row[t] >= 0 ? a.y[row[t]] : -1;
+        y[t] = yn < 0 ? -1 : yn < V ? (int)yn : (int)V;
         if (y[t] >= 0) x[t].load(a.x, row[t], D);
         else x[t].clear();
         ref[t] = neg_inf<A>();
@@ -368,7 +372,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
             if (VJP) {
                 a.lse[n] = none ? -neg_inf<A>() : lse;
                 a.w[n] = w / largest;
-                a.at[n] = known ? (int)y[t] : -1;
+                a.at[n] = known ? y[t] : -1;
             }
         }
         if (VJP) {
@@ -398,7 +402,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 }
 
 // WV groups of 16 NT classes x WR shares of the rows of this workgroup's share
-template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds__(256, 2) void class_narrow_classes(NarrowArgs<T> a) {
+template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds__(256, (WAVES_<T, DT>)) void class_narrow_classes(NarrowArgs<T> a) {
     typedef Narrow<T, DT> W;
     typedef typename W::A A;
     typedef typename W::C C;
@@ -534,7 +538,7 @@ template <typename T> struct NarrowPlan {
     static constexpr int NT = sizeof(T) == 8 ? 1 : 2;
     bool many_rows, many_classes, indexed;
     int64_t share, shares;
-    size_t lse, w, at, scale, order, y_of, count, part, bytes;
+    size_t lse, w, at, scale, order, y_of, count, runs, part, bytes;
     NarrowPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
         const size_t A = sizeof(acc_t<T>);
         many_rows = tiles_of(rows, 64 * NT) >= 512;
@@ -555,11 +559,12 @@ template <typename T> struct NarrowPlan {
             to += (n + 255) / 256 * 256;
             return p;
         };
-        order = y_of = count = 0;
+        order = y_of = count = runs = 0;
         if (indexed) {
             order = take(4 * (size_t)rows);
             y_of = take(4 * (size_t)rows);
             count = take(4);
+            runs = take(4 * (size_t)tiles_of(rows, INDEX_ROWS));
         }
         if (vjp) {
             lse = take(A * (size_t)rows);
@@ -603,8 +608,8 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     a.features = c.features;
     a.lp = (A*)c.lp;
     if (p.indexed) {
-        class_index<A><<<dim3((unsigned)tiles_of(c.rows, INDEX_ROWS)), dim3(1024), 0, st>>>(
-            c.y, c.rows, c.classes, nullptr, (int*)(ws + p.order), (int*)(ws + p.y_of), (int*)(ws + p.count), a.lp, nullptr, nullptr);
+        number_rows<A>(c.y, c.rows, c.classes, nullptr, (int*)(ws + p.order), (int*)(ws + p.y_of), (int*)(ws + p.count), a.lp, nullptr,
+                       nullptr, (int*)(ws + p.runs), st);
         a.order = (const int*)(ws + p.order);
         a.count = (const int*)(ws + p.count);
     }
