@@ -59,6 +59,9 @@ template <typename T> struct LogitArgs {
     int64_t ldr, ldrt, r_plane, rt_plane;
     A* part_alpha; // [tiles_n][ldr] or null
     Largest<A> largest;
+    // logits of the first kept_classes classes, as the first sweep leaves them for the second: tile by tile, a lane's fragments
+    typename T::Tl::C* kept;
+    int64_t kept_classes;
 };
 
 // One way to run the products: data type, tile, type and number of planes of its operands
@@ -78,11 +81,11 @@ template <typename W> __device__ __forceinline__ void words(float a, float b, ui
     } else u[0] = pack2<typename W::Element>(a, b);
 }
 
-// Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r.
-template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) void class_logits(LogitArgs<W> a) {
+// Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r. KEPT: eta was kept.
+template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class_logits(LogitArgs<W> a) {
     typedef typename W::Acc A;
     typedef typename W::Tl Tl;
-    __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
+    __shared__ typename Tl::Vec lds[KEPT ? 1 : Tl::LDS_BYTES / 16];
     __shared__ A red[2][Tl::WM > Tl::WN ? Tl::WM : Tl::WN][Tl::BM > Tl::BN ? Tl::BM : Tl::BN];
     const int64_t rows = *a.count, ld = a.x.rows;
     int64_t tm, tn;
@@ -90,11 +93,11 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
     const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
     const int nv = (int)(a.beta.rows - m0 < Tl::BM ? a.beta.rows - m0 : Tl::BM); // classes of this tile
     // what the tile's classes and rows need besides, on its way into LDS while the product runs (which ends with a barrier)
-    __shared__ A al[Tl::BM], lse_of[STATS ? 1 : Tl::BN], w_of[STATS ? 1 : Tl::BN];
+    __shared__ A al[KEPT ? 1 : Tl::BM], lse_of[STATS ? 1 : Tl::BN], w_of[STATS ? 1 : Tl::BN];
     __shared__ int at_of[Tl::BN];
     A largest = 1;
     if (!STATS) largest = a.largest.get();
-    for (int c = threadIdx.x; c < Tl::BM; c += Tl::THREADS)
+    for (int c = threadIdx.x; !KEPT && c < Tl::BM; c += Tl::THREADS)
         al[c] = c < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + c]) : (A)0) : neg_inf<A>();
     for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
         const int64_t n = n0 + c, y = n < rows ? a.y[n] : -1, from = y - (a.v0 + m0);
@@ -108,17 +111,33 @@ template <typename W, bool STATS> __global__ __launch_bounds__(W::Tl::THREADS) v
         }
     }
     a.x.rows = rows;
-    Tl tl;
-    tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
     const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Tl::WN, wn = (threadIdx.x >> 6) % Tl::WN;
+    const int64_t kept_tile = (a.v0 + m0) / Tl::BM * ((ld + Tl::BN - 1) / Tl::BN) + tn;
+    auto* kept = a.kept + kept_tile * (Tl::TM * Tl::TN * Tl::THREADS) + threadIdx.x;
+    Tl tl;
+    if constexpr (KEPT) {
 #pragma unroll
-    for (int i = 0; i < Tl::TM; ++i)
+        for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const A v = al[Tl::row(i, r)];
+            for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j] = kept[(i * Tl::TN + j) * Tl::THREADS];
+        __syncthreads();
+    } else {
+        tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
 #pragma unroll
-            for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + v;
-        }
+        for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const A v = al[Tl::row(i, r)];
+#pragma unroll
+                for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + v;
+            }
+    }
+    if (STATS && m0 < a.kept_classes) {
+#pragma unroll
+        for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < Tl::TN; ++j) kept[(i * Tl::TN + j) * Tl::THREADS] = tl.acc[i][j];
+    }
     if (STATS) {
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j) {
@@ -546,7 +565,7 @@ template <typename W> struct ProductsArgs {
     AlphaArgs<typename W::Data> alpha;
     int end[2];
 };
-template <typename W> __global__ __launch_bounds__(W::Tl::THREADS) void class_products(ProductsArgs<W> a) {
+template <typename W> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class_products(ProductsArgs<W> a) {
     typedef typename W::Tl Tl;
     __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
     const int id = blockIdx.x;
@@ -584,6 +603,7 @@ int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
 
 constexpr int64_t ROW_BLOCK = 1 << 18;              // rows taken at a time
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20; // r in both orders, of a piece of the classes and a block of the rows
+constexpr int64_t KEPT_BYTES = (int64_t)1 << 30;    // logits kept from the first sweep for the second
 constexpr int64_t FILL = 512;                       // workgroups that fill the card
 constexpr int64_t WIDE_TILES = 192;                 // 256 x 256 tiles from this many on
 
@@ -597,17 +617,22 @@ int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
 // 256 x 256 tiles for a product of m x n results?
 bool wide(int64_t m, int64_t n) { return tiles_of(m, 256) * tiles_of(n, 256) >= WIDE_TILES; }
 
+// Features from which writing a logit and reading it again takes less time than computing it again. With and without, in us: bf16 4096 x
+// 32000, 512 features 763 / 724, 1024 features 1125 / 1188; fp32 100 features (2000 x 8000) 205 / 194, 270 (275 x 13636) 192 / 215; fp64
+// 100 (2000 x 2000) 194 / 211
+template <typename T> constexpr int64_t keep_features() { return sizeof(T) == 2 ? 768 : sizeof(T) == 4 ? 160 : 64; }
+
 // W: the way of the logits. The products with r take the larger tile or the smaller by themselves
 template <typename W> struct Plan {
     typedef typename W::Data T;
     typedef typename W::Element E;
     static constexpr int64_t EDGE = W::Tl::BM;
     int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
-    int64_t xsplits, bsplits;
+    int64_t xsplits, bsplits, kept_pieces;
     bool xwide, bwide; // wide tiles for xbar, betabar
     bool copy;         // beta as operands of its own
     // offsets in bytes
-    size_t place, row, y, count, runs, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
+    size_t kept, place, row, y, count, runs, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
     // (a product's splits of k count too: 16 rows of large tiles with a sixteenth of a long k each fill the card as well)
     static bool product_wide(int64_t m, int64_t n, int64_t K) {
         const int64_t tiles = tiles_of(m, 256) * tiles_of(n, 256);
@@ -646,6 +671,10 @@ template <typename W> struct Plan {
             pieces = tiles_of(classes, piece);
             ldr = piece;
             ldrt = up_to(block, EDGE);
+            const int64_t logits = (int64_t)A * piece * ldrt;
+            kept_pieces = features >= keep_features<T>() ? KEPT_BYTES / logits : 0;
+            if (kept_pieces > pieces) kept_pieces = pieces;
+            kept = take((size_t)(kept_pieces * logits));
             lse = take(A * (size_t)block);
             scale = take(A * SCALE_PARTS);
             r = take(S * (size_t)(ldrt * ldr));
@@ -670,10 +699,10 @@ template <typename W> struct Plan {
     }
 };
 
-template <typename W, bool STATS> void logits(LogitArgs<W> l, hipStream_t st) {
+template <typename W, bool STATS, bool KEPT> void logits(LogitArgs<W> l, hipStream_t st) {
     typedef typename W::Tl Tl;
     l.tiles_v = tiles_of(l.beta.rows, Tl::BM);
-    class_logits<W, STATS><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
+    class_logits<W, STATS, KEPT><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
 // xbar and betabar of a piece (each complete if its `last`), alphabar (blocks: its workgroups, or none)
@@ -786,7 +815,9 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         l.part_sum = (A*)(ws + p.part_sum);
         l.eta_y = (A*)(ws + p.eta_y);
         l.largest = largest;
-        logits<W, true>(l, st);
+        l.kept = (typename W::Tl::C*)(ws + p.kept);
+        l.kept_classes = vjp ? p.kept_pieces * p.piece : 0;
+        logits<W, true, false>(l, st);
         A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
         class_join<A><<<dim3((unsigned)tiles_of(N, 8)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
                                                                             tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
@@ -812,7 +843,8 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
             l.ldr = up_to(nv, EDGE);
             l.r_plane = ldrt * l.ldr;
             l.rt_plane = l.ldr * ldrt;
-            logits<W, false>(l, st);
+            if (v0 < l.kept_classes) logits<W, false, true>(l, st);
+            else logits<W, false, false>(l, st);
             ProductsArgs<W> m = {};
             m.x.A = {bt, l.ldr, D, D * l.ldr};
             m.x.B = {r, l.ldr, N, l.r_plane};

@@ -115,12 +115,31 @@ template <typename T> struct SmallTile {
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = C{0, 0, 0, 0};
         Vec next[LOADS];
-        auto fetch = [&](int64_t k) {
+        // rows behind the last repeat it: their products are not used
+        const T* from[LOADS];
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int id = i * THREADS + t, row = id / TILE_CHUNKS, c = id % TILE_CHUNKS;
-                const int64_t kk = k + c * Vec16<T>::N;
-                next[i] = row < BM ? tile_chunk(A, m0 + row, kk, k1) : tile_chunk(B, n0 + (row - BM), kk, k1);
+        for (int i = 0; i < LOADS; ++i) {
+            const int id = i * THREADS + t, row = id / TILE_CHUNKS, c = id % TILE_CHUNKS;
+            const bool a = row < BM;
+            const int64_t r = a ? m0 + row : n0 + (row - BM), last = (a ? A.rows : B.rows) - 1;
+            from[i] = (a ? A.p : B.p) + (r < last ? r : last) * (a ? A.ld : B.ld) + c * Vec16<T>::N;
+        }
+        auto fetch = [&](int64_t k) {
+            if (k + tile_k<T>() <= k1) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) next[i] = load16(from[i] + k);
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) { // the rest of k: zeros behind it
+                const int64_t left = k1 - k - (i * THREADS + t) % TILE_CHUNKS * Vec16<T>::N;
+                next[i] = Vec{};
+                if (left >= Vec16<T>::N) next[i] = load16(from[i] + k);
+                else {
+#pragma unroll
+                    for (int e = 0; e < Vec16<T>::N; ++e)
+                        if (e < left) next[i][e] = from[i][k + e];
+                }
             }
         };
         auto put = [&](Vec* to) {
