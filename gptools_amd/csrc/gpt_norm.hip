@@ -15,23 +15,69 @@ using namespace gptt;
 namespace {
 
 // ---- rows that fit the registers of one workgroup ---------------------------------------------------------------------
-// THREADS consecutive threads take a row, ITER 16-byte vectors each, THREADS apart.
+// THREADS consecutive threads take a row, ITER 16-byte vectors each, THREADS apart. load() only issues loads, whole vectors without a
+// branch, so that none waits for another: those behind the row's end read its last N values, and so does the one that the end cuts.
+// settle() puts them right when they have come: the cut one moved to its place, zeros behind the end. (8191 rows of 1001 fp32 values,
+// reverse mode: 19 us against 22 with a branch at every vector.) Where every value is taken by itself, nothing need move: mine()
+// says which values of a vector are the row's and no other vector's. FULL: n is THREADS * ITER * N.
+template <typename T, int THREADS, int ITER> struct RowRaw {
+    static constexpr int N = Vec16<T>::N;
+    typename Vec16<T>::V v[ITER];
+    template <bool FULL = false> __device__ __forceinline__ void load(const T* p, int64_t n, int t) {
+        if (!FULL && n < N) {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i][e] = p[e < n ? e : 0];
+            return;
+        }
+        const int last = (int)n - N;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int k = (i * THREADS + t) * N;
+            v[i] = load16(p + (FULL || k < last ? k : last));
+        }
+    }
+    template <bool FULL = false> __device__ __forceinline__ void settle(int64_t n, int t) {
+        if (FULL) return;
+        const int whole = (int)n / N, rest = (int)n % N;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int at = i * THREADS + t;
+            if (rest && n > N) { // (the same for all threads)
+                const int by = N - rest;
+#pragma unroll
+                for (int m = N / 2; m >= 1; m >>= 1) {
+                    if (!(by & m)) continue;
+#pragma unroll
+                    for (int e = 0; e + m < N; ++e) v[i][e] = at == whole ? v[i][e + m] : v[i][e];
+                }
+            }
+            if (rest) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i][e] = e < rest || at != whole ? v[i][e] : (T)0;
+            }
+            const bool in = at < whole + (rest > 0);
+            uint4 u = __builtin_bit_cast(uint4, v[i]);
+            u = make_uint4(in ? u.x : 0, in ? u.y : 0, in ? u.z : 0, in ? u.w : 0);
+            v[i] = __builtin_bit_cast(typename Vec16<T>::V, u);
+        }
+    }
+    static __device__ __forceinline__ bool mine(int j, int64_t n, int t) {
+        const int whole = (int)n / N, rest = (int)n % N, at = j / N * THREADS + t, e = j % N;
+        return at < whole || (at == whole && (n < N ? e < rest : e >= N - rest));
+    }
+    __device__ __forceinline__ acc_t<T> at(int j) const { return (acc_t<T>)v[j / N][j % N]; }
+};
 template <typename T, int THREADS, int ITER> struct RowRegs {
     static constexpr int N = Vec16<T>::N;
     acc_t<T> v[ITER * N];
-    __device__ __forceinline__ void load(const T* p, int64_t n, int t) {
+    template <bool FULL = false> __device__ __forceinline__ void load(const T* p, int64_t n, int t) {
+        RowRaw<T, THREADS, ITER> u;
+        u.template load<FULL>(p, n, t);
+        u.template settle<FULL>(n, t);
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            const int64_t k = (int64_t)(i * THREADS + t) * N;
-            if (k + N <= n) {
-                const auto u = load16(p + k);
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[i * N + e] = (acc_t<T>)u[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[i * N + e] = k + e < n ? (acc_t<T>)p[k + e] : (acc_t<T>)0;
-            }
-        }
+        for (int j = 0; j < ITER * N; ++j) v[j] = u.at(j);
     }
     __device__ __forceinline__ void store(T* p, int64_t n, int t) const {
 #pragma unroll
@@ -64,18 +110,23 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row(NormAr
     const int64_t row = (int64_t)blockIdx.x * (BLOCK / THREADS) + threadIdx.x / THREADS;
     if (row >= a.rows) return; // (whole waves; a workgroup with barriers has one row)
     const int64_t n = a.width;
-    RowRegs<T, THREADS, ITER> x;
-    x.load((const T*)a.x + row * n, n, t);
-    A s[1] = {0};
+    typedef RowRaw<T, THREADS, ITER> Raw;
+    constexpr int N = Vec16<T>::N;
+    Raw u;
+    u.load((const T*)a.x + row * n, n, t);
+    A x[K], s[1] = {0};
 #pragma unroll
-    for (int j = 0; j < K; ++j) s[0] += x.v[j];
+    for (int j = 0; j < K; ++j) {
+        x[j] = u.at(j);
+        if (Raw::mine(j, n, t)) s[0] += x[j];
+    }
     row_sum<THREADS>(s, red, false);
     const A mean = s[0] / (A)n;
     s[0] = 0;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        x.v[j] -= mean;
-        if (RowRegs<T, THREADS, ITER>::inside(j, n, t)) s[0] += x.v[j] * x.v[j];
+        x[j] -= mean;
+        if (Raw::mine(j, n, t)) s[0] += x[j] * x[j];
     }
     row_sum<THREADS>(s, red, true);
     const A rstd = (A)1 / sqrt(s[0] / (A)n + (A)a.eps);
@@ -83,39 +134,34 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row(NormAr
         ((A*)a.mean)[row] = mean;
         ((A*)a.rstd)[row] = rstd;
     }
-    RowRegs<T, THREADS, ITER> w;
 #pragma unroll
-    for (int j = 0; j < K; ++j) x.v[j] *= rstd;
+    for (int j = 0; j < K; ++j) x[j] *= rstd;
     if (a.weight) {
-        w.load((const T*)a.weight, n, t);
+        u.load((const T*)a.weight, n, t);
 #pragma unroll
-        for (int j = 0; j < K; ++j) x.v[j] *= w.v[j];
+        for (int j = 0; j < K; ++j) x[j] *= u.at(j);
     }
     if (a.bias) {
-        w.load((const T*)a.bias, n, t);
+        u.load((const T*)a.bias, n, t);
 #pragma unroll
-        for (int j = 0; j < K; ++j) x.v[j] += w.v[j];
+        for (int j = 0; j < K; ++j) x[j] += u.at(j);
     }
-    x.store((T*)a.y + row * n, n, t);
+    T* y = (T*)a.y + row * n;
+    if (n < N) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (Raw::mine(e, n, t)) y[e] = (T)x[e];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int k = (i * THREADS + t) * N, last = (int)n - N;
+        typename Vec16<T>::V v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = (T)x[i * N + e];
+        if (k < n) store16(y + (k < last ? k : last), v); // (values that two vectors hold are the same in both)
+    }
 }
-
-// A row's vectors as they lie in memory
-template <typename T, int THREADS, int ITER> struct RowRaw {
-    static constexpr int N = Vec16<T>::N;
-    typename Vec16<T>::V v[ITER];
-    __device__ __forceinline__ void load(const T* p, int64_t n, int t) {
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            const int64_t k = (int64_t)(i * THREADS + t) * N;
-            if (k + N <= n) v[i] = load16(p + k);
-            else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[i][e] = k + e < n ? p[k + e] : (T)0;
-            }
-        }
-    }
-    __device__ __forceinline__ acc_t<T> at(int j) const { return (acc_t<T>)v[j / N][j % N]; }
-};
 
 // Rows go round the workgroups' groups of THREADS threads; the next row's vectors are on their way while this one is
 // reduced. The sums for the parameters' gradients stay in registers, and go to partial[2][gridDim.x][n] at the end
@@ -135,7 +181,10 @@ __global__ __launch_bounds__(THREADS * GROUPS) void norm_row_vjp(NormArgs a) {
         for (int j = 0; j < K; ++j) wbar[j] = bbar[j] = 0;
     }
     RowRaw<T, THREADS, ITER> w, xn, gn;
-    if (a.weight) w.load((const T*)a.weight, n, t);
+    if (a.weight) {
+        w.load((const T*)a.weight, n, t);
+        w.settle(n, t);
+    }
     int64_t row = (int64_t)blockIdx.x * GROUPS + group;
     A mean = 0, rstd = 0;
     if (row < a.rows) {
@@ -148,6 +197,8 @@ __global__ __launch_bounds__(THREADS * GROUPS) void norm_row_vjp(NormArgs a) {
         RowRegs<T, THREADS, ITER> x, g;
         const A mu = mean, rs = rstd;
         A s[2] = {0, 0};
+        xn.settle(n, t);
+        gn.settle(n, t);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             x.v[j] = (xn.at(j) - mu) * rs;
@@ -267,6 +318,8 @@ template <typename T, int COLS> __global__ __launch_bounds__(1024) void norm_par
 constexpr int LONG_THREADS = 256;
 constexpr int LONG_ITER = 8; // a sweep of a workgroup: 256 threads x 8 vectors = 32 KB, in registers
 template <typename T> constexpr int64_t long_sweep() { return (int64_t)LONG_THREADS * LONG_ITER * Vec16<T>::N; }
+constexpr int LONGB_ITER = 4; // 16 KB where more than x is held
+template <typename T> constexpr int64_t longb_sweep() { return (int64_t)LONG_THREADS * LONGB_ITER * Vec16<T>::N; }
 
 // Statistics of piece blockIdx.x of row blockIdx.y: partial[row][piece] = (c, sum (x - c), sum (x - c)^2) with c the mean of
 // the piece's first values, as rounded. Sums about a value near the piece's mean keep what a level far from zero would take
@@ -287,13 +340,23 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
 #pragma unroll
     for (int j = 0; j < N; ++j) c += r0.v[j];
     c = wave_sum(c) / (A)lead;
-    for (int64_t k = k0; k < k1; k += long_sweep<T>()) {
-        const int64_t n = k1 - k < long_sweep<T>() ? k1 - k : long_sweep<T>();
+    int64_t k = k0;
+    for (; k + long_sweep<T>() <= k1; k += long_sweep<T>()) {
         RowRegs<T, LONG_THREADS, LONG_ITER> r;
-        r.load(x + k, n, t);
+        r.template load<true>(x + k, long_sweep<T>(), t);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            const A d = RowRegs<T, LONG_THREADS, LONG_ITER>::inside(j, n, t) ? r.v[j] - c : (A)0;
+            const A d = r.v[j] - c;
+            s[0] += d;
+            s[1] += d * d;
+        }
+    }
+    if (k < k1) {
+        RowRegs<T, LONG_THREADS, LONG_ITER> r;
+        r.load(x + k, k1 - k, t);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const A d = RowRegs<T, LONG_THREADS, LONG_ITER>::inside(j, k1 - k, t) ? r.v[j] - c : (A)0;
             s[0] += d;
             s[1] += d * d;
         }
@@ -310,20 +373,20 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
 // mean and rstd of a row from its pieces', for a whole workgroup
 template <typename T> __device__ __forceinline__ void long_moments(const NormArgs& a, int64_t row, int pieces, acc_t<T>& mean, acc_t<T>& rstd) {
     typedef acc_t<T> A;
-    __shared__ A red[LONG_THREADS / 64];
+    __shared__ A red[2][LONG_THREADS / 64]; // (in turn: one barrier a sum, also from row to row)
     const int t = threadIdx.x;
     const A* p = (const A*)a.partial + row * pieces * 3;
     const A whole = (A)a.piece, tail = (A)(a.width - (int64_t)(pieces - 1) * a.piece); // values of a piece, of the last
     A s[1] = {0};
     for (int i = t; i < pieces; i += LONG_THREADS) s[0] += (i + 1 < pieces ? whole : tail) * p[3 * i] + p[3 * i + 1];
-    row_sum<LONG_THREADS>(s, red, false);
+    row_sum<LONG_THREADS>(s, red[0], true);
     mean = s[0] / (A)a.width;
     s[0] = 0;
     for (int i = t; i < pieces; i += LONG_THREADS) {
         const A d = p[3 * i] - mean;
         s[0] += p[3 * i + 2] + d * ((A)2 * p[3 * i + 1] + (i + 1 < pieces ? whole : tail) * d);
     }
-    row_sum<LONG_THREADS>(s, red, true);
+    row_sum<LONG_THREADS>(s, red[1], true);
     rstd = (A)1 / sqrt(s[0] / (A)a.width + (A)a.eps);
 }
 // ... one workgroup a row
@@ -336,72 +399,91 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
     }
 }
 
-// The second sweep, 32 KB a workgroup. join > 0: the row's moments from that many pieces, by each workgroup for itself. (Taking the rows one lattice at a time, so that it finds them in the last-level cache,
-// costs more in short launches than it saves: 16 lattices of 4096 x 4096 in fp64 1350 us against 1170.)
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a, int join) {
+// The second sweep, 16 KB of a row at a time. join > 0: the row's moments from that many pieces, by each workgroup for itself.
+// Bound by HBM: 16 lattices of 4096 x 4096 in fp64 765 us, 5.6 TB/s, after 380 us for their statistics. (Taking the rows one
+// lattice at a time, so that it finds them in the last-level cache, costs more in short launches than it saves: 1350 us
+// against 1170 for both sweeps.)
+template <typename T, bool FULL> __device__ __forceinline__ void long_apply(NormArgs a, int join) {
     typedef acc_t<T> A;
-    constexpr int K = LONG_ITER * Vec16<T>::N;
+    constexpr int K = LONGB_ITER * Vec16<T>::N;
     const int t = threadIdx.x;
-    const int64_t row = blockIdx.y, k = (int64_t)blockIdx.x * long_sweep<T>();
-    const int64_t n = a.width - k < long_sweep<T>() ? a.width - k : long_sweep<T>();
-    RowRegs<T, LONG_THREADS, LONG_ITER> r, w;
-    r.load((const T*)a.x + row * a.width + k, n, t);
-    A mean, rstd;
-    if (join) {
-        long_moments<T>(a, row, join, mean, rstd);
-        if (t == 0 && blockIdx.x == 0) {
-            ((A*)a.mean)[row] = mean;
-            ((A*)a.rstd)[row] = rstd;
+    const int64_t k = (int64_t)blockIdx.x * longb_sweep<T>();
+    const int64_t n = a.width - k < longb_sweep<T>() ? a.width - k : longb_sweep<T>();
+    RowRaw<T, LONG_THREADS, LONGB_ITER> w, b;
+    if (a.weight) w.template load<FULL>((const T*)a.weight + k, n, t);
+    if (a.bias) b.template load<FULL>((const T*)a.bias + k, n, t);
+    if (a.weight) w.template settle<FULL>(n, t);
+    if (a.bias) b.template settle<FULL>(n, t);
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        RowRegs<T, LONG_THREADS, LONGB_ITER> r;
+        r.template load<FULL>((const T*)a.x + row * a.width + k, n, t);
+        A mean, rstd;
+        if (join) {
+            long_moments<T>(a, row, join, mean, rstd);
+            if (t == 0 && blockIdx.x == 0) {
+                ((A*)a.mean)[row] = mean;
+                ((A*)a.rstd)[row] = rstd;
+            }
+        } else mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            r.v[j] = (r.v[j] - mean) * rstd;
+            if (a.weight) r.v[j] *= w.at(j);
+            if (a.bias) r.v[j] += b.at(j);
         }
-    } else mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
-#pragma unroll
-    for (int j = 0; j < K; ++j) r.v[j] = (r.v[j] - mean) * rstd;
-    if (a.weight) {
-        w.load((const T*)a.weight + k, n, t);
-#pragma unroll
-        for (int j = 0; j < K; ++j) r.v[j] *= w.v[j];
+        r.store((T*)a.y + row * a.width + k, n, t);
     }
-    if (a.bias) {
-        w.load((const T*)a.bias + k, n, t);
-#pragma unroll
-        for (int j = 0; j < K; ++j) r.v[j] += w.v[j];
-    }
-    r.store((T*)a.y + row * a.width + k, n, t);
+}
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_apply(NormArgs a, int join) {
+    if (((int64_t)blockIdx.x + 1) * longb_sweep<T>() <= a.width) long_apply<T, true>(a, join);
+    else long_apply<T, false>(a, join);
 }
 
 // Reverse mode, first sweep: columns [blockIdx.x * sweep, + sweep) of the rows of group blockIdx.y: the columns' gradient
 // sums over these rows (partial2[2][groups][n], or the outputs themselves where there is one group) and this piece's part of
 // the rows' two sums, partial[row][piece] = (sum g, sum g h).
-constexpr int LONGB_ITER = 4;
-template <typename T> constexpr int64_t longb_sweep() { return (int64_t)LONG_THREADS * LONGB_ITER * Vec16<T>::N; }
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_sums(NormArgs a) {
+template <typename T, bool FULL> __device__ __forceinline__ void long_vjp_sums(NormArgs a) {
     typedef acc_t<T> A;
     constexpr int K = LONGB_ITER * Vec16<T>::N;
-    __shared__ A red[LONG_THREADS / 64 * 2];
+    __shared__ A red[2][LONG_THREADS / 64 * 2];
     const int t = threadIdx.x;
     const int64_t k0 = (int64_t)blockIdx.x * longb_sweep<T>();
     const int64_t n = a.width - k0 < longb_sweep<T>() ? a.width - k0 : longb_sweep<T>();
-    RowRegs<T, LONG_THREADS, LONGB_ITER> w;
-    if (a.weight) w.load((const T*)a.weight + k0, n, t);
-    A wbar[K], bbar[K];
+    RowRaw<T, LONG_THREADS, LONGB_ITER> w, xn, gn;
+    if (a.weight) {
+        w.template load<FULL>((const T*)a.weight + k0, n, t);
+        w.template settle<FULL>(n, t);
+    }
+    A wbar[K], bbar[K], mean = 0, rstd = 0;
 #pragma unroll
     for (int j = 0; j < K; ++j) wbar[j] = bbar[j] = 0;
+    auto fetch = [&](int64_t row) {
+        xn.template load<FULL>((const T*)a.x + row * a.width + k0, n, t);
+        gn.template load<FULL>((const T*)a.ybar + row * a.width + k0, n, t);
+        mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+    };
+    if (blockIdx.y < a.rows) fetch(blockIdx.y);
+    int side = 0;
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        RowRegs<T, LONG_THREADS, LONGB_ITER> x, g;
-        x.load((const T*)a.x + row * a.width + k0, n, t);
-        g.load((const T*)a.ybar + row * a.width + k0, n, t);
-        const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
-        A s[2] = {0, 0};
+        A h[K], g[K], s[2] = {0, 0};
+        xn.template settle<FULL>(n, t);
+        gn.template settle<FULL>(n, t);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            const A h = (x.v[j] - mean) * rstd;
-            wbar[j] += g.v[j] * h;
-            bbar[j] += g.v[j];
-            const A gw = a.weight ? g.v[j] * w.v[j] : g.v[j];
-            s[0] += gw;
-            s[1] += gw * h;
+            h[j] = (xn.at(j) - mean) * rstd;
+            g[j] = gn.at(j);
         }
-        row_sum<LONG_THREADS>(s, red, false);
+        if (row + gridDim.y < a.rows) fetch(row + gridDim.y);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            wbar[j] += g[j] * h[j];
+            bbar[j] += g[j];
+            const A gw = a.weight ? g[j] * w.at(j) : g[j];
+            s[0] += gw;
+            s[1] += gw * h[j];
+        }
+        row_sum<LONG_THREADS>(s, red[side], true); // (the other half is next: one barrier a row)
+        side ^= 1;
         if (t == 0) {
             A* p = (A*)a.partial + (row * gridDim.x + blockIdx.x) * 2;
             p[0] = s[0];
@@ -425,25 +507,29 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
         }
     }
 }
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_sums(NormArgs a) {
+    if (((int64_t)blockIdx.x + 1) * longb_sweep<T>() <= a.width) long_vjp_sums<T, true>(a);
+    else long_vjp_sums<T, false>(a);
+}
 
 // (<g>, <g h>) of a row from its pieces', for a whole workgroup
-template <typename T> __device__ __forceinline__ void long_means(const NormArgs& a, int64_t row, int64_t pieces, acc_t<T> (&s)[2]) {
+template <typename T> __device__ __forceinline__ void long_means(const NormArgs& a, int64_t row, int64_t pieces, int side, acc_t<T> (&s)[2]) {
     typedef acc_t<T> A;
-    __shared__ A red[LONG_THREADS / 64 * 2];
+    __shared__ A red[2][LONG_THREADS / 64 * 2]; // (side: in turn from row to row)
     const A* p = (const A*)a.partial + row * pieces * 2;
     s[0] = s[1] = 0;
     for (int64_t i = threadIdx.x; i < pieces; i += LONG_THREADS) {
         s[0] += p[2 * i];
         s[1] += p[2 * i + 1];
     }
-    row_sum<LONG_THREADS>(s, red, true);
+    row_sum<LONG_THREADS>(s, red[side], true);
     s[0] /= (A)a.width;
     s[1] /= (A)a.width;
 }
 // ... one workgroup a row, into sums
 template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_rows(NormArgs a, int64_t pieces) {
     acc_t<T> s[2];
-    long_means<T>(a, blockIdx.x, pieces, s);
+    long_means<T>(a, blockIdx.x, pieces, 0, s);
     if (threadIdx.x == 0) {
         ((acc_t<T>*)a.sums)[2 * (int64_t)blockIdx.x] = s[0];
         ((acc_t<T>*)a.sums)[2 * (int64_t)blockIdx.x + 1] = s[1];
@@ -451,34 +537,46 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
 }
 
 // second sweep: xbar. join > 0: the row's means from that many pieces, by each workgroup for itself
-template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_apply(NormArgs a, int64_t join) {
+template <typename T, bool FULL> __device__ __forceinline__ void long_vjp_apply(NormArgs a, int64_t join) {
     typedef acc_t<T> A;
     constexpr int K = LONGB_ITER * Vec16<T>::N;
     const int t = threadIdx.x;
-    const int64_t row = blockIdx.y, k0 = (int64_t)blockIdx.x * longb_sweep<T>();
+    const int64_t k0 = (int64_t)blockIdx.x * longb_sweep<T>();
     const int64_t n = a.width - k0 < longb_sweep<T>() ? a.width - k0 : longb_sweep<T>();
-    const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
-    RowRegs<T, LONG_THREADS, LONGB_ITER> x, g, w;
-    x.load((const T*)a.x + row * a.width + k0, n, t);
-    g.load((const T*)a.ybar + row * a.width + k0, n, t);
-    A c[2];
-    if (join) long_means<T>(a, row, join, c);
-    else c[0] = ((const A*)a.sums)[2 * row], c[1] = ((const A*)a.sums)[2 * row + 1];
+    RowRaw<T, LONG_THREADS, LONGB_ITER> w;
     if (a.weight) {
-        w.load((const T*)a.weight + k0, n, t);
-#pragma unroll
-        for (int j = 0; j < K; ++j) g.v[j] *= w.v[j];
+        w.template load<FULL>((const T*)a.weight + k0, n, t);
+        w.template settle<FULL>(n, t);
     }
+    int side = 0;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y, side ^= 1) {
+        const A mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
+        RowRegs<T, LONG_THREADS, LONGB_ITER> x, g;
+        x.template load<FULL>((const T*)a.x + row * a.width + k0, n, t);
+        g.template load<FULL>((const T*)a.ybar + row * a.width + k0, n, t);
+        A c[2];
+        if (join) long_means<T>(a, row, join, side, c);
+        else c[0] = ((const A*)a.sums)[2 * row], c[1] = ((const A*)a.sums)[2 * row + 1];
 #pragma unroll
-    for (int j = 0; j < K; ++j) x.v[j] = rstd * (g.v[j] - c[0] - (x.v[j] - mean) * rstd * c[1]);
-    x.store((T*)a.xbar + row * a.width + k0, n, t);
+        for (int j = 0; j < K; ++j) {
+            if (a.weight) g.v[j] *= w.at(j);
+            x.v[j] = rstd * (g.v[j] - c[0] - (x.v[j] - mean) * rstd * c[1]);
+        }
+        x.store((T*)a.xbar + row * a.width + k0, n, t);
+    }
+}
+template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_vjp_apply(NormArgs a, int64_t join) {
+    if (((int64_t)blockIdx.x + 1) * longb_sweep<T>() <= a.width) long_vjp_apply<T, true>(a, join);
+    else long_vjp_apply<T, false>(a, join);
 }
 
 // ---- plans ------------------------------------------------------------------------------------------------------------
 constexpr int64_t ROW_BYTES = 65536;   // longest row that one workgroup keeps in registers (1024 threads x 4 vectors)
 constexpr int64_t VJP_ROW_BYTES = 32768; // ... with its cotangent and its gradient sums (1024 threads x 2 vectors)
 constexpr int64_t MAX_GRID_Y = 65535;
-constexpr int64_t FEW_PIECES = 256; // of a row that the second sweep's workgroups add up for themselves rather than in a launch before
+// Pieces of a row that the second sweep's workgroups add up for themselves rather than in a launch before (four fp64 lattices of 1024 x
+// 1024, 512 pieces each, reverse mode: 34 us against 37)
+constexpr int64_t FEW_PIECES = 512;
 
 struct LongPlan {
     int64_t piece, pieces;   // forward: elements of a piece (a multiple of the sweep), pieces of a row
@@ -487,8 +585,8 @@ struct LongPlan {
 template <typename T> LongPlan long_plan(int64_t rows, int64_t n) {
     LongPlan p;
     const int64_t sweeps = (n + long_sweep<T>() - 1) / long_sweep<T>();
-    // at most 2048 pieces a row: one row alone fills the card, and its join stays short
-    const int64_t per = (sweeps + 2047) / 2048;
+    // pieces of all rows enough to fill the card, and at most 2048 of one: its join stays short
+    const int64_t fill = sweeps * rows / 4096, per = fill > (sweeps + 2047) / 2048 ? fill : (sweeps + 2047) / 2048;
     p.piece = per * long_sweep<T>();
     p.pieces = (n + p.piece - 1) / p.piece;
     p.vpieces = (n + longb_sweep<T>() - 1) / longb_sweep<T>();
@@ -504,6 +602,14 @@ int64_t row_blocks(int64_t rows, bool small) {
     if (rows <= (small ? 32 : 2)) return 1;
     const int64_t groups = small ? (rows + 3) / 4 : rows;
     return groups < 256 ? groups : groups < 8192 ? (groups / 8 > 256 ? groups / 8 : 256) : 1024;
+}
+// Row groups of a second sweep: a workgroup that has weights takes several rows with them, if enough workgroups are left to fill the
+// card (32 lattices of 1024 x 1500 in fp64: 142 us against 214 with one row each). Not so in the reverse mode, with three streams
+// for the one of weights: 64 lattices of 300 x 1500 128 us against 111
+unsigned apply_groups(int64_t rows, int64_t pieces, bool weights) {
+    int64_t g = weights ? (2048 + pieces - 1) / pieces : rows;
+    if (g > rows) g = rows;
+    return (unsigned)(g < MAX_GRID_Y ? g : MAX_GRID_Y);
 }
 template <typename T> bool small_row(int64_t n) { return n <= 128 * Vec16<T>::N; }
 
@@ -530,7 +636,7 @@ template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
         else if (vecs <= 128) launch_row<T, 64, 2>(a, st);
         else if (vecs <= 256) launch_row<T, 256, 1>(a, st);
         else if (vecs <= 512) launch_row<T, 256, 2>(a, st);
-        else if (vecs <= 1024) launch_row<T, 256, 4>(a, st);
+        else if (vecs <= 1024) launch_row<T, 512, 2>(a, st);
         else if (vecs <= 2048) launch_row<T, 1024, 2>(a, st);
         else launch_row<T, 1024, 4>(a, st);
         return hipGetLastError();
@@ -549,7 +655,8 @@ template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
         norm_long_stats<T><<<dim3((unsigned)p.pieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s);
         const bool small = p.pieces <= FEW_PIECES;
         if (!small) norm_long_join<T><<<dim3((unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s, (int)p.pieces);
-        norm_long_apply<T><<<dim3((unsigned)((a.width + long_sweep<T>() - 1) / long_sweep<T>()), (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(
+        const int64_t sweeps = (a.width + longb_sweep<T>() - 1) / longb_sweep<T>();
+        norm_long_apply<T><<<dim3((unsigned)sweeps, apply_groups(s.rows, sweeps, a.weight || a.bias)), dim3(LONG_THREADS), 0, st>>>(
             s, small ? (int)p.pieces : 0);
     }
     return hipGetLastError();
@@ -586,22 +693,14 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
         norm_long_vjp_sums<T><<<dim3((unsigned)p.vpieces, (unsigned)p.groups), dim3(LONG_THREADS), 0, st>>>(a);
         const bool small = p.vpieces <= FEW_PIECES;
         if (!small) norm_long_vjp_rows<T><<<dim3((unsigned)a.rows), dim3(LONG_THREADS), 0, st>>>(a, p.vpieces);
-        for (int64_t r0 = 0; r0 < a.rows; r0 += MAX_GRID_Y) {
-            NormArgs s = a;
-            s.rows = a.rows - r0 < MAX_GRID_Y ? a.rows - r0 : MAX_GRID_Y;
-            s.x = (const T*)a.x + r0 * n;
-            s.ybar = (const T*)a.ybar + r0 * n;
-            s.xbar = (T*)a.xbar + r0 * n;
-            s.mean = (A*)a.mean + r0;
-            s.rstd = (A*)a.rstd + r0;
-            s.sums = (A*)a.sums + 2 * r0;
-            s.partial = (A*)a.partial + 2 * r0 * p.vpieces;
-            norm_long_vjp_apply<T><<<dim3((unsigned)p.vpieces, (unsigned)s.rows), dim3(LONG_THREADS), 0, st>>>(s, small ? p.vpieces : 0);
-        }
+        norm_long_vjp_apply<T><<<dim3((unsigned)p.vpieces, apply_groups(a.rows, p.vpieces, false)), dim3(LONG_THREADS), 0, st>>>(
+            a, small ? p.vpieces : 0);
         parts = p.groups > 1 ? p.groups : 0;
         parted = (A*)a.partial2;
     }
-    if (a.wbar && parts > 16)
+    if (a.wbar && parts > 16 && n <= 2048)
+        norm_param_sum<T, 16><<<dim3((unsigned)((n + 15) / 16), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
+    else if (a.wbar && parts > 16)
         norm_param_sum<T, 64><<<dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
     else if (a.wbar && parts > 0)
         norm_param_sum<T, 512><<<dim3((unsigned)((n + 511) / 512), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
