@@ -3,10 +3,14 @@
 //   eta[n][v] = alpha[v] + beta[v] . x[n],  lse[n] = log sum_v exp eta[n][v],  lp[n] = eta[n][y[n]] - lse[n]
 //   r[n][v] = lpbar[n] ([v = y[n]] - exp(eta[n][v] - lse[n])),  xbar = r beta,  alphabar = sum_n r,  betabar = r^T x
 //
-// The logits eta are never kept: one pass over the classes leaves a maximum and a sum for every row and tile of classes; the
-// reverse mode computes eta once more, a piece of the classes at a time, and turns it into the piece's r in a workspace of
-// bounded size, from which two more matrix products take xbar and betabar. Everything that a product sums over stands
-// contiguously for both operands: r is written in both orders, x and the piece of beta are transposed once.
+// Two passes over the classes. The first leaves a maximum and a sum for every row and tile of classes; the second takes a piece of
+// the classes at a time and turns its logits into the piece's r in a workspace of bounded size, from which two more matrix
+// products take xbar and betabar. Of the logits a bounded part is kept from the first pass (the tiles' registers as they are, up to
+// KEPT_BYTES), the rest is computed again. Everything that a product sums over stands contiguously for both operands: r is written in both
+// orders, x and the piece of beta are transposed once.
+//
+// What bounds it are the matrix cores: 4096 rows x 4096 features x 128000 classes in bf16 take 12.5 ms, 1.13 PFLOP/s in the products at the
+// 1.85-1.9 GHz that the power leaves (60-63 % busy).
 //
 // Sums, statistics and accumulators are Acc (fp32; fp64 for fp64 data). One intermediate is rounded to 16 bits where the data
 // have 16 bits: r, because the matrix instructions take both operands in one type. Its error (half a step of each entry) is

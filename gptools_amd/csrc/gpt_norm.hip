@@ -28,7 +28,7 @@ template <typename T, int THREADS, int ITER> struct RowRaw {
 #pragma unroll
             for (int i = 0; i < ITER; ++i)
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[i][e] = p[e < n ? e : 0];
+                for (int e = 0; e < N; ++e) v[i][e] = e < n ? p[e] : (T)0;
             return;
         }
         const int last = (int)n - N;
@@ -40,25 +40,22 @@ template <typename T, int THREADS, int ITER> struct RowRaw {
     }
     template <bool FULL = false> __device__ __forceinline__ void settle(int64_t n, int t) {
         if (FULL) return;
-        const int whole = (int)n / N, rest = (int)n % N;
+        const int whole = (int)n / N, rest = (int)n % N, by = rest && n > N ? (N - rest) * (int)sizeof(T) : 0; // bytes
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int at = i * THREADS + t;
-            if (rest && n > N) { // (the same for all threads)
-                const int by = N - rest;
-#pragma unroll
-                for (int m = N / 2; m >= 1; m >>= 1) {
-                    if (!(by & m)) continue;
-#pragma unroll
-                    for (int e = 0; e + m < N; ++e) v[i][e] = at == whole ? v[i][e + m] : v[i][e];
-                }
-            }
-            if (rest) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[i][e] = e < rest || at != whole ? v[i][e] : (T)0;
+            uint4 u = __builtin_bit_cast(uint4, v[i]);
+            if (by) { // (the same for all threads)
+                uint4 s = u;
+                if (by & 8) s = make_uint4(s.z, s.w, 0, 0);
+                if (by & 4) s = make_uint4(s.y, s.z, s.w, 0);
+                if (by & 2)
+                    s = make_uint4(__builtin_amdgcn_alignbyte(s.y, s.x, 2), __builtin_amdgcn_alignbyte(s.z, s.y, 2),
+                                   __builtin_amdgcn_alignbyte(s.w, s.z, 2), s.w >> 16);
+                const bool cut = at == whole;
+                u = make_uint4(cut ? s.x : u.x, cut ? s.y : u.y, cut ? s.z : u.z, cut ? s.w : u.w);
             }
             const bool in = at < whole + (rest > 0);
-            uint4 u = __builtin_bit_cast(uint4, v[i]);
             u = make_uint4(in ? u.x : 0, in ? u.y : 0, in ? u.z : 0, in ? u.w : 0);
             v[i] = __builtin_bit_cast(typename Vec16<T>::V, u);
         }
@@ -187,14 +184,17 @@ __global__ __launch_bounds__(THREADS * GROUPS) void norm_row_vjp(NormArgs a) {
     }
     int64_t row = (int64_t)blockIdx.x * GROUPS + group;
     A mean = 0, rstd = 0;
-    if (row < a.rows) {
-        xn.load((const T*)a.x + row * n, n, t);
-        gn.load((const T*)a.ybar + row * n, n, t);
-        mean = ((const A*)a.mean)[row], rstd = ((const A*)a.rstd)[row];
-    }
+    auto fetch = [&](int64_t r) {
+        xn.load((const T*)a.x + r * n, n, t);
+        gn.load((const T*)a.ybar + r * n, n, t);
+        mean = ((const A*)a.mean)[r], rstd = ((const A*)a.rstd)[r];
+    };
+    constexpr bool AHEAD = sizeof(T) > 2 || ITER < 4; // (else the registers do not suffice)
+    if (AHEAD && row < a.rows) fetch(row);
     int side = 0;
     for (; row < a.rows; row += step) { // (a group of several waves is the whole workgroup: its barriers are met by all)
         RowRegs<T, THREADS, ITER> x, g;
+        if (!AHEAD) fetch(row);
         const A mu = mean, rs = rstd;
         A s[2] = {0, 0};
         xn.settle(n, t);
@@ -204,11 +204,7 @@ __global__ __launch_bounds__(THREADS * GROUPS) void norm_row_vjp(NormArgs a) {
             x.v[j] = (xn.at(j) - mu) * rs;
             g.v[j] = gn.at(j);
         }
-        if (row + step < a.rows) {
-            xn.load((const T*)a.x + (row + step) * n, n, t);
-            gn.load((const T*)a.ybar + (row + step) * n, n, t);
-            mean = ((const A*)a.mean)[row + step], rstd = ((const A*)a.rstd)[row + step];
-        }
+        if (AHEAD && row + step < a.rows) fetch(row + step);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             if (PARAMS) {
@@ -572,7 +568,7 @@ template <typename T> __global__ __launch_bounds__(LONG_THREADS) void norm_long_
 
 // ---- plans ------------------------------------------------------------------------------------------------------------
 constexpr int64_t ROW_BYTES = 65536;   // longest row that one workgroup keeps in registers (1024 threads x 4 vectors)
-constexpr int64_t VJP_ROW_BYTES = 32768; // ... with its cotangent and its gradient sums (1024 threads x 2 vectors)
+constexpr int64_t VJP_ROW_BYTES = 32768; // ... with its cotangent and its gradient sums (512 threads x 4 vectors)
 constexpr int64_t MAX_GRID_Y = 65535;
 // Pieces of a row that the second sweep's workgroups add up for themselves rather than in a launch before (four fp64 lattices of 1024 x
 // 1024, 512 pieces each, reverse mode: 34 us against 37)
@@ -595,14 +591,20 @@ template <typename T> LongPlan long_plan(int64_t rows, int64_t n) {
     if (p.groups > rows) p.groups = rows;
     return p;
 }
+template <typename T> bool small_row(int64_t n) { return n <= 128 * Vec16<T>::N; }
 // Workgroups of the reverse mode on whole rows: one where the rows are few (its rounds are shorter than another launch), else
-// enough to fill the card, and at least 8 rows each where there are as many (each leaves 2 n partial sums). small: a wave takes a
-// row, a workgroup 4 at a time, or 16 if it is alone
-int64_t row_blocks(int64_t rows, bool small) {
+// enough to fill the card, and at least 8 rows each where there are as many (each leaves 2 n partial sums), at most those that stay on it at
+// once: a CU holds one of 512 threads or more, three of 256 with sums of 16 values, four others (bf16, 16384 rows of 8192: 163 us
+// against 180 with 1024). Short rows: a wave takes a row, a workgroup 4 at a time, or 16 if it is alone
+template <typename T> int64_t row_blocks(int64_t rows, int64_t n) {
+    const bool small = small_row<T>(n);
     if (rows <= (small ? 32 : 2)) return 1;
-    const int64_t groups = small ? (rows + 3) / 4 : rows;
-    return groups < 256 ? groups : groups < 8192 ? (groups / 8 > 256 ? groups / 8 : 256) : 1024;
+    const int64_t groups = small ? (rows + 3) / 4 : rows, vecs = (n + Vec16<T>::N - 1) / Vec16<T>::N;
+    const int64_t most = vecs > 512 ? 256 : vecs > 256 && sizeof(T) == 2 ? 768 : 1024;
+    if (groups < 256) return groups;
+    return groups / 8 < 256 ? 256 : groups / 8 < most ? groups / 8 : most;
 }
+
 // Row groups of a second sweep: a workgroup that has weights takes several rows with them, if enough workgroups are left to fill the
 // card (32 lattices of 1024 x 1500 in fp64: 142 us against 214 with one row each). Not so in the reverse mode, with three streams
 // for the one of weights: 64 lattices of 300 x 1500 128 us against 111
@@ -611,12 +613,10 @@ unsigned apply_groups(int64_t rows, int64_t pieces, bool weights) {
     if (g > rows) g = rows;
     return (unsigned)(g < MAX_GRID_Y ? g : MAX_GRID_Y);
 }
-template <typename T> bool small_row(int64_t n) { return n <= 128 * Vec16<T>::N; }
-
 template <typename T> size_t workspace(int64_t rows, int64_t n, bool vjp) {
     const size_t A = sizeof(acc_t<T>);
     if (n * (int64_t)sizeof(T) <= (vjp ? VJP_ROW_BYTES : ROW_BYTES)) {
-        const int64_t blocks = vjp ? row_blocks(rows, small_row<T>(n)) : 1;
+        const int64_t blocks = vjp ? row_blocks<T>(rows, n) : 1;
         return blocks > 1 ? A * 2 * (size_t)(blocks * n) : 0;
     }
     const LongPlan p = long_plan<T>(rows, n);
@@ -677,7 +677,7 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
     int64_t parts = 0;
     A* parted = (A*)a.partial;
     if (n * (int64_t)sizeof(T) <= VJP_ROW_BYTES) {
-        parts = row_blocks(a.rows, small_row<T>(n));
+        parts = row_blocks<T>(a.rows, n);
         const unsigned b = (unsigned)parts;
         if (parts == 1) parts = 0; // (nothing left to add up)
         if (vecs <= 64) launch_row_vjp<T, 64, 1>(a, b, st);
@@ -685,7 +685,7 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
         else if (vecs <= 256) launch_row_vjp<T, 256, 1>(a, b, st);
         else if (vecs <= 512) launch_row_vjp<T, 256, 2>(a, b, st);
         else if (vecs <= 1024) launch_row_vjp<T, 1024, 1>(a, b, st);
-        else launch_row_vjp<T, 1024, 2>(a, b, st);
+        else launch_row_vjp<T, 512, 4>(a, b, st);
     } else {
         const LongPlan p = long_plan<T>(a.rows, n);
         a.sums = (A*)a.partial + 2 * a.rows * p.vpieces;
@@ -698,9 +698,7 @@ template <typename T> hipError_t reverse(NormArgs a, hipStream_t st) {
         parts = p.groups > 1 ? p.groups : 0;
         parted = (A*)a.partial2;
     }
-    if (a.wbar && parts > 16 && n <= 2048)
-        norm_param_sum<T, 16><<<dim3((unsigned)((n + 15) / 16), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
-    else if (a.wbar && parts > 16)
+    if (a.wbar && parts > 16)
         norm_param_sum<T, 64><<<dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
     else if (a.wbar && parts > 0)
         norm_param_sum<T, 512><<<dim3((unsigned)((n + 511) / 512), 2), dim3(1024), 0, st>>>(parted, parts, n, (T*)a.wbar, (T*)a.bbar);
