@@ -86,38 +86,38 @@ template <typename W> __device__ __forceinline__ void words(float a, float b, ui
 }
 
 // Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r. KEPT: eta was kept.
-template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class_logits(LogitArgs<W> a) {
+template <typename W> struct LogitRoom { // LDS
     typedef typename W::Acc A;
     typedef typename W::Tl Tl;
-    __shared__ typename Tl::Vec lds[KEPT ? 1 : Tl::LDS_BYTES / 16];
-    __shared__ A red[2][Tl::WM > Tl::WN ? Tl::WM : Tl::WN][Tl::BM > Tl::BN ? Tl::BM : Tl::BN];
-    const int64_t rows = *a.count, ld = a.x.rows;
-    int64_t tm, tn;
-    if (!tile_place(blockIdx.x, a.tiles_v, (rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
-    const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN;
+    A red[2][Tl::WM > Tl::WN ? Tl::WM : Tl::WN][Tl::BM > Tl::BN ? Tl::BM : Tl::BN];
+    A al[Tl::BM], lse[Tl::BN], w[Tl::BN];
+    int at[Tl::BN];
+};
+template <typename W, typename Tl, bool STATS, bool KEPT>
+__device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_t tm, int64_t tn, LogitRoom<W>& room, typename Tl::Vec* lds) {
+    typedef typename W::Acc A;
+    const int64_t ld = a.x.rows, m0 = tm * W::Tl::BM, n0 = tn * W::Tl::BN;
     const int nv = (int)(a.beta.rows - m0 < Tl::BM ? a.beta.rows - m0 : Tl::BM); // classes of this tile
     // what the tile's classes and rows need besides, on its way into LDS while the product runs (which ends with a barrier)
-    __shared__ A al[KEPT ? 1 : Tl::BM], lse_of[STATS ? 1 : Tl::BN], w_of[STATS ? 1 : Tl::BN];
-    __shared__ int at_of[Tl::BN];
     A largest = 1;
     if (!STATS) largest = a.largest.get();
     for (int c = threadIdx.x; !KEPT && c < Tl::BM; c += Tl::THREADS)
-        al[c] = c < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + c]) : (A)0) : neg_inf<A>();
+        room.al[c] = c < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + c]) : (A)0) : neg_inf<A>();
     for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
         const int64_t n = n0 + c, y = n < rows ? a.y[n] : -1, from = y - (a.v0 + m0);
-        at_of[c] = y >= 0 && from >= 0 && from < nv ? (int)from : -1; // the row's class within the tile
+        room.at[c] = y >= 0 && from >= 0 && from < nv ? (int)from : -1; // the row's class within the tile
         if (!STATS) {
             // lse: NaN where the row's class is none, infinite (no probability) behind the last row and without a possible class
             const A l = y < 0 ? neg_inf<A>() : y >= a.classes ? (A)__builtin_nan("") : a.lse[n];
             const bool none = l == neg_inf<A>();
-            lse_of[c] = none ? -neg_inf<A>() : l;
-            w_of[c] = none ? (A)0 : a.lpbar ? a.lpbar[a.row[n]] / largest : (A)1;
+            room.lse[c] = none ? -neg_inf<A>() : l;
+            room.w[c] = none ? (A)0 : a.lpbar ? a.lpbar[a.row[n]] / largest : (A)1;
         }
     }
     a.x.rows = rows;
     const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Tl::WN, wn = (threadIdx.x >> 6) % Tl::WN;
-    const int64_t kept_tile = (a.v0 + m0) / Tl::BM * ((ld + Tl::BN - 1) / Tl::BN) + tn;
-    auto* kept = a.kept + kept_tile * (Tl::TM * Tl::TN * Tl::THREADS) + threadIdx.x;
+    const int64_t kept_tile = (a.v0 + m0) / Tl::BM * ((ld + W::Tl::BN - 1) / W::Tl::BN) + tn;
+    auto* kept = a.kept + kept_tile * (W::Tl::TM * W::Tl::TN * W::Tl::THREADS) + threadIdx.x;
     Tl tl;
     if constexpr (KEPT) {
 #pragma unroll
@@ -131,7 +131,7 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
         for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const A v = al[Tl::row(i, r)];
+                const A v = room.al[Tl::row(i, r)];
 #pragma unroll
                 for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j][r] = times_log2e(tl.acc[i][j][r]) + v;
             }
@@ -145,7 +145,7 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
     if (STATS) {
 #pragma unroll
         for (int j = 0; j < Tl::TN; ++j) {
-            const int at = at_of[Tl::col(j)];
+            const int at = room.at[Tl::col(j)];
             A mx = neg_inf<A>();
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
@@ -169,15 +169,15 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
 #pragma unroll
             for (int k = 16; k <= 32; k <<= 1) join(mx, s, __shfl_xor(mx, k, 64), __shfl_xor(s, k, 64));
             if (lane < 16) {
-                red[0][wm][Tl::col(j)] = mx;
-                red[1][wm][Tl::col(j)] = s;
+                room.red[0][wm][Tl::col(j)] = mx;
+                room.red[1][wm][Tl::col(j)] = s;
             }
         }
         __syncthreads();
         for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
-            A mx = red[0][0][c], s = red[1][0][c];
+            A mx = room.red[0][0][c], s = room.red[1][0][c];
 #pragma unroll
-            for (int w = 1; w < Tl::WM; ++w) join(mx, s, red[0][w][c], red[1][w][c]);
+            for (int w = 1; w < Tl::WM; ++w) join(mx, s, room.red[0][w][c], room.red[1][w][c]);
             if (n0 + c < rows) {
                 a.part_max[tm * ld + n0 + c] = mx;
                 a.part_sum[tm * ld + n0 + c] = s;
@@ -189,9 +189,9 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
     int at[Tl::TN];
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
-        lse[j] = lse_of[Tl::col(j)];
-        w[j] = w_of[Tl::col(j)];
-        at[j] = lse[j] == -neg_inf<A>() ? -1 : at_of[Tl::col(j)];
+        lse[j] = room.lse[Tl::col(j)];
+        w[j] = room.w[Tl::col(j)];
+        at[j] = lse[j] == -neg_inf<A>() ? -1 : room.at[Tl::col(j)];
     }
     constexpr A up = stored_scale<typename W::Data>();
     A total[Tl::TM][4];
@@ -267,15 +267,32 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const A s = sum16(total[i][r]);
-            if ((lane & 15) == 0) red[0][wn][Tl::row(i, r)] = s;
+            if ((lane & 15) == 0) room.red[0][wn][Tl::row(i, r)] = s;
         }
     __syncthreads();
     for (int c = threadIdx.x; c < nv; c += Tl::THREADS) {
-        A s = red[0][0][c];
+        A s = room.red[0][0][c];
 #pragma unroll
-        for (int k = 1; k < Tl::WN; ++k) s += red[0][k][c];
+        for (int k = 1; k < Tl::WN; ++k) s += room.red[0][k][c];
         a.part_alpha[tn * a.ldr + m0 + c] = s * (largest / up);
     }
+}
+template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class_logits(LogitArgs<W> a) {
+    typedef typename W::Tl Tl;
+    typedef typename HalfOf<Tl>::Tile Half;
+    __shared__ typename Tl::Vec lds[KEPT ? 1 : Tl::LDS_BYTES / 16];
+    __shared__ LogitRoom<W> room;
+    const int64_t rows = *a.count;
+    int64_t tm, tn;
+    bool half;
+    if (!tile_place<Tl>(blockIdx.x, a.tiles_v, rows, tm, tn, half)) return;
+    if constexpr (!std::is_void<Half>::value) {
+        if (half) {
+            logits_tile<W, Half, STATS, KEPT>(a, rows, tm, tn, room, lds);
+            return;
+        }
+    }
+    logits_tile<W, Tl, STATS, KEPT>(a, rows, tm, tn, room, lds);
 }
 
 // The observed rows of x side by side, as operands (zeros behind their features); zeros into xbar's other rows
@@ -453,17 +470,12 @@ template <typename T, typename E> struct ProductArgs {
     const Acc* lpbar;
     Largest<Acc> largest;
 };
-template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<typename W::Data, typename W::Element> a, int64_t id,
-                                                                   typename W::Tl::Vec* lds) {
+template <typename W, typename Tl>
+__device__ __forceinline__ void product_at(const ProductArgs<typename W::Data, typename W::Element>& a, int64_t split, int64_t tm, int64_t tn,
+                                           typename Tl::Vec* lds) {
     typedef typename W::Acc A;
     typedef typename W::Data T;
-    typedef typename W::Tl Tl;
-    const int64_t split = id / a.grid;
-    if (a.row) a.B.rows = *a.count;
-    else a.K = (*a.count + a.k_edge - 1) / a.k_edge * a.k_edge;
-    int64_t tm, tn;
-    if (!tile_place(id - split * a.grid, a.tiles_m, (a.B.rows + Tl::BN - 1) / Tl::BN, tm, tn)) return;
-    const int64_t m0 = tm * Tl::BM, n0 = tn * Tl::BN, step = tile_k<typename W::Element>();
+    const int64_t m0 = tm * W::Tl::BM, n0 = tn * W::Tl::BN, step = tile_k<typename W::Element>();
     const int64_t share = ((a.K + a.splits - 1) / a.splits + step - 1) / step * step;
     const int64_t k0 = split * share, k1 = k0 + share < a.K ? k0 + share : a.K;
     Tl tl;
@@ -536,6 +548,24 @@ template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<t
                 }
         }
     }
+}
+template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<typename W::Data, typename W::Element> a, int64_t id,
+                                                                   typename W::Tl::Vec* lds) {
+    typedef typename W::Tl Tl;
+    typedef typename HalfOf<Tl>::Tile Half;
+    const int64_t split = id / a.grid;
+    if (a.row) a.B.rows = *a.count;
+    else a.K = (*a.count + a.k_edge - 1) / a.k_edge * a.k_edge;
+    int64_t tm, tn;
+    bool half;
+    if (!tile_place<Tl>(id - split * a.grid, a.tiles_m, a.B.rows, tm, tn, half)) return;
+    if constexpr (!std::is_void<Half>::value) {
+        if (half) {
+            product_at<W, Half>(a, split, tm, tn, lds);
+            return;
+        }
+    }
+    product_at<W, Tl>(a, split, tm, tn, lds);
 }
 // alphabar of a piece from the tiles' sums: 64 classes a workgroup, its waves share the tiles. acc: sums over row blocks
 template <typename T> struct AlphaArgs {
@@ -706,7 +736,7 @@ template <typename W> struct Plan {
 template <typename W, bool STATS, bool KEPT> void logits(LogitArgs<W> l, hipStream_t st) {
     typedef typename W::Tl Tl;
     l.tiles_v = tiles_of(l.beta.rows, Tl::BM);
-    class_logits<W, STATS, KEPT><<<dim3(tile_grid(l.tiles_v, tiles_of(l.x.rows, Tl::BN))), dim3(Tl::THREADS), 0, st>>>(l);
+    class_logits<W, STATS, KEPT><<<dim3(tile_grid<Tl>(l.tiles_v, l.x.rows)), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
 // xbar and betabar of a piece (each complete if its `last`), alphabar (blocks: its workgroups, or none)
@@ -727,7 +757,7 @@ template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan
         ProductsArgs<U> u = {p.x, p.b, p.alpha, {0, 0}};
         auto size = [](auto& q) {
             q.tiles_m = tiles_of(q.A.rows, Tl::BM);
-            q.grid = tile_grid(q.tiles_m, tiles_of(q.B.rows, Tl::BN));
+            q.grid = tile_grid<Tl>(q.tiles_m, q.B.rows);
             return (int)(q.grid * q.splits);
         };
         u.end[0] = x ? size(u.x) : 0;

@@ -637,7 +637,7 @@ template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
         else if (vecs <= 256) launch_row<T, 256, 1>(a, st);
         else if (vecs <= 512) launch_row<T, 256, 2>(a, st);
         else if (vecs <= 1024) launch_row<T, 512, 2>(a, st);
-        else if (vecs <= 2048) launch_row<T, 1024, 2>(a, st);
+        else if (vecs <= 2048) launch_row<T, 512, 4>(a, st);
         else launch_row<T, 1024, 4>(a, st);
         return hipGetLastError();
     }
