@@ -663,7 +663,7 @@ template <typename W> struct Plan {
     static constexpr int64_t EDGE = W::Tl::BM;
     int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
     int64_t xsplits, bsplits, kept_pieces;
-    bool xwide, bwide; // wide tiles for xbar, betabar
+    bool wide_products; // wide tiles for xbar and betabar
     bool copy;         // beta as operands of its own
     // offsets in bytes
     size_t kept, place, row, y, count, runs, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
@@ -717,8 +717,7 @@ template <typename W> struct Plan {
             bt = take(S * (size_t)(features * ldr));
             part_alpha = take(A * (size_t)(tiles_n * ldr));
             alpha_acc = blocks > 1 ? take(A * (size_t)classes) : 0;
-            xwide = product_wide(features, block, piece);
-            bwide = product_wide(features, piece, block);
+            wide_products = product_wide(features, block, piece) && product_wide(features, piece, block);
             xsplits = product_splits(features, block, piece);
             bsplits = product_splits(features, piece, block);
             xacc = xsplits > 1 || pieces > 1 ? take(A * (size_t)(xsplits * block * features)) : 0;
@@ -727,8 +726,8 @@ template <typename W> struct Plan {
         }
         bytes = at;
     }
-    static int64_t product_splits(int64_t m, int64_t n, int64_t K) {
-        const int64_t large = product_wide(m, n, K) ? 2 : 1, edge = 128 * large;
+    int64_t product_splits(int64_t m, int64_t n, int64_t K) const {
+        const int64_t large = wide_products ? 2 : 1, edge = 128 * large;
         return splits_of(tiles_of(m, edge) * tiles_of(n, edge) * large, K, 2 * large * tile_k<E>());
     }
 };
@@ -751,7 +750,7 @@ template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan
     };
     ready(p.x, plan.xsplits, xlast, xbar);
     ready(p.b, plan.bsplits, blast, betabar);
-    auto run = [&](auto way, bool x, bool b) {
+    auto run = [&](auto way) {
         typedef decltype(way) U;
         typedef typename U::Tl Tl;
         ProductsArgs<U> u = {p.x, p.b, p.alpha, {0, 0}};
@@ -760,23 +759,16 @@ template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan
             q.grid = tile_grid<Tl>(q.tiles_m, q.B.rows);
             return (int)(q.grid * q.splits);
         };
-        u.end[0] = x ? size(u.x) : 0;
-        u.end[1] = u.end[0] + (b ? size(u.b) : 0);
-        class_products<U><<<dim3((unsigned)(u.end[1] + (b ? alpha_blocks : 0))), dim3(Tl::THREADS), 0, st>>>(u);
+        u.end[0] = size(u.x);
+        u.end[1] = u.end[0] + size(u.b);
+        class_products<U><<<dim3((unsigned)(u.end[1] + alpha_blocks)), dim3(Tl::THREADS), 0, st>>>(u);
     };
     if constexpr (W::LINES) {
         typedef Way<T, WideTile<E, W::PLANES>, W::PLANES> Wide;
         typedef Way<T, MidTile<E, W::PLANES>, W::PLANES> Mid;
-        if (plan.xwide == plan.bwide) {
-            if (plan.xwide) run(Wide(), true, true);
-            else run(Mid(), true, true);
-        } else {
-            if (plan.xwide) run(Wide(), true, false);
-            else run(Mid(), true, false);
-            if (plan.bwide) run(Wide(), false, true);
-            else run(Mid(), false, true);
-        }
-    } else run(W(), true, true);
+        if (plan.wide_products) run(Wide());
+        else run(Mid());
+    } else run(W());
     const bool xjoin = xlast && plan.xsplits > 1, bjoin = blast && plan.bsplits > 1;
     if (xjoin || bjoin) {
         auto args = [](const auto& q, T* out) {
