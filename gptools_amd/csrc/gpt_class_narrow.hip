@@ -301,14 +301,15 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
                     mx[t] = fmax(mx[t], p[t][v][r]);
                 }
             }
-            mx[t] = fmax(mx[t], __shfl_xor(mx[t], 16, 64));
-            mx[t] = fmax(mx[t], __shfl_xor(mx[t], 32, 64));
-            // the reference follows the maximum only where it falls behind by more than 8 (exponentials up to 2^8, or e^8)
+            // the reference follows the maximum only where it falls behind by more than 8 (exponentials up to 2^8, or e^8); whether it
+            // does shows without joining the four lane groups' maxima
             far |= mx[t] > ref[t] + (A)8 || (ref[t] == neg_inf<A>() && mx[t] > ref[t]);
         }
         if (__any(far)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
+                mx[t] = fmax(mx[t], __shfl_xor(mx[t], 16, 64));
+                mx[t] = fmax(mx[t], __shfl_xor(mx[t], 32, 64));
                 const A to = fmax(ref[t], mx[t]);
                 const A f = exp_log2e(ref[t] - about(to));
                 ref[t] = to;
