@@ -63,6 +63,8 @@ template <typename T, int DT> struct Narrow {
     typedef Vec16<bf16_t>::V SVec;
     // rows of a step in LDS, and what they take: the rows, their transpose [DP][STEP + 4] or planes [3][STEP][SLD]
     template <int STEP> static constexpr int stage() { return STEP * LD + (TURN ? DP * (STEP + 4) : SPLIT ? 3 * STEP * SLD / 2 : 0); }
+    // fp32: what stands in registers is times log2(e) already, so that logits come in that unit
+    static constexpr bool UNIT = sizeof(T) >= 4;
     // a lane's part of one row (its column of the logits): chunks 4 g + q
     struct Part {
         Vec v[SPLIT ? 1 : G];
@@ -76,8 +78,8 @@ template <typename T, int DT> struct Narrow {
                     for (int h = 0; h < 2; ++h) {
                         const Vec u = tile_chunk(o, row, (int64_t)((4 * g + q) * 8 + 4 * h), D);
                         uint32_t w[2][3];
-                        split3(u[0], u[1], w[0]);
-                        split3(u[2], u[3], w[1]);
+                        split3(times_log2e(u[0]), times_log2e(u[1]), w[0]);
+                        split3(times_log2e(u[2]), times_log2e(u[3]), w[1]);
 #pragma unroll
                         for (int p = 0; p < 3; ++p) {
                             uint4 k = __builtin_bit_cast(uint4, s[p][g]);
@@ -88,7 +90,13 @@ template <typename T, int DT> struct Narrow {
                     }
             } else {
 #pragma unroll
-                for (int g = 0; g < G; ++g) v[g] = tile_chunk(o, row, (int64_t)(4 * g + q) * N, D);
+                for (int g = 0; g < G; ++g) {
+                    v[g] = tile_chunk(o, row, (int64_t)(4 * g + q) * N, D);
+                    if constexpr (UNIT) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) v[g][e] = times_log2e(v[g][e]);
+                    }
+                }
             }
         }
         __device__ __forceinline__ void clear() {
@@ -128,56 +136,60 @@ template <typename T, int DT> struct Narrow {
     template <int STEP> static constexpr int loads() { return STEP * (DP / N) / 256 > 0 ? STEP * (DP / N) / 256 : 1; }
 
     // Rows r0.. of an operand (order given: order[r0..], rows of which y says that they are observed) into registers, and from
-    // there into LDS
-    template <int STEP> static __device__ __forceinline__ void fetch(Vec (&v)[loads<STEP>()], const Operand<T>& o, int64_t r0, int64_t D,
-                                                                     const int* order, const int64_t* y) {
-        const int left = (int)(o.rows - r0 < STEP ? o.rows - r0 : STEP);
-        const T* first = o.p + r0 * o.ld;
-        const int d = (int)D;
+    // there into LDS. Rows behind the last repeat it (nothing counts them); no branch keeps a load from leaving before the one ahead of it
+    // is back, unless a row ends within 16 bytes
+    template <int STEP> struct Rows {
+        Vec v[loads<STEP>()];
+        bool seen[loads<STEP>()];
+        __device__ __forceinline__ void fetch(const Operand<T>& o, int64_t r0, int64_t D, const int* order, const int64_t* y) {
+            const int last = (int)(o.rows - r0 < STEP ? o.rows - r0 : STEP) - 1, d = (int)D;
 #pragma unroll
-        for (int i = 0; i < loads<STEP>(); ++i) {
-            const int id = i * 256 + threadIdx.x, r = id / (DP / N), k = id % (DP / N) * N;
-            v[i] = Vec{};
-            if (r >= left || k >= d) continue;
-            const T* from = first + ((int64_t)r * o.ld + k);
-            if (order || y) {
-                const int64_t row = order ? order[r0 + r] : r0 + r;
-                if (y && y[row] < 0) continue;
-                from = o.p + row * o.ld + k;
-            }
-            if (k + N <= d) v[i] = load16(from);
-            else {
+            for (int i = 0; i < loads<STEP>(); ++i) {
+                const int id = i * 256 + threadIdx.x, k = id % (DP / N) * N;
+                int64_t row = r0 + (id / (DP / N) < last ? id / (DP / N) : last);
+                if (order) row = order[row];
+                seen[i] = k < d && (!y || y[row] >= 0);
+                const T* from = o.p + row * o.ld;
+                if (d % N == 0) v[i] = load16(from + (k < d ? k : 0));
+                else {
+                    v[i] = Vec{};
+                    if (k + N <= d) v[i] = load16(from + k);
+                    else {
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (k + e < d) v[i][e] = from[e];
-            }
-        }
-    }
-    template <int STEP> static __device__ __forceinline__ void put(const Vec (&v)[loads<STEP>()], T* lds) {
-#pragma unroll
-        for (int i = 0; i < loads<STEP>(); ++i) {
-            const int id = i * 256 + threadIdx.x, r = id / (DP / N), c = id % (DP / N);
-            if (r >= STEP) continue;
-            *reinterpret_cast<Vec*>(lds + r * LD + c * N) = v[i];
-            if constexpr (TURN) {
-                T* t = lds + STEP * LD + c * N * (STEP + 4) + r;
-#pragma unroll
-                for (int e = 0; e < N; ++e) t[e * (STEP + 4)] = v[i][e];
-            }
-            if constexpr (SPLIT) {
-                bf16_t* t = reinterpret_cast<bf16_t*>(lds + STEP * LD) + r * SLD + c * N;
-                uint32_t u[2][3];
-                split3(v[i][0], v[i][1], u[0]);
-                split3(v[i][2], v[i][3], u[1]);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(t + p * STEP * SLD) = make_uint2(u[0][p], u[1][p]);
+                        for (int e = 0; e < N; ++e)
+                            if (k + e < d) v[i][e] = from[k + e];
+                    }
+                }
             }
         }
-    }
-    // C[row base + .. of lds][column held in f] and its use as an operand
-    template <int STEP> static __device__ __forceinline__ C logits(const T* lds, int base, const Part& f) {
+        __device__ __forceinline__ void put(T* lds) const {
+#pragma unroll
+            for (int i = 0; i < loads<STEP>(); ++i) {
+                const int id = i * 256 + threadIdx.x, r = id / (DP / N), c = id % (DP / N);
+                if (r >= STEP) continue;
+                uint4 word = __builtin_bit_cast(uint4, v[i]);
+                if (!seen[i]) word = make_uint4(0, 0, 0, 0);
+                const Vec w = __builtin_bit_cast(Vec, word);
+                *reinterpret_cast<Vec*>(lds + r * LD + c * N) = w;
+                if constexpr (TURN) {
+                    T* t = lds + STEP * LD + c * N * (STEP + 4) + r;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) t[e * (STEP + 4)] = w[e];
+                }
+                if constexpr (SPLIT) {
+                    bf16_t* t = reinterpret_cast<bf16_t*>(lds + STEP * LD) + r * SLD + c * N;
+                    uint32_t u[2][3];
+                    split3(w[0], w[1], u[0]);
+                    split3(w[2], w[3], u[1]);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(t + p * STEP * SLD) = make_uint2(u[0][p], u[1][p]);
+                }
+            }
+        }
+    };
+    // C[row base + .. of lds][column held in f] plus c in UNIT, and its use as an operand
+    template <int STEP> static __device__ __forceinline__ C logits(const T* lds, int base, const Part& f, C c) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
-        C c = {0, 0, 0, 0};
         if constexpr (SPLIT) {
             const bf16_t* t = reinterpret_cast<const bf16_t*>(lds + STEP * LD) + (base + (lane & 15)) * SLD;
 #pragma unroll
@@ -269,10 +281,10 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = C{0, 0, 0, 0};
     }
-    Vec next[W::template loads<STEP>()];
+    typename W::template Rows<STEP> next;
     A next_al = 0;
     auto fetch = [&](int64_t v0) {
-        W::template fetch<STEP>(next, a.beta, v0, D, nullptr, nullptr);
+        next.fetch(a.beta, v0, D, nullptr, nullptr);
         if (threadIdx.x < STEP) {
             const int64_t v = v0 + threadIdx.x;
             next_al = v < V ? (a.alpha ? level_log2e((A)a.alpha[v]) : (A)0) : neg_inf<A>();
@@ -281,7 +293,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
     fetch(0);
     for (int64_t v0 = 0; v0 < V; v0 += STEP) {
         __syncthreads();
-        W::template put<STEP>(next, lds);
+        next.put(lds);
         if (threadIdx.x < STEP) al[threadIdx.x] = next_al;
         __syncthreads();
         if (v0 + STEP < V) fetch(v0 + STEP);
@@ -294,16 +306,19 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 #pragma unroll
             for (int v = 0; v < VT; ++v) {
                 const int base = (wv * VT + v) * 16;
-                p[t][v] = W::template logits<STEP>(lds, base, x[t]);
+                C level;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) level[r] = al[base + Mma<T>::row(q, r)];
+                p[t][v] = W::template logits<STEP>(lds, base, x[t], W::UNIT ? level : C{0, 0, 0, 0});
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[t][v][r] = times_log2e(p[t][v][r]) + al[base + Mma<T>::row(q, r)];
+                    if (!W::UNIT) p[t][v][r] = times_log2e(p[t][v][r]) + level[r];
                     mx[t] = fmax(mx[t], p[t][v][r]);
                 }
             }
             // the reference follows the maximum only where it falls behind by more than 8 (exponentials up to 2^8, or e^8); whether it
             // does shows without joining the four lane groups' maxima
-            far |= mx[t] > ref[t] + (A)8 || (ref[t] == neg_inf<A>() && mx[t] > ref[t]);
+            far |= mx[t] > ref[t] + (A)8;
         }
         if (__any(far)) {
 #pragma unroll
@@ -361,7 +376,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         if (wv == 0 && known) eta = x[t].dot(a.beta, y[t], D);
         eta += __shfl_xor(eta, 16, 64);
         eta += __shfl_xor(eta, 32, 64);
-        eta = times_log2e(eta);
+        if (!W::UNIT) eta = times_log2e(eta);
         if (known && a.alpha) eta += level_log2e((A)a.alpha[y[t]]);
         A lse;
         const A lp = row_lp(y[t], V, mx, s, eta, lse);
@@ -438,11 +453,11 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     }
     const int64_t r0 = (int64_t)blockIdx.y * share, r1 = r0 + share < rows ? r0 + share : rows;
     const Operand<T> x = {a.x.p, a.x.ld, r1, 0};
-    Vec next[W::template loads<STEP>()];
+    typename W::template Rows<STEP> next;
     A next_lse = 0, next_w = 0;
     int next_y = -1;
     auto fetch = [&](int64_t n0) {
-        W::template fetch<STEP>(next, x, n0, D, a.order, a.order ? nullptr : a.y);
+        next.fetch(x, n0, D, a.order, a.order ? nullptr : a.y);
         if (threadIdx.x < STEP) {
             const int64_t n = n0 + threadIdx.x;
             next_lse = n < r1 ? a.lse[n] : -neg_inf<A>();
@@ -453,7 +468,7 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     if (r0 < r1) fetch(r0);
     for (int64_t n0 = r0; n0 < r1; n0 += STEP) {
         __syncthreads();
-        W::template put<STEP>(next, lds);
+        next.put(lds);
         if (threadIdx.x < STEP) {
             lse[threadIdx.x] = next_lse;
             wt[threadIdx.x] = next_w;
@@ -466,11 +481,12 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
             const int base = (wr * VT + u) * 16;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                C p = W::template logits<STEP>(lds, base, b[t]);
+                const A level = W::UNIT ? al[t] : (A)0;
+                C p = W::template logits<STEP>(lds, base, b[t], C{level, level, level, level});
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int n = base + Mma<T>::row(q, r);
-                    const A e = exp_log2e(times_log2e(p[r]) + al[t] - lse[n]);
+                    const A e = exp_log2e((W::UNIT ? p[r] : times_log2e(p[r]) + al[t]) - lse[n]);
                     p[r] = wt[n] * ((yt[n] == me[t] ? (A)1 : (A)0) - e);
                     abar[t] += p[r];
                 }
