@@ -45,8 +45,10 @@ template <typename T> struct NarrowArgs {
 // waves' shares, have not the registers and the LDS for two)
 template <typename T, int DT, int SHARES> constexpr int VT_ = sizeof(T) >= 4 && DT == 4 && SHARES == 4 ? 1 : 2;
 
-// waves of a SIMD that the registers have to leave room for
-template <typename T, int DT> constexpr int WAVES_ = sizeof(T) == 8 || (sizeof(T) == 4 && DT == 4) ? 2 : 4;
+// Waves of a SIMD that the registers have to leave room for (bf16 5000 rows x 64 x 1000, fp32 5000 x 32 x 1000, whose waves share the rows:
+// 39 and 41 us with two, 43 and 46 with four, which spill)
+template <typename T, int DT, int SHARES>
+constexpr int WAVES_ = sizeof(T) == 8 || (sizeof(T) == 4 && DT == 4) || (SHARES == 4 && DT * (int)sizeof(T) == 8) ? 2 : 4;
 
 template <typename T, int DT> struct Narrow {
     typedef acc_t<T> A;
@@ -243,11 +245,10 @@ template <typename T, int DT> struct Narrow {
 constexpr int larger(int a, int b) { return a > b ? a : b; }
 
 // WR groups of 16 NT rows x WV shares of the classes a workgroup
-template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __launch_bounds__(256, (WAVES_<T, DT>)) void class_narrow_rows(NarrowArgs<T> a) {
+template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __launch_bounds__(256, (WAVES_<T, DT, WV>)) void class_narrow_rows(NarrowArgs<T> a) {
     typedef Narrow<T, DT> W;
     typedef typename W::A A;
     typedef typename W::C C;
-    typedef typename W::Vec Vec;
     constexpr int VT = VT_<T, DT, WV>, STEP = 16 * VT * WV, ROWS = 16 * NT * WR;
     constexpr int STAGE = W::template stage<STEP>() * (int)sizeof(T), SPILL = VJP ? WV * ROWS * W::OLD * (int)sizeof(A) : 0;
     __shared__ uint4 room[(larger(STAGE, SPILL) + 15) / 16];
@@ -418,11 +419,10 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 }
 
 // WV groups of 16 NT classes x WR shares of the rows of this workgroup's share
-template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds__(256, (WAVES_<T, DT>)) void class_narrow_classes(NarrowArgs<T> a) {
+template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds__(256, (WAVES_<T, DT, WR>)) void class_narrow_classes(NarrowArgs<T> a) {
     typedef Narrow<T, DT> W;
     typedef typename W::A A;
     typedef typename W::C C;
-    typedef typename W::Vec Vec;
     constexpr int VT = VT_<T, DT, WR>, STEP = 16 * VT * WR, CLASSES = 16 * NT * WV;
     constexpr int STAGE = W::template stage<STEP>() * (int)sizeof(T), SPILL = WR * CLASSES * W::OLD * (int)sizeof(A);
     __shared__ uint4 room[(larger(STAGE, SPILL) + 15) / 16];
@@ -519,7 +519,8 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     }
 }
 
-// betabar, alphabar <- sums over the shares
+// betabar, alphabar <- sums over the shares. (The last share to arrive could add them up without this launch, but making its values
+// visible across the XCDs costs more: fp64 2100 rows x 8 x 300 49 us against 23)
 template <typename T> __global__ __launch_bounds__(256) void class_narrow_join(const acc_t<T>* part, int shares, int64_t V, int64_t D,
                                                                               Largest<acc_t<T>> largest, T* betabar, T* alphabar) {
     typedef acc_t<T> A;
