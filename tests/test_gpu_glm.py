@@ -125,6 +125,14 @@ def test_layer_norm_lattices(glm, name, rows, core):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("rows,core", [((300,), (2049,)), ((270,), (4095,)), ((520,), (8191,)), ((260,), (10001,)), ((300,), (16001,)),
+                                       ((300,), (5,)), ((3000,), (17,)), ((3,), (40961,)), ((290,), (40961,)), ((64,), (300, 1000))])
+def test_layer_norm_several_rows_a_workgroup(glm, name, rows, core):
+    """More rows than workgroups, at lengths that a part vector, a part sweep or one value ends; lattices that share weights."""
+    _check_norm(glm, name, rows, core, seed=core[0])
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
 @pytest.mark.parametrize("width", [40, 3000, 70001])
 def test_layer_norm_without_parameters(glm, name, width):
     _check_norm(glm, name, (5,), (width,), affine=False, seed=width)
@@ -348,6 +356,47 @@ def test_class_many_rows(glm, name, n, d, v):
     y, x, alpha, beta = _class_data(name, n, d, v, 29, masked=0.1)
     lpbar = torch.full((n,), 1 / 1024, dtype=_wide(DTYPES[name]), device="cuda")
     _check_class(glm, name, y, x, alpha, beta, lpbar)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n,d,v", [(100, 72, 50000), (257, 72, 25000), (384, 72, 25000), (385, 72, 25000), (1100, 1000, 24680)])
+def test_class_last_rows_and_classes_fill_part_of_a_tile(glm, name, n, d, v):
+    _check_class(glm, name, *_class_data(name, n, d, v, seed=n + v))
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_class_observed_rows_fill_part_of_a_tile(glm, name):
+    for masked in (0.5, 0.6, 0.9):  # of 700 rows, about 350, 280, 70
+        y, x, alpha, beta = _class_data(name, 700, 72, 20000, 5, masked)
+        x[y < 0] = float("nan")
+        _check_class(glm, name, y, x, alpha, beta)
+
+
+@pytest.mark.parametrize("name,n,d,v", [("bf16", 16500, 768, 18000), ("f16", 16500, 800, 18000), ("f32", 4100, 170, 80000), ("f64", 2000, 70, 90000)])
+def test_class_some_logits_are_kept(glm, name, n, d, v):
+    """Several pieces of the classes, the logits of some of them kept and of the others computed again."""
+    y, x, alpha, beta = _class_data(name, n, d, v, 31, masked=0.1)
+    alpha[v // 2 : v // 2 + 300] = -float("inf")
+    y[(y >= v // 2) & (y < v // 2 + 300)] = 0
+    lpbar = torch.full((n,), -1 / 1024, dtype=_wide(DTYPES[name]), device="cuda")
+    _check_class(glm, name, y, x, alpha, beta, lpbar)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_class_kept_logits_of_rows_without_any(glm, name):
+    """Rows whose classes are all excluded, or whose values are spoilt, where the logits are kept."""
+    y, x, alpha, beta = _class_data(name, 300, 800, 1500, 37, masked=0.2)
+    lp, xbar, alphabar, betabar = glm.categorical_logit_glm_lpmf_vjp(y, x, torch.full_like(alpha, -float("inf")), beta)
+    seen = y >= 0
+    assert bool((lp[seen] == -float("inf")).all()) and not bool(lp[~seen].any())
+    assert not bool(xbar.any()) and not bool(alphabar.any()) and not bool(betabar.any())
+    want = glm.categorical_logit_glm_lpmf_vjp(y, x, alpha, beta)
+    row = int(seen.nonzero()[3])
+    x[row, 5] = float("nan")
+    got = glm.categorical_logit_glm_lpmf_vjp(y, x, alpha, beta)
+    rest = torch.arange(300, device="cuda") != row
+    assert bool(torch.isnan(got[0][row])) and torch.equal(got[0][rest], want[0][rest])
+    assert bool(torch.isnan(got[1][row]).all()) and torch.equal(got[1][rest], want[1][rest])
 
 
 def test_class_empty(glm):
