@@ -256,7 +256,8 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
     __shared__ A red[2][WV][ROWS];
     T* lds = reinterpret_cast<T*>(room);
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6, wr = wave / WV, wv = wave % WV;
-    const int64_t n0 = (int64_t)blockIdx.x * ROWS, V = a.beta.rows, D = a.features;
+    const int64_t n0 = wide_block() * ROWS, V = a.beta.rows, D = a.features;
+    if (n0 >= a.x.rows) return;
     if (a.count && n0 >= *a.count) { // nothing observed here: zeros (lp has them)
         if (VJP)
             for (int id = threadIdx.x; id < ROWS * (int)D; id += 256) {
@@ -598,7 +599,7 @@ template <typename T> struct NarrowPlan {
 template <typename T, int DT, bool VJP> void rows_kernel(const NarrowArgs<T>& a, const NarrowPlan<T>& p, hipStream_t st) {
     constexpr int NT = NarrowPlan<T>::NT;
     if (p.many_rows)
-        class_narrow_rows<T, DT, 2, 2, NT, VJP><<<dim3((unsigned)tiles_of(a.x.rows, 32 * NT)), dim3(256), 0, st>>>(a);
+        class_narrow_rows<T, DT, 2, 2, NT, VJP><<<wide_grid(tiles_of(a.x.rows, 32 * NT)), dim3(256), 0, st>>>(a);
     else class_narrow_rows<T, DT, 1, 4, 1, VJP><<<dim3((unsigned)tiles_of(a.x.rows, 16)), dim3(256), 0, st>>>(a);
 }
 template <typename T, int DT> void run(const NarrowArgs<T>& a, const NarrowPlan<T>& p, bool vjp, hipStream_t st) {

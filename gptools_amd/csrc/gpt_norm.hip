@@ -104,7 +104,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_row(NormAr
     constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, K = ITER * Vec16<T>::N;
     __shared__ A red[THREADS / 64];
     const int t = threadIdx.x % THREADS;
-    const int64_t row = (int64_t)blockIdx.x * (BLOCK / THREADS) + threadIdx.x / THREADS;
+    const int64_t row = wide_block() * (BLOCK / THREADS) + threadIdx.x / THREADS;
     if (row >= a.rows) return; // (whole waves; a workgroup with barriers has one row)
     const int64_t n = a.width;
     typedef RowRaw<T, THREADS, ITER> Raw;
@@ -626,7 +626,7 @@ template <typename T> size_t workspace(int64_t rows, int64_t n, bool vjp) {
 
 template <typename T, int THREADS, int ITER> void launch_row(const NormArgs& a, hipStream_t st) {
     constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, RPB = BLOCK / THREADS;
-    norm_row<T, THREADS, ITER><<<dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, st>>>(a);
+    norm_row<T, THREADS, ITER><<<wide_grid((a.rows + RPB - 1) / RPB), dim3(BLOCK), 0, st>>>(a);
 }
 template <typename T> hipError_t forward(NormArgs a, hipStream_t st) {
     const int64_t vecs = (a.width + Vec16<T>::N - 1) / Vec16<T>::N;

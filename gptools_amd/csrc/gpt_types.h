@@ -31,6 +31,13 @@ template <typename T> __device__ __forceinline__ void store16(T* p, typename Vec
     *reinterpret_cast<typename Vec16<T>::U*>(p) = v;
 }
 
+// A grid of many workgroups, in two dimensions (one counts its threads in 32 bits); workgroups behind the last of them may be there
+inline dim3 wide_grid(int64_t blocks) {
+    constexpr int64_t ROW = (int64_t)1 << 20;
+    return blocks <= ROW ? dim3((unsigned)blocks) : dim3((unsigned)ROW, (unsigned)((blocks + ROW - 1) / ROW));
+}
+__device__ __forceinline__ int64_t wide_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // sum over the 64 lanes of a wave, in every lane
 template <typename A> __device__ __forceinline__ A wave_sum(A v) {
 #pragma unroll

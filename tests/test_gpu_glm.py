@@ -175,6 +175,21 @@ def test_layer_norm_views_empty_batches_and_no_parameter_gradients(glm):
     assert xbar.shape == empty.shape and not bool(wbar.any()) and not bool(bbar.any())
 
 
+def test_layer_norm_of_very_many_rows(glm):
+    """More threads than a grid's dimension counts (2^32), and more values than 32 bits."""
+    rows, width = (1 << 26) + 1001, 65
+    x = torch.randint(-100, 100, (rows, width), dtype=torch.int8, device="cuda").to(torch.bfloat16)
+    y, mean, rstd = glm.layer_norm(x)
+    for at in (0, 1 << 25, rows - 700):
+        some = x[at:at + 700].clone()
+        want = glm.layer_norm(some)
+        assert torch.equal(y[at:at + 700], want[0]) and torch.equal(mean[at:at + 700], want[1]) and torch.equal(rstd[at:at + 700], want[2])
+    xbar = glm.layer_norm_vjp(x, None, mean, rstd, y, need_param_grad=False)[0]
+    for at in (0, 1 << 25, rows - 700):
+        c = slice(at, at + 700)
+        assert torch.equal(xbar[c], glm.layer_norm_vjp(x[c].clone(), None, mean[c], rstd[c], y[c], need_param_grad=False)[0])
+
+
 # ---- categorical log density -------------------------------------------------------------------------------------------
 def _class_want(y, x, alpha, beta, lpbar, seen):
     xd = torch.where(seen.unsqueeze(1), x.double(), torch.zeros((), dtype=torch.float64, device="cuda"))
@@ -356,6 +371,22 @@ def test_class_many_rows(glm, name, n, d, v):
     y, x, alpha, beta = _class_data(name, n, d, v, 29, masked=0.1)
     lpbar = torch.full((n,), 1 / 1024, dtype=_wide(DTYPES[name]), device="cuda")
     _check_class(glm, name, y, x, alpha, beta, lpbar)
+
+
+def test_class_of_very_many_rows(glm):
+    """More threads than a grid's dimension counts (2^32)."""
+    n = (1 << 29) + 77
+    x = torch.zeros(n, 1, dtype=torch.float64, device="cuda")
+    x[-5:, 0] = torch.arange(1.0, 6.0, dtype=torch.float64, device="cuda")
+    y = torch.zeros(n, dtype=torch.int64, device="cuda")
+    y[: n - 3 : 2] = -1
+    beta = torch.tensor([[0.5], [-0.25]], dtype=torch.float64, device="cuda")
+    lp = glm.categorical_logit_glm_lpmf(y, x, None, beta)
+    want = glm.categorical_logit_glm_lpmf(y[-100:].clone(), x[-100:].clone(), None, beta)
+    assert torch.allclose(lp[-100:], want, rtol=16 * 2.0**-53, atol=16 * 2.0**-53)
+    some = torch.arange(0, n - 5, 1001, device="cuda")
+    some_lp = -math.log(2) * (y[some] >= 0).double()
+    assert torch.allclose(lp[some], some_lp, rtol=16 * 2.0**-53, atol=0)
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
