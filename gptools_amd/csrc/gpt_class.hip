@@ -990,6 +990,13 @@ template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStr
     return launch_few<T, 4>(c, vjp, st);
 }
 
+// fp32 products of few rows and many classes stay with the fp32 instructions: splitting beta takes longer than they do. With and
+// without splitting, in us: 100 rows x 1024 x 32000 146 / 88, with the reverse mode 428 / 386; 200 rows 166 / 151 and 577 / 576; but
+// 200 x 128 x 20000 with the reverse mode 133 / 187, and where the tiles do not fill the card (130 x 2000 x 5000) 132 / 160
+bool whole(int64_t rows, int64_t classes, bool vjp) {
+    return rows <= (vjp ? 128 : 256) && tiles_of(classes, 128) * tiles_of(rows, 128) >= WIDE_TILES;
+}
+
 // fp32 runs in three planes of bf16; fp64 has neither the instructions nor the registers for line tiles
 template <typename T> struct Ways {
     typedef Way<T, WideTile<T>, 1> Wide;
@@ -999,6 +1006,7 @@ template <typename T> struct Ways {
 template <> struct Ways<float> {
     typedef Way<float, WideTile<bf16_t, 3>, 3> Wide;
     typedef Way<float, MidTile<bf16_t, 3>, 3> Mid;
+    typedef Way<float, SmallTile<float>, 1> Other; // few rows
 };
 template <> struct Ways<double> {
     typedef Way<double, SmallTile<double>, 1> Other;
@@ -1010,6 +1018,7 @@ template <typename T> size_t space(int64_t rows, int64_t features, int64_t class
     else {
         const bool large = wide(classes, rows < ROW_BLOCK ? rows : ROW_BLOCK);
         const size_t n = large ? Plan<typename Y::Wide>(rows, features, classes, vjp).bytes : Plan<typename Y::Mid>(rows, features, classes, vjp).bytes;
+        if (sizeof(T) == 4 && whole(rows, classes, vjp)) return Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
         if constexpr (sizeof(T) == 2) { // (whether beta starts on 16 bytes shows only in the call)
             const size_t other = Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
             return n > other ? n : other;
@@ -1022,6 +1031,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     typedef Ways<T> Y;
     if constexpr (sizeof(T) == 8) return launch_rows<typename Y::Other>(c, vjp, st);
     else {
+        if (sizeof(T) == 4 && whole(c.rows, c.classes, vjp)) return launch_rows<typename Y::Other>(c, vjp, st);
         if constexpr (sizeof(T) == 2) {
             // (rows of an odd length are copied, whole ones need to start on 16 bytes where they are)
             if (c.features * sizeof(T) % 16 == 0 && !tile_fits(Operand<T>{(const T*)c.beta, c.ldbeta, c.classes, 0}))
