@@ -66,6 +66,8 @@ template <typename T> struct LogitArgs {
     // logits of the first kept_classes classes, as the first sweep leaves them for the second: tile by tile, a lane's fragments
     typename T::Tl::C* kept;
     int64_t kept_classes;
+    // ... or, if the first sweep's tiles are few, shares of k that are added up then: [splits] of those, `plane` apart
+    int64_t splits, plane, grid; // grid: workgroups of one share
 };
 
 // One way to run the products: data type, tile, type and number of planes of its operands
@@ -85,7 +87,8 @@ template <typename W> __device__ __forceinline__ void words(float a, float b, ui
     } else u[0] = pack2<typename W::Element>(a, b);
 }
 
-// Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r. KEPT: eta was kept.
+// Tiles of eta, classes x rows. STATS: each tile's maximum and sum of exponentials for every row. else: r. KEPT: eta was kept (STATS: the
+// shares of class_partial).
 template <typename W> struct LogitRoom { // LDS
     typedef typename W::Acc A;
     typedef typename W::Tl Tl;
@@ -101,7 +104,7 @@ __device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_
     // what the tile's classes and rows need besides, on its way into LDS while the product runs (which ends with a barrier)
     A largest = 1;
     if (!STATS) largest = a.largest.get();
-    for (int c = threadIdx.x; !KEPT && c < Tl::BM; c += Tl::THREADS)
+    for (int c = threadIdx.x; (STATS || !KEPT) && c < Tl::BM; c += Tl::THREADS)
         room.al[c] = c < nv ? (a.alpha ? level_log2e((A)a.alpha[m0 + c]) : (A)0) : neg_inf<A>();
     for (int c = threadIdx.x; c < Tl::BN; c += Tl::THREADS) {
         const int64_t n = n0 + c, y = n < rows ? a.y[n] : -1, from = y - (a.v0 + m0);
@@ -124,9 +127,14 @@ __device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_
         for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
             for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j] = kept[(i * Tl::TN + j) * Tl::THREADS];
+        for (int64_t k = 1; STATS && k < a.splits; ++k)
+#pragma unroll
+            for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j] += kept[k * a.plane + (i * Tl::TN + j) * Tl::THREADS];
         __syncthreads();
-    } else {
-        tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
+    } else tl.run(a.beta, m0, a.x, n0, 0, a.features, lds);
+    if (STATS || !KEPT) {
 #pragma unroll
         for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
@@ -293,6 +301,26 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
         }
     }
     logits_tile<W, Tl, STATS, KEPT>(a, rows, tm, tn, room, lds);
+}
+
+// A share of k's part of eta's tiles, as they are
+template <typename W> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class_partial(LogitArgs<W> a) {
+    typedef typename W::Tl Tl;
+    __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
+    const int64_t ld = a.x.rows, split = blockIdx.x / a.grid, step = tile_k<typename W::Element>();
+    a.x.rows = *a.count;
+    int64_t tm, tn;
+    bool half;
+    if (!tile_place<Tl>(blockIdx.x - split * a.grid, a.tiles_v, a.x.rows, tm, tn, half)) return;
+    const int64_t share = ((a.features + a.splits - 1) / a.splits + step - 1) / step * step;
+    const int64_t k0 = split * share, k1 = k0 + share < a.features ? k0 + share : a.features;
+    Tl tl;
+    tl.run(a.beta, tm * Tl::BM, a.x, tn * Tl::BN, k0, k1, lds);
+    auto* to = a.kept + split * a.plane + (tm * ((ld + Tl::BN - 1) / Tl::BN) + tn) * (Tl::TM * Tl::TN * Tl::THREADS) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < Tl::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < Tl::TN; ++j) to[(i * Tl::TN + j) * Tl::THREADS] = tl.acc[i][j];
 }
 
 // The observed rows of x side by side, as operands (zeros behind their features); zeros into xbar's other rows
@@ -648,6 +676,11 @@ int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
     if (s > most) s = most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
 }
+// Shares of k of the first sweep's tiles where these are few: at least 24 steps of k each, 8 in fp64 (fp32 65 rows x 4000 x 8000 170 us
+// against 308, fp64 500 x 500 x 2000 71 against 100; but fp32 1000 x 500 x 1500 in five shares 53 against 48)
+template <typename E> int64_t logit_splits(int64_t tiles, int64_t K) {
+    return tiles < FILL / 2 ? splits_of(tiles, K, (sizeof(E) == 8 ? 2 : 6) * tile_k<E>()) : 1;
+}
 // 256 x 256 tiles for a product of m x n results?
 bool wide(int64_t m, int64_t n) { return tiles_of(m, 256) * tiles_of(n, 256) >= WIDE_TILES; }
 
@@ -662,7 +695,7 @@ template <typename W> struct Plan {
     typedef typename W::Element E;
     static constexpr int64_t EDGE = W::Tl::BM;
     int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
-    int64_t xsplits, bsplits, kept_pieces;
+    int64_t lsplits, xsplits, bsplits, kept_pieces;
     bool wide_products; // wide tiles for xbar and betabar
     bool copy;         // beta as operands of its own
     // offsets in bytes
@@ -696,6 +729,10 @@ template <typename W> struct Plan {
         xa = take(S * (size_t)(block * ldk));
         copy = W::PLANES == 3 || (W::LINES && features * sizeof(T) % 16);
         if (copy) ba = take(S * (size_t)(classes * ldk));
+        const int64_t tiles = tiles_v * tiles_n;
+        lsplits = std::is_void<typename HalfOf<typename W::Tl>::Tile>::value ? logit_splits<E>(tiles, (W::PLANES == 3 ? 6 : 1) * features) : 1;
+        kept_pieces = 0;
+        if (lsplits > 1) kept = take((size_t)(lsplits * tiles * EDGE * EDGE) * A);
         if (vjp) {
             piece = PIECE_BYTES / (int64_t)(2 * S) / up_to(block, EDGE) / EDGE * EDGE;
             if (piece < EDGE) piece = EDGE;
@@ -706,9 +743,9 @@ template <typename W> struct Plan {
             ldr = piece;
             ldrt = up_to(block, EDGE);
             const int64_t logits = (int64_t)A * piece * ldrt;
-            kept_pieces = features >= keep_features<T>() ? KEPT_BYTES / logits : 0;
+            kept_pieces = lsplits > 1 || features >= keep_features<T>() ? KEPT_BYTES / logits : 0;
             if (kept_pieces > pieces) kept_pieces = pieces;
-            kept = take((size_t)(kept_pieces * logits));
+            if (lsplits == 1) kept = take((size_t)(kept_pieces * logits)); // (else in the first share's place)
             lse = take(A * (size_t)block);
             scale = take(A * SCALE_PARTS);
             r = take(S * (size_t)(ldrt * ldr));
@@ -785,6 +822,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
     typedef typename W::Element E;
     typedef acc_t<T> A;
     constexpr int64_t EDGE = W::Tl::BM;
+    constexpr bool PARTED = std::is_void<typename HalfOf<typename W::Tl>::Tile>::value;
     const Plan<W> p(c.rows, c.features, c.classes, vjp);
     char* ws = (char*)c.ws;
     const int64_t D = c.features, V = c.classes;
@@ -843,7 +881,17 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         l.largest = largest;
         l.kept = (typename W::Tl::C*)(ws + p.kept);
         l.kept_classes = vjp ? p.kept_pieces * p.piece : 0;
-        logits<W, true, false>(l, st);
+        l.splits = p.lsplits;
+        if constexpr (!PARTED) logits<W, true, false>(l, st);
+        else if (p.lsplits == 1) logits<W, true, false>(l, st);
+        else {
+            typedef typename W::Tl Tl;
+            l.tiles_v = p.tiles_v;
+            l.grid = tile_grid<Tl>(l.tiles_v, N);
+            l.plane = p.tiles_v * p.tiles_n * (Tl::TM * Tl::TN * Tl::THREADS);
+            class_partial<W><<<dim3((unsigned)(l.grid * l.splits)), dim3(Tl::THREADS), 0, st>>>(l);
+            logits<W, true, true>(l, st);
+        }
         A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
         class_join<A><<<dim3((unsigned)tiles_of(N, 8)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
                                                                             tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
@@ -993,8 +1041,9 @@ template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStr
 // fp32 products of few rows and many classes stay with the fp32 instructions: splitting beta takes longer than they do. With and
 // without splitting, in us: 100 rows x 1024 x 32000 146 / 88, with the reverse mode 428 / 386; 200 rows 166 / 151 and 577 / 576; but
 // 200 x 128 x 20000 with the reverse mode 133 / 187, and where the tiles do not fill the card (130 x 2000 x 5000) 132 / 160
-bool whole(int64_t rows, int64_t classes, bool vjp) {
-    return rows <= (vjp ? 128 : 256) && tiles_of(classes, 128) * tiles_of(rows, 128) >= WIDE_TILES;
+bool whole(int64_t rows, int64_t features, int64_t classes, bool vjp) {
+    const int64_t tiles = tiles_of(classes, 128) * tiles_of(rows, 128);
+    return rows <= (vjp ? 128 : 256) && tiles * logit_splits<float>(tiles, features) >= WIDE_TILES;
 }
 
 // fp32 runs in three planes of bf16; fp64 has neither the instructions nor the registers for line tiles
@@ -1018,7 +1067,7 @@ template <typename T> size_t space(int64_t rows, int64_t features, int64_t class
     else {
         const bool large = wide(classes, rows < ROW_BLOCK ? rows : ROW_BLOCK);
         const size_t n = large ? Plan<typename Y::Wide>(rows, features, classes, vjp).bytes : Plan<typename Y::Mid>(rows, features, classes, vjp).bytes;
-        if (sizeof(T) == 4 && whole(rows, classes, vjp)) return Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
+        if (sizeof(T) == 4 && whole(rows, features, classes, vjp)) return Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
         if constexpr (sizeof(T) == 2) { // (whether beta starts on 16 bytes shows only in the call)
             const size_t other = Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
             return n > other ? n : other;
@@ -1031,7 +1080,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     typedef Ways<T> Y;
     if constexpr (sizeof(T) == 8) return launch_rows<typename Y::Other>(c, vjp, st);
     else {
-        if (sizeof(T) == 4 && whole(c.rows, c.classes, vjp)) return launch_rows<typename Y::Other>(c, vjp, st);
+        if (sizeof(T) == 4 && whole(c.rows, c.features, c.classes, vjp)) return launch_rows<typename Y::Other>(c, vjp, st);
         if constexpr (sizeof(T) == 2) {
             // (rows of an odd length are copied, whole ones need to start on 16 bytes where they are)
             if (c.features * sizeof(T) % 16 == 0 && !tile_fits(Operand<T>{(const T*)c.beta, c.ldbeta, c.classes, 0}))
