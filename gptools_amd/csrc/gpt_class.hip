@@ -127,6 +127,7 @@ __device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_
         for (int i = 0; i < Tl::TM; ++i)
 #pragma unroll
             for (int j = 0; j < Tl::TN; ++j) tl.acc[i][j] = kept[(i * Tl::TN + j) * Tl::THREADS];
+#pragma unroll 2
         for (int64_t k = 1; STATS && k < a.splits; ++k)
 #pragma unroll
             for (int i = 0; i < Tl::TM; ++i)
@@ -676,10 +677,10 @@ int64_t splits_of(int64_t tiles, int64_t K, int64_t step) {
     if (s > most) s = most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
 }
-// Shares of k of the first sweep's tiles where these are few: at least 24 steps of k each, 8 in fp64 (fp32 65 rows x 4000 x 8000 170 us
+// Shares of k of the first sweep's tiles where these are few: at least 24 steps of k each, 16 of the fp32 instructions', 8 of fp64's (fp32 65 rows x 4000 x 8000 170 us
 // against 308, fp64 500 x 500 x 2000 71 against 100; but fp32 1000 x 500 x 1500 in five shares 53 against 48)
 template <typename E> int64_t logit_splits(int64_t tiles, int64_t K) {
-    return tiles < FILL / 2 ? splits_of(tiles, K, (sizeof(E) == 8 ? 2 : 6) * tile_k<E>()) : 1;
+    return tiles < FILL / 2 ? splits_of(tiles, K, (sizeof(E) == 8 ? 2 : sizeof(E) == 4 ? 4 : 6) * tile_k<E>()) : 1;
 }
 // 256 x 256 tiles for a product of m x n results?
 bool wide(int64_t m, int64_t n) { return tiles_of(m, 256) * tiles_of(n, 256) >= WIDE_TILES; }
