@@ -6,8 +6,9 @@
 // Two passes over the classes. The first leaves a maximum and a sum for every row and tile of classes; the second takes a piece of
 // the classes at a time and turns its logits into the piece's r in a workspace of bounded size, from which two more matrix
 // products take xbar and betabar. Of the logits a bounded part is kept from the first pass (the tiles' registers as they are, up to
-// KEPT_BYTES), the rest is computed again. Everything that a product sums over stands contiguously for both operands: r is written in both
-// orders, x and the piece of beta are transposed once.
+// KEPT_BYTES), the rest is computed again. r is written in both orders, so that what a product sums over stands contiguously in it; of beta
+// and x, whose sums run down their columns there, the large tiles take transposed reads from LDS (for 65 rows x 4096 x 32000 in bf16 a
+// transposed copy of beta cost 400 us against 301), the small one transposed copies.
 //
 // What bounds it are the matrix cores: 4096 rows x 4096 features x 128000 classes in bf16 take 12.5 ms, 1.13 PFLOP/s in the products at the
 // 1.85-1.9 GHz that the power leaves (60-63 % busy).
@@ -75,6 +76,7 @@ template <typename T, typename Tl_, int PLANES_> struct Way {
     typedef T Data;
     typedef acc_t<T> Acc;
     typedef Tl_ Tl;
+    typedef typename TurnedOf<Tl>::Tile Product; // of the products with r
     typedef typename Tl::Element Element;
     static constexpr int PLANES = PLANES_;
     static constexpr bool LINES = Tl::TN == 4 && !std::is_same<Tl, SmallTile<T>>::value; // a LineTile
@@ -324,6 +326,8 @@ template <typename W> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class
         for (int j = 0; j < Tl::TN; ++j) to[(i * Tl::TN + j) * Tl::THREADS] = tl.acc[i][j];
 }
 
+__host__ __device__ __forceinline__ int64_t tiles_up(int64_t n, int64_t b) { return (n + b - 1) / b; }
+
 // The observed rows of x side by side, as operands (zeros behind their features); zeros into xbar's other rows
 template <typename W> struct GatherArgs {
     const typename W::Data* x;
@@ -332,6 +336,7 @@ template <typename W> struct GatherArgs {
     typename W::Element* out;
     int64_t ldo, plane;
     typename W::Data* xbar;
+    const int* count; // rows of out (null: rows), which zeros fill up to a multiple of 64 where a product runs along them
 };
 template <typename W> __device__ __forceinline__ void gather(const GatherArgs<W>& a, int64_t block, int64_t blocks) {
     typedef typename W::Data T;
@@ -340,6 +345,12 @@ template <typename W> __device__ __forceinline__ void gather(const GatherArgs<W>
     const int64_t ld = a.ld, rows = a.rows, cols = a.cols, ldo = a.ldo, plane = a.plane, per = ldo / N, total = rows * per;
     const int* place = a.place;
     T* xbar = a.xbar;
+    if (W::LINES) {
+        const int64_t from = a.count ? *a.count : rows, more = (tiles_up(from, 64) * 64 - from) * per;
+        for (int64_t i = block * 256 + threadIdx.x; i < more; i += blocks * 256)
+#pragma unroll
+            for (int p = 0; p < W::PLANES; ++p) *reinterpret_cast<uint4*>(a.out + p * plane + from * ldo + i * N) = make_uint4(0, 0, 0, 0);
+    }
     for (int64_t i = block * 256 + threadIdx.x; i < total; i += blocks * 256) {
         const int64_t r = i / per, k = (i - r * per) * N;
         const int at = place ? place[r] : (int)r;
@@ -467,7 +478,7 @@ template <typename W> __device__ __forceinline__ void transpose(const TransposeA
 }
 
 // All that is copied before the logits, in one launch: the workgroups up to end[k] do part k. end[0], end[1]: x side by side, and beta
-// with rows that start on 16 bytes (gather); end[2], end[3]: the transposes of x and of beta's first piece
+// with rows that start on 16 bytes (gather); end[2], end[3]: the transposes of x and of beta's first piece for the small tile
 template <typename W> struct PrepareArgs {
     GatherArgs<W> g[2];
     TransposeArgs<W> t[2];
@@ -517,49 +528,32 @@ __device__ __forceinline__ void product_at(const ProductArgs<typename W::Data, t
         if (n >= a.B.rows) continue;
         const int64_t to = a.row ? a.row[n] : n;
         const A back = (a.row && a.lpbar ? a.lpbar[to] : largest) / (A)stored_scale<T>();
-        if constexpr (W::LINES) {
-            // 16 neighbouring values a lane: whole vectors where the rows of the result allow them
+        if constexpr (W::LINES) { // four neighbouring values a lane
 #pragma unroll
-            for (int h = 0; h < Tl::TM / 4; ++h) {
-                const int64_t m = m0 + Tl::row(4 * h, 0);
-                A v[16];
+            for (int i = 0; i < Tl::TM; ++i) {
+                const int64_t m = m0 + Tl::row(i, 0);
+                A v[4];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = tl.acc[4 * h + k / 4][j][k % 4] * back;
+                for (int r = 0; r < 4; ++r) v[r] = tl.acc[i][j][r] * back;
                 A* s = acc + n * a.A.rows + m;
                 T* o = a.out + to * a.ldo + m;
-                if (m + 16 <= a.A.rows) {
+                if (m + 4 <= a.A.rows) {
                     if (a.add) {
+                        const auto u = load16(s);
 #pragma unroll
-                        for (int k = 0; k < 16; k += Vec16<A>::N) {
-                            const auto u = load16(s + k);
-#pragma unroll
-                            for (int e = 0; e < Vec16<A>::N; ++e) v[k + e] += u[e];
-                        }
+                        for (int r = 0; r < 4; ++r) v[r] += u[r];
                     }
                     if (a.out) {
-#pragma unroll
-                        for (int k = 0; k < 16; k += Vec16<T>::N) {
-                            typename Vec16<T>::V u;
-#pragma unroll
-                            for (int e = 0; e < Vec16<T>::N; ++e) u[e] = (T)v[k + e];
-                            store16(o + k, u);
-                        }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 16; k += Vec16<A>::N) {
-                            typename Vec16<A>::V u;
-#pragma unroll
-                            for (int e = 0; e < Vec16<A>::N; ++e) u[e] = v[k + e];
-                            store16(s + k, u);
-                        }
-                    }
+                        const T u[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+                        store4(o, u);
+                    } else store4(s, v);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        if (m + k >= a.A.rows) continue;
-                        if (a.add) v[k] += s[k];
-                        if (a.out) o[k] = (T)v[k];
-                        else s[k] = v[k];
+                    for (int r = 0; r < 4; ++r) {
+                        if (m + r >= a.A.rows) continue;
+                        if (a.add) v[r] += s[r];
+                        if (a.out) o[r] = (T)v[r];
+                        else s[r] = v[r];
                     }
                 }
             }
@@ -580,7 +574,7 @@ __device__ __forceinline__ void product_at(const ProductArgs<typename W::Data, t
 }
 template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<typename W::Data, typename W::Element> a, int64_t id,
                                                                    typename W::Tl::Vec* lds) {
-    typedef typename W::Tl Tl;
+    typedef typename W::Product Tl;
     typedef typename HalfOf<Tl>::Tile Half;
     const int64_t split = id / a.grid;
     if (a.row) a.B.rows = *a.count;
@@ -629,7 +623,7 @@ template <typename W> struct ProductsArgs {
     int end[2];
 };
 template <typename W> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class_products(ProductsArgs<W> a) {
-    typedef typename W::Tl Tl;
+    typedef typename W::Product Tl;
     __shared__ typename Tl::Vec lds[Tl::LDS_BYTES / 16];
     const int id = blockIdx.x;
     if (id < a.end[1]) { // (one call: the tile's code stands once)
@@ -695,7 +689,7 @@ template <typename W> struct Plan {
     typedef typename W::Data T;
     typedef typename W::Element E;
     static constexpr int64_t EDGE = W::Tl::BM;
-    int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk;
+    int64_t block, blocks, piece, pieces, tiles_v, tiles_n, ldr, ldrt, ldk, xrows, brows;
     int64_t lsplits, xsplits, bsplits, kept_pieces;
     bool wide_products; // wide tiles for xbar and betabar
     bool copy;         // beta as operands of its own
@@ -727,9 +721,11 @@ template <typename W> struct Plan {
         part_sum = take(A * (size_t)(tiles_v * block));
         eta_y = take(A * (size_t)block);
         ldk = up_to(features, tile_k<E>());
-        xa = take(S * (size_t)(block * ldk));
+        xrows = up_to(block, 64);
+        brows = up_to(classes, 64);
+        xa = take(S * (size_t)(xrows * ldk));
         copy = W::PLANES == 3 || (W::LINES && features * sizeof(T) % 16);
-        if (copy) ba = take(S * (size_t)(classes * ldk));
+        if (copy) ba = take(S * (size_t)(brows * ldk));
         const int64_t tiles = tiles_v * tiles_n;
         lsplits = std::is_void<typename HalfOf<typename W::Tl>::Tile>::value ? logit_splits<E>(tiles, (W::PLANES == 3 ? 6 : 1) * features) : 1;
         kept_pieces = 0;
@@ -751,8 +747,11 @@ template <typename W> struct Plan {
             scale = take(A * SCALE_PARTS);
             r = take(S * (size_t)(ldrt * ldr));
             rt = take(S * (size_t)(ldr * ldrt));
-            xt = take(S * (size_t)(features * ldrt));
-            bt = take(S * (size_t)(features * ldr));
+            xt = bt = 0;
+            if (!W::LINES) {
+                xt = take(S * (size_t)(features * ldrt));
+                bt = take(S * (size_t)(features * ldr));
+            }
             part_alpha = take(A * (size_t)(tiles_n * ldr));
             alpha_acc = blocks > 1 ? take(A * (size_t)classes) : 0;
             wide_products = product_wide(features, block, piece) && product_wide(features, piece, block);
@@ -794,7 +793,7 @@ template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan
         ProductsArgs<U> u = {p.x, p.b, p.alpha, {0, 0}};
         auto size = [](auto& q) {
             q.tiles_m = tiles_of(q.A.rows, Tl::BM);
-            q.grid = tile_grid<Tl>(q.tiles_m, q.B.rows);
+            q.grid = tile_grid<typename U::Product>(q.tiles_m, q.B.rows);
             return (int)(q.grid * q.splits);
         };
         u.end[0] = size(u.x);
@@ -831,7 +830,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
     int *place = (int*)(ws + p.place), *row = (int*)(ws + p.row), *count = (int*)(ws + p.count);
     E *xa = (E*)(ws + p.xa), *ba = (E*)(ws + p.ba);
     E *r = (E*)(ws + p.r), *rt = (E*)(ws + p.rt), *xt = (E*)(ws + p.xt), *bt = (E*)(ws + p.bt);
-    const Operand<E> beta = p.copy ? Operand<E>{ba, p.ldk, V, V * p.ldk} : Operand<E>{(const E*)c.beta, c.ldbeta, V, 0};
+    const Operand<E> beta = p.copy ? Operand<E>{ba, p.ldk, V, p.brows * p.ldk} : Operand<E>{(const E*)c.beta, c.ldbeta, V, 0};
     Largest<A> largest = {nullptr};
     if (vjp && c.lpbar) {
         largest.parts = (A*)(ws + p.scale);
@@ -852,15 +851,15 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         number_rows<A>(c.y + n0, N, V, place, row, (int*)(ws + p.y), count, (A*)c.lp + n0, (const A*)c.lpbar,
                        scale_here ? (A*)(ws + p.scale) : nullptr, (int*)(ws + p.runs), st);
         PrepareArgs<W> q = {};
-        q.g[0] = {x, c.ldx, N, D, place, xa, p.ldk, p.block * p.ldk, vjp ? (T*)c.xbar + n0 * D : nullptr};
+        q.g[0] = {x, c.ldx, N, D, place, xa, p.ldk, p.xrows * p.ldk, vjp ? (T*)c.xbar + n0 * D : nullptr, count};
         q.end[0] = (int)(tiles_of(N * (p.ldk / 8), 256) < 1024 ? tiles_of(N * (p.ldk / 8), 256) : 1024);
         q.end[1] = q.end[0];
         if (p.copy && first_block) {
-            q.g[1] = {(const T*)c.beta, c.ldbeta, V, D, nullptr, ba, p.ldk, V * p.ldk, nullptr};
+            q.g[1] = {(const T*)c.beta, c.ldbeta, V, D, nullptr, ba, p.ldk, p.brows * p.ldk, nullptr, nullptr};
             q.end[1] += (int)(tiles_of(V * (p.ldk / 8), 256) < 2048 ? tiles_of(V * (p.ldk / 8), 256) : 2048);
         }
         q.end[2] = q.end[3] = q.end[1];
-        if (vjp) {
+        if (vjp && !W::LINES) {
             q.t[0] = {x, c.ldx, N, count, D, row, xt, ldrt, D * ldrt};
             q.t[1] = turn(0);
             q.end[2] += (int)blocks_of(q.t[0]);
@@ -869,7 +868,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         class_prepare<W><<<dim3((unsigned)q.end[3]), dim3(256), 0, st>>>(q);
         LogitArgs<W> l = {};
         l.beta = beta;
-        l.x = {xa, p.ldk, N, p.block * p.ldk};
+        l.x = {xa, p.ldk, N, p.xrows * p.ldk};
         l.count = count;
         l.alpha = (const T*)c.alpha;
         l.features = p.copy ? p.ldk : D;
@@ -907,7 +906,7 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
         for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
             const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
             const bool first = v0 == 0, last = v0 + nv == V;
-            if (!first) {
+            if (!first && !W::LINES) {
                 PrepareArgs<W> t = {};
                 t.t[1] = turn(v0);
                 class_prepare<W><<<dim3((unsigned)blocks_of(t.t[1])), dim3(256), 0, st>>>(t);
@@ -921,18 +920,20 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
             if (v0 < l.kept_classes) logits<W, false, true>(l, st);
             else logits<W, false, false>(l, st);
             ProductsArgs<W> m = {};
-            m.x.A = {bt, l.ldr, D, D * l.ldr};
+            if (W::LINES) m.x.A = {l.beta.p, l.beta.ld, D, l.beta.plane};
+            else m.x.A = {bt, l.ldr, D, D * l.ldr};
             m.x.B = {r, l.ldr, N, l.r_plane};
-            m.x.K = l.ldr;
+            m.x.K = !W::LINES ? l.ldr : W::PLANES == 3 ? up_to(nv, 64) : nv; // (r is zero from nv on)
             m.x.count = count;
             m.x.acc = (A*)(ws + p.xacc);
             m.x.plane = p.block * D;
             m.x.add = !first;
             m.x.row = row;
             m.x.lpbar = l.lpbar;
-            m.b.A = {xt, ldrt, D, D * ldrt};
+            if (W::LINES) m.b.A = {xa, p.ldk, D, p.xrows * p.ldk};
+            else m.b.A = {xt, ldrt, D, D * ldrt};
             m.b.B = {rt, ldrt, nv, l.rt_plane};
-            m.b.k_edge = tile_k<E>(); // (rt and xt are zero from the last row to ldrt)
+            m.b.k_edge = tile_k<E>(); // (rt and x are zero from the last row to there)
             m.b.count = count;
             m.b.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
             m.b.plane = (p.blocks > 1 ? V : p.piece) * D;

@@ -210,7 +210,9 @@ template <typename T> bool tile_fits(const Operand<T>& o) {
 // are swizzled by the row bits that differ within such a fragment.
 //
 // PLANES == 3: the operands are fp32 values split in three (split3), and k runs through six pairs of planes.
-template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
+// TURN: A stands the other way, [k][m] (A.rows: its columns). Its step is 64 rows of BM values; the LDS read that transposes takes 4 rows of
+// 4 times 4 columns for 16 lanes, which a swizzle of the chunks by the row spreads over all banks. Fragment i holds rows 16 i .. of C then.
+template <typename T, int PLANES, int BM_, int BN_, bool TURN = false> struct LineTile {
     typedef T Element;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
@@ -229,6 +231,27 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
         const int64_t last = o.rows - 1 - r0;
         const int64_t r = row < last ? row : last;
         return (uint32_t)(r * o.ld * (int64_t)sizeof(T)) + (uint32_t)(slot ^ key(row)) * 16;
+    }
+    static constexpr int ACROSS = BM / 8; // TURN: chunks of a row of A
+    // byte of A's chunk in row k, slot `slot` of the step (columns behind the last whole chunk repeat it)
+    static __device__ __forceinline__ uint32_t source_turned(const Operand<T>& o, int64_t m0, int k, int slot) {
+        const int64_t last = (o.rows + 7) / 8 - 1 - m0 / 8;
+        const int c = slot ^ (k & 3) << 1;
+        return (uint32_t)(k * o.ld * (int64_t)sizeof(T)) + (uint32_t)(c < last ? c : last) * 16;
+    }
+    // this lane's part of a fragment's address: see read_turned
+    static __device__ __forceinline__ uint32_t turned(int i, int wm) {
+        const int lane = threadIdx.x & 63, kk = lane >> 2 & 3;
+        return (8 * (lane >> 4) + kk) * (BM * 2) + (wm / 8 + 2 * (i ^ kk) + (lane >> 1 & 1)) * 16 + (lane & 1) * 8;
+    }
+    // fragment i, k = 32 g + 8 (lane group) + 0 .. 7
+    static __device__ __forceinline__ Vec read_turned(const Vec* at, const uint32_t (&from)[4], int i, int g) {
+        typedef short V4 __attribute__((ext_vector_type(4)));
+        typedef short V8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) V4 L;
+        auto* p = (__attribute__((address_space(3))) char*)at + from[i & 3] + (i >> 2) * 128 + 32 * g * (BM * 2);
+        const V4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(p + 4 * (BM * 2)));
+        return __builtin_bit_cast(Vec, (V8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     // LOADS loads of 16 bytes a lane into LDS (a wave's 64 lanes side by side). The LDS address goes through m0; the waits that
     // the hardware does not make by itself: a scalar register that a vector instruction wrote, m0 before its use
@@ -269,6 +292,15 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
             for (int j = 0; j < TN; ++j) acc[i][j] = C{0, 0, 0, 0};
         constexpr int PAIRS = PLANES == 3 ? 6 : 1;
         const int64_t each = (k1 - k0) / tile_k<T>(), steps = PAIRS * each; // (with planes k1 - k0 is a whole number of steps)
+        uint32_t turn[4];
+        if constexpr (TURN) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) turn[i] = turned(i, (wave / WN) * (BM / WM));
+        }
+        auto fragment_a = [&](const Vec* at, int i, int g, int cm) {
+            if constexpr (TURN) return read_turned(at, turn, i, g);
+            else return at[(fm + fragment(i)) * TILE_CHUNKS + cm];
+        };
         // one half step: acc += a b, while a and bn take the fragments of half g of the step at `at`
         Vec a[TM];
         auto half = [&](const Vec(&b)[TN], Vec(&bn)[TN], const Vec* at, int g) {
@@ -277,21 +309,21 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
             for (int i = 0; i < TM; ++i) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::mul(a[i], b[j], acc[i][j]);
-                a[i] = at[(fm + fragment(i)) * TILE_CHUNKS + cm];
+                a[i] = fragment_a(at, i, g, cm);
                 if (i < TN) bn[i] = at[(fn + fragment(i)) * TILE_CHUNKS + cn];
             }
 #pragma unroll
             for (int i = 0; i < TM; ++i) { // matrix instructions, reads of LDS
                 __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);
-                if (i < TN) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (i < TN) __builtin_amdgcn_sched_group_barrier(0x100, TURN ? 3 : 2, 0);
+                else __builtin_amdgcn_sched_group_barrier(0x100, TURN ? 2 : 1, 0);
             }
         };
         auto first = [&](Vec(&b)[TN], const Vec* at) {
 #pragma unroll
             for (int j = 0; j < TN; ++j) b[j] = at[(fn + fragment(j)) * TILE_CHUNKS + (q ^ key(fn))];
 #pragma unroll
-            for (int i = 0; i < TM; ++i) a[i] = at[(fm + fragment(i)) * TILE_CHUNKS + (q ^ key(fm))];
+            for (int i = 0; i < TM; ++i) a[i] = fragment_a(at, i, 0, q ^ key(fm));
         };
         auto mul = [&](const Vec(&b)[TN]) {
 #pragma unroll
@@ -303,7 +335,7 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
 #pragma unroll
             for (int j = 0; j < TN; ++j) b[j] = at[(fn + fragment(j)) * TILE_CHUNKS + ((4 + q) ^ key(fn))];
 #pragma unroll
-            for (int i = 0; i < TM; ++i) a[i] = at[(fm + fragment(i)) * TILE_CHUNKS + ((4 + q) ^ key(fm))];
+            for (int i = 0; i < TM; ++i) a[i] = fragment_a(at, i, 1, (4 + q) ^ key(fm));
         };
         Vec b0[TN], b1[TN];
         if (steps > 0) {
@@ -311,13 +343,14 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int id = (i & 3) * THREADS + t;
-                from[i] = source(i < 4 ? A : B, i < 4 ? m0 : n0, id / TILE_CHUNKS, id % TILE_CHUNKS);
+                from[i] = TURN && i < 4 ? source_turned(A, m0, id / ACROSS, id % ACROSS)
+                                        : source(i < 4 ? A : B, i < 4 ? m0 : n0, id / TILE_CHUNKS, id % TILE_CHUNKS);
             }
-            const T *const a0 = A.p + m0 * A.ld + k0, *const b0_ = B.p + n0 * B.ld + k0, *pa = a0, *pb = b0_;
+            const T *const a0 = TURN ? A.p + k0 * A.ld + m0 : A.p + m0 * A.ld + k0, *const b0_ = B.p + n0 * B.ld + k0, *pa = a0, *pb = b0_;
             int64_t left = each;
             int pair = 0;
             auto onward = [&]() {
-                pa += tile_k<T>(), pb += tile_k<T>();
+                pa += TURN ? tile_k<T>() * A.ld : tile_k<T>(), pb += tile_k<T>();
                 if (PLANES == 3 && --left == 0) { // pairs of planes (0,0) (0,1) (1,0) (1,1) (0,2) (2,0)
                     left = each;
                     ++pair;
@@ -351,7 +384,10 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int id = (i & 3) * THREADS + t, row = id / TILE_CHUNKS, c = id % TILE_CHUNKS;
-                lds[(i < 4 ? 0 : BM * TILE_CHUNKS) + row * TILE_CHUNKS + (c ^ key(row))] =
+                if (TURN && i < 4) {
+                    const int r = id / ACROSS, slot = id % ACROSS;
+                    lds[id] = k + r < k1 ? load16(A.p + (k + r) * A.ld + m0 + source_turned(A, m0, 0, slot ^ (r & 3) << 1) / sizeof(T)) : Vec{};
+                } else lds[(i < 4 ? 0 : BM * TILE_CHUNKS) + row * TILE_CHUNKS + (c ^ key(row))] =
                     tile_chunk(i < 4 ? A : B, (i < 4 ? m0 : n0) + row, k + c * Vec16<T>::N, k1);
             }
             __syncthreads();
@@ -366,7 +402,8 @@ template <typename T, int PLANES, int BM_, int BN_> struct LineTile {
         return m / (BM / WM) == (int)(threadIdx.x >> 6) / WN && (m >> 4 & 3) == (int)(threadIdx.x & 63) >> 4;
     }
     static __device__ __forceinline__ int row(int i, int r) {
-        return ((int)(threadIdx.x >> 6) / WN) * (BM / WM) + fragment(i) + 16 * ((threadIdx.x & 63) >> 4) + r;
+        const int q = (threadIdx.x & 63) >> 4;
+        return ((int)(threadIdx.x >> 6) / WN) * (BM / WM) + (TURN ? 16 * i + 4 * q : fragment(i) + 16 * q) + r;
     }
     static __device__ __forceinline__ int col(int j) {
         return ((int)(threadIdx.x >> 6) % WN) * (BN / WN) + fragment(j) + 16 * (threadIdx.x >> 2 & 3) + (threadIdx.x & 3);
@@ -380,8 +417,15 @@ template <typename T, int PLANES = 1> using MidTile = LineTile<T, PLANES, 128, 1
 template <typename Tl> struct HalfOf {
     typedef void Tile;
 };
-template <typename T, int PLANES> struct HalfOf<LineTile<T, PLANES, 256, 256>> {
-    typedef LineTile<T, PLANES, 256, 128> Tile;
+template <typename T, int PLANES, bool TURN> struct HalfOf<LineTile<T, PLANES, 256, 256, TURN>> {
+    typedef LineTile<T, PLANES, 256, 128, TURN> Tile;
+};
+// The tile with A the other way, where there is one
+template <typename Tl> struct TurnedOf {
+    typedef Tl Tile;
+};
+template <typename T, int PLANES, int BM, int BN> struct TurnedOf<LineTile<T, PLANES, BM, BN>> {
+    typedef LineTile<T, PLANES, BM, BN, true> Tile;
 };
 
 // Which tile a workgroup takes: workgroups go round the 8 XCDs, each of which has an L2 of its own, so each XCD takes a

@@ -31,6 +31,11 @@ template <typename T> __device__ __forceinline__ void store16(T* p, typename Vec
     *reinterpret_cast<typename Vec16<T>::U*>(p) = v;
 }
 
+template <typename T> __device__ __forceinline__ void store4(T* p, const T (&v)[4]) {
+    typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    *reinterpret_cast<V*>(p) = V{v[0], v[1], v[2], v[3]};
+}
+
 // A grid of many workgroups, in two dimensions (one counts its threads in 32 bits); workgroups behind the last of them may be there
 inline dim3 wide_grid(int64_t blocks) {
     constexpr int64_t ROW = (int64_t)1 << 20;
