@@ -817,7 +817,8 @@ template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan
     return hipGetLastError();
 }
 
-template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipStream_t st) {
+// (REVERSE: that mode is asked of it at all)
+template <typename W, bool REVERSE = true> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipStream_t st) {
     typedef typename W::Data T;
     typedef typename W::Element E;
     typedef acc_t<T> A;
@@ -897,53 +898,55 @@ template <typename W> hipError_t launch_rows(const ClassArgs& c, bool vjp, hipSt
                                                                             tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if (!vjp) continue;
-        l.lse = lse;
-        l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
-        l.r = r;
-        l.rt = rt;
-        l.ldrt = ldrt;
-        l.part_alpha = c.alphabar ? (A*)(ws + p.part_alpha) : nullptr;
-        for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
-            const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
-            const bool first = v0 == 0, last = v0 + nv == V;
-            if (!first && !W::LINES) {
-                PrepareArgs<W> t = {};
-                t.t[1] = turn(v0);
-                class_prepare<W><<<dim3((unsigned)blocks_of(t.t[1])), dim3(256), 0, st>>>(t);
+        if constexpr (REVERSE) {
+            l.lse = lse;
+            l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
+            l.r = r;
+            l.rt = rt;
+            l.ldrt = ldrt;
+            l.part_alpha = c.alphabar ? (A*)(ws + p.part_alpha) : nullptr;
+            for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+                const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
+                const bool first = v0 == 0, last = v0 + nv == V;
+                if (!first && !W::LINES) {
+                    PrepareArgs<W> t = {};
+                    t.t[1] = turn(v0);
+                    class_prepare<W><<<dim3((unsigned)blocks_of(t.t[1])), dim3(256), 0, st>>>(t);
+                }
+                l.beta = {beta.p + v0 * beta.ld, beta.ld, nv, beta.plane};
+                l.alpha = c.alpha ? (const T*)c.alpha + v0 : nullptr;
+                l.v0 = v0;
+                l.ldr = up_to(nv, EDGE);
+                l.r_plane = ldrt * l.ldr;
+                l.rt_plane = l.ldr * ldrt;
+                if (v0 < l.kept_classes) logits<W, false, true>(l, st);
+                else logits<W, false, false>(l, st);
+                ProductsArgs<W> m = {};
+                if (W::LINES) m.x.A = {l.beta.p, l.beta.ld, D, l.beta.plane};
+                else m.x.A = {bt, l.ldr, D, D * l.ldr};
+                m.x.B = {r, l.ldr, N, l.r_plane};
+                m.x.K = !W::LINES ? l.ldr : W::PLANES == 3 ? up_to(nv, 64) : nv; // (r is zero from nv on)
+                m.x.count = count;
+                m.x.acc = (A*)(ws + p.xacc);
+                m.x.plane = p.block * D;
+                m.x.add = !first;
+                m.x.row = row;
+                m.x.lpbar = l.lpbar;
+                if (W::LINES) m.b.A = {xa, p.ldk, D, p.xrows * p.ldk};
+                else m.b.A = {xt, ldrt, D, D * ldrt};
+                m.b.B = {rt, ldrt, nv, l.rt_plane};
+                m.b.k_edge = tile_k<E>(); // (rt and x are zero from the last row to there)
+                m.b.count = count;
+                m.b.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
+                m.b.plane = (p.blocks > 1 ? V : p.piece) * D;
+                m.b.add = !first_block;
+                m.b.largest = largest;
+                if (c.alphabar)
+                    m.alpha = {l.part_alpha, count, EDGE, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
+                               last_block ? (T*)c.alphabar + v0 : nullptr};
+                e = products<W>(m, p, last, (T*)c.xbar + n0 * D, last_block, (T*)c.betabar + v0 * D, c.alphabar ? tiles_of(nv, 64) : 0, st);
+                if (e != hipSuccess) return e;
             }
-            l.beta = {beta.p + v0 * beta.ld, beta.ld, nv, beta.plane};
-            l.alpha = c.alpha ? (const T*)c.alpha + v0 : nullptr;
-            l.v0 = v0;
-            l.ldr = up_to(nv, EDGE);
-            l.r_plane = ldrt * l.ldr;
-            l.rt_plane = l.ldr * ldrt;
-            if (v0 < l.kept_classes) logits<W, false, true>(l, st);
-            else logits<W, false, false>(l, st);
-            ProductsArgs<W> m = {};
-            if (W::LINES) m.x.A = {l.beta.p, l.beta.ld, D, l.beta.plane};
-            else m.x.A = {bt, l.ldr, D, D * l.ldr};
-            m.x.B = {r, l.ldr, N, l.r_plane};
-            m.x.K = !W::LINES ? l.ldr : W::PLANES == 3 ? up_to(nv, 64) : nv; // (r is zero from nv on)
-            m.x.count = count;
-            m.x.acc = (A*)(ws + p.xacc);
-            m.x.plane = p.block * D;
-            m.x.add = !first;
-            m.x.row = row;
-            m.x.lpbar = l.lpbar;
-            if (W::LINES) m.b.A = {xa, p.ldk, D, p.xrows * p.ldk};
-            else m.b.A = {xt, ldrt, D, D * ldrt};
-            m.b.B = {rt, ldrt, nv, l.rt_plane};
-            m.b.k_edge = tile_k<E>(); // (rt and x are zero from the last row to there)
-            m.b.count = count;
-            m.b.acc = (A*)(ws + p.bacc) + (p.blocks > 1 ? v0 * D : 0);
-            m.b.plane = (p.blocks > 1 ? V : p.piece) * D;
-            m.b.add = !first_block;
-            m.b.largest = largest;
-            if (c.alphabar)
-                m.alpha = {l.part_alpha, count, EDGE, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
-                           last_block ? (T*)c.alphabar + v0 : nullptr};
-            e = products<W>(m, p, last, (T*)c.xbar + n0 * D, last_block, (T*)c.betabar + v0 * D, c.alphabar ? tiles_of(nv, 64) : 0, st);
-            if (e != hipSuccess) return e;
         }
     }
     return hipSuccess;
@@ -1040,12 +1043,12 @@ template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStr
     return launch_few<T, 4>(c, vjp, st);
 }
 
-// fp32 products of few rows and many classes stay with the fp32 instructions: splitting beta takes longer than they do. With and
-// without splitting, in us: 100 rows x 1024 x 32000 146 / 88, with the reverse mode 428 / 386; 200 rows 166 / 151 and 577 / 576; but
-// 200 x 128 x 20000 with the reverse mode 133 / 187, and where the tiles do not fill the card (130 x 2000 x 5000) 132 / 160
-bool whole(int64_t rows, int64_t features, int64_t classes, bool vjp) {
+// The fp32 log density of few rows and many classes stays with the fp32 instructions: splitting beta takes longer than they do. With and
+// without splitting, in us: 100 rows x 1024 x 32000 146 / 88, 200 rows 166 / 151; but where the tiles do not fill the card (130 x 2000 x 5000)
+// 132 / 160, and with the reverse mode (100 x 4000 x 8000) 311 / 395
+bool whole(int64_t rows, int64_t features, int64_t classes) {
     const int64_t tiles = tiles_of(classes, 128) * tiles_of(rows, 128);
-    return rows <= (vjp ? 128 : 256) && tiles * logit_splits<float>(tiles, features) >= WIDE_TILES;
+    return rows <= 256 && tiles * logit_splits<float>(tiles, features) >= WIDE_TILES;
 }
 
 // fp32 runs in three planes of bf16; fp64 has neither the instructions nor the registers for line tiles
@@ -1057,7 +1060,7 @@ template <typename T> struct Ways {
 template <> struct Ways<float> {
     typedef Way<float, WideTile<bf16_t, 3>, 3> Wide;
     typedef Way<float, MidTile<bf16_t, 3>, 3> Mid;
-    typedef Way<float, SmallTile<float>, 1> Other; // few rows
+    typedef Way<float, SmallTile<float>, 1> Other; // the log density of few rows
 };
 template <> struct Ways<double> {
     typedef Way<double, SmallTile<double>, 1> Other;
@@ -1069,7 +1072,7 @@ template <typename T> size_t space(int64_t rows, int64_t features, int64_t class
     else {
         const bool large = wide(classes, rows < ROW_BLOCK ? rows : ROW_BLOCK);
         const size_t n = large ? Plan<typename Y::Wide>(rows, features, classes, vjp).bytes : Plan<typename Y::Mid>(rows, features, classes, vjp).bytes;
-        if (sizeof(T) == 4 && whole(rows, features, classes, vjp)) return Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
+        if (sizeof(T) == 4 && !vjp && whole(rows, features, classes)) return Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
         if constexpr (sizeof(T) == 2) { // (whether beta starts on 16 bytes shows only in the call)
             const size_t other = Plan<typename Y::Other>(rows, features, classes, vjp).bytes;
             return n > other ? n : other;
@@ -1082,7 +1085,9 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     typedef Ways<T> Y;
     if constexpr (sizeof(T) == 8) return launch_rows<typename Y::Other>(c, vjp, st);
     else {
-        if (sizeof(T) == 4 && whole(c.rows, c.features, c.classes, vjp)) return launch_rows<typename Y::Other>(c, vjp, st);
+        if constexpr (sizeof(T) == 4) {
+            if (!vjp && whole(c.rows, c.features, c.classes)) return launch_rows<typename Y::Other, false>(c, false, st);
+        }
         if constexpr (sizeof(T) == 2) {
             // (rows of an odd length are copied, whole ones need to start on 16 bytes where they are)
             if (c.features * sizeof(T) % 16 == 0 && !tile_fits(Operand<T>{(const T*)c.beta, c.ldbeta, c.classes, 0}))
