@@ -590,11 +590,13 @@ template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<t
     }
     product_at<W, Tl>(a, split, tm, tn, lds);
 }
-// alphabar of a piece from the tiles' sums: 64 classes a workgroup, its waves share the tiles. acc: sums over row blocks
+// alphabar of a piece from the tiles' sums, 64 classes a wave, or a workgroup whose waves share the tiles where these are many.
+// acc: sums over row blocks
 template <typename T> struct AlphaArgs {
     const acc_t<T>* part;
     const int* count;
     int64_t edge, ld, nv;
+    bool shared;
     acc_t<T>* acc;
     bool add;
     T* out;
@@ -602,15 +604,20 @@ template <typename T> struct AlphaArgs {
 template <typename T, int WAVES> __device__ __forceinline__ void alpha_sums(const AlphaArgs<T>& a, int64_t block, acc_t<T>* red) {
     typedef acc_t<T> A;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t v = block * 64 + lane, tiles = (*a.count + a.edge - 1) / a.edge;
+    const int64_t v = (a.shared ? block : block * WAVES + w) * 64 + lane, tiles = (*a.count + a.edge - 1) / a.edge;
     A s = 0;
-    if (v < a.nv)
-        for (int64_t i = w; i < tiles; i += WAVES) s += a.part[i * a.ld + v];
-    red[w * 64 + lane] = s;
-    __syncthreads();
-    if (w || v >= a.nv) return;
+    if (v < a.nv) {
+#pragma unroll 4
+        for (int64_t i = a.shared ? w : 0; i < tiles; i += a.shared ? WAVES : 1) s += a.part[i * a.ld + v];
+    }
+    if (a.shared) {
+        red[w * 64 + lane] = s;
+        __syncthreads();
+        if (w) return;
 #pragma unroll
-    for (int k = 1; k < WAVES; ++k) s += red[k * 64 + lane];
+        for (int k = 1; k < WAVES; ++k) s += red[k * 64 + lane];
+    }
+    if (v >= a.nv) return;
     if (a.add) s += a.acc[v];
     if (a.out) a.out[v] = (T)s;
     else a.acc[v] = s;
@@ -775,9 +782,9 @@ template <typename W, bool STATS, bool KEPT> void logits(LogitArgs<W> l, hipStre
     class_logits<W, STATS, KEPT><<<dim3(tile_grid<Tl>(l.tiles_v, l.x.rows)), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
-// xbar and betabar of a piece (each complete if its `last`), alphabar (blocks: its workgroups, or none)
+// xbar and betabar of a piece (each complete if its `last`), alphabar (of alpha.nv classes)
 template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan, bool xlast, typename W::Data* xbar, bool blast,
-                                          typename W::Data* betabar, int64_t alpha_blocks, hipStream_t st) {
+                                          typename W::Data* betabar, hipStream_t st) {
     typedef typename W::Data T;
     typedef typename W::Element E;
     auto ready = [](auto& q, int64_t splits, bool last, T* out) {
@@ -796,9 +803,10 @@ template <typename W> hipError_t products(ProductsArgs<W> p, const Plan<W>& plan
             q.grid = tile_grid<typename U::Product>(q.tiles_m, q.B.rows);
             return (int)(q.grid * q.splits);
         };
+        const int64_t alpha = p.alpha.shared ? 64 : Tl::THREADS;
         u.end[0] = size(u.x);
         u.end[1] = u.end[0] + size(u.b);
-        class_products<U><<<dim3((unsigned)(u.end[1] + alpha_blocks)), dim3(Tl::THREADS), 0, st>>>(u);
+        class_products<U><<<dim3((unsigned)(u.end[1] + tiles_of(p.alpha.nv, alpha))), dim3(Tl::THREADS), 0, st>>>(u);
     };
     if constexpr (W::LINES) {
         typedef Way<T, WideTile<E, W::PLANES>, W::PLANES> Wide;
@@ -942,9 +950,9 @@ template <typename W, bool REVERSE = true> hipError_t launch_rows(const ClassArg
                 m.b.add = !first_block;
                 m.b.largest = largest;
                 if (c.alphabar)
-                    m.alpha = {l.part_alpha, count, EDGE, l.ldr, nv, (A*)(ws + p.alpha_acc) + v0, !first_block,
+                    m.alpha = {l.part_alpha, count, EDGE, l.ldr, nv, tiles_of(N, EDGE) > 32, (A*)(ws + p.alpha_acc) + v0, !first_block,
                                last_block ? (T*)c.alphabar + v0 : nullptr};
-                e = products<W>(m, p, last, (T*)c.xbar + n0 * D, last_block, (T*)c.betabar + v0 * D, c.alphabar ? tiles_of(nv, 64) : 0, st);
+                e = products<W>(m, p, last, (T*)c.xbar + n0 * D, last_block, (T*)c.betabar + v0 * D, st);
                 if (e != hipSuccess) return e;
             }
         }
