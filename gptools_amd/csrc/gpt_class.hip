@@ -314,7 +314,8 @@ template <typename W> __global__ __launch_bounds__(W::Tl::THREADS, 2) void class
     a.x.rows = *a.count;
     int64_t tm, tn;
     bool half;
-    if (!tile_place<Tl>(blockIdx.x - split * a.grid, a.tiles_v, a.x.rows, tm, tn, half)) return;
+    const int64_t in = split_place(blockIdx.x - split * a.grid, split, a.tiles_v * ((a.x.rows + Tl::BN - 1) / Tl::BN));
+    if (!tile_place<Tl>(in, a.tiles_v, a.x.rows, tm, tn, half)) return;
     const int64_t share = ((a.features + a.splits - 1) / a.splits + step - 1) / step * step;
     const int64_t k0 = split * share, k1 = k0 + share < a.features ? k0 + share : a.features;
     Tl tl;
@@ -581,7 +582,8 @@ template <typename W> __device__ __forceinline__ void product_tile(ProductArgs<t
     else a.K = (*a.count + a.k_edge - 1) / a.k_edge * a.k_edge;
     int64_t tm, tn;
     bool half;
-    if (!tile_place<Tl>(id - split * a.grid, a.tiles_m, a.B.rows, tm, tn, half)) return;
+    const int64_t in = split_place(id - split * a.grid, split, a.tiles_m * ((a.B.rows + Tl::BN - 1) / Tl::BN));
+    if (!tile_place<Tl>(in, a.tiles_m, a.B.rows, tm, tn, half)) return;
     if constexpr (!std::is_void<Half>::value) {
         if (half) {
             product_at<W, Half>(a, split, tm, tn, lds);

@@ -480,6 +480,11 @@ template <typename Tl> __device__ __forceinline__ bool tile_place(int64_t id, in
     if (half) n = whole;
     return true;
 }
+// The number of workgroup `in` of split `split`: the splits of fewer tiles than there are XCDs start on different ones (fp32 100 rows x
+// 300 x 30000 with the reverse mode: 130 us against 172)
+__device__ __forceinline__ int64_t split_place(int64_t in, int64_t split, int64_t tiles) {
+    return (in & ~(int64_t)7) | ((in + split * tiles) & 7);
+}
 template <typename Tl> unsigned tile_grid(int64_t tiles_m, int64_t cols) {
     const int64_t tiles_n = (cols + Tl::BN - 1) / Tl::BN;
     if (std::is_void<typename HalfOf<Tl>::Tile>::value) return (unsigned)((tiles_m * tiles_n + 7) / 8 * 8);
