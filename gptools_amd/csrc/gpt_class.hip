@@ -704,10 +704,12 @@ template <typename W> struct Plan {
     bool copy;         // beta as operands of its own
     // offsets in bytes
     size_t kept, place, row, y, count, runs, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
-    // (a product's splits of k count too: 16 rows of large tiles with a sixteenth of a long k each fill the card as well)
+    // (a product's splits of k count too: 16 large tiles with a sixteenth of a long k each fill the card as well. Fewer than nine would need
+    // too many of them: bf16 200 rows x 1000 x 100000 472 us against 372 with small ones, fp32 500 x 500 x 60000 1061 against 831, but
+    // 700 x 700 x 60000 1445 against 1617)
     static bool product_wide(int64_t m, int64_t n, int64_t K) {
         const int64_t tiles = tiles_of(m, 256) * tiles_of(n, 256);
-        return W::LINES && tiles * splits_of(2 * tiles, K, 4 * tile_k<E>()) >= WIDE_TILES;
+        return W::LINES && tiles > 8 && tiles * splits_of(2 * tiles, K, 4 * tile_k<E>()) >= WIDE_TILES;
     }
     Plan(int64_t rows, int64_t features, int64_t classes, bool vjp) {
         const size_t A = sizeof(acc_t<T>), S = sizeof(E) * W::PLANES;
