@@ -211,7 +211,8 @@ template <typename T> bool tile_fits(const Operand<T>& o) {
 //
 // PLANES == 3: the operands are fp32 values split in three (split3), and k runs through six pairs of planes.
 // TURN: A stands the other way, [k][m] (A.rows: its columns). Its step is 64 rows of BM values; the LDS read that transposes takes 4 rows of
-// 4 times 4 columns for 16 lanes, which a swizzle of the chunks by the row spreads over all banks. Fragment i holds rows 16 i .. of C then.
+// 4 times 4 columns for 16 lanes, which a swizzle of the chunks by the row spreads over half of the banks. (Over all of them, for 32 lanes at
+// once, takes one more addition for every other fragment: no conflicts, and 1 % more time.) Fragment i holds rows 16 i .. of C then.
 template <typename T, int PLANES, int BM_, int BN_, bool TURN = false> struct LineTile {
     typedef T Element;
     typedef typename Vec16<T>::V Vec;
