@@ -11,6 +11,7 @@ struct NormArgs {
     void *y, *xbar, *wbar, *bbar;         // wbar and bbar both null: not wanted
     void *partial, *partial2, *sums;      // workspace (partial), and parts of it
     int64_t rows, width, piece;
+    unsigned column_blocks; // workgroups of columns before those of rows
     double eps;
 };
 size_t gpt_norm_workspace(int dtype, int64_t rows, int64_t width, bool vjp);
