@@ -1033,8 +1033,15 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
         a.share = p.share;
     }
     const dim3 grid((unsigned)p.tiles);
-    if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4><<<grid, dim3(256), 0, st>>>(a);
-    else class_few_logits<T, NT, 1, 8><<<grid, dim3(512), 0, st>>>(a);
+    auto first = [&](auto half) {
+        constexpr bool HALF = decltype(half)::value;
+        if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4, HALF><<<grid, dim3(256), 0, st>>>(a);
+        else class_few_logits<T, NT, 1, 8, HALF><<<grid, dim3(512), 0, st>>>(a);
+    };
+    if constexpr (sizeof(T) == 2) {
+        if ((((uintptr_t)c.beta | (uintptr_t)c.x) & 2) || (c.ldbeta | c.ldx) & 1) first(std::true_type());
+        else first(std::false_type());
+    } else first(std::false_type());
     T* xt = vjp ? (T*)(ws + p.xt) : nullptr;
     class_few_join<T><<<dim3((unsigned)(c.rows + (vjp ? tiles_of(D, 64) : 0))), dim3(256), 0, st>>>(a, xt);
     if (!vjp) return hipGetLastError();

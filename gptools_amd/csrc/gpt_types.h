@@ -27,6 +27,19 @@ template <typename T> struct Vec16 {
 template <typename T> __device__ __forceinline__ typename Vec16<T>::V load16(const T* p) {
     return *reinterpret_cast<const typename Vec16<T>::U*>(p);
 }
+// The same for 16-bit elements that may start in the middle of a word, where lanes read rows of their own (such reads take twice the
+// time): whole words, and one more (which the last element lies in), moved by half a word
+template <typename T> __device__ __forceinline__ typename Vec16<T>::V load16_words(const T* p) {
+    static_assert(sizeof(T) == 2, "two elements a word");
+    typedef uint32_t W __attribute__((ext_vector_type(4), aligned(4)));
+    const uint32_t odd = (uint32_t)(uintptr_t)p & 2;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(p) - odd);
+    const W w = *reinterpret_cast<const W*>(q);
+    const uint32_t e = q[odd ? 4 : 3];
+    const uint4 u = make_uint4(__builtin_amdgcn_alignbyte(w[1], w[0], odd), __builtin_amdgcn_alignbyte(w[2], w[1], odd),
+                               __builtin_amdgcn_alignbyte(w[3], w[2], odd), __builtin_amdgcn_alignbyte(e, w[3], odd));
+    return __builtin_bit_cast(typename Vec16<T>::V, u);
+}
 template <typename T> __device__ __forceinline__ void store16(T* p, typename Vec16<T>::V v) {
     *reinterpret_cast<typename Vec16<T>::U*>(p) = v;
 }
