@@ -1033,15 +1033,22 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
         a.share = p.share;
     }
     const dim3 grid((unsigned)p.tiles);
-    auto first = [&](auto half) {
+    bool odd = false; // rows that start in the middle of a word
+    if (sizeof(T) == 2) odd = (((uintptr_t)c.beta | (uintptr_t)c.x) & 2) || ((c.ldbeta | c.ldx) & 1);
+    auto with = [&](auto run) {
+        if constexpr (sizeof(T) == 2) {
+            if (odd) {
+                run(std::true_type());
+                return;
+            }
+        }
+        run(std::false_type());
+    };
+    with([&](auto half) {
         constexpr bool HALF = decltype(half)::value;
         if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4, HALF><<<grid, dim3(256), 0, st>>>(a);
         else class_few_logits<T, NT, 1, 8, HALF><<<grid, dim3(512), 0, st>>>(a);
-    };
-    if constexpr (sizeof(T) == 2) {
-        if ((((uintptr_t)c.beta | (uintptr_t)c.x) & 2) || (c.ldbeta | c.ldx) & 1) first(std::true_type());
-        else first(std::false_type());
-    } else first(std::false_type());
+    });
     T* xt = vjp ? (T*)(ws + p.xt) : nullptr;
     class_few_join<T><<<dim3((unsigned)(c.rows + (vjp ? tiles_of(D, 64) : 0))), dim3(256), 0, st>>>(a, xt);
     if (!vjp) return hipGetLastError();
@@ -1051,8 +1058,10 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
     const int64_t xslabs = tiles_of(D, 16 * Vec16<T>::N), bslabs = tiles_of(D, Slab<T>::WIDTH);
     int64_t shares = tiles_of(4 * FILL, bslabs);
     if (shares > tiles_of(V, 128)) shares = tiles_of(V, 128);
-    class_few_back<T, NT, NG><<<dim3((unsigned)(xslabs * p.splits + bslabs * shares)), dim3(256), 0, st>>>(
-        a, xt, (T*)c.betabar, largest, (int)xslabs, (int)p.splits, (int)bslabs, (int)shares);
+    with([&](auto half) {
+        class_few_back<T, NT, NG, decltype(half)::value><<<dim3((unsigned)(xslabs * p.splits + bslabs * shares)), dim3(256), 0, st>>>(
+            a, xt, (T*)c.betabar, largest, (int)xslabs, (int)p.splits, (int)bslabs, (int)shares);
+    });
     if (p.splits > 1) class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits);
     return hipGetLastError();
 }

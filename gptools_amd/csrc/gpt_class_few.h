@@ -268,28 +268,33 @@ template <typename T> __device__ __forceinline__ T few_cotangent(const FewArgs<T
 }
 
 // xbar's sums over a share of the classes for 16 chunks of features: four waves with a quarter of the share each
-template <typename T, int NT> __device__ __forceinline__ void few_xbar(const FewArgs<T>& a, int64_t slab, int64_t split) {
+template <typename T, int NT, bool HALF> __device__ __forceinline__ void few_xbar(const FewArgs<T>& a, int64_t slab, int64_t split) {
     typedef acc_t<T> A;
     typedef typename Vec16<T>::V Vec;
     typedef typename Mma<T>::C C;
     constexpr int N = Vec16<T>::N;
     __shared__ A sum[4][16][16 * N + 1];
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
-    const int64_t d0 = slab * 16 * N, d = d0 + (lane & 15) * N, D = a.features, V = a.beta.rows;
+    // a chunk that lies behind the last whole one is taken as the last N features (some of which the one before has too, with the same
+    // sums): no guard holds a load back (bf16 12 rows x 1958 x 34026 with the reverse mode 126 us against 157)
+    const int64_t d0 = slab * 16 * N, D = a.features, V = a.beta.rows;
+    const auto start = [=](int chunk) { return D < N || d0 + (chunk + 1) * N <= D ? d0 + chunk * N : D - N; };
+    const int64_t d = start(lane & 15);
     const int64_t s0 = split * a.share, s1 = s0 + a.share < V ? s0 + a.share : V;
     C c[NT][N];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < N; ++j) c[t][j] = C{0, 0, 0, 0};
-    const bool full = d0 + 16 * N <= D;
     // lane group q: classes v + 8 q .. + 7 (r is zero behind the last class, up to ldv, a multiple of 32)
     for (int64_t v = s0 + 32 * wave; v < s1; v += 128) {
         Vec b[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int64_t at = v + 8 * q + u, row = at < V ? at : V - 1;
-            b[u] = full ? load16(a.beta.p + row * a.beta.ld + d) : tile_chunk(a.beta, row, d, D);
+            if (D < N) b[u] = tile_chunk(a.beta, row, d, D);
+            else if constexpr (HALF) b[u] = load16_words(a.beta.p + row * a.beta.ld + d);
+            else b[u] = load16(a.beta.p + row * a.beta.ld + d);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -315,10 +320,11 @@ template <typename T, int NT> __device__ __forceinline__ void few_xbar(const Few
         __syncthreads();
         for (int id = threadIdx.x; id < 16 * 16 * N; id += 256) {
             const int n = id / (16 * N), k = id % (16 * N);
-            if (16 * t + n >= a.x.rows || d0 + k >= D) continue;
+            const int64_t to = start(k / N) + k % N;
+            if (16 * t + n >= a.x.rows || d0 + k / N * N >= D || to >= D) continue;
             const A s = (sum[0][n][k] + sum[1][n][k]) + (sum[2][n][k] + sum[3][n][k]);
-            if (a.xpart) a.xpart[(split * a.x.rows + 16 * t + n) * D + d0 + k] = s;
-            else a.xbar[(16 * t + n) * D + d0 + k] = few_cotangent(a, 16 * t + n, s);
+            if (a.xpart) a.xpart[(split * a.x.rows + 16 * t + n) * D + to] = s;
+            else a.xbar[(16 * t + n) * D + to] = few_cotangent(a, 16 * t + n, s);
         }
         __syncthreads();
     }
@@ -408,11 +414,11 @@ template <typename T, int NG> __device__ __forceinline__ void few_beta(const Few
 }
 
 // xbar's sums by the first xslabs x splits workgroups, betabar by the others
-template <typename T, int NT, int NG> __global__ __launch_bounds__(256) void class_few_back(FewArgs<T> a, const T* xt, T* betabar,
+template <typename T, int NT, int NG, bool HALF> __global__ __launch_bounds__(256) void class_few_back(FewArgs<T> a, const T* xt, T* betabar,
                                                                                            Largest<acc_t<T>> largest, int xslabs, int splits,
                                                                                            int bslabs, int shares) {
     const int id = blockIdx.x;
-    if (id < xslabs * splits) few_xbar<T, NT>(a, id % xslabs, id / xslabs);
+    if (id < xslabs * splits) few_xbar<T, NT, HALF>(a, id % xslabs, id / xslabs);
     else few_beta<T, NG>(a, xt, betabar, largest, (id - xslabs * splits) % bslabs, (id - xslabs * splits) / bslabs, shares);
 }
 
