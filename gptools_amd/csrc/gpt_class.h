@@ -8,7 +8,8 @@ namespace gptt {
 template <typename A> __device__ __forceinline__ A neg_inf() { return -(A)__builtin_inf(); }
 
 // In fp32 logits, maxima and lse are kept times log2(e): an exponential is one instruction then
-__device__ __forceinline__ float times_log2e(float v) { return v * 1.44269504088896340736f; }
+constexpr float LOG2E = 1.44269504088896340736f;
+__device__ __forceinline__ float times_log2e(float v) { return v * LOG2E; }
 __device__ __forceinline__ float from_log2e(float v) { return v * 0.69314718055994530942f; }
 __device__ __forceinline__ float exp_log2e(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ double times_log2e(double v) { return v; }

@@ -15,6 +15,10 @@
 //
 // In 16 bits p and r are rounded for the second products, as their operands are of one type. p is at most 2^8 of the row's
 // running reference; r is taken relative to the largest cotangent, in fp16 times 2^14, as in gpt_class.hip.
+// p of the row's own class meets beta_y's other coefficient, 1, there: where it is nearly 1 xbar is small against both, and half a
+// step of p_y would be as large as xbar. That one rounding is therefore known and taken back: the class's logit is computed once more
+// after the walk, in the same order of operations and so to the same bit, and p_y with the reference that it met. What is left
+// are roundings of entries of r, and of Acc.
 #include "gpt_class.h"
 #include "gpt_readout.h"
 #include "gpt_tile.h"
@@ -110,30 +114,6 @@ template <typename T, int DT> struct Narrow {
                 for (int g = 0; g < G; ++g) v[g] = Vec{};
             }
         }
-        // this lane's share of the dot product with another row
-        __device__ __forceinline__ A dot(const Operand<T>& o, int64_t row, int64_t D) const {
-            const int q = (threadIdx.x & 63) >> 4;
-            A t = 0;
-            if constexpr (SPLIT) {
-#pragma unroll
-                for (int g = 0; g < SG; ++g)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const Vec u = tile_chunk(o, row, (int64_t)((4 * g + q) * 8 + 4 * h), D);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            t += ((float)s[0][g][4 * h + e] + ((float)s[1][g][4 * h + e] + (float)s[2][g][4 * h + e])) * u[e];
-                    }
-            } else {
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const Vec u = tile_chunk(o, row, (int64_t)(4 * g + q) * N, D);
-#pragma unroll
-                    for (int e = 0; e < N; ++e) t += (A)v[g][e] * (A)u[e];
-                }
-            }
-            return t;
-        }
     };
     template <int STEP> static constexpr int loads() { return STEP * (DP / N) / 256 > 0 ? STEP * (DP / N) / 256 : 1; }
 
@@ -189,6 +169,51 @@ template <typename T, int DT> struct Narrow {
             }
         }
     };
+    static __device__ __forceinline__ C split_mul(const SVec (&a)[3], const Part& f, int g, C c) {
+        c = Mma<bf16_t>::mul(a[2], f.s[0][g], c); // (the smallest first)
+        c = Mma<bf16_t>::mul(a[0], f.s[2][g], c);
+        c = Mma<bf16_t>::mul(a[1], f.s[1][g], c);
+        c = Mma<bf16_t>::mul(a[1], f.s[0][g], c);
+        c = Mma<bf16_t>::mul(a[0], f.s[1][g], c);
+        return Mma<bf16_t>::mul(a[0], f.s[0][g], c);
+    }
+    // a logit (times log2(e) in fp32) from the product with its level, or without it
+    static __device__ __forceinline__ A eta(A p, A level) {
+        if constexpr (UNIT) return p;
+        else return __builtin_fmaf(p, LOG2E, level);
+    }
+    // the logit of row `row` of o (at least 0) for this lane's column, to the bit as logits() and eta() have it: the columns' rows
+    // make a tile, whose diagonal it is
+    static __device__ __forceinline__ A eta_at(const Operand<T>& o, int64_t row, int64_t D, const Part& f, A level) {
+        const int lane = threadIdx.x & 63, q = lane >> 4;
+        const A l = UNIT ? level : (A)0;
+        C c = {l, l, l, l};
+        if constexpr (SPLIT) {
+#pragma unroll
+            for (int g = 0; g < SG; ++g) {
+                uint32_t w[4][3];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Vec u = tile_chunk(o, row, (int64_t)((4 * g + q) * 8 + 4 * h), D);
+                    split3(u[0], u[1], w[2 * h]);
+                    split3(u[2], u[3], w[2 * h + 1]);
+                }
+                SVec a[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) a[p] = __builtin_bit_cast(SVec, make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]));
+                c = split_mul(a, f, g, c);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; ++g) c = Mma<T>::mul(tile_chunk(o, row, (int64_t)(4 * g + q) * N, D), f.v[g], c);
+        }
+        A e = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e = Mma<T>::row(q, r) == (lane & 15) ? c[r] : e;
+        e += __shfl_xor(e, 16, 64); // (one of the four lane groups has it, the others zero)
+        e += __shfl_xor(e, 32, 64);
+        return eta(e, level);
+    }
     // C[row base + .. of lds][column held in f] plus c in UNIT, and its use as an operand
     template <int STEP> static __device__ __forceinline__ C logits(const T* lds, int base, const Part& f, C c) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
@@ -199,12 +224,7 @@ template <typename T, int DT> struct Narrow {
                 SVec a[3];
 #pragma unroll
                 for (int p = 0; p < 3; ++p) a[p] = *reinterpret_cast<const SVec*>(t + p * STEP * SLD + (4 * g + q) * 8);
-                c = Mma<bf16_t>::mul(a[2], f.s[0][g], c); // (the smallest first)
-                c = Mma<bf16_t>::mul(a[0], f.s[2][g], c);
-                c = Mma<bf16_t>::mul(a[1], f.s[1][g], c);
-                c = Mma<bf16_t>::mul(a[1], f.s[0][g], c);
-                c = Mma<bf16_t>::mul(a[0], f.s[1][g], c);
-                c = Mma<bf16_t>::mul(a[0], f.s[0][g], c);
+                c = split_mul(a, f, g, c);
             }
         } else {
 #pragma unroll
@@ -254,6 +274,8 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
     __shared__ uint4 room[(larger(STAGE, SPILL) + 15) / 16];
     __shared__ __attribute__((aligned(16))) A al[STEP];
     __shared__ A red[2][WV][ROWS];
+    constexpr bool BACK = VJP && W::TURN; // p is rounded
+    __shared__ A met[BACK ? ROWS : 1], own[VJP ? ROWS : 1]; // the reference that a row's class met; beta_y's coefficient in xbar
     T* lds = reinterpret_cast<T*>(room);
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6, wr = wave / WV, wv = wave % WV;
     const int64_t n0 = wide_block() * ROWS, V = a.beta.rows, D = a.features;
@@ -268,7 +290,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
     }
     typename W::Part x[NT];
     int y[NT], row[NT]; // y: -1 without an observation, V where it is no class
-    A ref[NT], sum[NT];
+    A ref[NT], sum[NT], ref_y[BACK ? NT : 1];
     C o[NT][DT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -279,6 +301,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         if (y[t] >= 0) x[t].load(a.x, row[t], D);
         else x[t].clear();
         ref[t] = neg_inf<A>();
+        if (BACK) ref_y[t] = neg_inf<A>();
         sum[t] = 0;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = C{0, 0, 0, 0};
@@ -314,7 +337,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
                 p[t][v] = W::template logits<STEP>(lds, base, x[t], W::UNIT ? level : C{0, 0, 0, 0});
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (!W::UNIT) p[t][v][r] = times_log2e(p[t][v][r]) + level[r];
+                    p[t][v][r] = W::eta(p[t][v][r], level[r]);
                     mx[t] = fmax(mx[t], p[t][v][r]);
                 }
             }
@@ -342,6 +365,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const A m = about(ref[t]);
+            if (BACK) ref_y[t] = (int)v0 <= y[t] ? ref[t] : ref_y[t]; // (the step that holds y is the last such)
 #pragma unroll
             for (int v = 0; v < VT; ++v) {
 #pragma unroll
@@ -361,6 +385,8 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         if (q == 0) {
             red[0][wv][(wr * NT + t) * 16 + lane] = ref[t];
             red[1][wv][(wr * NT + t) * 16 + lane] = sum[t];
+            // (of the waves that share the rows the one whose classes y is among)
+            if (BACK && y[t] >= 0 && y[t] / (16 * VT) % WV == wv) met[(wr * NT + t) * 16 + lane] = ref_y[t];
         }
     }
     __syncthreads(); // (and the last step's rows have been read)
@@ -374,12 +400,8 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
 #pragma unroll
         for (int k = 0; k < WV; ++k) join(mx, s, red[0][k][at], red[1][k][at]);
         const bool known = y[t] >= 0 && y[t] < V;
-        A eta = 0; // of the row's class, as the matrix cores have it up to rounding
-        if (wv == 0 && known) eta = x[t].dot(a.beta, y[t], D);
-        eta += __shfl_xor(eta, 16, 64);
-        eta += __shfl_xor(eta, 32, 64);
-        if (!W::UNIT) eta = times_log2e(eta);
-        if (known && a.alpha) eta += level_log2e((A)a.alpha[y[t]]);
+        A eta = 0; // of the row's class
+        if (wv == 0) eta = W::eta_at(a.beta, known ? y[t] : 0, D, x[t], known && a.alpha ? level_log2e((A)a.alpha[y[t]]) : (A)0);
         A lse;
         const A lp = row_lp(y[t], V, mx, s, eta, lse);
         const bool none = y[t] < 0 || lse == neg_inf<A>();
@@ -392,6 +414,16 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
                 a.w[n] = w / largest;
                 a.at[n] = known ? y[t] : -1;
             }
+        }
+        if (VJP && wv == 0 && q == 0) {
+            A more = 0; // what the rounding took from p_y, of the sum
+            if constexpr (BACK) {
+                if (known && !none) {
+                    const A p = exp_log2e(eta - about(met[at]));
+                    more = (p - (A)(T)p) * (exp_log2e(about(met[at]) - about(mx)) / s);
+                }
+            }
+            own[at] = w * ((A)1 - more);
         }
         if (VJP) {
             const A f = none ? (A)0 : w * (exp_log2e(ref[t] - about(mx)) / s);
@@ -410,7 +442,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         const int64_t n = n0 + r;
         if (d >= D || n >= a.x.rows) continue;
         const int64_t to = a.order ? a.order[n] : n, yn = a.at[n];
-        const A w = a.w[n] * largest;
+        const A w = own[r];
         A s = 0;
 #pragma unroll
         for (int k = 0; k < WV; ++k) s += spilt[(k * ROWS + r) * W::OLD + d];
