@@ -14,7 +14,8 @@
 // of the second's fall on different banks), in 16 bits from a transposed copy.
 //
 // In 16 bits p and r are rounded for the second products, as their operands are of one type. p is at most 2^8 of the row's
-// running reference; r is taken relative to the largest cotangent, in fp16 times 2^14, as in gpt_class.hip.
+// running reference; in fp16, which has too few exponents for the small probabilities, it is held times 2^13 and at most 2^2 of the
+// reference. r is taken relative to the largest cotangent, in fp16 times 2^14, as in gpt_class.hip.
 // p of the row's own class meets beta_y's other coefficient, 1, there: where it is nearly 1 xbar is small against both, and half a
 // step of p_y would be as large as xbar. That one rounding is therefore known and taken back: the class's logit is computed once more
 // after the walk, in the same order of operations and so to the same bit, and p_y with the reference that it met. What is left
@@ -71,6 +72,10 @@ template <typename T, int DT> struct Narrow {
     template <int STEP> static constexpr int stage() { return STEP * LD + (TURN ? DP * (STEP + 4) : SPLIT ? 3 * STEP * SLD / 2 : 0); }
     // fp32: what stands in registers is times log2(e) already, so that logits come in that unit
     static constexpr bool UNIT = sizeof(T) >= 4;
+    // fp16: p is 2^HEAD where the logit is the reference's own, and at most 2^15: a probability is off by 2^-38 at most besides its
+    // relative rounding, as r is, which holds 2^14 for one. The reference then follows the maximum more closely (65536 rows x 64 x 1000
+    // 124 us, with a HEAD of 7 121)
+    static constexpr int HEAD = std::is_same<T, half_t>::value ? 13 : 0;
     // a lane's part of one row (its column of the logits): chunks 4 g + q
     struct Part {
         Vec v[SPLIT ? 1 : G];
@@ -275,6 +280,7 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
     __shared__ __attribute__((aligned(16))) A al[STEP];
     __shared__ A red[2][WV][ROWS];
     constexpr bool BACK = VJP && W::TURN; // p is rounded
+    constexpr int HEAD = BACK ? W::HEAD : 0, LAG = HEAD ? 15 - HEAD : 8;
     __shared__ A met[BACK ? ROWS : 1], own[VJP ? ROWS : 1]; // the reference that a row's class met; beta_y's coefficient in xbar
     T* lds = reinterpret_cast<T*>(room);
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6, wr = wave / WV, wv = wave % WV;
@@ -341,16 +347,16 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
                     mx[t] = fmax(mx[t], p[t][v][r]);
                 }
             }
-            // the reference follows the maximum only where it falls behind by more than 8 (exponentials up to 2^8, or e^8); whether it
-            // does shows without joining the four lane groups' maxima
-            far |= mx[t] > ref[t] + (A)8;
+            // the reference follows the maximum only where it falls behind by more than LAG (exponentials up to 2^LAG, or e^LAG, over
+            // that of HEAD); whether it does shows without joining the four lane groups' maxima
+            far |= mx[t] > ref[t] + (A)(LAG + HEAD);
         }
         if (__any(far)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 mx[t] = fmax(mx[t], __shfl_xor(mx[t], 16, 64));
                 mx[t] = fmax(mx[t], __shfl_xor(mx[t], 32, 64));
-                const A to = fmax(ref[t], mx[t]);
+                const A to = fmax(ref[t], mx[t] - (A)HEAD);
                 const A f = exp_log2e(ref[t] - about(to));
                 ref[t] = to;
                 sum[t] *= f;

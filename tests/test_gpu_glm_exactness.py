@@ -44,3 +44,29 @@ def test_rows_predicted_with_confidence(glm, name, n, d, v, sure):
     y[::7] = -1
     lpbar = 0.5 + torch.rand(n, generator=_rng(2), device="cuda", dtype=_wide(DTYPES[name]))
     _check_class(glm, name, y, x, alpha, beta, lpbar)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n,d,v", [(150, 32, 1000), (66000, 8, 1000), (30, 100, 1000), (300, 100, 1000)])
+@pytest.mark.parametrize("lead", [8.0, 14.0, 17.5])
+def test_probabilities_far_below_the_likeliest(glm, name, n, d, v, lead):
+    """One class `lead` above all others, which alone have a coefficient: xbar is minus the sum of many small probabilities."""
+    dtype, wide = DTYPES[name], _wide(DTYPES[name])
+    x = torch.zeros(n, d, dtype=dtype, device="cuda")
+    for likely in (0, v // 2):
+        beta = torch.zeros(v, d, dtype=dtype, device="cuda")
+        beta[:, 0] = 1
+        beta[likely, 0] = 0
+        alpha = torch.zeros(v, dtype=dtype, device="cuda")
+        alpha[likely] = lead
+        y = torch.full((n,), likely, dtype=torch.int64, device="cuda")
+        lpbar = torch.full((n,), 1000.0, dtype=wide, device="cuda")
+        xbar = glm.categorical_logit_glm_lpmf_vjp(y, x, alpha, beta, lpbar=lpbar)[1]
+        p = torch.softmax(alpha.double(), 0)
+        want = -1000.0 * float(p.sum() - p[likely])
+        # a half step of the element type for r or p, one for the result; the exponential of `lead`, v additions; in fp16 what is
+        # stored times 2^13 at least is off by half of its smallest step 2^-24 besides
+        rel = 2 * (_eps(dtype) / 2) * 1.01 + (4 * lead + v + 16) * _eps(wide)
+        off = v * 1000.0 * 2.0**-38 + 2.0**-25 if name == "f16" else 0.0
+        assert not bool(xbar[:, 1:].any())
+        assert float((xbar[:, 0].double() - want).abs().max()) <= rel * abs(want) + off
