@@ -60,15 +60,22 @@ template <typename T> struct Operand {
     int64_t plane; // elements from one plane to the next
 };
 
-// fp32 as a sum of three bf16 values, by cutting off bits: each holds the eight leading bits of what is left (an infinity or a NaN
-// stands in the first). Six of the nine products of two such sums are taken; those left out are at most 2^-22 of the whole (the
-// second value is below 2^-7 of the first, the third below 2^-15), and 2^-26 on average. Here as fp32 values whose low halves are zero.
+// fp32 as a sum of three bf16 values, by cutting off bits: each holds the eight leading bits of what is left. Six of the nine products
+// of two such sums are taken; those left out are at most 2^-21 of the whole (the second value is below 2^-7 of the first, the third
+// below 2^-15; two of them are second times third), 2^-24.5 on average for normal data, and have the product's sign. Here as fp32
+// values whose low halves are zero.
+// An infinity is the largest bf16 number twice and an infinity in the third place, which meets the other operand's first value alone:
+// with a finite value other than zero all six products have one sign and one of them is infinite, as the product is. (In the first
+// place it would meet the zeros that the second and third values of a short number are.) A NaN stands in the third place too.
+__device__ __forceinline__ float split_high(float v) {
+    constexpr float MOST = 3.38953138925153547590e38f; // (bf16's largest)
+    return __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u), -MOST, MOST);
+}
 __device__ __forceinline__ void split3(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
-    a = __builtin_bit_cast(uint32_t, v) & 0xffff0000u;
-    const float fa = __builtin_bit_cast(float, a);
-    const float r = v == fa ? 0.f : v - fa; // (inf - inf is not 0)
-    b = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
-    c = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, b));
+    const float fa = split_high(v), r = v - fa, fb = split_high(r);
+    a = __builtin_bit_cast(uint32_t, fa);
+    b = __builtin_bit_cast(uint32_t, fb);
+    c = __builtin_bit_cast(uint32_t, r - fb);
 }
 // ... of two values, two bf16 in a word each
 __device__ __forceinline__ void split3(float v, float w, uint32_t (&u)[3]) {

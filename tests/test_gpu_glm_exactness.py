@@ -70,3 +70,33 @@ def test_probabilities_far_below_the_likeliest(glm, name, n, d, v, lead):
         off = v * 1000.0 * 2.0**-38 + 2.0**-25 if name == "f16" else 0.0
         assert not bool(xbar[:, 1:].any())
         assert float((xbar[:, 0].double() - want).abs().max()) <= rel * abs(want) + off
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n,d,v", [(60, 16, 70), (66, 17, 70), (100, 64, 300), (66000, 20, 70), (64, 65, 700), (65, 65, 700), (300, 128, 3000),
+                                   (700, 100, 9000)])
+def test_classes_excluded_by_their_coefficients(glm, name, n, d, v):
+    """An intercept column of ones whose coefficient is -inf for some classes: their probability is zero, at all sizes alike."""
+    dtype = DTYPES[name]
+    g = _rng(n + d + v)
+    x, beta = _normal(g, (n, d), dtype), _normal(g, (v, d), dtype, 1.5 / d**0.5)
+    x[:, 0] = 1
+    out = torch.zeros(v, dtype=torch.bool, device="cuda")
+    out[1::3] = True
+    y = torch.randint(0, v // 3, (n,), generator=g, device="cuda") * 3
+    finite = beta.clone()
+    finite[out, 0] = 0
+    beta[out, 0] = -float("inf")
+    alpha = torch.where(out, -float("inf"), 0.0).to(dtype)
+    want = glm.categorical_logit_glm_lpmf_vjp(y, x, alpha, finite)  # (tested elsewhere)
+    want_lp = glm.categorical_logit_glm_lpmf(y, x, alpha, finite)
+    lp = glm.categorical_logit_glm_lpmf(y, x, None, beta)
+    got = glm.categorical_logit_glm_lpmf_vjp(y, x, torch.zeros_like(alpha), beta)
+    # the same products, with zeros for the excluded classes' probabilities. (xbar's first column holds 0 times -inf)
+    assert torch.equal(lp, want_lp) and torch.equal(got[0], want[0])
+    assert torch.equal(got[1][:, 1:], want[1][:, 1:])
+    assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+    # both infinite, and an infinity times zero: as in any product
+    x[2, 0], x[3, 0] = float("inf"), 0
+    lp = glm.categorical_logit_glm_lpmf(y, x, None, beta)
+    assert bool(torch.isnan(lp[3])) and torch.equal(lp[4:], want_lp[4:])
