@@ -17,6 +17,8 @@ __device__ __forceinline__ double from_log2e(double v) { return v; }
 __device__ __forceinline__ double exp_log2e(double v) { return exp(v); }
 __device__ __forceinline__ float log_(float x) { return logf(x); }
 __device__ __forceinline__ double log_(double x) { return log(x); }
+__device__ __forceinline__ float log1p_(float x) { return log1pf(x); }
+__device__ __forceinline__ double log1p_(double x) { return log1p(x); }
 // alpha: a finite one stays finite (the type's lowest value is no exclusion)
 __device__ __forceinline__ float level_log2e(float v) {
     return v == neg_inf<float>() ? v : fmaxf(times_log2e(v), -3.40282346638528859812e38f);
@@ -31,12 +33,17 @@ template <typename A> __device__ __forceinline__ void join(A& mx, A& s, A mo, A 
     s = s * exp_log2e(mx - ref) + so * exp_log2e(mo - ref);
     mx = mm;
 }
-// a row's log probability from all classes' maximum and sum, and its lse (times log2(e) in fp32)
+// a row's log probability from all classes' maximum (or a reference below it) and sum, and its lse (times log2(e) in fp32). eta_y is
+// the logit that the sum holds, to the bit: where it takes more than half of the sum, the rest comes from the same values, and the log
+// probability is never above zero
 template <typename A> __device__ __forceinline__ A row_lp(int64_t y, int64_t classes, A mx, A s, A eta_y, A& lse) {
     const bool empty = mx == neg_inf<A>() && s == 0;
-    const A ls = log_(s);
+    const A ls = log_(s), p = exp_log2e(eta_y - about(mx));
     lse = empty ? neg_inf<A>() : about(mx) + times_log2e(ls);
-    return y < 0 ? (A)0 : y >= classes ? (A)__builtin_nan("") : empty ? neg_inf<A>() : from_log2e(eta_y - about(mx)) - ls;
+    if (y < 0) return 0;
+    if (y >= classes) return (A)__builtin_nan("");
+    if (empty) return neg_inf<A>();
+    return p > (A)0.5 * s ? -log1p_(fmax(s - p, (A)0) / p) : from_log2e(eta_y - about(mx)) - ls;
 }
 
 // sum over the 16 lanes of a row of lanes, in each of them

@@ -970,7 +970,7 @@ template <typename T> struct FewPlan {
     static constexpr int CT = sizeof(T) == 8 ? 2 : 4;
     bool large;
     int64_t tiles, ldv, ldrt, share, splits;
-    size_t part_max, part_sum, eta, lse, largest, r, rt, xt, xpart, bytes;
+    size_t part_max, part_sum, eta_y, eta, lse, largest, r, rt, xt, xpart, bytes;
     FewPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
         const size_t A = sizeof(acc_t<T>), E = sizeof(T);
         size_t at = 0;
@@ -983,6 +983,7 @@ template <typename T> struct FewPlan {
         tiles = tiles_of(V, large ? 16 * CT : 16);
         part_max = take(A * (size_t)(rows * tiles));
         part_sum = take(A * (size_t)(rows * tiles));
+        eta_y = take(A * (size_t)rows);
         if (vjp) {
             ldv = up_to(V, 64);
             ldrt = rows <= 32 ? 32 : 64;
@@ -1017,6 +1018,7 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
     a.features = D;
     a.part_max = (A*)(ws + p.part_max);
     a.part_sum = (A*)(ws + p.part_sum);
+    a.eta_y = (A*)(ws + p.eta_y);
     a.tiles = p.tiles;
     a.lp = (A*)c.lp;
     if (vjp) {

@@ -23,6 +23,7 @@ template <typename T> struct FewArgs {
     const acc_t<T>* lpbar;
     int64_t features;
     acc_t<T>*part_max, *part_sum; // [rows][tiles]
+    acc_t<T>* eta_y;              // [rows]: logits of the rows' classes, as the sums have them
     int64_t tiles;
     acc_t<T>* eta; // [rows][ldv], times log2(e) in fp32
     int64_t ldv;
@@ -117,6 +118,7 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
     const int k = threadIdx.x & 15;
     for (int n = threadIdx.x >> 4; n < NT * 16; n += 4 * WK) {
         A e[CT], mx = neg_inf<A>(), s = 0;
+        const int64_t y = n < a.x.rows ? a.y[n] : -1;
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
             const int64_t v = v0 + 16 * i + k;
@@ -125,6 +127,7 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
             for (int w = 0; w < WK; ++w) u += sum[w][16 * i + k][n];
             e[i] = times_log2e(u) + (v < V ? (a.alpha ? level_log2e((A)a.alpha[v]) : (A)0) : neg_inf<A>());
             mx = fmax(mx, e[i]);
+            if (v == y && v < V) a.eta_y[n] = e[i];
             if (a.eta && n < a.x.rows && v < a.ldv) a.eta[n * a.ldv + v] = e[i];
         }
 #pragma unroll
@@ -149,42 +152,30 @@ template <typename T> __device__ __forceinline__ void few_turn(const FewArgs<T>&
     for (int k = w; k < 64; k += 4)
         if (lane < a.ldrt && d0 + k < a.features) xt[(d0 + k) * a.ldrt + lane] = tile[lane][k];
 }
-// One workgroup a row: lse and lp. The row's logit of its class comes from x and beta again (one dot product). The workgroups behind
-// the last row turn x over
+// One workgroup a row: lse and lp. The workgroups behind the last row turn x over
 template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewArgs<T> a, T* xt) {
     typedef acc_t<T> A;
-    __shared__ A red[3][4];
+    __shared__ A red[2][4];
     if (blockIdx.x >= a.x.rows) {
         few_turn(a, (blockIdx.x - a.x.rows) * 64, xt);
         return;
     }
     const int64_t n = blockIdx.x, y = a.y[n], V = a.beta.rows;
     const bool known = y >= 0 && y < V;
-    A mx = neg_inf<A>(), s = 0, eta = 0;
+    A mx = neg_inf<A>(), s = 0;
+    const A eta = known ? a.eta_y[n] : (A)0;
     for (int64_t i = threadIdx.x; i < a.tiles; i += 256) join(mx, s, a.part_max[n * a.tiles + i], a.part_sum[n * a.tiles + i]);
-    if (known)
-#pragma unroll 4
-        for (int k = threadIdx.x; k < (int)a.features; k += 256) eta += (A)a.x.p[n * a.x.ld + k] * (A)a.beta.p[y * a.beta.ld + k];
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        join(mx, s, __shfl_xor(mx, m, 64), __shfl_xor(s, m, 64));
-        eta += __shfl_xor(eta, m, 64);
-    }
+    for (int m = 32; m >= 1; m >>= 1) join(mx, s, __shfl_xor(mx, m, 64), __shfl_xor(s, m, 64));
     if ((threadIdx.x & 63) == 0) {
         red[0][threadIdx.x >> 6] = mx;
         red[1][threadIdx.x >> 6] = s;
-        red[2][threadIdx.x >> 6] = eta;
     }
     __syncthreads();
     if (a.largest && n == 0) // (rows behind the last)
         for (int64_t i = a.x.rows + threadIdx.x; i < FEW; i += 256) a.largest[i] = 0;
     if (threadIdx.x) return;
-    for (int w = 1; w < 4; ++w) {
-        join(mx, s, red[0][w], red[1][w]);
-        eta += red[2][w];
-    }
-    eta = times_log2e(eta);
-    if (known && a.alpha) eta += level_log2e((A)a.alpha[y]);
+    for (int w = 1; w < 4; ++w) join(mx, s, red[0][w], red[1][w]);
     A lse;
     a.lp[n] = row_lp(y, V, mx, s, eta, lse);
     if (a.lse) a.lse[n] = lse;

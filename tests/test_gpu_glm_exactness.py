@@ -100,3 +100,15 @@ def test_classes_excluded_by_their_coefficients(glm, name, n, d, v):
     x[2, 0], x[3, 0] = float("inf"), 0
     lp = glm.categorical_logit_glm_lpmf(y, x, None, beta)
     assert bool(torch.isnan(lp[3])) and torch.equal(lp[4:], want_lp[4:])
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("n,d,v", [(1, 1000, 40), (40, 100, 2000), (64, 4096, 500), (17, 200, 40000), (150, 32, 300), (150, 8, 70),
+                                   (66000, 64, 70), (66000, 8, 300), (300, 100, 700), (700, 256, 9000)])
+def test_log_probabilities_are_at_most_zero(glm, name, n, d, v):
+    """The logit of a row's class is the one that the sum over the classes holds, not another rounding of it."""
+    y, x, beta = _towards(name, n, d, v, 0.999999, seed=n + d + v)
+    alpha = _normal(_rng(4), (v,), DTYPES[name], 0.1)
+    for al in (None, alpha):
+        assert bool((glm.categorical_logit_glm_lpmf(y, x, al, beta) <= 0).all())
+        assert bool((glm.categorical_logit_glm_lpmf_vjp(y, x, al, beta)[0] <= 0).all())
