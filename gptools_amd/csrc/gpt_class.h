@@ -33,17 +33,24 @@ template <typename A> __device__ __forceinline__ void join(A& mx, A& s, A mo, A 
     s = s * exp_log2e(mx - ref) + so * exp_log2e(mo - ref);
     mx = mm;
 }
-// a row's log probability from all classes' maximum (or a reference below it) and sum, and its lse (times log2(e) in fp32). eta_y is
-// the logit that the sum holds, to the bit: where it takes more than half of the sum, the rest comes from the same values, and the log
-// probability is never above zero
-template <typename A> __device__ __forceinline__ A row_lp(int64_t y, int64_t classes, A mx, A s, A eta_y, A& lse) {
-    const bool empty = mx == neg_inf<A>() && s == 0;
-    const A ls = log_(s), p = exp_log2e(eta_y - about(mx));
-    lse = empty ? neg_inf<A>() : about(mx) + times_log2e(ls);
+// What a row's probabilities come from: exp(eta - top) * share, share = 1 / (the sum of the exponentials about top). (exp(eta - lse)
+// is one operation less, but lse's own rounding is relative to its size: a level common to all classes, which cancels, would cost
+// them digits.) top infinite, share zero: none, where no class is possible; NaN where the row's class is none
+template <typename A> struct RowSum {
+    A top, share;
+};
+template <typename A> __device__ __forceinline__ RowSum<A> row_sum_of(int64_t y, int64_t classes, A mx, A s) {
+    if (mx == neg_inf<A>() && s == 0) return {(A)__builtin_inf(), (A)0};
+    return {about(mx), y >= classes ? (A)__builtin_nan("") : (A)1 / s};
+}
+// a row's log probability from all classes' maximum (or a reference below it) and sum. eta_y is the logit that the sum holds, to the
+// bit: where it takes more than half of the sum, the rest comes from the same values, and the log probability is never above zero
+template <typename A> __device__ __forceinline__ A row_lp(int64_t y, int64_t classes, A mx, A s, A eta_y) {
+    const A p = exp_log2e(eta_y - about(mx));
     if (y < 0) return 0;
     if (y >= classes) return (A)__builtin_nan("");
-    if (empty) return neg_inf<A>();
-    return p > (A)0.5 * s ? -log1p_(fmax(s - p, (A)0) / p) : from_log2e(eta_y - about(mx)) - ls;
+    if (mx == neg_inf<A>() && s == 0) return neg_inf<A>();
+    return p > (A)0.5 * s ? -log1p_(fmax(s - p, (A)0) / p) : from_log2e(eta_y - about(mx)) - log_(s);
 }
 
 // sum over the 16 lanes of a row of lanes, in each of them

@@ -59,7 +59,8 @@ template <typename T> struct LogitArgs {
     // statistics
     A *part_max, *part_sum, *eta_y; // [tiles_v][rows], [tiles_v][rows], [rows]
     // r, and r with the rows' cotangents in the other order: [rows][ldr] and [classes of the piece][ldrt], in whole tiles
-    const A *lse, *lpbar; // lpbar: of all rows
+    const RowSum<A>* of;
+    const A* lpbar; // of all rows
     E *r, *rt;
     int64_t ldr, ldrt, r_plane, rt_plane;
     A* part_alpha; // [tiles_n][ldr] or null
@@ -95,7 +96,7 @@ template <typename W> struct LogitRoom { // LDS
     typedef typename W::Acc A;
     typedef typename W::Tl Tl;
     A red[2][Tl::WM > Tl::WN ? Tl::WM : Tl::WN][Tl::BM > Tl::BN ? Tl::BM : Tl::BN];
-    A al[Tl::BM], lse[Tl::BN], w[Tl::BN];
+    A al[Tl::BM], top[Tl::BN], share[Tl::BN], w[Tl::BN];
     int at[Tl::BN];
 };
 template <typename W, typename Tl, bool STATS, bool KEPT>
@@ -112,10 +113,10 @@ __device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_
         const int64_t n = n0 + c, y = n < rows ? a.y[n] : -1, from = y - (a.v0 + m0);
         room.at[c] = y >= 0 && from >= 0 && from < nv ? (int)from : -1; // the row's class within the tile
         if (!STATS) {
-            // lse: NaN where the row's class is none, infinite (no probability) behind the last row and without a possible class
-            const A l = y < 0 ? neg_inf<A>() : y >= a.classes ? (A)__builtin_nan("") : a.lse[n];
-            const bool none = l == neg_inf<A>();
-            room.lse[c] = none ? -neg_inf<A>() : l;
+            const RowSum<A> of = y < 0 ? RowSum<A>{(A)__builtin_inf(), (A)0} : a.of[n]; // (behind the last row: none)
+            const bool none = of.share == 0;
+            room.top[c] = of.top;
+            room.share[c] = stored_scale<typename W::Data>() * of.share;
             room.w[c] = none ? (A)0 : a.lpbar ? a.lpbar[a.row[n]] / largest : (A)1;
         }
     }
@@ -196,13 +197,14 @@ __device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_
         }
         return;
     }
-    A lse[Tl::TN], w[Tl::TN];
+    A top[Tl::TN], share[Tl::TN], w[Tl::TN];
     int at[Tl::TN];
 #pragma unroll
     for (int j = 0; j < Tl::TN; ++j) {
-        lse[j] = room.lse[Tl::col(j)];
+        top[j] = room.top[Tl::col(j)];
+        share[j] = room.share[Tl::col(j)];
         w[j] = room.w[Tl::col(j)];
-        at[j] = lse[j] == -neg_inf<A>() ? -1 : room.at[Tl::col(j)];
+        at[j] = share[j] == 0 ? -1 : room.at[Tl::col(j)];
     }
     constexpr A up = stored_scale<typename W::Data>();
     A total[Tl::TM][4];
@@ -213,8 +215,7 @@ __device__ __forceinline__ void logits_tile(LogitArgs<W> a, int64_t rows, int64_
             total[i][r] = 0;
 #pragma unroll
             for (int j = 0; j < Tl::TN; ++j) {
-                const A p = exp_log2e(tl.acc[i][j][r] - lse[j]);
-                const A v = (Tl::row(i, r) == at[j] ? up : (A)0) - up * p;
+                const A v = (Tl::row(i, r) == at[j] ? up : (A)0) - share[j] * exp_log2e(tl.acc[i][j][r] - top[j]);
                 tl.acc[i][j][r] = v;
                 total[i][r] += v * w[j];
             }
@@ -388,10 +389,10 @@ template <typename W> __device__ __forceinline__ void gather(const GatherArgs<W>
     }
 }
 
-// lse (times log2(e) in fp32) and lp of 8 observed rows from their tiles' statistics, 32 slices of the tiles in parallel
+// The sums and lp of 8 observed rows from their tiles' statistics, 32 slices of the tiles in parallel
 template <typename A> __global__ __launch_bounds__(256) void class_join(const A* part_max, const A* part_sum, const A* eta_y, const int* y,
                                                                        const int* row, const int* count, int64_t tiles, int64_t ld,
-                                                                       int64_t classes, A* lse, A* lp) {
+                                                                       int64_t classes, RowSum<A>* of, A* lp) {
     __shared__ A red[2][32][9];
     const int c = threadIdx.x & 7, k = threadIdx.x >> 3;
     const int64_t n = (int64_t)blockIdx.x * 8 + c, rows = *count;
@@ -417,9 +418,8 @@ template <typename A> __global__ __launch_bounds__(256) void class_join(const A*
     if (k || n >= rows) return;
     for (int i = 1; i < 32; ++i) join(mx, s, red[0][i][c], red[1][i][c]);
     const int64_t yn = y[n];
-    A l;
-    lp[row[n]] = row_lp(yn, classes, mx, s, yn < classes ? eta_y[n] : (A)0, l);
-    if (lse) lse[n] = l;
+    lp[row[n]] = row_lp(yn, classes, mx, s, yn < classes ? eta_y[n] : (A)0);
+    if (of) of[n] = row_sum_of(yn, classes, mx, s);
 }
 
 // out[c][r] = in[row[r]][c] as operands (row null: r itself), zeros behind the last row up to ldo. 64 x 64 through LDS; each side in
@@ -703,7 +703,7 @@ template <typename W> struct Plan {
     bool wide_products; // wide tiles for xbar and betabar
     bool copy;         // beta as operands of its own
     // offsets in bytes
-    size_t kept, place, row, y, count, runs, part_max, part_sum, eta_y, lse, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
+    size_t kept, place, row, y, count, runs, part_max, part_sum, eta_y, of, scale, r, rt, xt, bt, part_alpha, alpha_acc, xacc, bacc, xa, ba, bytes;
     // (a product's splits of k count too: 16 large tiles with a sixteenth of a long k each fill the card as well. Fewer than nine would need
     // too many of them: bf16 200 rows x 1000 x 100000 472 us against 372 with small ones, fp32 500 x 500 x 60000 1061 against 831, but
     // 700 x 700 x 60000 1445 against 1617)
@@ -754,7 +754,7 @@ template <typename W> struct Plan {
             kept_pieces = lsplits > 1 || features >= keep_features<T>() ? KEPT_BYTES / logits : 0;
             if (kept_pieces > pieces) kept_pieces = pieces;
             if (lsplits == 1) kept = take((size_t)(kept_pieces * logits)); // (else in the first share's place)
-            lse = take(A * (size_t)block);
+            of = take(2 * A * (size_t)block);
             scale = take(A * SCALE_PARTS);
             r = take(S * (size_t)(ldrt * ldr));
             rt = take(S * (size_t)(ldr * ldrt));
@@ -905,13 +905,13 @@ template <typename W, bool REVERSE = true> hipError_t launch_rows(const ClassArg
             class_partial<W><<<dim3((unsigned)(l.grid * l.splits)), dim3(Tl::THREADS), 0, st>>>(l);
             logits<W, true, true>(l, st);
         }
-        A* lse = vjp ? (A*)(ws + p.lse) : nullptr;
+        RowSum<A>* of = vjp ? (RowSum<A>*)(ws + p.of) : nullptr;
         class_join<A><<<dim3((unsigned)tiles_of(N, 8)), dim3(256), 0, st>>>(l.part_max, l.part_sum, l.eta_y, l.y, row, count,
-                                                                            tiles_of(V, EDGE), N, V, lse, (A*)c.lp + n0);
+                                                                            tiles_of(V, EDGE), N, V, of, (A*)c.lp + n0);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if (!vjp) continue;
         if constexpr (REVERSE) {
-            l.lse = lse;
+            l.of = of;
             l.lpbar = c.lpbar ? (const A*)c.lpbar + n0 : nullptr;
             l.r = r;
             l.rt = rt;
@@ -970,7 +970,7 @@ template <typename T> struct FewPlan {
     static constexpr int CT = sizeof(T) == 8 ? 2 : 4;
     bool large;
     int64_t tiles, ldv, ldrt, share, splits;
-    size_t part_max, part_sum, eta_y, eta, lse, largest, r, rt, xt, xpart, bytes;
+    size_t part_max, part_sum, eta_y, eta, of, largest, r, rt, xt, xpart, bytes;
     FewPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
         const size_t A = sizeof(acc_t<T>), E = sizeof(T);
         size_t at = 0;
@@ -994,7 +994,7 @@ template <typename T> struct FewPlan {
             share = up_to(tiles_of(V, splits), 128);
             splits = tiles_of(V, share);
             eta = take(A * (size_t)(rows * ldv));
-            lse = take(A * (size_t)rows);
+            of = take(2 * A * (size_t)rows);
             largest = take(A * FEW);
             r = take(E * (size_t)(rows * ldv));
             rt = take(E * (size_t)(V * ldrt));
@@ -1024,7 +1024,7 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
     if (vjp) {
         a.eta = (A*)(ws + p.eta);
         a.ldv = p.ldv;
-        a.lse = (A*)(ws + p.lse);
+        a.of = (RowSum<A>*)(ws + p.of);
         a.largest = (A*)(ws + p.largest);
         a.r = (T*)(ws + p.r);
         a.rt = (T*)(ws + p.rt);

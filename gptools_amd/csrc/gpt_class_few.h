@@ -27,7 +27,8 @@ template <typename T> struct FewArgs {
     int64_t tiles;
     acc_t<T>* eta; // [rows][ldv], times log2(e) in fp32
     int64_t ldv;
-    acc_t<T>*lse, *lp, *largest; // largest: |lpbar| of each observed row, zero to FEW
+    RowSum<acc_t<T>>* of;  // [rows]; null: no reverse mode
+    acc_t<T>*lp, *largest; // largest: |lpbar| of each observed row, zero to FEW
     T *r, *rt;                   // [rows][ldv], [classes][ldrt]
     int64_t ldrt;
     T* alphabar;
@@ -152,7 +153,7 @@ template <typename T> __device__ __forceinline__ void few_turn(const FewArgs<T>&
     for (int k = w; k < 64; k += 4)
         if (lane < a.ldrt && d0 + k < a.features) xt[(d0 + k) * a.ldrt + lane] = tile[lane][k];
 }
-// One workgroup a row: lse and lp. The workgroups behind the last row turn x over
+// One workgroup a row: its sum and lp. The workgroups behind the last row turn x over
 template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewArgs<T> a, T* xt) {
     typedef acc_t<T> A;
     __shared__ A red[2][4];
@@ -176,9 +177,8 @@ template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewA
         for (int64_t i = a.x.rows + threadIdx.x; i < FEW; i += 256) a.largest[i] = 0;
     if (threadIdx.x) return;
     for (int w = 1; w < 4; ++w) join(mx, s, red[0][w], red[1][w]);
-    A lse;
-    a.lp[n] = row_lp(y, V, mx, s, eta, lse);
-    if (a.lse) a.lse[n] = lse;
+    a.lp[n] = row_lp(y, V, mx, s, eta);
+    if (a.of) a.of[n] = row_sum_of(y, V, mx, s);
     if (a.largest) a.largest[n] = y < 0 || !a.lpbar ? (A)0 : fabs(a.lpbar[n]);
 }
 
@@ -186,23 +186,24 @@ template <typename T> __global__ __launch_bounds__(256) void class_few_join(FewA
 template <typename T> __global__ __launch_bounds__(256) void class_few_r(FewArgs<T> a, Largest<acc_t<T>> largest_of) {
     typedef acc_t<T> A;
     constexpr int N = Vec16<T>::N;
-    __shared__ A lse[FEW], w[FEW], sum[4][64];
+    __shared__ A top[FEW], share_of[FEW], w[FEW], sum[4][64];
     __shared__ int64_t y[FEW];
     const A largest = largest_of.get();
+    constexpr A up = stored_scale<T>();
     const int64_t V = a.beta.rows;
     const int rows = (int)a.x.rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x < FEW) {
         const int n = threadIdx.x;
         const int64_t yn = n < rows ? a.y[n] : -1;
-        const A l = yn >= 0 ? a.lse[n] : neg_inf<A>();
-        const bool none = l == neg_inf<A>();
+        const RowSum<A> of = yn >= 0 ? a.of[n] : RowSum<A>{(A)__builtin_inf(), (A)0};
+        const bool none = of.share == 0;
         y[n] = none ? -1 : yn;
-        lse[n] = yn >= V ? (A)__builtin_nan("") : l;
+        top[n] = of.top;
+        share_of[n] = up * of.share;
         w[n] = none ? (A)0 : a.lpbar ? a.lpbar[n] / largest : (A)1;
     }
     __syncthreads();
     const int64_t v = (int64_t)blockIdx.x * 64 + lane; // (below ldv, a multiple of 64)
-    constexpr A up = stored_scale<T>();
     A total = 0;
     const int share = (int)a.ldrt / 4;
     for (int n0 = wave * share; n0 < (wave + 1) * share; n0 += N) {
@@ -212,7 +213,7 @@ template <typename T> __global__ __launch_bounds__(256) void class_few_r(FewArgs
             const int n = n0 + e;
             A g = 0;
             if (n < rows) {
-                g = y[n] < 0 || v >= V ? (A)0 : (y[n] == v ? up : (A)0) - up * exp_log2e(a.eta[n * a.ldv + v] - lse[n]);
+                g = y[n] < 0 || v >= V ? (A)0 : (y[n] == v ? up : (A)0) - share_of[n] * exp_log2e(a.eta[n * a.ldv + v] - top[n]);
                 a.r[n * a.ldv + v] = (T)g;
                 g *= w[n];
             }

@@ -4,7 +4,7 @@
 //
 //   class_narrow_rows    a wave holds 16 rows of x (or 32) and walks the classes 32 at a time: logits of 16 classes x 16 rows on the
 //                        matrix cores, their exponentials about a running reference, and sum_v p beta_v from the same registers.
-//                        Leaves lp, lse, and xbar = lpbar (beta_y - sum_v p beta_v).
+//                        Leaves lp, the sums, and xbar = lpbar (beta_y - sum_v p beta_v).
 //   class_narrow_classes a wave holds 16 classes (or 32) and walks the rows, logits again, r, betabar and alphabar.
 //
 // That the second product needs no shuffle is the matrix instruction's doing: it leaves value (v, n) of C in register r of lane
@@ -37,8 +37,10 @@ template <typename T> struct NarrowArgs {
     int64_t features;
     // rows in the order they are taken, the observed ones first, and how many those are (null: as they come, all)
     const int *order, *count;
-    A *lp, *lse, *w; // w: the row's cotangent over the largest, 0 without an observation; lse: infinite there. Both in that order
-    int* at;         // ... and the row's class
+    // in that order: w: the row's cotangent over the largest, 0 without an observation; top: what its exponentials are taken about,
+    // infinite there; share: w over their sum (16 bits: top is the lse and share is not there)
+    A *lp, *top, *share_of, *w;
+    int* at; // ... and the row's class
     Largest<A> largest;
     T* xbar;       // [rows][features]
     A* part;       // [shares][classes][features + 1]: betabar, alphabar; null: one share, the results themselves
@@ -72,6 +74,9 @@ template <typename T, int DT> struct Narrow {
     template <int STEP> static constexpr int stage() { return STEP * LD + (TURN ? DP * (STEP + 4) : SPLIT ? 3 * STEP * SLD / 2 : 0); }
     // fp32: what stands in registers is times log2(e) already, so that logits come in that unit
     static constexpr bool UNIT = sizeof(T) >= 4;
+    // the second kernel's probabilities as RowSum has them; in 16 bits about the lse, whose rounding (2^-24 of its size) is nothing
+    // beside r's, and which takes fewer registers (fp16 65536 x 64 x 1000 124 us against 160)
+    static constexpr bool SHARE = UNIT;
     // fp16: p is 2^HEAD where the logit is the reference's own, and at most 2^15: a probability is off by 2^-38 at most besides its
     // relative rounding, as r is, which holds 2^14 for one. The reference then follows the maximum more closely (65536 rows x 64 x 1000
     // 124 us, with a HEAD of 7 121)
@@ -408,16 +413,17 @@ template <typename T, int DT, int WR, int WV, int NT, bool VJP> __global__ __lau
         const bool known = y[t] >= 0 && y[t] < V;
         A eta = 0; // of the row's class
         if (wv == 0) eta = W::eta_at(a.beta, known ? y[t] : 0, D, x[t], known && a.alpha ? level_log2e((A)a.alpha[y[t]]) : (A)0);
-        A lse;
-        const A lp = row_lp(y[t], V, mx, s, eta, lse);
-        const bool none = y[t] < 0 || lse == neg_inf<A>();
+        const A lp = row_lp(y[t], V, mx, s, eta);
+        const RowSum<A> of = row_sum_of((int64_t)y[t], V, mx, s);
+        const bool none = y[t] < 0 || of.share == 0;
         A w = 0;
         if (VJP) w = none ? (A)0 : known ? (a.lpbar ? a.lpbar[row[t]] : (A)1) : (A)__builtin_nan("");
         if (wv == 0 && q == 0 && n < a.x.rows) {
             a.lp[row[t]] = lp;
             if (VJP) {
-                a.lse[n] = none ? -neg_inf<A>() : lse;
+                a.top[n] = none ? -neg_inf<A>() : W::SHARE ? of.top : of.top + times_log2e(log_(s));
                 a.w[n] = w / largest;
+                if (W::SHARE) a.share_of[n] = none ? (A)0 : w * of.share;
                 a.at[n] = known ? y[t] : -1;
             }
         }
@@ -465,7 +471,7 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     constexpr int VT = VT_<T, DT, WR>, STEP = 16 * VT * WR, CLASSES = 16 * NT * WV;
     constexpr int STAGE = W::template stage<STEP>() * (int)sizeof(T), SPILL = WR * CLASSES * W::OLD * (int)sizeof(A);
     __shared__ uint4 room[(larger(STAGE, SPILL) + 15) / 16];
-    __shared__ __attribute__((aligned(16))) A lse[STEP], wt[STEP];
+    __shared__ __attribute__((aligned(16))) A top[STEP], part_of[W::SHARE ? STEP : 4], wt[STEP];
     __shared__ __attribute__((aligned(16))) int yt[STEP];
     T* lds = reinterpret_cast<T*>(room);
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6, wv = wave / WR, wr = wave % WR;
@@ -493,13 +499,14 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
     const int64_t r0 = (int64_t)blockIdx.y * share, r1 = r0 + share < rows ? r0 + share : rows;
     const Operand<T> x = {a.x.p, a.x.ld, r1, 0};
     typename W::template Rows<STEP> next;
-    A next_lse = 0, next_w = 0;
+    A next_top = 0, next_part = 0, next_w = 0;
     int next_y = -1;
     auto fetch = [&](int64_t n0) {
         next.fetch(x, n0, D, a.order, a.order ? nullptr : a.y);
         if (threadIdx.x < STEP) {
             const int64_t n = n0 + threadIdx.x;
-            next_lse = n < r1 ? a.lse[n] : -neg_inf<A>();
+            next_top = n < r1 ? a.top[n] : -neg_inf<A>();
+            if (W::SHARE) next_part = n < r1 ? a.share_of[n] : (A)0;
             next_w = n < r1 ? a.w[n] * up : (A)0;
             next_y = n < r1 ? a.at[n] : -1;
         }
@@ -509,7 +516,8 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
         __syncthreads();
         next.put(lds);
         if (threadIdx.x < STEP) {
-            lse[threadIdx.x] = next_lse;
+            top[threadIdx.x] = next_top;
+            if (W::SHARE) part_of[threadIdx.x] = next_part;
             wt[threadIdx.x] = next_w;
             yt[threadIdx.x] = next_y;
         }
@@ -520,13 +528,21 @@ template <typename T, int DT, int WR, int WV, int NT> __global__ __launch_bounds
             const int base = (wr * VT + u) * 16;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const A level = W::UNIT ? al[t] : (A)0;
-                C p = W::template logits<STEP>(lds, base, b[t], C{level, level, level, level});
+                C p = {0, 0, 0, 0};
+                // fp32: the product starts from the level less the row's top, which is in no register afterwards. (fp64 65536 x 32 x 1000
+                // 459 us that way, 446 with the top taken off behind it)
+                constexpr bool BEFORE = sizeof(T) == 4;
+                if constexpr (W::SHARE) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = BEFORE ? al[t] - top[base + Mma<T>::row(q, r)] : al[t];
+                }
+                p = W::template logits<STEP>(lds, base, b[t], p);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int n = base + Mma<T>::row(q, r);
-                    const A e = exp_log2e((W::UNIT ? p[r] : times_log2e(p[r]) + al[t]) - lse[n]);
-                    p[r] = wt[n] * ((yt[n] == me[t] ? (A)1 : (A)0) - e);
+                    const bool own = yt[n] == me[t];
+                    if constexpr (W::SHARE) p[r] = (own ? wt[n] : (A)0) - part_of[n] * exp_log2e(BEFORE ? p[r] : p[r] - top[n]);
+                    else p[r] = wt[n] * ((own ? (A)1 : (A)0) - exp_log2e(W::eta(p[r], al[t]) - top[n]));
                     abar[t] += p[r];
                 }
                 W::template gather<STEP>(lds, base, p, o[t]);
@@ -595,7 +611,7 @@ template <typename T> struct NarrowPlan {
     static constexpr int NT = sizeof(T) == 8 ? 1 : 2;
     bool many_rows, many_classes, indexed;
     int64_t share, shares;
-    size_t lse, w, at, scale, order, y_of, count, runs, part, bytes;
+    size_t top, share_of, w, at, scale, order, y_of, count, runs, part, bytes;
     NarrowPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
         const size_t A = sizeof(acc_t<T>);
         many_rows = tiles_of(rows, 64 * NT) >= 512;
@@ -624,7 +640,8 @@ template <typename T> struct NarrowPlan {
             runs = take(4 * (size_t)tiles_of(rows, INDEX_ROWS));
         }
         if (vjp) {
-            lse = take(A * (size_t)rows);
+            top = take(A * (size_t)rows);
+            share_of = take(sizeof(T) >= 4 ? A * (size_t)rows : 0);
             w = take(A * (size_t)rows);
             at = take(4 * (size_t)rows);
             scale = take(A * SCALE_PARTS);
@@ -671,7 +688,8 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
         a.count = (const int*)(ws + p.count);
     }
     if (vjp) {
-        a.lse = (A*)(ws + p.lse);
+        a.top = (A*)(ws + p.top);
+        a.share_of = (A*)(ws + p.share_of);
         a.w = (A*)(ws + p.w);
         a.at = (int*)(ws + p.at);
         a.xbar = (T*)c.xbar;

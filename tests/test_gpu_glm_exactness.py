@@ -112,3 +112,27 @@ def test_log_probabilities_are_at_most_zero(glm, name, n, d, v):
     for al in (None, alpha):
         assert bool((glm.categorical_logit_glm_lpmf(y, x, al, beta) <= 0).all())
         assert bool((glm.categorical_logit_glm_lpmf_vjp(y, x, al, beta)[0] <= 0).all())
+
+
+@pytest.mark.parametrize("name", ["f64", "f32"])
+@pytest.mark.parametrize("n,d,v", [(40, 100, 2000), (300, 8, 300), (300, 40, 77), (66000, 8, 300), (300, 100, 700), (600, 100, 24680)])
+@pytest.mark.parametrize("level", [0.0, 1024.0, -1024.0])
+def test_a_level_common_to_all_classes(glm, name, n, d, v, level):
+    """It cancels in the probabilities, which are 1 / v here, and may not cost them digits."""
+    dtype, ea = DTYPES[name], _eps(DTYPES[name])
+    x = torch.zeros(n, d, dtype=dtype, device="cuda")
+    x[:, 0] = 1
+    beta = torch.zeros(v, d, dtype=dtype, device="cuda")
+    beta[:, 1] = 1  # (x is zero there)
+    alpha = torch.full((v,), level, dtype=dtype, device="cuda")
+    y = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    y[7:27] = 3
+    lp, xbar, alphabar, betabar = glm.categorical_logit_glm_lpmf_vjp(y, x, alpha, beta)
+    want = torch.full((v,), -20.0 / v, dtype=torch.float64, device="cuda")
+    want[3] += 20
+    # the logits are all equal, their exponentials about the largest are 1 and add up to v exactly; 1 / v, the product and the
+    # difference are rounded, and 20 additions of them
+    assert bool(((alphabar.double() - want).abs() <= 24 * ea * want.abs()).all())
+    assert bool(((betabar[:, 0].double() - want).abs() <= 24 * ea * want.abs()).all())
+    # one entry of size 1, v of 1 / v and their sum in any order
+    assert float(xbar[:, 1].abs().max()) <= (v + 8) * ea
