@@ -34,7 +34,7 @@ int zero(gpt_ctx* c, void* p, size_t bytes) {
 bool known_type(int dtype) { return dtype == GPT_F64 || dtype == GPT_F32 || dtype == GPT_F16 || dtype == GPT_BF16; }
 size_t size_of(int dtype) { return dtype == GPT_F64 ? 8 : dtype == GPT_F32 ? 4 : 2; }
 constexpr int64_t MOST = 2147483647LL;                                       // rows
-constexpr int64_t MOST_FEATURES = (int64_t)1 << 21, MOST_CLASSES = (int64_t)1 << 26; // (grids count their tiles in 32 bits)
+constexpr int64_t MOST_FEATURES = (int64_t)1 << 21, MOST_CLASSES = (int64_t)1 << 26;
 constexpr int64_t MOST_WIDTH = (int64_t)1 << 40;
 
 int check_norm(gpt_ctx* c, int dtype, int64_t rows, int64_t width) {

@@ -297,7 +297,7 @@ template <typename W, bool STATS, bool KEPT> __global__ __launch_bounds__(W::Tl:
     const int64_t rows = *a.count;
     int64_t tm, tn;
     bool half;
-    if (!tile_place<Tl>(blockIdx.x, a.tiles_v, rows, tm, tn, half)) return;
+    if (!tile_place<Tl>(wide_block(), a.tiles_v, rows, tm, tn, half)) return;
     if constexpr (!std::is_void<Half>::value) {
         if (half) {
             logits_tile<W, Half, STATS, KEPT>(a, rows, tm, tn, room, lds);
@@ -783,7 +783,7 @@ template <typename W> struct Plan {
 template <typename W, bool STATS, bool KEPT> void logits(LogitArgs<W> l, hipStream_t st) {
     typedef typename W::Tl Tl;
     l.tiles_v = tiles_of(l.beta.rows, Tl::BM);
-    class_logits<W, STATS, KEPT><<<dim3(tile_grid<Tl>(l.tiles_v, l.x.rows)), dim3(Tl::THREADS), 0, st>>>(l);
+    class_logits<W, STATS, KEPT><<<wide_grid(tile_grid<Tl>(l.tiles_v, l.x.rows)), dim3(Tl::THREADS), 0, st>>>(l);
 }
 
 // xbar and betabar of a piece (each complete if its `last`), alphabar (of alpha.nv classes)

@@ -493,11 +493,11 @@ template <typename Tl> __device__ __forceinline__ bool tile_place(int64_t id, in
 __device__ __forceinline__ int64_t split_place(int64_t in, int64_t split, int64_t tiles) {
     return (in & ~(int64_t)7) | ((in + split * tiles) & 7);
 }
-template <typename Tl> unsigned tile_grid(int64_t tiles_m, int64_t cols) {
+template <typename Tl> int64_t tile_grid(int64_t tiles_m, int64_t cols) {
     const int64_t tiles_n = (cols + Tl::BN - 1) / Tl::BN;
-    if (std::is_void<typename HalfOf<Tl>::Tile>::value) return (unsigned)((tiles_m * tiles_n + 7) / 8 * 8);
+    if (std::is_void<typename HalfOf<Tl>::Tile>::value) return (tiles_m * tiles_n + 7) / 8 * 8;
     const int64_t band = tile_band(tiles_m);
-    return (unsigned)((tiles_m + band - 1) / band * ((band * tiles_n + 7) / 8 * 8 + 8));
+    return (tiles_m + band - 1) / band * ((band * tiles_n + 7) / 8 * 8 + 8);
 }
 
 } // namespace gptt

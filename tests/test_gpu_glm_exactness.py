@@ -6,7 +6,7 @@ the largest calls. Inputs, formulas and bounds are those of test_gpu_glm.py unle
 import pytest
 import torch
 
-from test_gpu_glm import DTYPES, _check_class, _class_want, _eps, _normal, _rng, _wide, glm  # noqa: F401
+from test_gpu_glm import DTYPES, _check_class, _class_data, _class_want, _eps, _normal, _rng, _wide, glm  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,19 @@ def test_a_level_common_to_all_classes(glm, name, n, d, v, level):
     assert bool(((betabar[:, 0].double() - want).abs() <= 24 * ea * want.abs()).all())
     # one entry of size 1, v of 1 / v and their sum in any order
     assert float(xbar[:, 1].abs().max()) <= (v + 8) * ea
+
+
+@pytest.mark.parametrize("name,v", [("f64", 1 << 20), ("bf16", 2100001)])
+def test_more_tiles_than_a_grid_counts_threads(glm, name, v):
+    """Rows x classes whose tiles have more threads than a grid's first dimension counts (2^32)."""
+    n, d = 1 << 18, 65
+    y, x, alpha, beta = _class_data(name, n, d, v, 3)
+    lp = glm.categorical_logit_glm_lpmf(y, x, alpha, beta)
+    ea = _eps(_wide(DTYPES[name]))
+    for at in (0, n // 2 + 3, n - 50):
+        some = slice(at, at + 50)
+        xd, bd, eta, lse, want, *_ = _class_want(y[some], x[some], alpha, beta, None, y[some] >= 0)
+        # as in _check_class
+        de = (d + 2) * ea * (xd.abs() @ bd.abs().T + eta.abs()) + 4 * ea * (eta.abs() + lse.abs().unsqueeze(1))
+        tol = 2 * de.max(1).values + (96 + v / 2048) * ea + 2 * ea * (lse.abs() + want.abs())
+        assert bool(((lp[some].double() - want).abs() <= tol).all())
