@@ -969,7 +969,7 @@ template <typename T> struct FewPlan {
     // class tiles of a workgroup where the classes are enough to fill the card that way (fp64 has not the LDS for more)
     static constexpr int CT = sizeof(T) == 8 ? 2 : 4;
     bool large;
-    int64_t tiles, ldv, ldrt, share, splits;
+    int64_t tiles, piece, pieces, ldv, ldrt, share, splits; // (splits: of a piece)
     size_t part_max, part_sum, eta_y, eta, of, largest, r, rt, xt, xpart, bytes;
     FewPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
         const size_t A = sizeof(acc_t<T>), E = sizeof(T);
@@ -985,21 +985,27 @@ template <typename T> struct FewPlan {
         part_sum = take(A * (size_t)(rows * tiles));
         eta_y = take(A * (size_t)rows);
         if (vjp) {
-            ldv = up_to(V, 64);
             ldrt = rows <= 32 ? 32 : 64;
+            // logits, r and its transpose: as much as the other way's pieces and kept logits may take. (Beyond it logits are computed twice:
+            // one row x 128 x 24 M classes in bf16 6.6 ms against 5.7, 64 x 512 x 1.1 M in fp64 9.3 against 7.2; the other way 14.8 and 12.6)
+            const int64_t held = (int64_t)(rows * (A + E) + ldrt * E), most = (PIECE_BYTES + KEPT_BYTES) / held / 128 * 128;
+            pieces = tiles_of(V, most);
+            piece = pieces > 1 ? up_to(tiles_of(V, pieces), 128) : V;
+            pieces = tiles_of(V, piece);
+            ldv = up_to(piece, 64);
             const int64_t slabs = tiles_of(D, 16 * Vec16<T>::N);
             splits = tiles_of(2 * FILL, slabs);
-            if (splits > tiles_of(V, 128)) splits = tiles_of(V, 128);
+            if (splits > tiles_of(piece, 128)) splits = tiles_of(piece, 128);
             if (V <= 1024) splits = 1; // (eight rounds of one workgroup are shorter than another launch)
-            share = up_to(tiles_of(V, splits), 128);
-            splits = tiles_of(V, share);
+            share = up_to(tiles_of(piece, splits), 128);
+            splits = tiles_of(piece, share);
             eta = take(A * (size_t)(rows * ldv));
             of = take(2 * A * (size_t)rows);
             largest = take(A * FEW);
             r = take(E * (size_t)(rows * ldv));
-            rt = take(E * (size_t)(V * ldrt));
+            rt = take(E * (size_t)(piece * ldrt));
             xt = take(E * (size_t)(D * ldrt));
-            xpart = splits > 1 ? take(A * (size_t)(splits * rows * D)) : 0;
+            xpart = pieces * splits > 1 ? take(A * (size_t)(splits * rows * D)) : 0;
         }
         bytes = at;
     }
@@ -1022,7 +1028,7 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
     a.tiles = p.tiles;
     a.lp = (A*)c.lp;
     if (vjp) {
-        a.eta = (A*)(ws + p.eta);
+        a.eta = p.pieces == 1 ? (A*)(ws + p.eta) : nullptr;
         a.ldv = p.ldv;
         a.of = (RowSum<A>*)(ws + p.of);
         a.largest = (A*)(ws + p.largest);
@@ -1030,11 +1036,10 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
         a.rt = (T*)(ws + p.rt);
         a.ldrt = p.ldrt;
         a.alphabar = (T*)c.alphabar;
-        a.xpart = p.splits > 1 ? (A*)(ws + p.xpart) : nullptr;
+        a.xpart = p.pieces * p.splits > 1 ? (A*)(ws + p.xpart) : nullptr;
         a.xbar = (T*)c.xbar;
         a.share = p.share;
     }
-    const dim3 grid((unsigned)p.tiles);
     bool odd = false; // rows that start in the middle of a word
     if (sizeof(T) == 2) odd = (((uintptr_t)c.beta | (uintptr_t)c.x) & 2) || ((c.ldbeta | c.ldx) & 1);
     auto with = [&](auto run) {
@@ -1046,25 +1051,42 @@ template <typename T, int NT> hipError_t launch_few(const ClassArgs& c, bool vjp
         }
         run(std::false_type());
     };
-    with([&](auto half) {
-        constexpr bool HALF = decltype(half)::value;
-        if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4, HALF><<<grid, dim3(256), 0, st>>>(a);
-        else class_few_logits<T, NT, 1, 8, HALF><<<grid, dim3(512), 0, st>>>(a);
-    });
+    auto logits = [&](const FewArgs<T>& a) {
+        with([&](auto half) {
+            constexpr bool HALF = decltype(half)::value;
+            const unsigned large = (unsigned)tiles_of(a.beta.rows, 16 * FewPlan<T>::CT), small = (unsigned)tiles_of(a.beta.rows, 16);
+            if (p.large) class_few_logits<T, NT, FewPlan<T>::CT, 4, HALF><<<dim3(large), dim3(256), 0, st>>>(a);
+            else class_few_logits<T, NT, 1, 8, HALF><<<dim3(small), dim3(512), 0, st>>>(a);
+        });
+    };
+    logits(a);
     T* xt = vjp ? (T*)(ws + p.xt) : nullptr;
     class_few_join<T><<<dim3((unsigned)(c.rows + (vjp ? tiles_of(D, 64) : 0))), dim3(256), 0, st>>>(a, xt);
     if (!vjp) return hipGetLastError();
     const Largest<A> largest = {c.lpbar ? a.largest : nullptr};
-    class_few_r<T><<<dim3((unsigned)(p.ldv / 64)), dim3(256), 0, st>>>(a, largest);
     constexpr int NG = (NT <= 2 ? 32 : 64) / (4 * Vec16<T>::N);
     const int64_t xslabs = tiles_of(D, 16 * Vec16<T>::N), bslabs = tiles_of(D, Slab<T>::WIDTH);
-    int64_t shares = tiles_of(4 * FILL, bslabs);
-    if (shares > tiles_of(V, 128)) shares = tiles_of(V, 128);
-    with([&](auto half) {
-        class_few_back<T, NT, NG, decltype(half)::value><<<dim3((unsigned)(xslabs * p.splits + bslabs * shares)), dim3(256), 0, st>>>(
-            a, xt, (T*)c.betabar, largest, (int)xslabs, (int)p.splits, (int)bslabs, (int)shares);
-    });
-    if (p.splits > 1) class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits);
+    for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+        const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece, splits = tiles_of(nv, p.share);
+        FewArgs<T> b = a;
+        b.beta = {(const T*)c.beta + v0 * c.ldbeta, c.ldbeta, nv};
+        b.v0 = v0;
+        if (c.alpha) b.alpha = (const T*)c.alpha + v0;
+        if (c.alphabar) b.alphabar = (T*)c.alphabar + v0;
+        if (p.pieces > 1) {
+            b.eta = (A*)(ws + p.eta);
+            b.add = v0 > 0;
+            logits(b);
+        }
+        class_few_r<T><<<dim3((unsigned)tiles_of(nv, 64)), dim3(256), 0, st>>>(b, largest);
+        int64_t shares = tiles_of(4 * FILL, bslabs);
+        if (shares > tiles_of(nv, 128)) shares = tiles_of(nv, 128);
+        with([&](auto half) {
+            class_few_back<T, NT, NG, decltype(half)::value><<<dim3((unsigned)(xslabs * splits + bslabs * shares)), dim3(256), 0, st>>>(
+                b, xt, (T*)c.betabar + v0 * D, largest, (int)xslabs, (int)splits, (int)bslabs, (int)shares);
+        });
+    }
+    if (a.xpart) class_few_xbar_join<T><<<dim3((unsigned)tiles_of(c.rows * D, 256)), dim3(256), 0, st>>>(a, (int)p.splits);
     return hipGetLastError();
 }
 template <typename T> hipError_t launch_few(const ClassArgs& c, bool vjp, hipStream_t st) {

@@ -3,7 +3,8 @@
 // into the registers that the matrix instruction reads, no LDS between.
 //
 //   class_few_logits  16 classes a workgroup or 64 (32 in fp64), whose waves share the features; their logits' maximum and sum for every row,
-//                     and for the reverse mode the logits themselves (64 rows of logits are a piece as r is one)
+//                     and for the reverse mode the logits themselves, or, where the classes are too many to hold these and r
+//                     at once, those of a piece of the classes at a time when all sums are known
 //   class_few_r       r in both orders, alphabar
 //   class_few_back    xbar = r beta, and betabar = r^T x, which is bound by writing it. For xbar beta's rows lie along the
 //                     features, the sum runs over the classes: a lane reads 16 bytes of eight classes and turns the block over in
@@ -21,7 +22,7 @@ template <typename T> struct FewArgs {
     const T* alpha;
     const int64_t* y;
     const acc_t<T>* lpbar;
-    int64_t features;
+    int64_t features, v0; // v0: class of beta's first row
     acc_t<T>*part_max, *part_sum; // [rows][tiles]
     acc_t<T>* eta_y;              // [rows]: logits of the rows' classes, as the sums have them
     int64_t tiles;
@@ -33,6 +34,7 @@ template <typename T> struct FewArgs {
     int64_t ldrt;
     T* alphabar;
     acc_t<T>* xpart; // [splits][rows][features]; null: one split, the result itself
+    bool add;        // xpart holds earlier pieces' sums
     T* xbar;
     int64_t share;   // classes of a split
 };
@@ -128,7 +130,7 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
             for (int w = 0; w < WK; ++w) u += sum[w][16 * i + k][n];
             e[i] = times_log2e(u) + (v < V ? (a.alpha ? level_log2e((A)a.alpha[v]) : (A)0) : neg_inf<A>());
             mx = fmax(mx, e[i]);
-            if (v == y && v < V) a.eta_y[n] = e[i];
+            if (a.v0 + v == y && v < V) a.eta_y[n] = e[i];
             if (a.eta && n < a.x.rows && v < a.ldv) a.eta[n * a.ldv + v] = e[i];
         }
 #pragma unroll
@@ -213,7 +215,7 @@ template <typename T> __global__ __launch_bounds__(256) void class_few_r(FewArgs
             const int n = n0 + e;
             A g = 0;
             if (n < rows) {
-                g = y[n] < 0 || v >= V ? (A)0 : (y[n] == v ? up : (A)0) - share_of[n] * exp_log2e(a.eta[n * a.ldv + v] - top[n]);
+                g = y[n] < 0 || v >= V ? (A)0 : (y[n] == a.v0 + v ? up : (A)0) - share_of[n] * exp_log2e(a.eta[n * a.ldv + v] - top[n]);
                 a.r[n * a.ldv + v] = (T)g;
                 g *= w[n];
             }
@@ -267,8 +269,8 @@ template <typename T, int NT, bool HALF> __device__ __forceinline__ void few_xba
     constexpr int N = Vec16<T>::N;
     __shared__ A sum[4][16][16 * N + 1];
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
-    // a chunk that lies behind the last whole one is taken as the last N features (some of which the one before has too, with the same
-    // sums): no guard holds a load back (bf16 12 rows x 1958 x 34026 with the reverse mode 126 us against 157)
+    // a chunk that lies behind the last whole one is taken as the last N features (some of which the one before has too): no guard
+    // holds a load back (bf16 12 rows x 1958 x 34026 with the reverse mode 126 us against 157)
     const int64_t d0 = slab * 16 * N, D = a.features, V = a.beta.rows;
     const auto start = [=](int chunk) { return D < N || d0 + (chunk + 1) * N <= D ? d0 + chunk * N : D - N; };
     const int64_t d = start(lane & 15);
@@ -313,10 +315,12 @@ template <typename T, int NT, bool HALF> __device__ __forceinline__ void few_xba
         for (int id = threadIdx.x; id < 16 * 16 * N; id += 256) {
             const int n = id / (16 * N), k = id % (16 * N);
             const int64_t to = start(k / N) + k % N;
-            if (16 * t + n >= a.x.rows || d0 + k / N * N >= D || to >= D) continue;
+            if (16 * t + n >= a.x.rows || to < d0 + k / N * N || to >= D) continue; // (each feature by the chunk that it lies in)
             const A s = (sum[0][n][k] + sum[1][n][k]) + (sum[2][n][k] + sum[3][n][k]);
-            if (a.xpart) a.xpart[(split * a.x.rows + 16 * t + n) * D + to] = s;
-            else a.xbar[(16 * t + n) * D + to] = few_cotangent(a, 16 * t + n, s);
+            if (a.xpart) {
+                A* part = a.xpart + (split * a.x.rows + 16 * t + n) * D + to;
+                *part = a.add ? *part + s : s;
+            } else a.xbar[(16 * t + n) * D + to] = few_cotangent(a, 16 * t + n, s);
         }
         __syncthreads();
     }

@@ -183,8 +183,8 @@ def categorical_logit_glm_lpmf_vjp(y, x, alpha, beta, lpbar=None, check=True):
     """:func:`categorical_logit_glm_lpmf` and its reverse mode in one call: ``(lp, xbar, alphabar, betabar)`` for the cotangent
     ``lpbar`` of the log probabilities (``None``: ones, the gradients of their sum). ``alphabar`` and ``betabar`` are summed over all
     leading dimensions (``alphabar`` is ``None`` where ``alpha`` is). A row without an observation has no gradient. The classes are
-    taken in pieces: what is held per row and class stays below 1.5 GB, however
-    many there are, and a maximum and a sum for every row and 128 or 256 classes beside it."""
+    taken in pieces: what is held per row and class (logits and their gradients) stays below 1.61 GB (1.5 * 2**30), however many there are,
+    and a maximum and a sum for every row and 128 or 256 classes (up to 64 rows: 16 to 64) beside it."""
     y, x, alpha, beta, bshape = _glm(y, x, alpha, beta, check)
     xm, ldx = _matrix(x)
     bm, ldb = _matrix(beta)

@@ -56,3 +56,15 @@ def test_shapes_without_a_gpu():
     for kw in (dict(shape=(3,)), dict(dtype=torch.float64)):
         with pytest.raises(ValueError, match="weight"):
             glm._alike("weight", torch.zeros(5), kw.get("shape", (5,)), kw.get("dtype", torch.float32), torch.device("cpu"))
+
+
+@pytest.mark.parametrize("dtype,size,acc", [(0, 8, 8), (1, 4, 4), (2, 2, 4), (3, 2, 4)])
+@pytest.mark.parametrize("rows", [1, 20, 64, 65, 3000])
+def test_workspace_per_row_and_class_is_bounded(lib, dtype, size, acc, rows):
+    """1.5 GB of logits and r, however many classes there are; beside it a maximum and a sum for every row and 128 classes (up to 64 rows: 64, 32 in
+    fp64), in fp32 three planes of beta, and what does not grow with the classes (transposes of a piece, sums for xbar)."""
+    features = 64
+    tile = 128 if rows > 64 else 32 if size == 8 else 64
+    for classes in (1 << 20, 1 << 22, 1 << 24, 1 << 26):
+        rest = 2 * acc * rows * (classes // tile + 1) + (6 * features * (classes + 64) if size == 4 else 0) + (256 << 20)
+        assert lib.gpt_categorical_logit_glm_workspace(dtype, rows, features, classes, 1) <= (3 << 29) + rest

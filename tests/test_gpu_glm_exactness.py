@@ -152,3 +152,13 @@ def test_more_tiles_than_a_grid_counts_threads(glm, name, v):
         de = (d + 2) * ea * (xd.abs() @ bd.abs().T + eta.abs()) + 4 * ea * (eta.abs() + lse.abs().unsqueeze(1))
         tol = 2 * de.max(1).values + (96 + v / 2048) * ea + 2 * ea * (lse.abs() + want.abs())
         assert bool(((lp[some].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("name,n,d,v", [("f64", 64, 66, 1100001), ("f64", 3, 66, 6000001), ("f32", 64, 71, 2200001), ("f16", 50, 72, 3900001),
+                                        ("bf16", 64, 67, 3200001)])
+def test_few_rows_of_very_many_classes(glm, name, n, d, v):
+    """So many that the logits and r of all classes at once would be more than is held per row and class."""
+    y, x, alpha, beta = _class_data(name, n, d, v, 5)
+    y[n // 3] = -1
+    x[n // 3] = float("nan")
+    _check_class(glm, name, y, x, alpha, beta)
