@@ -47,6 +47,8 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
     typedef typename Mma<T>::C C;
     constexpr int N = Vec16<T>::N, STEP = 4 * N; // a wave's step: 64 bytes of a row
     __shared__ A sum[WK][CT * 16][NT * 16 + 1];
+    __shared__ int own[NT * 16]; // the rows' classes where they are among the workgroup's, counted from its first
+    const int64_t y = threadIdx.x < NT * 16 && threadIdx.x < a.x.rows ? a.y[threadIdx.x] : -1; // (on its way while the product runs)
     const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
     const int64_t v0 = (int64_t)blockIdx.x * CT * 16, V = a.beta.rows, D = a.features;
     C c[CT][NT];
@@ -116,12 +118,15 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum[wave][16 * i + Mma<T>::row(q, r)][16 * t + (lane & 15)] = c[i][t][r];
+    if (threadIdx.x < NT * 16) {
+        const int64_t at = y - a.v0 - v0;
+        own[threadIdx.x] = at >= 0 && at < V - v0 && at < 16 * CT ? (int)at : -1;
+    }
     __syncthreads();
     // 16 threads a row (NT * 16 rows; the workgroup may take them in several goes), CT classes each
     const int k = threadIdx.x & 15;
     for (int n = threadIdx.x >> 4; n < NT * 16; n += 4 * WK) {
         A e[CT], mx = neg_inf<A>(), s = 0;
-        const int64_t y = n < a.x.rows ? a.y[n] : -1;
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
             const int64_t v = v0 + 16 * i + k;
@@ -130,7 +135,6 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
             for (int w = 0; w < WK; ++w) u += sum[w][16 * i + k][n];
             e[i] = times_log2e(u) + (v < V ? (a.alpha ? level_log2e((A)a.alpha[v]) : (A)0) : neg_inf<A>());
             mx = fmax(mx, e[i]);
-            if (a.v0 + v == y && v < V) a.eta_y[n] = e[i];
             if (a.eta && n < a.x.rows && v < a.ldv) a.eta[n * a.ldv + v] = e[i];
         }
 #pragma unroll
@@ -138,6 +142,11 @@ template <typename T, int NT, int CT, int WK, bool HALF> __global__ __launch_bou
 #pragma unroll
         for (int i = 0; i < CT; ++i) s += exp_log2e(e[i] - about(mx));
         s = sum16(s);
+        if (own[n] >= 0) { // (few workgroups hold a row's class)
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+                if (own[n] == 16 * i + k) a.eta_y[n] = e[i];
+        }
         if (k == 0 && n < a.x.rows) {
             a.part_max[n * a.tiles + blockIdx.x] = mx;
             a.part_sum[n * a.tiles + blockIdx.x] = s;
