@@ -92,7 +92,7 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
 
 namespace { // (a kernel of its own in each of the two)
 
-// Numbers the observed rows: row[number], y[number] (any y that is no class as `classes`), their count; behind them row lists the
+// Numbers the observed rows: row[number], y[number] (or null; any y that is no class as `classes`), their count; behind them row lists the
 // others, whose lp is 0. place (or null): the rows' numbers, -1 where there is no observation. parts (or null): the largest |lpbar| of
 // the observed rows of a workgroup, as class_scale leaves it. A workgroup takes INDEX_ROWS rows; runs: the observed ones of every
 // INDEX_ROWS (class_count), or null, and it counts those before its own for itself.
@@ -172,7 +172,7 @@ template <typename A> __global__ __launch_bounds__(1024) void class_index(const 
         if (place) place[i] = seen ? at : -1;
         if (seen) {
             row[at] = (int)i;
-            y_of[at] = (int)(v[k] < classes ? v[k] : classes);
+            if (y_of) y_of[at] = (int)(v[k] < classes ? v[k] : classes);
             ++at;
         } else {
             row[rows - 1 - (i - at)] = (int)i; // (i - at rows before this one have no observation)

@@ -611,7 +611,7 @@ template <typename T> struct NarrowPlan {
     static constexpr int NT = sizeof(T) == 8 ? 1 : 2;
     bool many_rows, many_classes, indexed;
     int64_t share, shares;
-    size_t top, share_of, w, at, scale, order, y_of, count, runs, part, bytes;
+    size_t top, share_of, w, at, scale, order, count, runs, part, bytes;
     NarrowPlan(int64_t rows, int64_t D, int64_t V, bool vjp) {
         const size_t A = sizeof(acc_t<T>);
         many_rows = tiles_of(rows, 64 * NT) >= 512;
@@ -632,10 +632,9 @@ template <typename T> struct NarrowPlan {
             to += (n + 255) / 256 * 256;
             return p;
         };
-        order = y_of = count = runs = 0;
+        order = count = runs = 0;
         if (indexed) {
             order = take(4 * (size_t)rows);
-            y_of = take(4 * (size_t)rows);
             count = take(4);
             runs = take(4 * (size_t)tiles_of(rows, INDEX_ROWS));
         }
@@ -682,7 +681,7 @@ template <typename T> hipError_t launch(const ClassArgs& c, bool vjp, hipStream_
     a.features = c.features;
     a.lp = (A*)c.lp;
     if (p.indexed) {
-        number_rows<A>(c.y, c.rows, c.classes, nullptr, (int*)(ws + p.order), (int*)(ws + p.y_of), (int*)(ws + p.count), a.lp, nullptr,
+        number_rows<A>(c.y, c.rows, c.classes, nullptr, (int*)(ws + p.order), nullptr, (int*)(ws + p.count), a.lp, nullptr,
                        nullptr, (int*)(ws + p.runs), st);
         a.order = (const int*)(ws + p.order);
         a.count = (const int*)(ws + p.count);

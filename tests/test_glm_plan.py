@@ -68,3 +68,10 @@ def test_workspace_per_row_and_class_is_bounded(lib, dtype, size, acc, rows):
     for classes in (1 << 20, 1 << 22, 1 << 24, 1 << 26):
         rest = 2 * acc * rows * (classes // tile + 1) + (6 * features * (classes + 64) if size == 4 else 0) + (256 << 20)
         assert lib.gpt_categorical_logit_glm_workspace(dtype, rows, features, classes, 1) <= (3 << 29) + rest
+
+
+@pytest.mark.parametrize("dtype", range(4))
+@pytest.mark.parametrize("rows", [20000, 1 << 20, 1 << 28])
+def test_few_features_take_one_number_a_row(lib, dtype, rows):
+    """The log density of many rows needs their order, a count for every 4096 of them and one in all, in pieces of 256 bytes."""
+    assert lib.gpt_categorical_logit_glm_workspace(dtype, rows, 8, 300, 0) <= 4 * rows + 4 * (rows // 4096 + 1) + 3 * 256
