@@ -10,8 +10,8 @@
 // and x, whose sums run down their columns there, the large tiles take transposed reads from LDS (for 65 rows x 4096 x 32000 in bf16 a
 // transposed copy of beta cost 400 us against 301), the small one transposed copies.
 //
-// What bounds it are the matrix cores: 4096 rows x 4096 features x 128000 classes in bf16 take 12.1 ms, 1.31 PFLOP/s in the first
-// sweep's logits and 1.15 in the products, at the 1.85-1.9 GHz that the power leaves (matrix cores 63 % busy).
+// What bounds it are the matrix cores: 4096 rows (3892 observed) x 4096 features x 128000 classes in bf16 take 12.1 to 12.5 ms, 1.14
+// PFLOP/s in the first sweep's logits and 1.19 in the products, at the 1.85-1.9 GHz that the power leaves (matrix cores 63 % busy).
 //
 // Sums, statistics and accumulators are Acc (fp32; fp64 for fp64 data). One intermediate is rounded to 16 bits where the data
 // have 16 bits: r, because the matrix instructions take both operands in one type. Its error (half a step of each entry) is

@@ -368,9 +368,10 @@ int gpt_layer_norm_vjp(gpt_ctx*, int dtype, const void* x, const void* weight, c
 /* Log probability of observed classes, Stan's categorical_logit_glm_lpmf row by row: eta = alpha + beta x,
  * lp[n] = eta[y[n]] - log sum_v exp eta[v] (Acc). x: `rows` rows of `features` T, ldx elements apart; beta: `classes` rows of
  * `features` T, ldbeta apart (the memory of Stan's column-major features x classes matrix); alpha: [classes] T or NULL, -inf
- * excludes a class (a row whose classes are all excluded has lp = -inf and no gradient). y: [rows] classes from 0;
- * y < 0: not observed -- lp = 0, no gradient, and that row of x may hold anything; y >= classes: lp and the gradients of
- * that row (so the sums over rows too) are NaN. Of the rows x classes logits a bounded part is stored at most (the workspace). */
+ * excludes a class, as an entry of beta does whose product is -inf (a row whose classes are all excluded has lp = -inf and no
+ * gradient). y: [rows] classes from 0; y < 0: not observed -- lp = 0, no gradient, and that row of x may hold anything;
+ * y >= classes: lp and the gradients of that row (so the sums over rows too) are NaN. lp is never above zero. Of the
+ * rows x classes logits a bounded part is stored at most (the workspace). */
 size_t gpt_categorical_logit_glm_workspace(int dtype, int64_t rows, int64_t features, int64_t classes, int vjp);
 int gpt_categorical_logit_glm_lpmf(gpt_ctx*, int dtype, const int64_t* y, const void* x, int64_t ldx, const void* alpha,
                                    const void* beta, int64_t ldbeta, int64_t rows, int64_t features, int64_t classes, void* lp,
